@@ -430,6 +430,85 @@ int msda_attention_bwd_dropout(const void* q, const void* k, const void* v, cons
 int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float rate, uint64_t seed,
                                 uint8_t* keep, void* stream);
 
+/* ---- Attention over packed sequences --------------------------------------------------------
+ * Softmax attention of sequences of different lengths that lie behind one another, with fewer key
+ * heads than query heads (heads a multiple of kv_heads: query head h reads key head
+ * h / (heads / kv_heads)), causal or not. No counterpart in the reference, whose attention
+ * (layers.py:54-99) takes one length, one number of heads and an explicit mask.
+ *   q, out, grad_out, grad_q   [q_rows, heads, head_dim]       dtype
+ *   k, v, grad_k, grad_v       [k_rows, kv_heads, head_dim]    dtype
+ *   q_offsets, k_offsets       [sequences + 1] int32, device memory, rising
+ *   k_lengths                  [sequences] int32, device memory, or NULL
+ * Sequence i holds the query rows q_offsets[i] .. q_offsets[i + 1] - 1 (n of them) and the m key rows
+ * from k_offsets[i] on: as many as k_lengths[i] says, or all before k_offsets[i + 1] (a cache has room
+ * for more rows than it holds). Query t of a sequence sees its keys j < m, with `causal` those with
+ * j <= t + m - n: the last query sees every key, so one new token over a cache of m keys is n = 1.
+ *   out = softmax(scale q k^T over the seen keys) v, 0 where no key is seen.
+ * A pair that is not seen takes no part, whatever its rows hold. Rows of out and of the gradients that
+ * belong to no sequence, and of grad_k and grad_v from the m-th of a sequence on, are written as zeros.
+ * Offsets and lengths are clamped to the tensors' rows: others than rising ones give unspecified
+ * values, never an access out of bounds.
+ *
+ * head_dim: a multiple of 8, at most 128. `strides` holds the element strides (row, head) of each
+ * tensor; channels are contiguous, and rows start on 16-byte boundaries (bases, and strides in bytes, are
+ * multiples of 16). scale > 0. q_rows * heads / kv_heads and k_rows below 2^31 less 128 rows a sequence.
+ * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
+ * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them and uses entry 2
+ * for rowsum(grad_out * out). May be NULL in a forward whose backward is not wanted.
+ * Sums, softmax and statistics are f32; bf16 products run on bf16 matrix instructions, with the softmax
+ * weights and their gradients rounded to bf16, f32 products on f32 ones. No result depends on an order of
+ * atomics.
+ */
+
+/*
+ * Device workspace of msda_packed_attention_fwd in bytes (a function of the shape only), or a negative
+ * code: the partial sums of calls with so few query rows that the keys of a sequence are split over
+ * several workgroups, else 0.
+ */
+int64_t msda_packed_attention_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);
+
+/* strides: [4 tensors: q, k, v, out][2]. The workspace is 16-byte aligned; NULL when its size is 0. */
+int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, float* stats,
+                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
+                              int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
+                              const int64_t* strides, int causal, float scale, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/*
+ * Backward of msda_packed_attention_fwd for the cotangent grad_out: grad_q, grad_k, grad_v (each may be
+ * NULL to skip it). out and stats are the forward's (stats entry 2 is overwritten).
+ * strides: [8 tensors: q, k, v, out, grad_out, grad_q, grad_k, grad_v][2].
+ */
+int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, float* stats,
+                              const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
+                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
+                              int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
+                              const int64_t* strides, int causal, float scale, void* stream);
+
+/* ---- Rotary positions on several axes -------------------------------------------------------
+ * Rotates channel pairs of queries and keys by angles that grow with the token's position on each of
+ * `axes` axes (time, height, width, ...). No counterpart in the reference.
+ *   q, q_out  [tokens, heads, head_dim], k, k_out  [tokens, kv_heads, head_dim]   dtype
+ *   positions [tokens, axes]  int32, int64 or f32 (enum msda_position_type), device memory
+ *   sections  host int32 [axes]: the number of pairs of each axis, in order; n is their sum, 2 n <= head_dim
+ * Pair i, the j-th of axis a, turns by positions[t][a] * base^-e: with shared_frequencies e = i / n (the
+ * axes share one falling sequence), else e = j / sections[a] (each axis has its own). Its channels are
+ * (i, i + n), or (2 i, 2 i + 1) with `interleaved`:
+ *   (u, w) -> (u cos - w sin, u sin + w cos).
+ * Channels from 2 n on are copied. inverse: by the negative angles (the gradient for the cotangents of
+ * q_out and k_out). Angles are formed in f64 and reduced to one turn before cos and sin, so that far
+ * positions keep their precision; the products are f32, rounded once.
+ * strides: element strides (token, head) of q, q_out, k, k_out [4][2], channels contiguous;
+ * position_strides: (token, axis). An output may be its input. heads or kv_heads may be 0 (its pointers
+ * NULL). head_dim even, at most 256; at most 8 axes.
+ */
+enum msda_position_type { MSDA_POSITION_I32 = 0, MSDA_POSITION_I64 = 1, MSDA_POSITION_F32 = 2 };
+
+int msda_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtype,
+                const void* positions, int position_type, int tokens, int heads, int kv_heads, int head_dim,
+                const int64_t* strides, const int64_t* position_strides, const int32_t* sections, int axes,
+                double base, int shared_frequencies, int interleaved, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,12 +28,10 @@
 
 #include <cstdint>
 
+#include "attention_common.h"
 #include "msda_kernels.h"  // bf16_t
 
 namespace msda {
-
-typedef float at_f4 __attribute__((ext_vector_type(4)));
-typedef float at_f16 __attribute__((ext_vector_type(16)));
 
 enum AttnTensor { kAtQ = 0, kAtK, kAtV, kAtO, kAtGO, kAtGQ, kAtGK, kAtGV, kAtTensors };
 
@@ -124,17 +122,6 @@ __device__ __forceinline__ void at_st1(VT* p, int64_t i, float v) {
   } else {
     p[i] = v;
   }
-}
-
-// 2^x by v_exp_f32 alone: results below 2^-126 flush to zero (a weight that small is below the
-// f32 resolution of any row sum it enters), 2^-inf = 0.
-__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-__device__ __forceinline__ at_f16 at_zero16() {
-  at_f16 z;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-  return z;
 }
 
 // A (slice, head) pair zh = z * H + h, and a tensor's base offset there.
@@ -260,18 +247,6 @@ __device__ __forceinline__ void at_accum1(at_f16 (&acc)[D / 32], const float* Xs
         acc[nd] = __builtin_amdgcn_mfma_f32_32x32x2f32(Xs[(8 * c4 + 4 * grp + j) * LD + 32 * nd + col], w[4 * c4 + j], acc[nd], 0, 0, 0);
 }
 
-// Reductions over the two halves of a wave (lanes l and l ^ 32, which hold the same query) by
-// v_permlane32_swap: both lanes get the same bits.
-__device__ __forceinline__ float at_max_halves(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-__device__ __forceinline__ float at_sum_halves(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // Scale two transposed score blocks (keys k0 + 32 h + 8 (i / 4) + 4 grp + i % 4 of register i, the
 // lane's query qi) by scale2, give keys past L the score -inf and blocked keys finfo.min (the mask
 // row of qi; qi < 0: no row), and take their maximum into bm. The mask test is hoisted out of the
@@ -316,8 +291,6 @@ __device__ __forceinline__ void at_scale_scores(at_f16& s0, at_f16& s1, int k0, 
 // Without a mask, on a full chunk, each score costs one fma (x - m) before exp2, and the maximum
 // is taken on those (a computed float is canonical, so the maximum needs no quieting of its
 // operands).
-constexpr float kAtLazy = 8.0f;
-constexpr float kAtLow = 64.0f;
 
 template <bool MASK>
 __device__ __forceinline__ float at_softmax_chunk(at_f16& s0, at_f16& s1, int k0, int L, float scale2, const uint8_t* mask, int qi, int grp,
@@ -363,17 +336,6 @@ __device__ __forceinline__ float at_softmax_chunk(at_f16& s0, at_f16& s1, int k0
   for (int i = 0; i < 16; ++i) rs += s0[i] + s1[i];
   l = l * alpha + at_sum_halves(rs);
   return alpha;
-}
-
-typedef __bf16 at_bf8 __attribute__((ext_vector_type(8)));
-typedef float at_f8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ at_bf8 at_bf8_of(uint2 lo, uint2 hi) { return __builtin_bit_cast(at_bf8, uint4{lo.x, lo.y, hi.x, hi.y}); }
-
-// registers i0 .. i0 + 7 of a result block, rounded to bf16 (v_cvt_pk_bf16_f32, nearest even)
-__device__ __forceinline__ at_bf8 at_bf8_regs(const at_f16& v, int i0) {
-  const at_f8 f = {v[i0], v[i0 + 1], v[i0 + 2], v[i0 + 3], v[i0 + 4], v[i0 + 5], v[i0 + 6], v[i0 + 7]};
-  return __builtin_convertvector(f, at_bf8);
 }
 
 // Stores a 32 x 32 result block v * scale (lane l: row r0 + l % 32, channels 8 c + 4 (l / 32) + e in
@@ -738,16 +700,6 @@ __device__ __forceinline__ int at_sw(int r) {
 template <int D>
 __device__ __forceinline__ int at_swo(int r, int ch) {
   return r * D + 8 * ((ch >> 3) ^ at_sw<D>(r)) + (ch & 7);
-}
-
-typedef short at_s4 __attribute__((ext_vector_type(4)));
-
-// ds_read_b64_tr_b16: within each group of 16 lanes, lane 4a + b receives element b of the 8 bytes
-// that lanes a, 4 + a, 8 + a and 12 + a address (in that order): the 16 x 4 block of 16-bit
-// elements the group addresses, transposed.
-__device__ __forceinline__ uint2 at_read_tr(const uint16_t* p) {
-  const at_s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(p));
-  return __builtin_bit_cast(uint2, r);
 }
 
 // A raw bf16 chunk (64 rows x D) in registers: 4-element vectors, rows clamped to L - 1.
@@ -1251,7 +1203,6 @@ __global__ void __launch_bounds__(64 * RB, D == 32 ? (MASK ? 2 : 3) : 1) attn_bw
     }
   }
 }
-
 
 // Fused backward (bf16, D = 32, L <= 32 kAtFusedBlocks, no mask: a masked kernel would not fit three
 // waves per SIMD without spilling): a workgroup is one (slice, head). Waves 0 .. nb - 1 own one key

@@ -1,0 +1,177 @@
+// packed_attention_abi.hip — C ABI of the attention over packed sequences (include/msda.h): validation,
+// launch planning, kernel launches. Validation runs before any HIP call.
+#include "msda.h"
+#include "packed_attention_launch.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace {
+
+using msda_host::aligned_to;
+using msda_host::fail;
+
+struct PackShape {
+  int dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim;
+};
+
+int64_t slots_of(int64_t rows, int sequences) { return rows / msda::kPkTile + sequences + 2; }
+
+int pk_shape(const PackShape& s) {
+  if (s.dtype != MSDA_DTYPE_F32 && s.dtype != MSDA_DTYPE_BF16) return fail(MSDA_ERR_UNSUPPORTED, "packed attention: unsupported dtype code %d", s.dtype);
+  if (s.sequences < 0 || s.q_rows < 0 || s.k_rows < 0 || s.heads < 0 || s.kv_heads < 0)
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: negative extent");
+  if (s.head_dim < 8 || s.head_dim > 128 || s.head_dim % 8 != 0)
+    return fail(MSDA_ERR_UNSUPPORTED, "packed attention: head_dim %d (multiples of 8 up to 128 supported)", s.head_dim);
+  if (s.heads != 0 && (s.kv_heads == 0 || s.heads % s.kv_heads != 0))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: %d heads do not divide into %d key heads", s.heads, s.kv_heads);
+  // row numbers of a key head's matrix, tiles included, are formed in 32 bits
+  const int64_t group = s.heads == 0 ? 1 : s.heads / s.kv_heads, tiles = (static_cast<int64_t>(s.sequences) + 3) * msda::kPkTile;
+  if (s.q_rows * group + tiles >= (int64_t{1} << 31) || s.k_rows + tiles >= (int64_t{1} << 31))
+    return fail(MSDA_ERR_UNSUPPORTED, "packed attention: too many rows");
+  return MSDA_OK;
+}
+
+// The number of parts that the keys are split into: with fewer workgroups than CUs hold (two each), as
+// many as fill them, of at least kLeast chunks of 64 keys of an average sequence.
+int pk_splits(const PackShape& s) {
+  constexpr int64_t kWant = 512, kLeast = 4, kMost = 64;
+  if (s.heads == 0 || s.sequences == 0) return 1;
+  const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads);
+  const int64_t groups = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
+  const int64_t chunks = (s.k_rows / s.sequences + msda::kPkChunk - 1) / msda::kPkChunk;
+  if (groups == 0) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / groups, chunks / kLeast, kMost})));
+}
+
+// Bytes of the split forward's parts: f32 sums, then (m, l) of every row.
+int64_t pk_workspace(const PackShape& s) {
+  const int splits = pk_splits(s);
+  return splits == 1 ? 0 : static_cast<int64_t>(splits) * s.q_rows * s.heads * (s.head_dim + 2) * 4;
+}
+
+int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
+  if (strides == nullptr) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: NULL strides");
+  const int64_t e = s.dtype == MSDA_DTYPE_BF16 ? 8 : 4;
+  for (int i = 0; i < 2 * ntensors; ++i)
+    if (strides[i] < 0 || strides[i] % e != 0)
+      return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: stride %d (%lld) must be a non-negative multiple of 16 bytes", i,
+                  static_cast<long long>(strides[i]));
+  return MSDA_OK;
+}
+
+msda::PackParams pk_params(const PackShape& s, const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, const int64_t* strides,
+                           int ntensors, const int* order, int causal, float scale) {
+  msda::PackParams p{};
+  p.q_offsets = q_offsets;
+  p.k_offsets = k_offsets;
+  p.k_lengths = k_lengths;
+  p.sequences = s.sequences;
+  p.q_rows = s.q_rows;
+  p.k_rows = s.k_rows;
+  p.heads = s.heads;
+  p.kv_heads = s.kv_heads;
+  p.group = s.heads / s.kv_heads;
+  p.dim = s.head_dim;
+  p.causal = causal != 0;
+  p.splits = 1;
+  p.scale = scale;
+  p.scale2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+  for (int t = 0; t < ntensors; ++t)
+    for (int j = 0; j < 2; ++j) p.st[order[t]][j] = strides[2 * t + j];
+  return p;
+}
+
+int pk_scale(float scale) {
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: scale %g must be positive and finite", static_cast<double>(scale));
+  return MSDA_OK;
+}
+
+int pk_offsets(const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths) {
+  if (q_offsets == nullptr || k_offsets == nullptr) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: NULL offsets");
+  if (!aligned_to(q_offsets, 4) || !aligned_to(k_offsets, 4) || !aligned_to(k_lengths, 4))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: offsets and lengths must be aligned to 4 bytes");
+  return MSDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t msda_packed_attention_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  const int rc = pk_shape(s);
+  return rc != MSDA_OK ? rc : pk_workspace(s);
+}
+
+int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, float* stats, const int32_t* q_offsets,
+                              const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                              int head_dim, const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  int rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 4)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
+  if (q_rows == 0 || heads == 0) return MSDA_OK;
+  if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
+  if (q == nullptr || out == nullptr || (k_rows != 0 && (k == nullptr || v == nullptr)))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: NULL tensor pointer");
+  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(stats, 16))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: tensors must be aligned to 16 bytes");
+  static const int order[4] = {msda::kPkQ, msda::kPkK, msda::kPkV, msda::kPkO};
+  msda::PackParams p = pk_params(s, q_offsets, k_offsets, k_lengths, strides, 4, order, causal, scale);
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.stats = stats;
+  p.slots = static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
+  p.splits = pk_splits(s);
+  if (p.splits > 1) {
+    const int64_t need = pk_workspace(s);
+    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+      return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * q_rows * heads * head_dim;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_fwd<msda::bf16_t>(p, st) : msda_host::dispatch_pk_fwd<float>(p, st);
+}
+
+int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, float* stats, const void* grad_out, int dtype,
+                              void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
+                              const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
+                              const int64_t* strides, int causal, float scale, void* stream) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  int rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 8)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
+  if (heads == 0 || (grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
+  if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
+  if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: NULL tensor pointer");
+  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(stats, 16) || !aligned_to(grad_out, 16) ||
+      !aligned_to(grad_q, 16) || !aligned_to(grad_k, 16) || !aligned_to(grad_v, 16))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: tensors must be aligned to 16 bytes");
+  static const int order[8] = {msda::kPkQ, msda::kPkK, msda::kPkV, msda::kPkO, msda::kPkGO, msda::kPkGQ, msda::kPkGK, msda::kPkGV};
+  msda::PackParams p = pk_params(s, q_offsets, k_offsets, k_lengths, strides, 8, order, causal, scale);
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.o = out;
+  p.go = grad_out;
+  p.gq = grad_q;
+  p.gk = grad_k;
+  p.gv = grad_v;
+  p.stats = stats;
+  const int q_slots = q_rows == 0 ? 0 : static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
+  const int k_slots = k_rows == 0 ? 0 : static_cast<int>(slots_of(k_rows, sequences));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_bwd<msda::bf16_t>(p, q_slots, k_slots, st)
+                                  : msda_host::dispatch_pk_bwd<float>(p, q_slots, k_slots, st);
+}
+
+}  // extern "C"

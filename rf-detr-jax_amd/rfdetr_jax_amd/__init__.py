@@ -6,7 +6,9 @@ backed by hand-written HIP kernels through the C ABI in include/msda.h. Also the
 (``MSDeformAttn``, ops.py:326-411) with its prologue, value projection and head split fused into the
 kernels, the segmentation head's point sampling (``bilinear_grid_sample``, ``point_sample``), and the
 decoder's grouped self-attention (``MultiheadAttention``, ``scaled_dot_product_attention``,
-layers.py:54-99, :491-548).
+layers.py:54-99, :491-548). Beside it, without a counterpart in the reference, attention over packed
+sequences of different lengths with grouped heads (``packed_attention``) and rotary positions on several
+axes (``rotary_embed``).
 """
 
 from .attention import (
@@ -28,6 +30,8 @@ from .ops import (
     ms_deform_attn_fused_backward,
     ms_deform_attn_fused_forward,
 )
+from .packed_attention import packed_attention, packed_attention_backward, packed_attention_forward
+from .rotary import rotary_embed
 from .value_proj import MSDeformAttn, value_proj_rows
 
 __all__ = [
@@ -46,7 +50,11 @@ __all__ = [
     "ms_deform_attn_fused",
     "ms_deform_attn_fused_backward",
     "ms_deform_attn_fused_forward",
+    "packed_attention",
+    "packed_attention_backward",
+    "packed_attention_forward",
     "point_sample",
+    "rotary_embed",
     "scaled_dot_product_attention",
     "value_proj_rows",
 ]

@@ -1,0 +1,315 @@
+"""The attention over packed sequences (msda_packed_attention_fwd / _bwd through rfdetr_jax_amd.packed_attention)
+on an MI355X, against the float64 oracle.
+
+Tolerances are the oracle's ``bounds``: element by element, from half a step of the type for each weight
+and result and 2^-24 for each term of an f32 sum.
+"""
+
+from __future__ import annotations
+
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import packed_attention_ref as PA
+from rfdetr_jax_amd import packed_attention, packed_attention_backward, packed_attention_forward, rotary_embed
+
+pytestmark = pytest.mark.gpu
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def _note(msg):
+    sys.stderr.write(f"[gpu] {msg}\n")
+    sys.stderr.flush()
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    return torch.device("cuda:0")
+
+
+def _int(x):
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device=_dev())
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _normal(seed, dtype, *shapes):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(dtype).to(_dev()) for s in shapes]
+
+
+def _within(got, want, bound, what):
+    got = _np(got)
+    assert got.shape == want.shape, what
+    assert np.isfinite(got).all(), f"{what}: not finite"
+    over = np.abs(got - want) - bound
+    at = np.unravel_index(np.argmax(over), over.shape)
+    assert over[at] <= 0, f"{what}: off by {abs(got[at] - want[at]):.3e} at {at}, {bound[at]:.3e} allowed"
+
+
+def _compare(q, k, v, g, got, seqs, causal, scale=None):
+    arrays = [_np(x) for x in (q, k, v, g)]
+    want = [PA.attention(*arrays[:3], seqs, causal, scale), *PA.attention_vjp(*arrays, seqs, causal, scale)]
+    bound = PA.bounds(*arrays, seqs, HALF_STEP[q.dtype], causal, scale)
+    for name, x, w, b in zip(("out", "grad_q", "grad_k", "grad_v"), got, want, bound):
+        if x is not None:
+            _within(x, w, b, name)
+
+
+def _run(q, k, v, g, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None):
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = packed_attention(*leaves, offsets, key_offsets, key_lengths, causal, scale)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    return (out, *torch.autograd.grad(out, leaves, g))
+
+
+#      lengths, keys, heads, key heads, head dim
+SHAPES = {
+    "one_token": ([1], [1], 1, 1, 32),
+    "ragged": ([5, 64, 1, 130, 33, 0, 63], None, 4, 2, 64),
+    "odd_group": ([43, 7, 90], None, 6, 2, 128),       # rows of a tile in groups of 3
+    "one_key_head": ([100, 29], None, 8, 1, 64),
+    "dim8": ([70, 3], None, 2, 2, 8),
+    "dim40": ([65, 31], None, 3, 1, 40),
+    "dim96": ([129, 40], None, 2, 1, 96),
+    "dim120": ([50, 66], None, 2, 2, 120),
+    "more_keys": ([3, 70, 0, 20], [200, 70, 5, 65], 4, 2, 64),
+    "fewer_keys": ([40, 9, 130], [10, 0, 127], 4, 2, 32),  # rows that see no key
+    "long": ([700, 1], None, 2, 1, 128),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("name", sorted(SHAPES))
+def test_against_oracle(name, causal, dtype):
+    lengths, keys, h, hk, d = SHAPES[name]
+    keys = lengths if keys is None else keys
+    _note(f"packed attention {name} causal={causal} {dtype}")
+    off, koff = np.cumsum([0, *lengths]), np.cumsum([0, *keys])
+    q, k, v, g = _normal(5, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d), (off[-1], h, d))
+    got = _run(q, k, v, g, _int(off), _int(koff), causal=causal)
+    _compare(q, k, v, g, got, PA.sequences(off, koff), causal)
+
+
+@TYPES
+def test_large_scores_and_scale(dtype):
+    """Scores that rise and fall by hundreds along the keys: the running reference score moves and rows are dominated by
+    one key."""
+    off = [0, 300, 333]
+    q, k, v, g = _normal(6, dtype, (333, 2, 64), (333, 1, 64), (333, 1, 64), (333, 2, 64))
+    ramp = torch.linspace(0.2, 6.0, 333, device=_dev())[:, None, None].to(dtype)
+    for kk in (k * ramp, k * ramp.flip(0)):
+        for scale in (None, 0.7):
+            got = _run(q, kk, v, g, _int(off), scale=scale)
+            _compare(q, kk, v, g, got, PA.sequences(off), True, scale)
+
+
+@TYPES
+def test_rows_outside_the_sequences(dtype):
+    """Rows before the first sequence, behind the last, and of a cache behind its keys: they hold NaN, take no part and
+    come out as zeros."""
+    off, koff, lengths = [3, 60, 60, 190], [7, 90, 140, 300], [57, 20, 130]
+    q, k, v, g = _normal(7, dtype, (200, 4, 64), (320, 2, 64), (320, 2, 64), (200, 4, 64))
+    seqs = PA.sequences(off, koff, lengths)
+    for x in (q, g):
+        x[:3] = x[190:] = float("nan")
+    outside = torch.ones(320, dtype=torch.bool, device=_dev())
+    for _, _, k0, m in seqs:
+        outside[k0:k0 + m] = False
+    k[outside] = v[outside] = float("nan")
+    got = _run(q, k, v, g, _int(off), _int(koff), _int(lengths))
+    for x in (got[0], got[1]):
+        assert not x[:3].any() and not x[190:].any()
+    for x in got[2:]:
+        assert not x[outside].any()
+    clean = [torch.nan_to_num(x) for x in (q, k, v, g)]
+    _compare(*clean, got, seqs, True)
+
+
+@TYPES
+def test_slices_of_a_projection_and_other_strides(dtype):
+    """q, k and v as slices of one projection's rows; head-major tensors; rows off their 16-byte boundaries (copied);
+    channels that are not contiguous; a key head for all rows by stride 0; a cotangent by stride 0."""
+    off = [0, 50, 131]
+    h, hk, d, seqs = 4, 2, 64, PA.sequences(off)
+    (qkv,) = _normal(8, dtype, (131, (h + 2 * hk) * d + 8))
+    flat = qkv[:, :-8].unflatten(1, (h + 2 * hk, d))
+    parts = [flat[:, :h], flat[:, h:h + hk], flat[:, h + hk:]]
+    (g,) = _normal(9, dtype, (131, h, d))
+    want = _run(*(x.contiguous() for x in parts), g, _int(off))
+    _compare(*parts, g, want, seqs, True)
+    head_major = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in parts]
+    shifted = [torch.empty(x.numel() + 1, dtype=dtype, device=_dev())[1:].view(x.shape).copy_(x) for x in parts]
+    channels = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in parts]
+    for other in (parts, head_major, shifted, channels):
+        got = _run(*other, g, _int(off))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = [parts[0], parts[1][:1].expand(131, hk, d), parts[2]]
+    got = _run(*one, g, _int(off))
+    _compare(*one, g, got, seqs, True)
+    ones = torch.ones((), dtype=dtype, device=_dev()).expand(131, h, d)
+    _compare(*parts, ones, _run(*parts, ones, _int(off)), seqs, True)
+
+
+@TYPES
+@pytest.mark.parametrize("new", [1, 7], ids=["one_token", "chunk"])
+@pytest.mark.parametrize("heads", [(8, 1), (4, 4), (16, 2)], ids=["8to1", "4to4", "16to2"])
+def test_tokens_over_a_cache(heads, new, dtype):
+    """Few new tokens over caches of different fill (one key, a tile less one, many), whose keys are split over
+    workgroups; unfilled rows hold NaN. A sequence without new tokens and one without keys are among them."""
+    h, hk = heads
+    room, fill, d = 2500, [2500, 1, 63, 0, 1999, 64], 128
+    lengths = [min(new, max(m, 1)) for m in fill]
+    lengths[4] = 0
+    off, koff = np.cumsum([0, *lengths]), np.arange(len(fill) + 1) * room
+    q, k, v = _normal(10, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d))
+    for i, m in enumerate(fill):
+        k[koff[i] + m:koff[i + 1]] = v[koff[i] + m:koff[i + 1]] = float("nan")
+    out = packed_attention(q, k, v, _int(off), _int(koff), _int(fill))
+    seqs = PA.sequences(off, koff, fill)
+    _compare(q, torch.nan_to_num(k), torch.nan_to_num(v), torch.zeros_like(q), (out,), seqs, True)
+    out2, stats = packed_attention_forward(q, k, v, _int(off), _int(koff), _int(fill))
+    assert torch.equal(out, out2)
+    (g,) = _normal(11, dtype, q.shape)
+    grads = packed_attention_backward(q, k, v, out2, stats, g, _int(off), _int(koff), _int(fill))
+    _compare(q, torch.nan_to_num(k), torch.nan_to_num(v), g, (out2, *grads), seqs, True)
+
+
+@TYPES
+def test_gradients_wanted_one_by_one(dtype):
+    off = [0, 77, 140]
+    q, k, v, g = _normal(12, dtype, (140, 4, 64), (140, 2, 64), (140, 2, 64), (140, 4, 64))
+    out, stats = packed_attention_forward(q, k, v, _int(off))
+    want = packed_attention_backward(q, k, v, out, stats, g, _int(off))
+    for i in range(3):
+        needs = [j == i for j in range(3)]
+        got = packed_attention_backward(q, k, v, out, stats, g, _int(off), needs=needs)
+        assert [x is not None for x in got] == needs and torch.equal(got[i], want[i])
+        leaves = [x.detach().requires_grad_(j == i) for j, x in enumerate((q, k, v))]
+        (grad,) = torch.autograd.grad(packed_attention(*leaves, _int(off)), [leaves[i]], g)
+        assert torch.equal(grad, want[i])
+    with torch.no_grad():
+        assert torch.equal(packed_attention(q, k, v, _int(off)), out)
+
+
+def test_empty_calls():
+    d = _dev()
+    for t, s, n in ((0, 0, 0), (0, 5, 1), (4, 0, 1), (4, 5, 0), (4, 5, 2)):
+        q = torch.randn(t, 2, 32, device=d, requires_grad=True)
+        k, v = (torch.randn(s, 1, 32, device=d, requires_grad=True) for _ in range(2))
+        off, koff = torch.zeros(n + 1, dtype=torch.int32, device=d), torch.zeros(n + 1, dtype=torch.int32, device=d)
+        out = packed_attention(q, k, v, off, koff)
+        grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+        assert not out.any() and not any(x.any() for x in grads)
+
+
+def test_offsets_that_do_not_rise_stay_in_bounds():
+    """Falling, negative and too large offsets and lengths are clamped: the call ends and a following right call is right."""
+    q, k, v, g = _normal(13, torch.float32, (150, 4, 32), (300, 2, 32), (300, 2, 32), (150, 4, 32))
+    for off, koff, lengths in (([0, 150, 20, 150], [0, 300, 10, 300], None), ([-5, 40, 1000, 2000], [-9, 100, 400, 9000], [900, -3, 50]),
+                               ([150, 0, 0, 0], [300, 0, 0, 0], [3, 3, 3])):
+        got = _run(q, k, v, g, _int(off), _int(koff), None if lengths is None else _int(lengths))
+        assert [x.shape for x in got] == [q.shape, q.shape, k.shape, v.shape]
+    off, koff = [0, 100, 150], [0, 200, 300]
+    _compare(q, k, v, g, _run(q, k, v, g, _int(off), _int(koff)), PA.sequences(off, koff), True)
+
+
+@TYPES
+def test_the_same_bits_each_time_and_beside_other_work(dtype):
+    """Two calls at once on two streams, and again: the same bits."""
+    off = _int([0, 200, 513, 600])
+    a = _normal(14, dtype, (600, 8, 64), (600, 2, 64), (600, 2, 64), (600, 8, 64))
+    b = _normal(15, dtype, (600, 8, 64), (600, 2, 64), (600, 2, 64), (600, 8, 64))
+    want = [_run(*x, off) for x in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for x, s in zip((a, b), streams):
+            with torch.cuda.stream(s):
+                got.append(_run(*x, off))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for x, y in zip(got, want) for p, q in zip(x, y))
+
+
+@TYPES
+def test_in_a_graph_with_other_lengths(dtype):
+    """One captured forward and backward, and a captured call with split keys, replayed with other lengths, offsets and
+    inputs and other eager work between: each replay gives the eager call's bits."""
+    q, k, v, g = _normal(16, dtype, (300, 4, 64), (300, 2, 64), (300, 2, 64), (300, 4, 64))
+    off = _int([0, 100, 300])
+    cq, ck, cv = _normal(17, dtype, (2, 4, 64), (4000, 2, 64), (4000, 2, 64))
+    coff, ckoff, fill = _int([0, 1, 2]), _int([0, 2000, 4000]), _int([2000, 5])
+
+    def work():
+        out, stats = packed_attention_forward(q, k, v, off)
+        return (out, *packed_attention_backward(q, k, v, out, stats, g, off), packed_attention(cq, ck, cv, coff, ckoff, fill))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = work()
+    for lengths, filled in (([0, 100, 300], [2000, 5]), ([0, 0, 177], [1, 1999]), ([20, 21, 290], [0, 700])):
+        off.copy_(_int(lengths))
+        fill.copy_(_int(filled))
+        q.mul_(-0.5)
+        eager = work()
+        torch.cuda.synchronize()
+        for x in outs:
+            x.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager)), (lengths, filled)
+
+
+@TYPES
+def test_rotary_prompt_and_tokens(dtype):
+    """As they are used together: a step of training on packed sequences with positions on three axes, and the same
+    sequences again token by token over a cache, whose last tokens agree with the prompt's within the bounds."""
+    h, hk, d, lengths, room = 4, 2, 64, [37, 70], 128
+    off = np.cumsum([0, *lengths])
+    (qkv,) = _normal(18, dtype, (off[-1], h + 2 * hk, d))
+    (g,) = _normal(19, dtype, (off[-1], h, d))
+    pos = torch.stack([torch.cat([torch.arange(n) for n in lengths])] * 3, 1).to(torch.int32).to(_dev())
+    leaf = qkv.detach().requires_grad_(True)
+    q, k = rotary_embed(leaf[:, :h], leaf[:, h:h + hk], pos, (8, 12, 12), shared_frequencies=True)
+    out = packed_attention(q, k, leaf[:, h + hk:], _int(off))
+    (grad,) = torch.autograd.grad(out, leaf, g)
+    seqs = PA.sequences(off)
+    v = qkv[:, h + hk:]
+    arrays = [_np(x) for x in (q, k, v, g)]
+    bound = PA.bounds(*arrays, seqs, HALF_STEP[dtype])
+    _within(out, PA.attention(*arrays[:3], seqs), bound[0], "out")
+    _within(grad[:, h + hk:], PA.attention_vjp(*arrays, seqs)[2], bound[3], "grad_v")
+    # the gradient of the unrotated keys: a rotation mixes two channels' errors, and rounds once
+    from oracle import rotary_ref as RO
+
+    for at, i in ((slice(0, h), 1), (slice(h, h + hk), 2)):
+        want = RO.rotate(PA.attention_vjp(*arrays, seqs)[i - 1], pos.cpu().numpy(), (8, 12, 12), shared=True, sign=-1.0)
+        e = bound[i]
+        both = np.concatenate([e[..., :32] + e[..., 32:]] * 2, -1)
+        _within(grad[:, at], want, both + (HALF_STEP[dtype] + 2.0 ** -20) * (np.abs(want) + both), "grad of the projection")
+    # token by token
+    cache = [torch.full((len(lengths) * room, hk, d), float("nan"), dtype=dtype, device=_dev()) for _ in range(2)]
+    starts = _int(np.arange(len(lengths) + 1) * room)
+    for i, n in enumerate(lengths):
+        cache[0][i * room:i * room + n - 1], cache[1][i * room:i * room + n - 1] = k.detach()[off[i]:off[i + 1] - 1], v[off[i]:off[i + 1] - 1]
+    last = torch.tensor(off[1:] - 1, device=_dev())
+    nq, nk = rotary_embed(qkv[last, :h], qkv[last, h:h + hk], pos[last], (8, 12, 12), shared_frequencies=True)
+    assert torch.equal(nq, q[last]) and torch.equal(nk, k[last])
+    rows = torch.tensor([i * room + n - 1 for i, n in enumerate(lengths)], device=_dev())
+    cache[0][rows], cache[1][rows] = nk, v[last]
+    got = packed_attention(nq, *cache, _int([0, 1, 2]), starts, _int(lengths))
+    at = last.cpu().numpy()
+    _within(got, PA.attention(*arrays[:3], seqs)[at], bound[0][at], "token by token")
