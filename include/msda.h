@@ -451,39 +451,43 @@ int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float
  *
  * head_dim: a multiple of 8, at most 128. `strides` holds the element strides (row, head) of each
  * tensor; channels are contiguous, and rows start on 16-byte boundaries (bases, and strides in bytes, are
- * multiples of 16). scale > 0. q_rows * heads / kv_heads and k_rows below 2^31 less 128 rows a sequence.
+ * multiples of 16), head_dim to 2^22 elements apart, a row's heads within 2^23 elements. scale > 0. q_rows * heads / kv_heads and k_rows below 2^31 less 128 rows a sequence.
  * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
- * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them and uses entry 2
- * for rowsum(grad_out * out). May be NULL in a forward whose backward is not wanted.
+ * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them and uses entries 2
+ * and 3 between its kernels. May be NULL in a forward whose backward is not wanted.
+ * out_rest: NULL, or for bf16 a tensor of out's strides: the forward writes what out's rounding left, the
+ * backward reads out + out_rest for rowsum(grad_out * out), whose error is then that of f32 sums.
  * Sums, softmax and statistics are f32; bf16 products run on bf16 matrix instructions, with the softmax
  * weights and their gradients rounded to bf16, f32 products on f32 ones. No result depends on an order of
  * atomics.
  */
 
 /*
- * Device workspace of msda_packed_attention_fwd in bytes (a function of the shape only), or a negative
- * code: the partial sums of calls with so few query rows that the keys of a sequence are split over
- * several workgroups, else 0.
+ * Device workspaces in bytes (functions of the shape only), or a negative code: partial sums of forward
+ * calls with so few query rows that the keys of a sequence are split over several workgroups, and of
+ * backward calls with so few key tiles that the rows seeing one are; else 0.
  */
-int64_t msda_packed_attention_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);
+int64_t msda_packed_attention_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);
+int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);
 
 /* strides: [4 tensors: q, k, v, out][2]. The workspace is 16-byte aligned; NULL when its size is 0. */
-int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, float* stats,
-                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
-                              int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
-                              const int64_t* strides, int causal, float scale, void* workspace,
-                              int64_t workspace_bytes, void* stream);
+int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest,
+                              float* stats, const int32_t* q_offsets, const int32_t* k_offsets,
+                              const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads,
+                              int kv_heads, int head_dim, const int64_t* strides, int causal, float scale,
+                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Backward of msda_packed_attention_fwd for the cotangent grad_out: grad_q, grad_k, grad_v (each may be
- * NULL to skip it). out and stats are the forward's (stats entry 2 is overwritten).
+ * NULL to skip it). out, out_rest and stats are the forward's (stats entries 2 and 3 are overwritten).
  * strides: [8 tensors: q, k, v, out, grad_out, grad_q, grad_k, grad_v][2].
  */
-int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, float* stats,
-                              const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
-                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
-                              int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
-                              const int64_t* strides, int causal, float scale, void* stream);
+int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                              float* stats, const void* grad_out, int dtype, void* grad_q, void* grad_k,
+                              void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
+                              const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads,
+                              int kv_heads, int head_dim, const int64_t* strides, int causal, float scale,
+                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Rotary positions on several axes -------------------------------------------------------
  * Rotates channel pairs of queries and keys by angles that grow with the token's position on each of

@@ -47,9 +47,26 @@ int pk_splits(const PackShape& s) {
 }
 
 // Bytes of the split forward's parts: f32 sums, then (m, l) of every row.
-int64_t pk_workspace(const PackShape& s) {
+int64_t pk_fwd_workspace(const PackShape& s) {
   const int splits = pk_splits(s);
   return splits == 1 ? 0 : static_cast<int64_t>(splits) * s.q_rows * s.heads * (s.head_dim + 2) * 4;
+}
+
+// The number of workgroups that may share a tile of keys in the backward: a causal sequence's first keys are
+// seen by all its rows, so with few tiles the longest one sets the time. Twice two workgroups a CU, and no
+// more than the rows of one long sequence are worth.
+int pk_parts(const PackShape& s) {
+  constexpr int64_t kWant = 1024, kMost = 8;
+  if (s.heads == 0 || s.sequences == 0 || s.k_rows == 0) return 1;
+  const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
+  const int64_t chunks = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / msda::kPkChunk;
+  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, chunks / msda::kPkLeastPart, kMost})));
+}
+
+// Bytes of the parts' f32 sums of dk and dv.
+int64_t pk_bwd_workspace(const PackShape& s) {
+  const int parts = pk_parts(s);
+  return parts == 1 ? 0 : static_cast<int64_t>(parts) * 2 * s.k_rows * s.kv_heads * s.head_dim * 4;
 }
 
 int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
@@ -59,6 +76,11 @@ int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
     if (strides[i] < 0 || strides[i] % e != 0)
       return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: stride %d (%lld) must be a non-negative multiple of 16 bytes", i,
                   static_cast<long long>(strides[i]));
+  for (int i = 0; i < ntensors; ++i)  // a tile's byte offsets are formed in 31 bits, its end from its rows
+    if (strides[2 * i] != 0 || strides[2 * i + 1] != 0)
+      if (strides[2 * i] < s.head_dim || strides[2 * i] >= (int64_t{1} << 22) || strides[2 * i + 1] * s.heads >= (int64_t{1} << 23))
+        return fail(MSDA_ERR_UNSUPPORTED, "packed attention: strides %lld, %lld of tensor %d: rows must lie head_dim to 2^22 elements apart, a row's heads within 2^23",
+                    static_cast<long long>(strides[2 * i]), static_cast<long long>(strides[2 * i + 1]), i);
   return MSDA_OK;
 }
 
@@ -100,15 +122,22 @@ int pk_offsets(const int32_t* q_offsets, const int32_t* k_offsets, const int32_t
 
 extern "C" {
 
-int64_t msda_packed_attention_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
+int64_t msda_packed_attention_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   const int rc = pk_shape(s);
-  return rc != MSDA_OK ? rc : pk_workspace(s);
+  return rc != MSDA_OK ? rc : pk_fwd_workspace(s);
 }
 
-int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, float* stats, const int32_t* q_offsets,
-                              const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  const int rc = pk_shape(s);
+  return rc != MSDA_OK ? rc : pk_bwd_workspace(s);
+}
+
+int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest, float* stats,
+                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
                               int head_dim, const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes,
                               void* stream) {
   msda_host::clear_error();
@@ -119,7 +148,7 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if (q == nullptr || out == nullptr || (k_rows != 0 && (k == nullptr || v == nullptr)))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: NULL tensor pointer");
-  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(stats, 16))
+  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(out_rest, 16) || !aligned_to(stats, 16))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: tensors must be aligned to 16 bytes");
   static const int order[4] = {msda::kPkQ, msda::kPkK, msda::kPkV, msda::kPkO};
   msda::PackParams p = pk_params(s, q_offsets, k_offsets, k_lengths, strides, 4, order, causal, scale);
@@ -127,11 +156,12 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   p.k = k;
   p.v = v;
   p.out = out;
+  p.rest = dtype == MSDA_DTYPE_BF16 ? out_rest : nullptr;
   p.stats = stats;
   p.slots = static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
   p.splits = pk_splits(s);
   if (p.splits > 1) {
-    const int64_t need = pk_workspace(s);
+    const int64_t need = pk_fwd_workspace(s);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
     p.part_o = static_cast<float*>(workspace);
@@ -141,10 +171,10 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_fwd<msda::bf16_t>(p, st) : msda_host::dispatch_pk_fwd<float>(p, st);
 }
 
-int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, float* stats, const void* grad_out, int dtype,
-                              void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
+int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, float* stats,
+                              const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
                               const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
-                              const int64_t* strides, int causal, float scale, void* stream) {
+                              const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
@@ -153,8 +183,8 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: NULL tensor pointer");
-  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(stats, 16) || !aligned_to(grad_out, 16) ||
-      !aligned_to(grad_q, 16) || !aligned_to(grad_k, 16) || !aligned_to(grad_v, 16))
+  if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(out_rest, 16) || !aligned_to(stats, 16) ||
+      !aligned_to(grad_out, 16) || !aligned_to(grad_q, 16) || !aligned_to(grad_k, 16) || !aligned_to(grad_v, 16))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: tensors must be aligned to 16 bytes");
   static const int order[8] = {msda::kPkQ, msda::kPkK, msda::kPkV, msda::kPkO, msda::kPkGO, msda::kPkGQ, msda::kPkGK, msda::kPkGV};
   msda::PackParams p = pk_params(s, q_offsets, k_offsets, k_lengths, strides, 8, order, causal, scale);
@@ -162,11 +192,19 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
   p.k = k;
   p.v = v;
   p.o = out;
+  p.rest = dtype == MSDA_DTYPE_BF16 ? const_cast<void*>(out_rest) : nullptr;
   p.go = grad_out;
   p.gq = grad_q;
   p.gk = grad_k;
   p.gv = grad_v;
   p.stats = stats;
+  if (grad_k != nullptr || grad_v != nullptr) p.splits = pk_parts(s);
+  if (p.splits > 1) {
+    const int64_t need = pk_bwd_workspace(s);
+    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+      return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
+    p.part_kv = static_cast<float*>(workspace);
+  }
   const int q_slots = q_rows == 0 ? 0 : static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
   const int k_slots = k_rows == 0 ? 0 : static_cast<int>(slots_of(k_rows, sequences));
   hipStream_t st = static_cast<hipStream_t>(stream);

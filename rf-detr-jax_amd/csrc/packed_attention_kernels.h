@@ -22,13 +22,14 @@
 // rows), a lane owns one own row (its softmax statistics stay in the lane), and the weights in their
 // result registers are the B operand of the next product, whose A operand is read from the streamed
 // tile by transposing LDS reads. Streamed tiles of 64 rows lie in LDS as swizzled rows, written by
-// global_load_lds (no registers, two buffers, one barrier a tile); rows past a sequence's end and
-// channels past head_dim come from a page of zeros.
+// buffer loads into LDS (no registers, two buffers, one barrier a tile), which bring zeros for rows past a
+// sequence's end and channels past head_dim.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "attention_common.h"
 #include "msda_kernels.h"  // bf16_t, wait_vmem
@@ -44,15 +45,17 @@ struct PackParams {
   const void* o;   // backward: the forward output
   const void* go;  // backward: grad of the output
   void* out;
+  void* rest;  // forward: what out's rounding left (out's type and strides), or null; backward: the same, read
   void* gq;  // backward outputs (each may be null)
   void* gk;
   void* gv;
-  float* stats;  // [q_rows * heads][4]: m, log2 l (forward), delta (backward), unused; row (token, head)
+  float* stats;  // [q_rows * heads][4]: m, log2 l (forward); two numbers of the backward (pk_bwd_q_kernel); row (token, head)
   const int32_t* q_offsets;  // [sequences + 1]
   const int32_t* k_offsets;  // [sequences + 1]
   const int32_t* k_lengths;  // [sequences], or null: all rows of a sequence's range
   float* part_o;             // split forward: [splits][q_rows * heads][dim], sums relative to part_ml's m
   float* part_ml;            // [splits][q_rows * heads][2]: m, l
+  float* part_kv;            // key side: [splits][dk, dv][k_rows * kv_heads][dim]
   int64_t st[kPkTensors][2];  // element strides (row, head) of each tensor
   int sequences, q_rows, k_rows, heads, kv_heads, group, dim, causal, splits;
   int slots;     // tiles of the kernel's own side
@@ -62,6 +65,7 @@ struct PackParams {
 
 constexpr int kPkTile = 128;  // own rows of a workgroup: 32 a wave
 constexpr int kPkChunk = 64;  // streamed rows of a tile
+constexpr int kPkLeastPart = 16;  // chunks that are worth a workgroup of their own on the key side
 
 __device__ __align__(16) const uint32_t pk_zeros[4] = {0u, 0u, 0u, 0u};
 
@@ -105,18 +109,41 @@ __device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequence
 
 // ---- operands ----------------------------------------------------------------------------------
 
+using PkLds = const MSDA_LDS unsigned char*;
+
 // DT: channels that the products run over (head_dim rounded up to 32); a tile's rows lie DP apart.
 template <typename T, int DT>
 struct PkTile {
   static constexpr int DP = DT == 96 ? 128 : DT;
   static constexpr int E = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte chunk
   static constexpr int CPR = DP / E;                          // chunks of a row
-  static constexpr int BYTES = kPkChunk * DP * static_cast<int>(sizeof(T));
-  static constexpr int ND = DT / 32;
+  static constexpr int ROW = DP * static_cast<int>(sizeof(T));  // bytes of a row
+  static constexpr int BYTES = kPkChunk * ROW;
   // 16-byte chunk c of row r sits at slot c ^ swizzle(r): the rows that a read takes together fall on
   // distinct banks
   static __device__ __forceinline__ int swizzle(int r) { return CPR >= 16 ? (r & 15) : ((r / (16 / CPR)) & (CPR - 1)); }
-  static __device__ __forceinline__ int at(int r, int ch) { return r * DP + E * ((ch / E) ^ swizzle(r)) + (ch % E); }
+};
+
+// A lane's byte offsets in a tile. The chunks that one lane reads differ in bits that neither its row's
+// swizzle nor a carry reaches, so they are an exclusive or with a constant away from one offset, and rows
+// 8 apart the mask kRows8: an offset costs one instruction, and a few registers serve a whole tile.
+template <typename T, int DT>
+struct PkLane {
+  using Tile = PkTile<T, DT>;
+  static constexpr uint32_t kRows8 = Tile::CPR >= 16 ? 128 : 8 * Tile::CPR;  // swizzle(r) ^ swizzle(r + 8), as bytes
+  uint32_t row;  // row col, chunk grp: operands along the channels
+  uint32_t tr;   // bf16: rows 4 grp + (lane % 16) / 4, channels 16 (lane / 16 % 2) + 4 (lane % 4)
+                 // f32: row 4 grp, channel col: operands along the rows
+  __device__ __forceinline__ explicit PkLane(int lane) {
+    const int grp = lane >> 5, col = lane & 31;
+    row = col * Tile::ROW + ((grp ^ Tile::swizzle(col)) << 4);
+    if constexpr (sizeof(T) == 2) {
+      const int g = (lane >> 4) & 1, r = lane & 15, ro = 4 * grp + (r >> 2);
+      tr = ro * Tile::ROW + (((2 * g + ((r & 3) >> 1)) ^ Tile::swizzle(ro)) << 4) + (r & 1) * 8;
+    } else {
+      tr = 4 * grp * Tile::ROW + (((col >> 2) ^ Tile::swizzle(4 * grp)) << 4) + (col & 3) * 4;
+    }
+  }
 };
 
 // One row's channels as the B operand of the score products.
@@ -165,58 +192,126 @@ struct PkRow<float, DT> {
   }
 };
 
-// Scores of the 32-row block at row x0 of a tile against the lane's row: register i holds streamed row
-// x0 + 8 (i / 4) + 4 grp + i % 4.
-template <typename T, int DT>
-__device__ __forceinline__ at_f16 pk_scores(const T* X, int x0, const PkRow<T, DT>& r, int col, int grp) {
-  using Tile = PkTile<T, DT>;
-  at_f16 s = at_zero16();
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < DT / 16; ++i) {
-      const at_bf8 a = __builtin_bit_cast(at_bf8, *reinterpret_cast<const uint4*>(&X[Tile::at(x0 + col, 16 * i + 8 * grp)]));
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, r.x[i], s, 0, 0, 0);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < DT / 8; ++c) {
-      const at_f4 a = *reinterpret_cast<const at_f4*>(&X[Tile::at(x0 + col, 8 * c + 4 * grp)]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], r.x[c][j], s, 0, 0, 0);
-    }
-  }
-  return s;
+__device__ __forceinline__ uint2 pk_read_tr(PkLds p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MSDA_LDS at_s4*)(p)));
 }
 
-// acc += X^T w for the 32-row block at row x0 of a tile, w in result-layout registers: acc[nd] register i
-// holds channel 32 nd + 8 (i / 4) + 4 grp + i % 4 of the lane's row. bf16: w is rounded to bf16 for the
-// product (half a step, 2^-8 of each weight at most: as much as the inputs' and the result's own rounding).
-template <typename T, int DT>
-__device__ __forceinline__ void pk_accumulate(at_f16 (&acc)[DT / 32], const T* X, int x0, const at_f16& w, int lane) {
-  using Tile = PkTile<T, DT>;
-  const int grp = lane >> 5;
-  if constexpr (sizeof(T) == 2) {
-    const int g = lane >> 4, r = lane & 15;
-    const uint16_t* U = reinterpret_cast<const uint16_t*>(X);
+// N products, the operand of each read from LDS PF products ahead. The barriers hold LDS reads and products
+// in this order (vector and scalar instructions may pass): left to itself the compiler reads an operand,
+// waits for it, and multiplies, one at a time.
+template <int N, int PF, typename Read, typename Use>
+__device__ __forceinline__ void pk_pipe(Read&& read, Use&& use) {
+  decltype(read(0)) a[PF];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const at_bf8 b = at_bf8_regs(w, 8 * s);
+  for (int i = 0; i < PF; ++i) a[i] = read(i);
+  __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
-      for (int nd = 0; nd < DT / 32; ++nd) {
-        const int c = 32 * nd + 16 * (g & 1) + 4 * (r & 3), ro = x0 + 16 * s + 4 * grp + (r >> 2);
-        const at_bf8 a = at_bf8_of(at_read_tr(U + Tile::at(ro, c)), at_read_tr(U + Tile::at(ro + 8, c)));
-        acc[nd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[nd], 0, 0, 0);
-      }
-    }
-  } else {
-    const int col = lane & 31;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-      for (int nd = 0; nd < DT / 32; ++nd)
-        acc[nd] = __builtin_amdgcn_mfma_f32_32x32x2f32(X[Tile::at(x0 + 8 * (i >> 2) + 4 * grp + (i & 3), 32 * nd + col)], w[i], acc[nd], 0, 0, 0);
+  for (int i = 0; i < N; ++i) {
+    use(i, a[i % PF]);
+    if (i + PF < N) a[i % PF] = read(i + PF);
+    __builtin_amdgcn_sched_barrier(0x6);
   }
 }
+
+// Operands of one 32-row block of a tile. Scores of block X against the lane's row r: register i of the
+// result holds streamed row 8 (i / 4) + 4 grp + i % 4. Sums X^T w, w in result-layout registers: register
+// i of acc[nd] holds channel 32 nd + 8 (i / 4) + 4 grp + i % 4 of the lane's row; bf16: w is rounded to
+// bf16 for the product (half a step, 2^-8 of each weight at most: as much as the inputs' and the result's
+// own rounding).
+template <typename T, int DT>
+struct PkProducts;
+
+template <int DT>
+struct PkProducts<bf16_t, DT> {
+  using T = bf16_t;
+  static constexpr int ROW = PkTile<T, DT>::ROW, KS = DT / 16, ND = DT / 32;
+  static constexpr int kScores = KS, kSums = 2 * ND;  // products of a block
+  static __device__ __forceinline__ at_bf8 row_operand(PkLds X, const PkLane<T, DT>& at, int i) {
+    return *reinterpret_cast<const MSDA_LDS at_bf8*>(X + (at.row ^ (i << 5)));
+  }
+  static __device__ __forceinline__ void score(at_f16& s, const at_bf8& a, const PkRow<T, DT>& r, int i) {
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, r.x[i], s, 0, 0, 0);
+  }
+  // product j: rows 16 (j / ND) .. + 15, channels of block j % ND
+  static __device__ __forceinline__ at_bf8 sum_operand(PkLds X, const PkLane<T, DT>& at, int j) {
+    const int s = j / ND, nd = j % ND;
+    const uint32_t o = at.tr ^ (nd << 6);
+    return at_bf8_of(pk_read_tr(X + o + 16 * s * ROW), pk_read_tr(X + (o ^ PkLane<T, DT>::kRows8) + (16 * s + 8) * ROW));
+  }
+  struct Weights {
+    at_bf8 b[2];
+    __device__ __forceinline__ explicit Weights(const at_f16& w) : b{at_bf8_regs(w, 0), at_bf8_regs(w, 8)} {}
+  };
+  static __device__ __forceinline__ void sum(at_f16 (&acc)[ND], const at_bf8& a, const Weights& w, int j) {
+    acc[j % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.b[j / ND], acc[j % ND], 0, 0, 0);
+  }
+};
+
+template <int DT>
+struct PkProducts<float, DT> {
+  using T = float;
+  static constexpr int ROW = PkTile<T, DT>::ROW, ND = DT / 32;
+  static constexpr int kScores = DT / 8, kSums = 16;  // steps of a block (4 and ND products each)
+  static __device__ __forceinline__ at_f4 row_operand(PkLds X, const PkLane<T, DT>& at, int c) {
+    return *reinterpret_cast<const MSDA_LDS at_f4*>(X + (at.row ^ (c << 5)));
+  }
+  static __device__ __forceinline__ void score(at_f16& s, const at_f4& a, const PkRow<T, DT>& r, int c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], r.x[c][j], s, 0, 0, 0);
+  }
+  struct Operand {
+    float a[ND];
+  };
+  static __device__ __forceinline__ Operand sum_operand(PkLds X, const PkLane<T, DT>& at, int i) {
+    constexpr int S = PkTile<T, DT>::CPR;
+    const int ro = 8 * (i >> 2) + (i & 3);  // its swizzle: row 4 grp's, and a constant (4 grp + i % 4 carries nothing)
+    const uint32_t x = S >= 16 ? (ro & 15) : ((ro / (16 / S)) & (S - 1));
+    Operand o;
+#pragma unroll
+    for (int nd = 0; nd < ND; ++nd) o.a[nd] = *reinterpret_cast<const MSDA_LDS float*>(X + (at.tr ^ ((x ^ (8 * nd)) << 4)) + ro * ROW);
+    return o;
+  }
+  struct Weights {
+    at_f16 b;
+    __device__ __forceinline__ explicit Weights(const at_f16& w) : b(w) {}
+  };
+  static __device__ __forceinline__ void sum(at_f16 (&acc)[ND], const Operand& o, const Weights& w, int i) {
+#pragma unroll
+    for (int nd = 0; nd < ND; ++nd) acc[nd] = __builtin_amdgcn_mfma_f32_32x32x2f32(o.a[nd], w.b[i], acc[nd], 0, 0, 0);
+  }
+};
+
+// s += scores of X with x, t += scores of Y with y.
+template <typename T, int DT, int PF>
+__device__ __forceinline__ void pk_scores2(at_f16& s, PkLds X, const PkRow<T, DT>& x, at_f16& t, PkLds Y, const PkRow<T, DT>& y,
+                                           const PkLane<T, DT>& at) {
+  using P = PkProducts<T, DT>;
+  constexpr int N = P::kScores;
+  pk_pipe<2 * N, PF>([&](int i) { return P::row_operand(i < N ? X : Y, at, i % N); },
+                     [&](int i, const auto& a) { P::score(i < N ? s : t, a, i < N ? x : y, i % N); });
+}
+
+// acc += X^T w
+template <typename T, int DT, int PF>
+__device__ __forceinline__ void pk_accumulate(at_f16 (&acc)[DT / 32], PkLds X, const at_f16& w, const PkLane<T, DT>& at) {
+  using P = PkProducts<T, DT>;
+  const typename P::Weights b(w);
+  pk_pipe<P::kSums, PF>([&](int i) { return P::sum_operand(X, at, i); }, [&](int i, const auto& a) { P::sum(acc, a, b, i); });
+}
+
+// ax += X^T wx, ay += Y^T wy
+template <typename T, int DT, int PF>
+__device__ __forceinline__ void pk_accumulate2(at_f16 (&ax)[DT / 32], PkLds X, const at_f16& wx, at_f16 (&ay)[DT / 32], PkLds Y, const at_f16& wy,
+                                               const PkLane<T, DT>& at) {
+  using P = PkProducts<T, DT>;
+  constexpr int N = P::kSums;
+  const typename P::Weights bx(wx), by(wy);
+  pk_pipe<2 * N, PF>([&](int i) { return P::sum_operand(i < N ? X : Y, at, i % N); },
+                     [&](int i, const auto& a) { P::sum(i < N ? ax : ay, a, i < N ? bx : by, i % N); });
+}
+
+typedef __bf16 pk_bf16 __attribute__((ext_vector_type(16)));
+typedef __bf16 pk_bf4 __attribute__((ext_vector_type(4)));
 
 // A wave's LDS accesses are in order; this keeps the compiler from exchanging them.
 __device__ __forceinline__ void pk_wave_sync() {
@@ -227,14 +322,16 @@ __device__ __forceinline__ void pk_wave_sync() {
 
 // Writes acc * f (f: of the lane's row) as rows of T: through the wave's LDS scratch, so that each lane
 // stores 16 bytes and the wave whole rows. `row(r)`: the address of own row r of the wave's 32, or null.
-template <typename T, int DT, typename R>
+// REST: what the rounding to T leaves of them instead.
+template <typename T, int DT, bool REST = false, typename R>
 __device__ __forceinline__ void pk_store(const at_f16 (&acc)[DT / 32], float f, T* scratch, int dim, int lane, R&& row) {
   constexpr int E = 16 / static_cast<int>(sizeof(T)), LD = DT + E, C = DT / E;
   static_assert(32 * LD * sizeof(T) <= PkTile<T, DT>::BYTES, "the scratch fits a tile");
   const int grp = lane >> 5, col = lane & 31;
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) {
-    const at_f16 v = acc[nd] * f;
+    at_f16 v = acc[nd] * f;
+    if constexpr (REST) v -= __builtin_convertvector(__builtin_convertvector(v, pk_bf16), at_f16);
     if constexpr (sizeof(T) == 2) {
       uint16_t* t = reinterpret_cast<uint16_t*>(scratch) + col * LD + 32 * nd + 4 * grp;
 #pragma unroll
@@ -250,7 +347,7 @@ __device__ __forceinline__ void pk_store(const at_f16 (&acc)[DT / 32], float f, 
     }
   }
   pk_wave_sync();
-#pragma unroll
+#pragma unroll 2
   for (int k = 0; k < C / 2; ++k) {
     const int idx = lane + 64 * k, r = idx / C, ch = E * (idx - r * C);
     T* to = row(r);
@@ -272,34 +369,57 @@ __device__ __forceinline__ void pk_zero_rows(int r0, int r1, int dim, R&& row) {
 
 // ---- streaming ---------------------------------------------------------------------------------
 
+constexpr int kPkFar = 0x7fffff00;  // a byte offset behind every tile: its transfer brings zeros
+
+// A buffer of `bytes` from p on (both uniform): transfers from behind it bring zeros, so rows past a
+// sequence's end and channels past head_dim need no test of their own. Buffer instructions also count as
+// memory accesses alone; global ones into LDS count as LDS accesses too, after which every wait for an
+// operand from LDS would wait for all of them.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+
 // The transfers of one 64-row tile by the workgroup's 256 threads: piece u is row u / CPR, slot u % CPR,
-// which holds the row's chunk slot ^ swizzle(row).
+// which holds the row's chunk slot ^ swizzle(row). A thread's pieces are kStep rows apart. Row strides are
+// below 2^22 elements (the host's check), so a tile's offsets fit 31 bits.
 template <typename T, int DT>
 struct PkStream {
   using Tile = PkTile<T, DT>;
-  static constexpr int NV = kPkChunk * Tile::CPR / 256;  // pieces of a thread
+  static constexpr int kStep = 256 / Tile::CPR, NV = kPkChunk / kStep;
+  static __device__ __forceinline__ void transfer(__amdgpu_buffer_rsrc_t src, int offset, unsigned char* lds, int v) {
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (MSDA_LDS void*)(lds + (256 * v + 64 * wave) * 16), 16, offset, 0, 0, 0);
+  }
+  // row and channel of piece v of thread t
+  static __device__ __forceinline__ int row(int t, int v) { return t / Tile::CPR + kStep * v; }
+  static __device__ __forceinline__ int channel(int t, int v) { return Tile::E * ((t % Tile::CPR) ^ Tile::swizzle(row(t, v))); }
   // rows [first, first + 64) of a tensor whose row r is base + r stride; rows from `end` on are zeros
   static __device__ __forceinline__ void load(unsigned char* lds, const T* base, int64_t stride, int first, int end, int dim) {
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int st = static_cast<int>(stride) * static_cast<int>(sizeof(T));
+    const __amdgpu_buffer_rsrc_t src = pk_buffer(base + first * stride, min(end - first, kPkChunk) * st);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int u = threadIdx.x + 256 * v, row = u / Tile::CPR, ch = Tile::E * ((u % Tile::CPR) ^ Tile::swizzle(row));
-      const void* src = first + row < end && ch < dim ? static_cast<const void*>(base + (first + row) * stride + ch) : static_cast<const void*>(pk_zeros);
-      __builtin_amdgcn_global_load_lds(static_cast<const uint4*>(src), (MSDA_LDS void*)(lds + (256 * v + 64 * wave) * 16), 16, 0, 0);
+      const int t = static_cast<int>(threadIdx.x), ch = channel(t, v);
+      transfer(src, dim == Tile::DP || ch < dim ? row(t, v) * st + ch * static_cast<int>(sizeof(T)) : kPkFar, lds, v);
     }
   }
-  // the same for rows r = t group + g of queries: row r at base + t stride + g head
-  static __device__ __forceinline__ void load_rows(unsigned char* lds, const T* base, int64_t stride, int64_t head, int group, int first, int end,
-                                                   int dim) {
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int u = threadIdx.x + 256 * v, row = u / Tile::CPR, ch = Tile::E * ((u % Tile::CPR) ^ Tile::swizzle(row));
-      const int r = first + row, t = r / group, g = r - t * group;
-      const void* src = r < end && ch < dim ? static_cast<const void*>(base + t * stride + g * head + ch) : static_cast<const void*>(pk_zeros);
-      __builtin_amdgcn_global_load_lds(static_cast<const uint4*>(src), (MSDA_LDS void*)(lds + (256 * v + 64 * wave) * 16), 16, 0, 0);
-    }
+};
+
+// The rows r = t G + g of a key head's queries, in chunks of at most 64: whole tokens while 64 rows hold one
+// (then a row's place in its chunk gives its token and head whatever the chunk), 64 rows otherwise.
+struct PkRows {
+  int group, tokens, rows;   // tokens of a chunk (0: not whole ones), its rows
+  uint32_t magic;            // x / group = x magic >> 16 for x < 64, group <= 64 (x (magic group - 2^16) < 2^16)
+  __device__ __forceinline__ explicit PkRows(int g) : group(g) {
+    tokens = g <= kPkChunk ? kPkChunk / g : 0;
+    rows = tokens != 0 ? tokens * g : kPkChunk;
+    magic = tokens != 0 ? (65536 + g - 1) / g : 0;
   }
+  // token and head of row x of a chunk whose first row has head g0 (0 in chunks of whole tokens)
+  __device__ __forceinline__ int token(int x, int g0) const {
+    return tokens != 0 ? static_cast<int>((static_cast<uint32_t>(x) * magic) >> 16) : (g0 + x >= group ? 1 : 0);
+  }
+  __device__ __forceinline__ int head(int x, int g0, int token) const { return g0 + x - token * group; }
 };
 
 // ---- queries on their own side: forward and dq -------------------------------------------------
@@ -366,7 +486,9 @@ template <typename T, int DT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   __shared__ __align__(16) unsigned char K0[Tile::BYTES], V0[Tile::BYTES], K1[Tile::BYTES], V1[Tile::BYTES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 5, col = lane & 31;
+  constexpr int PF = sizeof(T) == 2 ? 3 : 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
+  const PkLane<T, DT> at(lane);
   const PkQueries w(p, lane);
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
@@ -406,11 +528,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(con
     PkStream<T, DT>::load(V, vp, p.st[kPkV][0], c * kPkChunk, w.m, p.dim);
   };
   auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c) {
-    const T* K = reinterpret_cast<const T*>(Kb);
-    const T* V = reinterpret_cast<const T*>(Vb);
+    PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
     if (k0 >= wend) return;
-    at_f16 s0 = pk_scores<T, DT>(K, 0, q, col, grp), s1 = pk_scores<T, DT>(K, 32, q, col, grp);
+    at_f16 s0 = at_zero16(), s1 = at_zero16();
+    pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
     if (k0 + kPkChunk > wfull) {
       pk_mask(s0, k0, lim, grp);
       pk_mask(s1, k0 + 32, lim, grp);
@@ -434,8 +556,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(con
       rs += s0[i] + s1[i];
     }
     l += at_sum_halves(rs);
-    pk_accumulate<T, DT>(o, V, 0, s0, lane);
-    pk_accumulate<T, DT>(o, V, 32, s1, lane);
+    pk_accumulate2<T, DT, PF>(o, V, s0, o, V + 32 * Tile::ROW, s1, at);
   };
   if (c0 < c1) stage(K0, V0, c0);
   for (int c = c0; c < c1; c += 2) {
@@ -454,8 +575,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(con
   T* scratch = reinterpret_cast<T*>(wave == 0 ? tiles[0] : wave == 1 ? tiles[1] : wave == 2 ? tiles[2] : tiles[3]);
   if (p.splits > 1) {  // sums as they are: registers hold 4 consecutive channels of the lane's row
     if (!valid) return;
-    const int64_t at = static_cast<int64_t>(w.split) * p.q_rows * p.heads + w.stat(p, ri);
-    float* po = p.part_o + at * p.dim;
+    const int64_t part = static_cast<int64_t>(w.split) * p.q_rows * p.heads + w.stat(p, ri);
+    float* po = p.part_o + part * p.dim;
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
@@ -463,13 +584,28 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(con
         const int ch = 32 * nd + 8 * c + 4 * grp;
         if (ch < p.dim) *reinterpret_cast<at_f4*>(po + ch) = at_f4{o[nd][4 * c], o[nd][4 * c + 1], o[nd][4 * c + 2], o[nd][4 * c + 3]};
       }
-    if (grp == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = float2{m, l};
+    if (grp == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = float2{m, l};
     return;
   }
-  pk_store<T, DT>(o, l == 0.0f ? 0.0f : 1.0f / l, scratch, p.dim, lane,
-                  [&](int r) { return wr0 + r < w.rows ? w.row(p, out, kPkO, wr0 + r) : static_cast<T*>(nullptr); });
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  pk_store<T, DT>(o, inv, scratch, p.dim, lane, [&](int r) { return wr0 + r < w.rows ? w.row(p, out, kPkO, wr0 + r) : static_cast<T*>(nullptr); });
+  if constexpr (sizeof(T) == 2) {
+    T* rest = static_cast<T*>(p.rest);
+    if (rest != nullptr)
+      pk_store<T, DT, true>(o, inv, scratch, p.dim, lane,
+                            [&](int r) { return wr0 + r < w.rows ? w.row(p, rest, kPkO, wr0 + r) : static_cast<T*>(nullptr); });
+  }
   if (p.stats != nullptr && valid && grp == 0)
     *reinterpret_cast<float2*>(p.stats + 4 * w.stat(p, ri)) = pk_stats(m, l);
+}
+
+template <typename T>
+__device__ __forceinline__ void pk_put4(T* to, at_f4 v) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint2*>(to) = __builtin_bit_cast(uint2, __builtin_convertvector(v, pk_bf4));
+  } else {
+    *reinterpret_cast<at_f4*>(to) = v;
+  }
 }
 
 // The split forward's parts joined: one row (token, head) to a wave's quarter, 16 lanes a row.
@@ -497,12 +633,10 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
       if (ml.y != 0.0f) a += *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch) * at_exp2(ml.x - m);
     }
     a *= inv;
-    if constexpr (sizeof(T) == 2) {
-      typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + ch) = __builtin_bit_cast(uint2, __builtin_convertvector(a, bf4));
-    } else {
-      *reinterpret_cast<at_f4*>(out + ch) = a;
-    }
+    pk_put4(out + ch, a);
+    if constexpr (sizeof(T) == 2)
+      if (p.rest != nullptr)
+        pk_put4(static_cast<T*>(p.rest) + (out - static_cast<T*>(p.out)) + ch, a - __builtin_convertvector(__builtin_convertvector(a, pk_bf4), at_f4));
   }
   if (p.stats != nullptr && lane == 0)
     *reinterpret_cast<float2*>(p.stats + 4 * row) = pk_stats(m, l);
@@ -513,7 +647,9 @@ template <typename T, int DT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   __shared__ __align__(16) unsigned char K0[Tile::BYTES], V0[Tile::BYTES], K1[Tile::BYTES], V1[Tile::BYTES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 5, col = lane & 31;
+  constexpr int PF = sizeof(T) == 2 ? 3 : 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
+  const PkLane<T, DT> at(lane);
   const PkQueries w(p, lane);
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
@@ -536,13 +672,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(c
   {
     PkRow<T, DT> o;
     o.load(w.row(p, static_cast<const T*>(p.o), kPkO, rc), valid, p.dim, grp);
-    delta = at_sum_halves(go.dot(o));
+    delta = go.dot(o);
+    if constexpr (sizeof(T) == 2) {
+      // with what out's rounding left: delta's error from the rounding would be as large as that of ds's own
+      // (packed training, error of grad_q and grad_k against f64: 2.6e-3 without, 2.4e-3 with it)
+      if (p.rest != nullptr) {
+        o.load(w.row(p, static_cast<const T*>(p.rest), kPkO, rc), valid, p.dim, grp);
+        delta += go.dot(o);
+      }
+    }
+    delta = at_sum_halves(delta);
     float* st = p.stats + 4 * w.stat(p, rc);
     m = st[0];
     ll = st[1];
-    if (valid && grp == 0) st[2] = delta;
+    // for the key side: delta; bf16: -delta and -(m + log2 l) / scale2, which its sums start from (the weight is
+    // 2^(scale2 s) then; the number is rounded at its own size, 2^-24 of it)
+    if (valid && grp == 0) *reinterpret_cast<float2*>(st + 2) = sizeof(T) == 2 ? float2{-delta, -(m + ll) / p.scale2} : float2{delta, 0.0f};
   }
   if (gq == nullptr) return;
+  constexpr bool bf = sizeof(T) == 2;
+  if (bf) m += ll;  // rounded at its own size, 2^-24 of it
   const T* kp = static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
   const T* vp = static_cast<const T*>(p.v) + w.k_first * p.st[kPkV][0] + w.kv_head * p.st[kPkV][1];
   at_f16 dq[DT / 32];
@@ -554,20 +703,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(c
     PkStream<T, DT>::load(V, vp, p.st[kPkV][0], c * kPkChunk, w.m, p.dim);
   };
   auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c) {
-    const T* K = reinterpret_cast<const T*>(Kb);
-    const T* V = reinterpret_cast<const T*>(Vb);
+    PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
     if (k0 >= wend) return;
+#pragma unroll 1
+    for (int h = 0; h < kPkChunk; h += 32) {
+      PkLane<T, DT> now = at;  // as in pk_bwd_kv_kernel
+      asm volatile("" : "+v"(now.row), "+v"(now.tr));
+      at_f16 s = at_zero16(), dp = at_zero16();
+      pk_scores2<T, DT, PF>(s, K + h * Tile::ROW, q, dp, V + h * Tile::ROW, go, now);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      at_f16 s = pk_scores<T, DT>(K, 32 * h, q, col, grp), dp = pk_scores<T, DT>(V, 32 * h, go, col, grp);
-      const bool full = k0 + 32 * h + 32 <= wfull;
+      for (int i = 0; i < 16; ++i) s[i] = at_exp2(bf ? fmaf(s[i], p.scale2, -m) : fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
+      if (k0 + h + 32 > wfull) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float w2 = at_exp2(fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
-        s[i] = full || k0 + 32 * h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? w2 : 0.0f;
+        for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
       }
-      pk_accumulate<T, DT>(dq, K, 32 * h, s, lane);
+      pk_accumulate<T, DT, PF>(dq, K + h * Tile::ROW, s, now);
     }
   };
   if (chunks > 0) stage(K0, V0, 0);
@@ -589,134 +740,235 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(c
 }
 
 // ---- keys on their own side: dk and dv ---------------------------------------------------------
+
+struct PkKeys {
+  PkPlace w;
+  int kv_head, part;
+  int b0, b1;            // keys of the tile, in the sequence's range
+  int m, n, q_first;     // keys and queries of the sequence, its first query row
+  int rows, shift;
+  int first, chunks;     // the first token that sees a key of the tile; chunks of rows (token and head) from there
+  int parts;             // workgroups that share them
+  __device__ PkKeys(const PackParams& p, const PkRows& walk, int lane) {
+    // key heads fastest (PkQueries); the first tiles, which the most queries of a causal sequence see, first
+    const int b = static_cast<int>(blockIdx.x), rest = b / p.kv_heads;
+    kv_head = b - rest * p.kv_heads;
+    part = rest % p.splits;
+    w = pk_place<kPkTile>(p.k_offsets, p.sequences, p.k_rows, 1, rest / p.splits, lane);
+    b0 = w.tile * kPkTile;
+    b1 = min(b0 + kPkTile, w.own);
+    m = n = q_first = 0;
+    if (w.seq >= 0) {
+      m = p.k_lengths != nullptr ? min(max(p.k_lengths[w.seq], 0), w.own) : w.own;
+      q_first = min(max(p.q_offsets[w.seq], 0), p.q_rows);
+      n = min(max(p.q_offsets[w.seq + 1], q_first), p.q_rows) - q_first;
+    }
+    rows = n * p.group;
+    shift = m - n;
+    first = p.causal ? min(max(b0 - shift, 0), n) : 0;
+    chunks = b0 < m ? (rows - first * p.group + walk.rows - 1) / walk.rows : 0;
+    parts = min(max(chunks / kPkLeastPart, 1), p.splits);
+  }
+  template <typename T>
+  __device__ T* row(const PackParams& p, T* base, int t, int j) const {
+    return base + (static_cast<int64_t>(w.first) + j) * p.st[t][0] + kv_head * p.st[t][1];
+  }
+  // row of the parts' sums of key j
+  __device__ int64_t part_row(const PackParams& p, int which, int j) const {
+    return (static_cast<int64_t>(which) * p.k_rows + w.first + j) * p.kv_heads + kv_head;
+  }
+};
+
 // A workgroup takes 128 keys, 32 a wave in registers, and walks over the rows (tokens and heads of the key
-// head's group) that see them, 64 at a time.
+// head's group) that see them, 64 at a time. A tile that many rows see is shared by several workgroups,
+// whose sums pk_join_kv_kernel adds in their order.
 template <typename T, int DT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 && DT <= 64 ? 2 : 1) pk_bwd_kv_kernel(const PackParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
+  using Stream = PkStream<T, DT>;
   __shared__ __align__(16) unsigned char Q0[Tile::BYTES], G0[Tile::BYTES], Q1[Tile::BYTES], G1[Tile::BYTES];
-  __shared__ __align__(16) float row_m[2][kPkChunk], row_l[2][kPkChunk], row_d[2][kPkChunk];
+  // of the tile's rows: the numbers that its scores and dP start from (bf16), or m, log2 l and delta (f32);
+  // the keys that the row sees
+  __shared__ __align__(16) float row_s[2][kPkChunk], row_d[2][kPkChunk], row_l[2][sizeof(T) == 2 ? 4 : kPkChunk];
   __shared__ __align__(16) int row_lim[2][kPkChunk];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 5, col = lane & 31;
-  const int rest = static_cast<int>(blockIdx.x) / p.kv_heads, kv_head = static_cast<int>(blockIdx.x) - rest * p.kv_heads;
-  // the first tiles, which the most queries of a causal sequence see, first
-  const PkPlace w = pk_place<kPkTile>(p.k_offsets, p.sequences, p.k_rows, 1, rest, lane);
-  const int b0 = w.tile * kPkTile;
-  if (b0 >= w.own) return;
-  const int b1 = min(b0 + kPkTile, w.own);
+  constexpr bool bf = sizeof(T) == 2;
+  constexpr int PF = bf ? 3 : 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
+  const PkLane<T, DT> at(lane);
+  const PkRows walk(p.group);
+  const PkKeys w(p, walk, lane);
+  if (w.b0 >= w.w.own || w.part >= w.parts) return;
   T* gk = static_cast<T*>(p.gk);
   T* gv = static_cast<T*>(p.gv);
-  auto key_row = [&](T* base, int t, int j) { return base + (static_cast<int64_t>(w.first) + j) * p.st[t][0] + kv_head * p.st[t][1]; };
-  int m = 0, n = 0, q_first = 0;
-  if (w.seq >= 0) {
-    m = p.k_lengths != nullptr ? min(max(p.k_lengths[w.seq], 0), w.own) : w.own;
-    q_first = min(max(p.q_offsets[w.seq], 0), p.q_rows);
-    n = min(max(p.q_offsets[w.seq + 1], q_first), p.q_rows) - q_first;
-  }
-  if (b0 >= m || n == 0) {
-    if (gk != nullptr) pk_zero_rows<T, 256>(b0, b1, p.dim, [&](int j) { return key_row(gk, kPkGK, j); });
-    if (gv != nullptr) pk_zero_rows<T, 256>(b0, b1, p.dim, [&](int j) { return key_row(gv, kPkGV, j); });
+  if (w.chunks <= 0) {
+    if (gk != nullptr) pk_zero_rows<T, 256>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gk, kPkGK, j); });
+    if (gv != nullptr) pk_zero_rows<T, 256>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gv, kPkGV, j); });
     return;
   }
-  const int rows = n * p.group, shift = m - n;
-  const int wb0 = b0 + 32 * wave, kj = wb0 + col;
-  const bool valid = kj < m;
+  const int m = w.m, shift = w.shift, rows = w.rows;
+  const int wb0 = w.b0 + 32 * wave;
   PkRow<T, DT> k, v;
-  k.load(key_row(const_cast<T*>(static_cast<const T*>(p.k)), kPkK, min(kj, m - 1)), valid, p.dim, grp);
-  v.load(key_row(const_cast<T*>(static_cast<const T*>(p.v)), kPkV, min(kj, m - 1)), valid, p.dim, grp);
-  const T* qp = static_cast<const T*>(p.q) + q_first * p.st[kPkQ][0] + static_cast<int64_t>(kv_head) * p.group * p.st[kPkQ][1];
-  const T* gp = static_cast<const T*>(p.go) + q_first * p.st[kPkGO][0] + static_cast<int64_t>(kv_head) * p.group * p.st[kPkGO][1];
-  const float* sp = p.stats + 4 * (static_cast<int64_t>(q_first) * p.heads + kv_head * p.group);
-  const int first = p.causal ? min(max(b0 - shift, 0), n) * p.group : 0;  // the first row that sees a key of the tile
-  const int chunks = first < rows ? (rows - first + kPkChunk - 1) / kPkChunk : 0;
+  {
+    const int kj = wb0 + col;
+    k.load(w.row(p, static_cast<const T*>(p.k), kPkK, min(kj, m - 1)), kj < m, p.dim, grp);
+    v.load(w.row(p, static_cast<const T*>(p.v), kPkV, min(kj, m - 1)), kj < m, p.dim, grp);
+  }
+  const T* qp = static_cast<const T*>(p.q) + w.q_first * p.st[kPkQ][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkQ][1];
+  const T* gp = static_cast<const T*>(p.go) + w.q_first * p.st[kPkGO][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkGO][1];
+  const float* sp = p.stats + 4 * (static_cast<int64_t>(w.q_first) * p.heads + w.kv_head * p.group);
+  const int per = (w.chunks + w.parts - 1) / w.parts, c0 = w.part * per, c1 = min(w.chunks, c0 + per);
   at_f16 dk[DT / 32], dv[DT / 32];
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) dk[nd] = dv[nd] = at_zero16();
 
-  float4 st;  // statistics of row threadIdx.x of the next tile
-  int st_lim;
-  auto stage = [&](unsigned char* Q, unsigned char* G, int c) {
-    const int r0 = first + c * kPkChunk;
-    PkStream<T, DT>::load_rows(Q, qp, p.st[kPkQ][0], p.st[kPkQ][1], p.group, r0, rows, p.dim);
-    PkStream<T, DT>::load_rows(G, gp, p.st[kPkGO][0], p.st[kPkGO][1], p.group, r0, rows, p.dim);
+  // Chunk c: its first row, and that row's token and head
+  auto place = [&](int c, int& r0, int& t0, int& g0) {
+    r0 = w.first * p.group + c * walk.rows;
+    t0 = walk.tokens != 0 ? w.first + c * walk.tokens : r0 / p.group;
+    g0 = walk.tokens != 0 ? 0 : r0 - t0 * p.group;
   };
-  auto load_stats = [&](int c) {
-    const int r = first + c * kPkChunk + static_cast<int>(threadIdx.x);
-    st = float4{0.0f, INFINITY, 0.0f, 0.0f};
-    st_lim = 0;
-    if (threadIdx.x < kPkChunk && r < rows) {
-      const int t = r / p.group, g = r - t * p.group;
-      st = *reinterpret_cast<const float4*>(sp + 4 * (static_cast<int64_t>(t) * p.heads + g));
-      st_lim = p.causal ? min(max(t + shift + 1, 0), m) : m;
-    }
-  };
-  auto store_stats = [&](int buf) {
-    if (threadIdx.x < kPkChunk) {
-      row_m[buf][threadIdx.x] = st.x;
-      row_l[buf][threadIdx.x] = st.y;
-      row_d[buf][threadIdx.x] = st.z;
-      row_lim[buf][threadIdx.x] = st_lim;
-    }
-  };
-  auto chunk = [&](const unsigned char* Qb, const unsigned char* Gb, int buf, int c) {
-    const T* Q = reinterpret_cast<const T*>(Qb);
-    const T* G = reinterpret_cast<const T*>(Gb);
-    const int r0 = first + c * kPkChunk;
-    if (wb0 >= m || (p.causal && (min(r0 + kPkChunk, rows) - 1) / p.group + shift < wb0)) return;
-    // every row sees every key of the wave
-    const bool full = r0 + kPkChunk <= rows && (p.causal ? r0 / p.group + shift >= wb0 + 31 && wb0 + 32 <= m : wb0 + 32 <= m);
+  // Tile c into Q, G and the row arrays `buf`: the rows' numbers by one wave each, a row a lane.
+  auto stage = [&](unsigned char* Q, unsigned char* G, int buf, int c) {
+    int r0, t0, g0;
+    place(c, r0, t0, g0);
+    const int count = min(walk.rows, rows - r0);
+    constexpr int E = sizeof(T);
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // the pieces' offsets are formed anew (as in block)
+    const __amdgpu_buffer_rsrc_t qs = pk_buffer(qp + t0 * p.st[kPkQ][0], kPkFar), gs = pk_buffer(gp + t0 * p.st[kPkGO][0], kPkFar);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      at_f16 s = pk_scores<T, DT>(Q, 32 * h, k, col, grp), dp = pk_scores<T, DT>(G, 32 * h, v, col, grp);
+    for (int v = 0; v < Stream::NV; ++v) {
+      const int x = Stream::row(thread, v), t = walk.token(x, g0), g = walk.head(x, g0, t), ch = Stream::channel(thread, v);
+      const bool ok = x < count && (p.dim == Tile::DP || ch < p.dim);
+      Stream::transfer(qs, ok ? (t * static_cast<int>(p.st[kPkQ][0]) + g * static_cast<int>(p.st[kPkQ][1]) + ch) * E : kPkFar, Q, v);
+      Stream::transfer(gs, ok ? (t * static_cast<int>(p.st[kPkGO][0]) + g * static_cast<int>(p.st[kPkGO][1]) + ch) * E : kPkFar, G, v);
+    }
+    const int x = thread & 63, t = walk.token(x, g0), g = walk.head(x, g0, t), o = x < count ? (t * p.heads + g) * 16 : kPkFar;
+    const __amdgpu_buffer_rsrc_t ss = pk_buffer(sp + 4 * static_cast<int64_t>(t0) * p.heads, kPkFar);
+    if (wave == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_s[buf]), 4, o + (bf ? 12 : 0), 0, 0, 0);
+    if (wave == 1) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_d[buf]), 4, o + 8, 0, 0, 0);
+    if (wave == 2 && !bf) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_l[buf]), 4, o + 4, 0, 0, 0);
+    if (wave == 3) row_lim[buf][x] = x >= count ? 0 : p.causal ? min(max(t0 + t + shift + 1, 0), m) : m;
+  };
+  // One 32-row block; `all`: every row sees every key of the wave.
+  auto block = [&](bool all, PkLds Q, PkLds G, const float* rs, const float* rd, const float* rl, const int* lims) {
+    // formed anew in each step: kept over the loop, the offsets' dozen registers spill at 128 channels
+    PkLane<T, DT> now = at;
+    asm volatile("" : "+v"(now.row), "+v"(now.tr));
+    at_f16 s, dp;
+#pragma unroll
+    for (int c4 = 0; c4 < 4; ++c4) {  // bf16: the matrix units start from the rows' numbers
+      const at_f4 a = bf ? *reinterpret_cast<const at_f4*>(rs + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
+      const at_f4 b = bf ? *reinterpret_cast<const at_f4*>(rd + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[4 * c4 + j] = a[j];
+        dp[4 * c4 + j] = b[j];
+      }
+    }
+    pk_scores2<T, DT, PF>(s, Q, k, dp, G, v, now);
+    if constexpr (bf) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = at_exp2(s[i] * p.scale2);
+        dp[i] *= s[i];
+      }
+    } else {
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
-        const int at = 32 * h + 8 * c4 + 4 * grp;
-        const at_f4 mm = *reinterpret_cast<const at_f4*>(&row_m[buf][at]), ll = *reinterpret_cast<const at_f4*>(&row_l[buf][at]);
-        const at_f4 dd = *reinterpret_cast<const at_f4*>(&row_d[buf][at]);
-        const int4 lm = *reinterpret_cast<const int4*>(&row_lim[buf][at]);
+        const int a = 8 * c4 + 4 * grp;
+        const at_f4 mm = *reinterpret_cast<const at_f4*>(rs + a), ll = *reinterpret_cast<const at_f4*>(rl + a);
+        const at_f4 dd = *reinterpret_cast<const at_f4*>(rd + a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * c4 + j;
+          s[i] = at_exp2(fmaf(s[i], p.scale2, -mm[j]) - ll[j]);
+          dp[i] = s[i] * (dp[i] - dd[j]);
+        }
+      }
+    }
+    if (!all) {
+      const int kj = wb0 + col;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
         const int lim[4] = {lm.x, lm.y, lm.z, lm.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * c4 + j;
-          const bool sees = full || kj < lim[j];
-          s[i] = sees ? at_exp2(fmaf(s[i], p.scale2, -mm[j]) - ll[j]) : 0.0f;
-          dp[i] = sees ? s[i] * (dp[i] - dd[j]) : 0.0f;
+          s[i] = kj < lim[j] ? s[i] : 0.0f;
+          dp[i] = kj < lim[j] ? dp[i] : 0.0f;
         }
       }
-      pk_accumulate<T, DT>(dv, G, 32 * h, s, lane);
-      pk_accumulate<T, DT>(dk, Q, 32 * h, dp, lane);
     }
+    pk_accumulate2<T, DT, PF>(dv, G, s, dk, Q, dp, now);
   };
-  if (chunks > 0) {
-    load_stats(0);
-    stage(Q0, G0, 0);
-  }
-  for (int c = 0; c < chunks; c += 2) {
-    store_stats(0);
+  auto chunk = [&](const unsigned char* Qb, const unsigned char* Gb, int buf, int c) {
+    PkLds Q = (PkLds)(Qb), G = (PkLds)(Gb);
+    int r0, t0, g0;
+    place(c, r0, t0, g0);
+    const int r1 = min(r0 + walk.rows, rows), t1 = walk.tokens != 0 ? min(t0 + walk.tokens, w.n) : (r1 - 1) / p.group + 1;
+    if (wb0 >= m || (p.causal && t1 + shift <= wb0)) return;
+    // every row sees every key of the wave
+    const bool full = r0 + kPkChunk == r1 && wb0 + 32 <= m && (!p.causal || t0 + shift >= wb0 + 31);
+#pragma unroll 1
+    for (int h = 0; h < r1 - r0; h += 32)
+      block(full, Q + h * Tile::ROW, G + h * Tile::ROW, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h);
+  };
+  if (c0 < c1) stage(Q0, G0, 0, c0);
+  for (int c = c0; c < c1; c += 2) {
     wait_vmem();
     __syncthreads();
-    if (c + 1 < chunks) {
-      load_stats(c + 1);
-      stage(Q1, G1, c + 1);
-    }
+    if (c + 1 < c1) stage(Q1, G1, 1, c + 1);
     chunk(Q0, G0, 0, c);
-    if (c + 1 >= chunks) break;
-    store_stats(1);
+    if (c + 1 >= c1) break;
     wait_vmem();
     __syncthreads();
-    if (c + 2 < chunks) {
-      load_stats(c + 2);
-      stage(Q0, G0, c + 2);
-    }
+    if (c + 2 < c1) stage(Q0, G0, 0, c + 2);
     chunk(Q1, G1, 1, c + 1);
+  }
+  if (w.parts > 1) {
+    const int kj = wb0 + col;
+    if (kj >= w.b1) return;
+    float* pk = p.part_kv + w.part_row(p, 2 * w.part, kj) * p.dim;
+    float* pv = p.part_kv + w.part_row(p, 2 * w.part + 1, kj) * p.dim;
+#pragma unroll
+    for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int ch = 32 * nd + 8 * c + 4 * grp;
+        if (ch >= p.dim) continue;
+        *reinterpret_cast<at_f4*>(pk + ch) = at_f4{dk[nd][4 * c], dk[nd][4 * c + 1], dk[nd][4 * c + 2], dk[nd][4 * c + 3]};
+        *reinterpret_cast<at_f4*>(pv + ch) = at_f4{dv[nd][4 * c], dv[nd][4 * c + 1], dv[nd][4 * c + 2], dv[nd][4 * c + 3]};
+      }
+    return;
   }
   __syncthreads();
   T* scratch = reinterpret_cast<T*>(wave == 0 ? Q0 : wave == 1 ? G0 : wave == 2 ? Q1 : G1);
   // keys from m on (rows of the range behind the sequence's keys) hold zeros: their scores never counted
   if (gk != nullptr)
-    pk_store<T, DT>(dk, p.scale, scratch, p.dim, lane, [&](int r) { return wb0 + r < b1 ? key_row(gk, kPkGK, wb0 + r) : static_cast<T*>(nullptr); });
+    pk_store<T, DT>(dk, p.scale, scratch, p.dim, lane, [&](int r) { return wb0 + r < w.b1 ? w.row(p, gk, kPkGK, wb0 + r) : static_cast<T*>(nullptr); });
   if (gv != nullptr)
-    pk_store<T, DT>(dv, 1.0f, scratch, p.dim, lane, [&](int r) { return wb0 + r < b1 ? key_row(gv, kPkGV, wb0 + r) : static_cast<T*>(nullptr); });
+    pk_store<T, DT>(dv, 1.0f, scratch, p.dim, lane, [&](int r) { return wb0 + r < w.b1 ? w.row(p, gv, kPkGV, wb0 + r) : static_cast<T*>(nullptr); });
+}
+
+// The sums of a tile's parts, in their order (the grid of pk_bwd_kv_kernel with one part).
+template <typename T>
+__global__ void __launch_bounds__(256) pk_join_kv_kernel(const PackParams p) {
+  PackParams one = p;
+  one.splits = 1;
+  const PkKeys w(one, PkRows(p.group), threadIdx.x & 63);
+  const int parts = min(max(w.chunks / kPkLeastPart, 1), p.splits);
+  if (w.b0 >= w.w.own || parts == 1) return;
+  const int pieces = p.dim / 4;
+  for (int i = threadIdx.x; i < 2 * (w.b1 - w.b0) * pieces; i += 256) {
+    const int which = i & 1, key = w.b0 + (i >> 1) / pieces, ch = 4 * ((i >> 1) % pieces);
+    T* base = static_cast<T*>(which == 0 ? p.gk : p.gv);
+    if (base == nullptr) continue;
+    at_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < parts; ++s) a += *reinterpret_cast<const at_f4*>(p.part_kv + w.part_row(p, 2 * s + which, key) * p.dim + ch);
+    pk_put4(w.row(p, base, which == 0 ? kPkGK : kPkGV, key) + ch, which == 0 ? a * p.scale : a);
+  }
 }
 
 }  // namespace msda

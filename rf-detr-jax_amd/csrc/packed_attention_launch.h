@@ -23,14 +23,19 @@ int pk_fwd(const msda::PackParams& p, hipStream_t st) {
   return pk_launch(msda::pk_join_kernel<T>, (static_cast<int64_t>(p.q_rows) * p.heads + 15) / 16, p, st, "packed attention forward (join)");
 }
 
-// q_slots, k_slots: tiles of the queries' and of the keys' side
+// q_slots, k_slots: tiles of the queries' and of the keys' side; p.splits: parts of a key tile
 template <typename T, int DT>
 int pk_bwd(msda::PackParams p, int q_slots, int k_slots, hipStream_t st) {
-  p.slots = q_slots;
-  const int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT>, static_cast<int64_t>(q_slots) * p.kv_heads, p, st, "packed attention backward (queries)");
+  msda::PackParams q = p;
+  q.slots = q_slots;
+  q.splits = 1;
+  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT>, static_cast<int64_t>(q_slots) * p.kv_heads, q, st, "packed attention backward (queries)");
   if (rc != MSDA_OK || (p.gk == nullptr && p.gv == nullptr)) return rc;
   p.slots = k_slots;
-  return pk_launch(msda::pk_bwd_kv_kernel<T, DT>, static_cast<int64_t>(k_slots) * p.kv_heads, p, st, "packed attention backward (keys, values)");
+  rc = pk_launch(msda::pk_bwd_kv_kernel<T, DT>, static_cast<int64_t>(k_slots) * p.splits * p.kv_heads, p, st,
+                 "packed attention backward (keys, values)");
+  if (rc != MSDA_OK || p.splits == 1) return rc;
+  return pk_launch(msda::pk_join_kv_kernel<T>, static_cast<int64_t>(k_slots) * p.kv_heads, p, st, "packed attention backward (join)");
 }
 
 template <typename T>

@@ -33,9 +33,9 @@ def _stream(device):
 
 
 def _rows16(t):
-    """``t`` as the kernels read it: channels contiguous, rows on 16-byte boundaries (a copy where they are not)."""
-    step = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.stride(0) % step or t.stride(1) % step or t.data_ptr() % 16:
+    """``t`` as the kernels read it: channels contiguous, rows on 16-byte boundaries and apart (a copy where they are not)."""
+    step, (row, head, channel) = 16 // t.element_size(), t.stride()
+    if channel != 1 or row % step or head % step or t.data_ptr() % 16 or not t.shape[2] <= row < 1 << 22 or head * t.shape[1] >= 1 << 22:
         t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
     return t
 
@@ -99,53 +99,66 @@ def _strides(tensors):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _forward(q, k, v, seq, causal, scale, want_stats):
+def _forward(q, k, v, seq, causal, scale, backward):
+    """``(out, rest, stats)``; with ``backward`` what it needs: what out's rounding left (bfloat16) and statistics."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    stats = torch.empty((q.shape[0] * q.shape[1] * 4,), dtype=torch.float32, device=q.device) if want_stats else None
+    rest = torch.empty_like(out) if backward and q.dtype == torch.bfloat16 else None
+    stats = torch.empty((q.shape[0], q.shape[1], 4), dtype=torch.float32, device=q.device) if backward else None
     lib, code = _native.lib(), _DTYPES[q.dtype]
     dims = (seq.count, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
-    nbytes = lib.msda_packed_attention_workspace_size(code, *dims)
-    _native.check(min(nbytes, 0))
-    ws = _native.workspace(nbytes, q.device) if nbytes else None
     with torch.cuda.device(q.device):
-        rc = lib.msda_packed_attention_fwd(_ptr(q), _ptr(k), _ptr(v), code, _ptr(out), _ptr(stats), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths),
-                                           *dims, _strides((q, k, v, out)), int(causal), scale, _ptr(ws), nbytes, _stream(q.device))
+        nbytes = lib.msda_packed_attention_fwd_workspace_size(code, *dims)
+        _native.check(min(nbytes, 0))
+        ws = _native.workspace(nbytes, q.device) if nbytes else None
+        rc = lib.msda_packed_attention_fwd(_ptr(q), _ptr(k), _ptr(v), code, _ptr(out), _ptr(rest), _ptr(stats), _ptr(seq.q), _ptr(seq.k),
+                                           _ptr(seq.lengths), *dims, _strides((q, k, v, out)), int(causal), scale, _ptr(ws), nbytes,
+                                           _stream(q.device))
     _native.check(rc)
-    return out, stats
+    return out, rest, stats
 
 
-def _backward(q, k, v, out, stats, grad_out, seq, causal, scale, needs):
+def _backward(q, k, v, out, rest, stats, grad_out, seq, causal, scale, needs):
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None for t, need in zip((q, k, v), needs)]
-    lib = _native.lib()
+    lib, code = _native.lib(), _DTYPES[q.dtype]
+    dims = (seq.count, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
     with torch.cuda.device(q.device):
-        rc = lib.msda_packed_attention_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(stats), _ptr(grad_out), _DTYPES[q.dtype],
-                                           *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), seq.count, q.shape[0],
-                                           k.shape[0], q.shape[1], k.shape[1], q.shape[2], _strides((q, k, v, out, grad_out, *grads)),
-                                           int(causal), scale, _stream(q.device))
+        nbytes = lib.msda_packed_attention_bwd_workspace_size(code, *dims) if needs[1] or needs[2] else 0
+        _native.check(min(nbytes, 0))
+        ws = _native.workspace(nbytes, q.device) if nbytes else None
+        rc = lib.msda_packed_attention_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(stats), _ptr(grad_out), code,
+                                           *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), *dims,
+                                           _strides((q, k, v, out, grad_out, *grads)), int(causal), scale, _ptr(ws), nbytes, _stream(q.device))
     _native.check(rc)
     return grads
 
 
 def packed_attention_forward(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None):
-    """``(out, stats)`` of :func:`packed_attention`'s arguments, without autograd; ``stats`` is for
-    :func:`packed_attention_backward`."""
+    """``(out, saved)`` of :func:`packed_attention`'s arguments, without autograd; ``saved`` is for
+    :func:`packed_attention_backward`: the statistics ``[T, H, 4]``, and for bfloat16 what the rounding of ``out``
+    left, ``[T, H, D]`` (else None)."""
     _check(q, k, v)
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
-    return _forward(*(_rows16(t) for t in (q, k, v)), seq, causal, _scale(scale, q.shape[2]), True)
+    out, rest, stats = _forward(*(_rows16(t) for t in (q, k, v)), seq, causal, _scale(scale, q.shape[2]), True)
+    return out, (stats, rest)
 
 
-def packed_attention_backward(q, k, v, out, stats, grad_out, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None,
+def packed_attention_backward(q, k, v, out, saved, grad_out, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None,
                               needs=(True, True, True)):
     """``(grad_q, grad_k, grad_v)``, contiguous, for the cotangent ``grad_out`` of ``out``; ``out`` and
-    ``stats`` as :func:`packed_attention_forward` gave them. None where ``needs`` says so."""
+    ``saved`` as :func:`packed_attention_forward` gave them. None where ``needs`` says so."""
     _check(q, k, v)
-    if out.shape != q.shape or grad_out.shape != q.shape or stats.numel() != q.shape[0] * q.shape[1] * 4:
-        raise ValueError("out, stats and grad_out do not belong to these queries")
-    if any(t.device != q.device for t in (out, stats, grad_out)) or stats.dtype != torch.float32:
-        raise ValueError("out, stats and grad_out must be on the queries' device, stats in float32")
+    stats, rest = saved
+    if any(t.shape != q.shape for t in (out, grad_out, *(() if rest is None else (rest,)))) or tuple(stats.shape) != (*q.shape[:2], 4):
+        raise ValueError("out, its statistics or grad_out do not belong to these queries")
+    if any(t.device != q.device for t in (out, grad_out, stats, *(() if rest is None else (rest,)))):
+        raise ValueError("out, its statistics and grad_out must be on the queries' device")
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
-    tensors = [_rows16(t.to(q.dtype)) for t in (q, k, v, out)]
-    return tuple(_backward(*tensors, stats.contiguous(), _rows16(grad_out.to(q.dtype)), seq, causal, _scale(scale, q.shape[2]), needs))
+    # hooks on saved tensors may hand back other types and layouts: as the kernels read them
+    q, k, v, out, grad_out = (_rows16(t.to(q.dtype)) for t in (q, k, v, out, grad_out))
+    if rest is not None:
+        out, rest = out.contiguous(), rest.to(q.dtype).contiguous()  # of the same strides
+    stats = stats.to(torch.float32).contiguous()
+    return tuple(_backward(q, k, v, out, rest, stats, grad_out, seq, causal, _scale(scale, q.shape[2]), needs))
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -156,19 +169,18 @@ class _PackedAttention(torch.autograd.Function):
         scale = _scale(scale, q.shape[2])
         needs = any(ctx.needs_input_grad[:3])
         q, k, v = (_rows16(t) for t in (q, k, v))
-        out, stats = _forward(q, k, v, seq, causal, scale, needs)
+        out, rest, stats = _forward(q, k, v, seq, causal, scale, needs)
         if needs:
-            ctx.save_for_backward(q, k, v, out, stats, offsets, key_offsets, key_lengths)
+            ctx.save_for_backward(q, k, v, out, rest, stats, offsets, key_offsets, key_lengths)
             ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, stats, offsets, key_offsets, key_lengths = ctx.saved_tensors
-        # hooks on saved tensors may hand back other types and layouts: as the kernels read them
-        q, k, v, out = (t.to(grad_out.dtype) for t in (q, k, v, out))
-        grads = packed_attention_backward(q, k, v, out, stats.to(torch.float32), grad_out, offsets, key_offsets, key_lengths, ctx.causal, ctx.scale,
+        q, k, v, out, rest, stats, offsets, key_offsets, key_lengths = ctx.saved_tensors
+        q, k, v = (t.to(grad_out.dtype) for t in (q, k, v))
+        grads = packed_attention_backward(q, k, v, out, (stats, rest), grad_out, offsets, key_offsets, key_lengths, ctx.causal, ctx.scale,
                                           ctx.needs_input_grad[:3])
         return (*grads, None, None, None, None, None)
 

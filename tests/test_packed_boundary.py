@@ -19,18 +19,18 @@ def _i64(*v):
 
 
 def _attention(direction, **kw):
-    a = dict(q=PTR, k=PTR, v=PTR, dtype=1, out=PTR, stats=PTR, qo=PTR, ko=PTR, kl=None, n=1, t=4, s=4, h=4, hk=2, d=64, causal=1, scale=0.125,
+    a = dict(q=PTR, k=PTR, v=PTR, dtype=1, out=PTR, rest=None, stats=PTR, qo=PTR, ko=PTR, kl=None, n=1, t=4, s=4, h=4, hk=2, d=64, causal=1, scale=0.125,
              strides=None, ws=None, ws_bytes=0, go=PTR, gq=PTR, gk=PTR, gv=PTR)
     a.update(kw)
     lib = _native.lib()
     dims = (a["n"], a["t"], a["s"], a["h"], a["hk"], a["d"])
     strides = _i64(*([256, 64] * (4 if direction == "fwd" else 8))) if a["strides"] is None else a["strides"]
     if direction == "fwd":
-        rc = lib.msda_packed_attention_fwd(a["q"], a["k"], a["v"], a["dtype"], a["out"], a["stats"], a["qo"], a["ko"], a["kl"], *dims, strides,
+        rc = lib.msda_packed_attention_fwd(a["q"], a["k"], a["v"], a["dtype"], a["out"], a["rest"], a["stats"], a["qo"], a["ko"], a["kl"], *dims, strides,
                                            a["causal"], a["scale"], a["ws"], a["ws_bytes"], None)
     else:
-        rc = lib.msda_packed_attention_bwd(a["q"], a["k"], a["v"], a["out"], a["stats"], a["go"], a["dtype"], a["gq"], a["gk"], a["gv"], a["qo"],
-                                           a["ko"], a["kl"], *dims, strides, a["causal"], a["scale"], None)
+        rc = lib.msda_packed_attention_bwd(a["q"], a["k"], a["v"], a["out"], a["rest"], a["stats"], a["go"], a["dtype"], a["gq"], a["gk"], a["gv"], a["qo"],
+                                           a["ko"], a["kl"], *dims, strides, a["causal"], a["scale"], a["ws"], a["ws_bytes"], None)
     return rc, lib.msda_last_error().decode()
 
 
@@ -46,7 +46,9 @@ INVALID, UNSUPPORTED = _native.ERR_INVALID_ARGUMENT, _native.ERR_UNSUPPORTED
     ({"scale": float("inf")}, INVALID, "scale"), ({"q": None}, INVALID, "NULL"), ({"k": None}, INVALID, "NULL"), ({"out": None}, INVALID, "NULL"),
     ({"qo": None}, INVALID, "offsets"), ({"ko": None}, INVALID, "offsets"), ({"v": ODD}, INVALID, "16 bytes"), ({"stats": ODD}, INVALID, "16 bytes"),
     ({"kl": ctypes.c_void_p((1 << 20) + 2)}, INVALID, "4 bytes"), ({"strides": _i64(*([260, 64] * 8))}, INVALID, "stride"),
-    ({"strides": _i64(*([-256, 64] * 8))}, INVALID, "stride"),
+    ({"strides": _i64(*([-256, 64] * 8))}, INVALID, "stride"), ({"strides": _i64(*([56, 64] * 8))}, UNSUPPORTED, "apart"),
+    ({"strides": _i64(*([1 << 22, 64] * 8))}, UNSUPPORTED, "apart"), ({"strides": _i64(*([256, 1 << 21] * 8))}, UNSUPPORTED, "apart"),
+    ({"rest": ODD}, INVALID, "16 bytes"),
 ])
 def test_attention_refusals(direction, change, code, text):
     rc, msg = _attention(direction, **change)
@@ -58,13 +60,21 @@ def test_attention_backward_pointers_and_workspace():
     assert _attention("bwd", gk=ODD)[0] == INVALID
     assert _attention("bwd", gq=None, gk=None, gv=None)[0] == 0  # nothing wanted, nothing launched
     assert _attention("fwd", t=0)[0] == 0 and _attention("bwd", t=0, s=0)[0] == 0
-    size = _native.lib().msda_packed_attention_workspace_size
+    size = _native.lib().msda_packed_attention_fwd_workspace_size
     assert size(1, 1, 4096, 4096, 32, 8, 128) == 0
     need = size(1, 1, 1, 100000, 8, 8, 128)  # one token: its keys are split
     assert need > 0 and need % (8 * 130 * 4) == 0
     assert size(1, 1, 1, 100000, 8, 3, 128) == INVALID and size(7, 1, 1, 1, 8, 8, 128) == UNSUPPORTED
     for ws, n in ((None, 0), (PTR, need - 1), (ODD, need)):
         rc, msg = _attention("fwd", t=1, s=100000, h=8, hk=8, d=128, strides=_i64(*([1024, 128] * 4)), ws=ws, ws_bytes=n)
+        assert rc == INVALID and "workspace" in msg
+    size = _native.lib().msda_packed_attention_bwd_workspace_size
+    assert size(1, 16, 65536, 65536, 32, 8, 128) == 0
+    need = size(1, 1, 4096, 4096, 16, 2, 64)  # 64 tiles of keys: several workgroups share one
+    assert need > 0 and need % (2 * 4096 * 2 * 64 * 4) == 0
+    big = dict(t=4096, s=4096, h=16, hk=2, strides=_i64(*([1024, 64] * 8)))
+    for ws, n in ((None, 0), (PTR, need - 1), (ODD, need)):
+        rc, msg = _attention("bwd", ws=ws, ws_bytes=n, **big)
         assert rc == INVALID and "workspace" in msg
 
 
