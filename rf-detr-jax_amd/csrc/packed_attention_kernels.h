@@ -480,8 +480,8 @@ __device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lim, int grp) {
 }
 
 // Forward. A workgroup takes 128 rows and walks over the keys that they see, 64 at a time, with a running
-// reference score m (moved when a chunk's maximum exceeds it by 2^8, or lies 2^64 below it while nothing
-// is summed) and sum l.
+// reference score m and sum l. m starts at the first chunk's maximum (whose weight, the largest of a short
+// row, is then 1 and rounds to itself) and moves when a chunk's exceeds it by 2^8.
 template <typename T, int DT>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(con
 #pragma unroll
     for (int i = 0; i < 16; ++i) bm = fmaxf(bm, fmaxf(s0[i], s1[i]));
     bm = at_max_halves(bm) * p.scale2;
-    if (bm != -INFINITY && (bm > m + kAtLazy || (l == 0.0f && bm < m - kAtLow))) {
+    if (bm != -INFINITY && (bm > m + kAtLazy || l == 0.0f)) {
       const float alpha = l == 0.0f ? 0.0f : at_exp2(m - bm);
       m = bm;
       l *= alpha;

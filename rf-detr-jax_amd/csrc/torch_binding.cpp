@@ -16,11 +16,13 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
+#include <cmath>
 #include <optional>
 #include <vector>
 
@@ -49,6 +51,11 @@ struct Library {
   decltype(&msda_value_proj_bwd_workspace_size) value_proj_bwd_workspace_size;
   decltype(&msda_attention_fwd) attention_fwd;
   decltype(&msda_attention_bwd) attention_bwd;
+  decltype(&msda_packed_attention_fwd) packed_fwd;
+  decltype(&msda_packed_attention_bwd) packed_bwd;
+  decltype(&msda_packed_attention_fwd_workspace_size) packed_fwd_workspace_size;
+  decltype(&msda_packed_attention_bwd_workspace_size) packed_bwd_workspace_size;
+  decltype(&msda_rotary) rotary;
 };
 
 Library lib;
@@ -72,6 +79,11 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_value_proj_bwd_workspace_size", lib.value_proj_bwd_workspace_size);
   get("msda_attention_fwd", lib.attention_fwd);
   get("msda_attention_bwd", lib.attention_bwd);
+  get("msda_packed_attention_fwd", lib.packed_fwd);
+  get("msda_packed_attention_bwd", lib.packed_bwd);
+  get("msda_packed_attention_fwd_workspace_size", lib.packed_fwd_workspace_size);
+  get("msda_packed_attention_bwd_workspace_size", lib.packed_bwd_workspace_size);
+  get("msda_rotary", lib.rotary);
   check_status = py::object(check).release().ptr();
   parameter_type = reinterpret_cast<PyTypeObject*>(py::object(parameter).release().ptr());
 }
@@ -521,6 +533,249 @@ py::object attention(const py::handle& q, const py::handle& k, const py::handle&
   return py::cast(Attention::apply(*a, *b, *c, lay));
 }
 
+// ---- attention over packed sequences, rotary positions ----------------------------------------
+
+// Gradients that are not differentiable again: differentiating them raises.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (const Tensor& g : grads)
+    if (g.defined()) defined.push_back(g);
+  if (defined.empty()) return grads;
+  const auto node = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate the gradients of ") + what,
+                                                                    static_cast<int64_t>(defined.size()));
+  defined = (*node)(std::move(defined));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = defined[i++];
+  return grads;
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->requires_grad()) return true;
+  return false;
+}
+
+// [rows, heads, D] as the packed kernels read it: channels contiguous, rows on 16-byte boundaries and apart
+bool packed_rows(const Tensor& t) {
+  const int64_t step = 16 / t.element_size();
+  return t.dim() == 3 && t.stride(2) == 1 && t.stride(0) % step == 0 && t.stride(1) % step == 0 && t.stride(0) >= t.size(2) &&
+         t.stride(0) < (int64_t{1} << 22) && t.stride(1) * t.size(1) < (int64_t{1} << 22) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+struct Packed {  // one call's sizes
+  int sequences, q_rows, k_rows, heads, kv_heads, dim;
+  bool causal;
+  float scale;
+  Packed(const Tensor& q, const Tensor& k, const Tensor& offsets, bool c, double s)
+      : sequences(static_cast<int>(offsets.numel() - 1)), q_rows(static_cast<int>(q.size(0))), k_rows(static_cast<int>(k.size(0))),
+        heads(static_cast<int>(q.size(1))), kv_heads(static_cast<int>(k.size(1))), dim(static_cast<int>(q.size(2))), causal(c),
+        scale(static_cast<float>(s)) {}
+};
+
+const int32_t* iptr(const Tensor& t) { return static_cast<const int32_t*>(ptr(t)); }
+
+// (out, what its rounding left, statistics); the last two as the backward needs them
+std::array<Tensor, 3> packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& key_offsets,
+                                     const Tensor& key_lengths, const Packed& p, bool backward) {
+  Tensor out = at::empty(q.sizes(), q.options()), rest, stats, ws;
+  if (backward) {
+    if (q.scalar_type() == at::kBFloat16) rest = at::empty(q.sizes(), q.options());
+    stats = at::empty({q.size(0), q.size(1), 4}, q.options().dtype(at::kFloat));
+  }
+  const int64_t bytes = lib.packed_fwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim);
+  check(bytes);
+  if (bytes != 0) ws = workspace(bytes, q);
+  const int64_t st[8] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1)};
+  launch(q, [&](void* stream) {
+    return lib.packed_fwd(ptr(q), ptr(k), ptr(v), code(q), ptr(out), ptr(rest), fptr(stats), iptr(offsets), iptr(key_offsets), iptr(key_lengths),
+                          p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale, ptr(ws), bytes, stream);
+  });
+  return {out, rest, stats};
+}
+
+struct PackedAttention : torch::autograd::Function<PackedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& key_offsets,
+                        const std::optional<Tensor>& key_lengths, const Packed& p) {
+    const auto [out, rest, stats] = packed_forward(q, k, v, offsets, key_offsets, key_lengths.value_or(Tensor()), p, true);
+    ctx->save_for_backward({q, k, v, out, rest, stats, offsets, key_offsets, key_lengths.value_or(Tensor())});
+    ctx->saved_data["causal"] = p.causal;
+    ctx->saved_data["scale"] = static_cast<double>(p.scale);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::ScalarType type = grads[0].scalar_type();
+    const auto rows = [&](const Tensor& t) {
+      return t.defined() && t.is_cuda() && t.scalar_type() == type && packed_rows(t) ? t : aligned(restored(t, type));
+    };
+    const Tensor q = rows(saved[0]), k = rows(saved[1]), v = rows(saved[2]), out = aligned(restored(saved[3], type));
+    const Tensor rest = saved[4].defined() ? aligned(restored(saved[4], type)) : Tensor();
+    const Tensor stats = aligned(restored(saved[5], at::kFloat)), offsets = restored(saved[6], at::kInt), key_offsets = restored(saved[7], at::kInt);
+    const Tensor key_lengths = saved[8].defined() ? restored(saved[8], at::kInt) : Tensor(), g = rows(grads[0]);
+    saved_as(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.sizes() == g.sizes() && out.sizes() == q.sizes() &&
+             (!rest.defined() || rest.sizes() == q.sizes()) && stats.sizes().equals({q.size(0), q.size(1), 4}) && k.size(2) == q.size(2) &&
+             q.size(1) % k.size(1) == 0 && offsets.dim() == 1 && offsets.numel() >= 1 && key_offsets.sizes() == offsets.sizes() &&
+             (!key_lengths.defined() || (key_lengths.dim() == 1 && key_lengths.numel() == offsets.numel() - 1)));
+    for (const Tensor* t : {&k, &v, &out, &rest, &stats, &offsets, &key_offsets, &key_lengths, &g})
+      saved_as(!t->defined() || t->device() == q.device());
+    const Packed p(q, k, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    const auto like = [](bool wanted, const Tensor& t) { return wanted ? at::empty(t.sizes(), t.options()) : Tensor(); };
+    Tensor gq = like(ctx->needs_input_grad(0), q), gk = like(ctx->needs_input_grad(1), k), gv = like(ctx->needs_input_grad(2), v), ws;
+    const int64_t bytes = gk.defined() || gv.defined()
+                              ? lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim)
+                              : 0;
+    check(bytes);
+    if (bytes != 0) ws = workspace(bytes, q);
+    int64_t st[16] = {};
+    const Tensor* t[8] = {&q, &k, &v, &out, &g, &gq, &gk, &gv};
+    for (int i = 0; i < 8; ++i)
+      if (t[i]->defined()) {
+        st[2 * i] = t[i]->stride(0);
+        st[2 * i + 1] = t[i]->stride(1);
+      }
+    launch(q, [&](void* stream) {
+      return lib.packed_bwd(ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), fptr(stats), ptr(g), code(q), ptr(gq), ptr(gk), ptr(gv), iptr(offsets),
+                            iptr(key_offsets), iptr(key_lengths), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale,
+                            ptr(ws), bytes, stream);
+    });
+    return once({gq, gk, gv, Tensor(), Tensor(), Tensor(), Tensor()}, "packed_attention");
+  }
+
+  // a contiguous tensor on a 16-byte boundary
+  static Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
+};
+
+// q [T, H, D], k and v [S, Hk, D]; scale: a Python float, or None
+py::object packed_attention(const py::handle& q, const py::handle& k, const py::handle& v, const py::handle& offsets, const py::handle& key_offsets,
+                            const py::handle& key_lengths, bool causal, const py::handle& scale) {
+  const Tensor *a, *b, *c, *o, *ko, *kl = nullptr;
+  if (!ordinary_state() || (a = plain(q)) == nullptr || (b = plain(k)) == nullptr || (c = plain(v)) == nullptr || (o = plain(offsets)) == nullptr ||
+      (ko = key_offsets.is_none() ? o : plain(key_offsets)) == nullptr || (!key_lengths.is_none() && (kl = plain(key_lengths)) == nullptr))
+    return py::none();
+  if (!value_type(*a) || a->dim() != 3) return py::none();
+  for (const Tensor* t : {a, b, c}) {
+    if (t->scalar_type() != a->scalar_type() || t->device() != a->device() || !packed_rows(*t)) return py::none();
+    for (int64_t n : t->sizes())
+      if (n >= (int64_t{1} << 31)) return py::none();
+  }
+  if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || a->size(1) % b->size(1) != 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
+    return py::none();
+  for (const Tensor* t : {o, ko, kl})
+    if (t != nullptr && (t->dim() != 1 || t->scalar_type() != at::kInt || t->device() != a->device() || !t->is_contiguous())) return py::none();
+  if (ko->numel() != o->numel() || (kl != nullptr && kl->numel() != o->numel() - 1)) return py::none();
+  if (!scale.is_none() && !PyFloat_CheckExact(scale.ptr())) return py::none();
+  const double s = scale.is_none() ? 1.0 / std::sqrt(static_cast<double>(a->size(2))) : PyFloat_AS_DOUBLE(scale.ptr());
+  if (!(s > 0.0) || !std::isfinite(static_cast<float>(s)) || static_cast<float>(s) == 0.0f) return py::none();
+  const Packed p(*a, *b, *o, causal, s);
+  if (!wants_grad({a, b, c})) return py::cast(packed_forward(*a, *b, *c, *o, *ko, kl != nullptr ? *kl : Tensor(), p, false)[0]);
+  return py::cast(PackedAttention::apply(*a, *b, *c, *o, *ko, kl != nullptr ? std::optional<Tensor>(*kl) : std::nullopt, p));
+}
+
+struct RotaryPlan {
+  std::vector<int64_t> sections;
+  double base;
+  bool shared, interleaved;
+};
+
+// x and y [T, heads, D] with contiguous channels (y undefined: x alone), rotated into new tensors
+std::array<Tensor, 2> rotated(const Tensor& x, const Tensor& y, const Tensor& positions, const RotaryPlan& plan, bool inverse) {
+  std::array<Tensor, 2> out = {at::empty(x.sizes(), x.options()), y.defined() ? at::empty(y.sizes(), y.options()) : Tensor()};
+  int64_t st[8] = {x.stride(0), x.stride(1), out[0].stride(0), out[0].stride(1)};
+  if (y.defined()) {
+    st[4] = y.stride(0);
+    st[5] = y.stride(1);
+    st[6] = out[1].stride(0);
+    st[7] = out[1].stride(1);
+  }
+  const int64_t ps[2] = {positions.stride(0), positions.stride(1)};
+  int32_t sections[8];
+  for (size_t i = 0; i < plan.sections.size(); ++i) sections[i] = static_cast<int32_t>(plan.sections[i]);
+  const int type = positions.scalar_type() == at::kInt ? MSDA_POSITION_I32 : positions.scalar_type() == at::kLong ? MSDA_POSITION_I64 : MSDA_POSITION_F32;
+  launch(x, [&](void* stream) {
+    return lib.rotary(ptr(x), ptr(out[0]), ptr(y), ptr(out[1]), code(x), ptr(positions), type, static_cast<int>(x.size(0)), static_cast<int>(x.size(1)),
+                      y.defined() ? static_cast<int>(y.size(1)) : 0, static_cast<int>(x.size(2)), st, ps, sections,
+                      static_cast<int>(plan.sections.size()), plan.base, plan.shared, plan.interleaved, inverse, stream);
+  });
+  return out;
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& positions, const RotaryPlan& plan) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions});
+    ctx->saved_data["sections"] = plan.sections;
+    ctx->saved_data["base"] = plan.base;
+    ctx->saved_data["shared"] = plan.shared;
+    ctx->saved_data["interleaved"] = plan.interleaved;
+    ctx->saved_data["position_type"] = static_cast<int64_t>(positions.scalar_type());
+    auto out = rotated(q, k.value_or(Tensor()), positions, plan, false);
+    if (!k) return {out[0]};
+    return {out[0], out[1]};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const RotaryPlan plan{ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), ctx->saved_data["shared"].toBool(),
+                          ctx->saved_data["interleaved"].toBool()};
+    const Tensor positions = restored(ctx->get_saved_variables()[0], static_cast<at::ScalarType>(ctx->saved_data["position_type"].toInt()));
+    variable_list out(4);
+    Tensor g[2];
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) g[i] = grads[i].stride(2) == 1 ? grads[i] : grads[i].contiguous();
+    const int first = g[0].defined() ? 0 : 1;
+    if (!g[first].defined()) return out;
+    saved_as(positions.dim() == 2 && positions.size(0) == g[first].size(0) && positions.size(1) == static_cast<int64_t>(plan.sections.size()) &&
+             positions.device() == g[first].device());
+    auto turned = rotated(g[first], first == 0 ? g[1] : Tensor(), positions, plan, true);
+    out[first] = turned[0];
+    if (first == 0) out[1] = turned[1];
+    return once(out, "rotary_embed");
+  }
+};
+
+// q [T, H, D], k [T, Hk, D] or None, positions [T, A]; sections: a tuple of Python ints
+py::object rotary(const py::handle& q, const py::handle& k, const py::handle& positions, const py::handle& sections, const py::handle& base, bool shared,
+                  bool interleaved) {
+  const Tensor *a, *b = nullptr, *p;
+  if (!ordinary_state() || (a = plain(q)) == nullptr || (!k.is_none() && (b = plain(k)) == nullptr) || (p = plain(positions)) == nullptr ||
+      !PyTuple_CheckExact(sections.ptr()) || !PyFloat_CheckExact(base.ptr()))
+    return py::none();
+  RotaryPlan plan{{}, PyFloat_AS_DOUBLE(base.ptr()), shared, interleaved};
+  int64_t pairs = 0;
+  for (const py::handle& n : py::reinterpret_borrow<py::tuple>(sections)) {
+    if (!PyLong_CheckExact(n.ptr())) return py::none();
+    const int64_t x = PyLong_AsLongLong(n.ptr());
+    if (x < 1 || x > 128) {
+      PyErr_Clear();
+      return py::none();
+    }
+    plan.sections.push_back(x);
+    pairs += x;
+  }
+  if (plan.sections.empty() || plan.sections.size() > 8 || !(plan.base > 0.0) || !std::isfinite(plan.base)) return py::none();
+  if (a->dim() != 3 || !value_type(*a) || a->stride(2) != 1 || a->size(2) % 2 != 0 || a->size(2) > 256 || 2 * pairs > a->size(2)) return py::none();
+  if (b != nullptr && (b->dim() != 3 || b->scalar_type() != a->scalar_type() || b->device() != a->device() || b->stride(2) != 1 ||
+                       b->size(0) != a->size(0) || b->size(2) != a->size(2)))
+    return py::none();
+  for (const Tensor* t : {a, b})
+    if (t != nullptr && (t->size(0) >= (int64_t{1} << 31) || t->size(1) > (1 << 15))) return py::none();
+  const auto type = p->scalar_type();
+  if (p->dim() != 2 || p->size(0) != a->size(0) || p->size(1) != static_cast<int64_t>(plan.sections.size()) || p->device() != a->device() ||
+      (type != at::kInt && type != at::kLong && type != at::kFloat))
+    return py::none();
+  if (!wants_grad({a, b})) {
+    const auto out = rotated(*a, b != nullptr ? *b : Tensor(), *p, plan, false);
+    if (b == nullptr) return py::cast(out[0]);
+    return py::make_tuple(out[0], out[1]);
+  }
+  const auto out = Rotary::apply(*a, b != nullptr ? std::optional<Tensor>(*b) : std::nullopt, *p, plan);
+  if (b == nullptr) return py::cast(out[0]);
+  return py::make_tuple(out[0], out[1]);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
@@ -539,4 +794,6 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("value_proj", &value_proj);
   m.def("grid_sample", &grid_sample);
   m.def("attention", &attention);
+  m.def("packed_attention", &packed_attention);
+  m.def("rotary", &rotary);
 }

@@ -122,7 +122,7 @@ def lib(path: str | None = None) -> ctypes.CDLL:
 class _NoBinding:
     """Leaves every call to the Python autograd functions."""
 
-    core = fused = value_proj = grid_sample = attention = staticmethod(lambda *args: None)
+    core = fused = value_proj = grid_sample = attention = packed_attention = rotary = staticmethod(lambda *args: None)
 
 
 def binding():

@@ -210,4 +210,7 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
         TypeError: types other than the above.
         RuntimeError: tensors that are not on a GPU.
     """
+    out = _native.binding().packed_attention(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale)
+    if out is not None:
+        return out
     return _PackedAttention.apply(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale)

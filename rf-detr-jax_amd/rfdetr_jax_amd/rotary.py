@@ -99,6 +99,9 @@ def rotary_embed(q, k, positions, sections, base=10000.0, shared_frequencies=Fal
         RuntimeError: tensors that are not on a GPU.
     """
     sections = tuple(int(s) for s in sections)
+    out = _native.binding().rotary(q, k, positions, sections, base, bool(shared_frequencies), bool(interleaved))
+    if out is not None:
+        return out
     for name, t in (("q", q), ("k", k)):
         if t is None and name == "k":
             continue
