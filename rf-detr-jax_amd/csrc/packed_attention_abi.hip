@@ -27,6 +27,8 @@ int pk_shape(const PackShape& s) {
     return fail(MSDA_ERR_UNSUPPORTED, "packed attention: head_dim %d (multiples of 8 up to 128 supported)", s.head_dim);
   if (s.heads != 0 && (s.kv_heads == 0 || s.heads % s.kv_heads != 0))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: %d heads do not divide into %d key heads", s.heads, s.kv_heads);
+  if (s.heads != 0 && s.heads / s.kv_heads > msda::kPkChunk)
+    return fail(MSDA_ERR_UNSUPPORTED, "packed attention: %d query heads to a key head (at most %d)", s.heads / s.kv_heads, msda::kPkChunk);
   // row numbers of a key head's matrix, tiles included, are formed in 32 bits
   const int64_t group = s.heads == 0 ? 1 : s.heads / s.kv_heads, tiles = (static_cast<int64_t>(s.sequences) + 3) * msda::kPkTile;
   if (s.q_rows * group + tiles >= (int64_t{1} << 31) || s.k_rows + tiles >= (int64_t{1} << 31))
@@ -34,33 +36,52 @@ int pk_shape(const PackShape& s) {
   return MSDA_OK;
 }
 
-// The number of parts that the keys are split into: with fewer workgroups than CUs hold (two each), as
-// many as fill them, of at least kLeast chunks of 64 keys of an average sequence.
-int pk_splits(const PackShape& s) {
-  constexpr int64_t kWant = 512, kLeast = 4, kMost = 64;
-  if (s.heads == 0 || s.sequences == 0) return 1;
+// The forward's split of the keys over workgroups: how many at most share a tile of rows, and the chunks of 64 keys
+// that make one worth it. The lengths are not known here, only their sums; a workgroup finds its tile's number
+// of parts from the length (pk_fwd_kernel).
+struct PackSplit {
+  int most, part;
+};
+
+PackSplit pk_split(const PackShape& s) {
+  constexpr int64_t kSlots = 512;  // workgroups that the CUs hold, two each
+  const PackSplit none{1, 1 << 30};
+  if (s.heads == 0 || s.sequences == 0) return none;
   const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads);
-  const int64_t groups = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
-  const int64_t chunks = (s.k_rows / s.sequences + msda::kPkChunk - 1) / msda::kPkChunk;
-  if (groups == 0) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / groups, chunks / kLeast, kMost})));
+  const int64_t tiles = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
+  const int64_t chunks = (s.k_rows / s.sequences + msda::kPkChunk - 1) / msda::kPkChunk;  // of an average sequence
+  if (tiles == 0) return none;
+  // Few rows to a tile (new tokens over caches): a part's own cost is small against its keys, so even calls that
+  // fill the CUs are split, because the longest cache would set their time.
+  const bool few = rows <= int64_t{32} * s.sequences;
+  if (!few && 2 * tiles > kSlots) return none;
+  // Full tiles: a part writes and the join reads 128 rows of f32 sums, the time of about 6 chunks of keys at
+  // 128 channels in bf16, of 2 in f32. Of the parts that the CUs hold at once, each takes `even` chunks:
+  const int64_t even = (tiles * chunks + kSlots - 1) / kSlots, least = few ? 2 : s.dtype == MSDA_DTYPE_BF16 ? 6 : 2;
+  const int64_t part = few ? std::clamp<int64_t>(even, least, 16) : std::max(even, least);
+  // An average sequence's parts (a longer one's are longer), twice those where a causal tile's keys are half of them on average
+  const int64_t most = std::min<int64_t>((few ? 1 : 2) * ((chunks + part - 1) / part), msda::kPkMostParts);
+  return most <= 1 ? none : PackSplit{static_cast<int>(most), static_cast<int>(part)};
 }
 
-// Bytes of the split forward's parts: f32 sums, then (m, l) of every row.
+// Bytes of the split forward's parts: f32 sums, (m, l) of every row and part, the rows' numbers of parts.
 int64_t pk_fwd_workspace(const PackShape& s) {
-  const int splits = pk_splits(s);
-  return splits == 1 ? 0 : static_cast<int64_t>(splits) * s.q_rows * s.heads * (s.head_dim + 2) * 4;
+  const int64_t parts = pk_split(s).most, rows = static_cast<int64_t>(s.q_rows) * s.heads;
+  return parts == 1 ? 0 : (parts * (s.head_dim + 2) + 1) * rows * 4;
 }
 
 // The number of workgroups that may share a tile of keys in the backward: a causal sequence's first keys are
-// seen by all its rows, so with few tiles the longest one sets the time. Twice two workgroups a CU, and no
-// more than the rows of one long sequence are worth.
+// seen by all its rows, so with few tiles the longest one sets the time. A part is kPkPart chunks (more where
+// that makes more than kMost parts, or the tiles alone are several rounds of workgroups).
 int pk_parts(const PackShape& s) {
-  constexpr int64_t kWant = 1024, kMost = 8;
+  constexpr int64_t kWant = 2048, kMost = 8;
   if (s.heads == 0 || s.sequences == 0 || s.k_rows == 0) return 1;
   const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
-  const int64_t chunks = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) / msda::kPkChunk;
-  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, chunks / msda::kPkLeastPart, kMost})));
+  // The rows of one sequence, if it is 4 times the average: a longer one takes longer parts, and batches of short
+  // sequences start no second kernel (4 us).
+  const int64_t rows = std::min<int64_t>(s.q_rows, 4 * (static_cast<int64_t>(s.q_rows) / s.sequences + 1));
+  const int64_t chunks = rows * (s.heads / s.kv_heads) / msda::kPkChunk;
+  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, (chunks + msda::kPkPart - 1) / msda::kPkPart, kMost})));
 }
 
 // Bytes of the parts' f32 sums of dk and dv.
@@ -159,13 +180,16 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   p.rest = dtype == MSDA_DTYPE_BF16 ? out_rest : nullptr;
   p.stats = stats;
   p.slots = static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
-  p.splits = pk_splits(s);
+  const PackSplit split = pk_split(s);
+  p.splits = split.most;
+  p.part = split.part;
   if (p.splits > 1) {
     const int64_t need = pk_fwd_workspace(s);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + static_cast<int64_t>(p.splits) * q_rows * heads * head_dim;
+    p.part_n = reinterpret_cast<int32_t*>(p.part_ml + static_cast<int64_t>(p.splits) * q_rows * heads * 2);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_fwd<msda::bf16_t>(p, st) : msda_host::dispatch_pk_fwd<float>(p, st);

@@ -30,6 +30,7 @@
 
 #include <cstdint>
 #include <type_traits>
+#include <utility>
 
 #include "attention_common.h"
 #include "msda_kernels.h"  // bf16_t, wait_vmem
@@ -55,17 +56,23 @@ struct PackParams {
   const int32_t* k_lengths;  // [sequences], or null: all rows of a sequence's range
   float* part_o;             // split forward: [splits][q_rows * heads][dim], sums relative to part_ml's m
   float* part_ml;            // [splits][q_rows * heads][2]: m, l
+  int32_t* part_n;           // [q_rows * heads]: the row's parts
   float* part_kv;            // key side: [splits][dk, dv][k_rows * kv_heads][dim]
   int64_t st[kPkTensors][2];  // element strides (row, head) of each tensor
-  int sequences, q_rows, k_rows, heads, kv_heads, group, dim, causal, splits;
+  int sequences, q_rows, k_rows, heads, kv_heads, group, dim, causal;
+  int splits;    // at most so many workgroups share a tile's streamed rows
+  int part;      // forward: chunks of one of them, unless that makes more
   int slots;     // tiles of the kernel's own side
   float scale;   // of the scores
   float scale2;  // scale log2(e)
 };
 
-constexpr int kPkTile = 128;  // own rows of a workgroup: 32 a wave
-constexpr int kPkChunk = 64;  // streamed rows of a tile
-constexpr int kPkLeastPart = 16;  // chunks that are worth a workgroup of their own on the key side
+constexpr int kPkWaves = 4;              // of a workgroup
+constexpr int kPkTile = 32 * kPkWaves;   // own rows of a workgroup: 32 a wave
+constexpr int kPkChunk = 64;             // streamed rows of a tile
+constexpr int kPkMostParts = 64;  // of a forward tile's keys
+constexpr int kPkPart = 32;  // chunks of a workgroup on the key side, unless that makes more parts than the host gave room for
+constexpr int kPkJoin = 32;   // workgroups that join a key tile's parts
 
 __device__ __align__(16) const uint32_t pk_zeros[4] = {0u, 0u, 0u, 0u};
 
@@ -87,12 +94,11 @@ struct PkPlace {
 
 // The segment of `slot` (the wave searches 64 segments at a time): the last one that starts at or
 // before it. `unit`: rows of a tile's matrix to a row of the tensor.
-template <int BM>
 __device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequences, int rows, int unit, int slot, int lane) {
   int lo = 0, hi = sequences + 2;
   while (hi - lo > 1) {
     const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-    const bool at = s < hi && static_cast<int>(static_cast<uint32_t>(pk_bound(offsets, s, sequences, rows)) * unit / BM) + s <= slot;
+    const bool at = s < hi && static_cast<int>(static_cast<uint32_t>(pk_bound(offsets, s, sequences, rows)) * unit / kPkTile) + s <= slot;
     const int n = max(1, static_cast<int>(__popcll(__ballot(at))));
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
@@ -102,7 +108,7 @@ __device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequence
   w.first = pk_bound(offsets, lo, sequences, rows);
   w.own = max(0, pk_bound(offsets, lo + 1, sequences, rows) - w.first);
   w.seq = lo >= 1 && lo <= sequences ? lo - 1 : -1;
-  w.tile = slot - (static_cast<int>(static_cast<uint32_t>(w.first) * unit / BM) + lo);
+  w.tile = slot - (static_cast<int>(static_cast<uint32_t>(w.first) * unit / kPkTile) + lo);
   if (w.tile < 0) w.tile = w.own = 0;  // only where the offsets fall
   return w;
 }
@@ -119,9 +125,20 @@ struct PkTile {
   static constexpr int CPR = DP / E;                          // chunks of a row
   static constexpr int ROW = DP * static_cast<int>(sizeof(T));  // bytes of a row
   static constexpr int BYTES = kPkChunk * ROW;
-  // 16-byte chunk c of row r sits at slot c ^ swizzle(r): the rows that a read takes together fall on
-  // distinct banks
-  static __device__ __forceinline__ int swizzle(int r) { return CPR >= 16 ? (r & 15) : ((r / (16 / CPR)) & (CPR - 1)); }
+  // 16-byte chunk c of row r sits at slot c ^ swizzle(r), so that what one read takes together falls on
+  // distinct banks (256 bytes a clock): 16 rows of one chunk (operands along the channels); 4 rows of 4
+  // chunks (bf16, transposing reads: rows that share a 256-byte line differ in the slot's upper bits); 8
+  // chunks of rows 4 apart (f32, along the rows: their halves of a line differ). With r % 16 for a swizzle
+  // the transposing reads met 4 rows on the same banks, and the forward at 128 channels spent 60 % of its
+  // LDS time on conflicts.
+  static __device__ __forceinline__ constexpr int swizzle(int r) {
+    if (sizeof(T) == 2) {
+      if (CPR == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+      if (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+      return (r >> 2) & 3;
+    }
+    return CPR >= 16 ? ((((r >> 2) & 1) << 3) | (((r >> 3) & 1) << 2) | (r & 3)) : ((r >> 1) & 7);
+  }
 };
 
 // A lane's byte offsets in a tile. The chunks that one lane reads differ in bits that neither its row's
@@ -130,7 +147,7 @@ struct PkTile {
 template <typename T, int DT>
 struct PkLane {
   using Tile = PkTile<T, DT>;
-  static constexpr uint32_t kRows8 = Tile::CPR >= 16 ? 128 : 8 * Tile::CPR;  // swizzle(r) ^ swizzle(r + 8), as bytes
+  static constexpr uint32_t kRows8 = 32;  // bf16: swizzle(r) ^ swizzle(r + 8), as bytes
   uint32_t row;  // row col, chunk grp: operands along the channels
   uint32_t tr;   // bf16: rows 4 grp + (lane % 16) / 4, channels 16 (lane / 16 % 2) + 4 (lane % 4)
                  // f32: row 4 grp, channel col: operands along the rows
@@ -196,20 +213,42 @@ __device__ __forceinline__ uint2 pk_read_tr(PkLds p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MSDA_LDS at_s4*)(p)));
 }
 
-// N products, the operand of each read from LDS PF products ahead. The barriers hold LDS reads and products
-// in this order (vector and scalar instructions may pass): left to itself the compiler reads an operand,
-// waits for it, and multiplies, one at a time.
-template <int N, int PF, typename Read, typename Use>
-__device__ __forceinline__ void pk_pipe(Read&& read, Use&& use) {
-  decltype(read(0)) a[PF];
-#pragma unroll
-  for (int i = 0; i < PF; ++i) a[i] = read(i);
-  __builtin_amdgcn_sched_barrier(0x6);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
+// f(0) .. f(N - 1) with the number as a constant.
+template <int I>
+using PkInt = std::integral_constant<int, I>;
+template <typename F, int... I>
+__device__ __forceinline__ void pk_for_each(F&& f, std::integer_sequence<int, I...>) {
+  (f(PkInt<I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void pk_for(F&& f) {
+  pk_for_each(f, std::make_integer_sequence<int, N>{});
+}
+
+// N products, the operand of each read from LDS PF products ahead. The barriers hold everything in the order
+// that it is written in (MAY: but the kinds of instructions that may pass), the vector work `beside` a product
+// included: left to itself the compiler reads an operand, waits for it, and multiplies, one at a time, and all
+// vector work after that.
+template <int N, int PF, int MAY = 0, typename Read, typename Use, typename Beside>
+__device__ __forceinline__ void pk_pipe(Read&& read, Use&& use, Beside&& beside) {
+  decltype(read(PkInt<0>{})) a[PF];
+  pk_for<PF>([&](auto i) { a[i] = read(i); });
+  __builtin_amdgcn_sched_barrier(MAY);
+  pk_for<N>([&](auto i) {
     use(i, a[i % PF]);
-    if (i + PF < N) a[i % PF] = read(i + PF);
-    __builtin_amdgcn_sched_barrier(0x6);
+    if constexpr (i + PF < N) a[i % PF] = read(PkInt<i + PF>{});
+    beside(i);
+    __builtin_amdgcn_sched_barrier(MAY);
+  });
+}
+
+// Vector work beside the KS products of a phase: a product's result is there one product later, so step t
+// takes part t - 1 of KS - 1 of the 16 registers.
+template <int KS, int T, typename F>
+__device__ __forceinline__ void pk_beside(F&& f) {
+  if constexpr (T >= 1) {
+    constexpr int lo = 16 * (T - 1) / (KS - 1), hi = 16 * T / (KS - 1);
+    pk_for<hi - lo>([&](auto i) { f(lo + i); });
   }
 }
 
@@ -229,9 +268,10 @@ struct PkProducts<bf16_t, DT> {
   static __device__ __forceinline__ at_bf8 row_operand(PkLds X, const PkLane<T, DT>& at, int i) {
     return *reinterpret_cast<const MSDA_LDS at_bf8*>(X + (at.row ^ (i << 5)));
   }
-  static __device__ __forceinline__ void score(at_f16& s, const at_bf8& a, const PkRow<T, DT>& r, int i) {
-    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, r.x[i], s, 0, 0, 0);
+  static __device__ __forceinline__ void score(at_f16& s, const at_bf8& a, const at_bf8& b) {
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, s, 0, 0, 0);
   }
+  static __device__ __forceinline__ void score(at_f16& s, const at_bf8& a, const PkRow<T, DT>& r, int i) { score(s, a, r.x[i]); }
   // product j: rows 16 (j / ND) .. + 15, channels of block j % ND
   static __device__ __forceinline__ at_bf8 sum_operand(PkLds X, const PkLane<T, DT>& at, int j) {
     const int s = j / ND, nd = j % ND;
@@ -240,7 +280,10 @@ struct PkProducts<bf16_t, DT> {
   }
   struct Weights {
     at_bf8 b[2];
-    __device__ __forceinline__ explicit Weights(const at_f16& w) : b{at_bf8_regs(w, 0), at_bf8_regs(w, 8)} {}
+    __device__ __forceinline__ void set(const at_f16& w) {
+      b[0] = at_bf8_regs(w, 0);
+      b[1] = at_bf8_regs(w, 8);
+    }
   };
   static __device__ __forceinline__ void sum(at_f16 (&acc)[ND], const at_bf8& a, const Weights& w, int j) {
     acc[j % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.b[j / ND], acc[j % ND], 0, 0, 0);
@@ -263,9 +306,8 @@ struct PkProducts<float, DT> {
     float a[ND];
   };
   static __device__ __forceinline__ Operand sum_operand(PkLds X, const PkLane<T, DT>& at, int i) {
-    constexpr int S = PkTile<T, DT>::CPR;
-    const int ro = 8 * (i >> 2) + (i & 3);  // its swizzle: row 4 grp's, and a constant (4 grp + i % 4 carries nothing)
-    const uint32_t x = S >= 16 ? (ro & 15) : ((ro / (16 / S)) & (S - 1));
+    const int ro = 8 * (i >> 2) + (i & 3);  // row 4 grp + ro: the swizzle's bits of 4 grp (in at.tr) and of ro do not meet
+    const uint32_t x = PkTile<T, DT>::swizzle(ro);
     Operand o;
 #pragma unroll
     for (int nd = 0; nd < ND; ++nd) o.a[nd] = *reinterpret_cast<const MSDA_LDS float*>(X + (at.tr ^ ((x ^ (8 * nd)) << 4)) + ro * ROW);
@@ -273,7 +315,7 @@ struct PkProducts<float, DT> {
   }
   struct Weights {
     at_f16 b;
-    __device__ __forceinline__ explicit Weights(const at_f16& w) : b(w) {}
+    __device__ __forceinline__ void set(const at_f16& w) { b = w; }
   };
   static __device__ __forceinline__ void sum(at_f16 (&acc)[ND], const Operand& o, const Weights& w, int i) {
 #pragma unroll
@@ -287,16 +329,21 @@ __device__ __forceinline__ void pk_scores2(at_f16& s, PkLds X, const PkRow<T, DT
                                            const PkLane<T, DT>& at) {
   using P = PkProducts<T, DT>;
   constexpr int N = P::kScores;
-  pk_pipe<2 * N, PF>([&](int i) { return P::row_operand(i < N ? X : Y, at, i % N); },
-                     [&](int i, const auto& a) { P::score(i < N ? s : t, a, i < N ? x : y, i % N); });
+  pk_pipe<2 * N, PF, 0x6>([&](auto i) { return P::row_operand(i < N ? X : Y, at, i % N); },
+                     [&](auto i, const auto& a) {
+                       if constexpr (i < N) P::score(s, a, x, i);
+                       else P::score(t, a, y, i - N);
+                     },
+                     [](auto) {});
 }
 
 // acc += X^T w
 template <typename T, int DT, int PF>
 __device__ __forceinline__ void pk_accumulate(at_f16 (&acc)[DT / 32], PkLds X, const at_f16& w, const PkLane<T, DT>& at) {
   using P = PkProducts<T, DT>;
-  const typename P::Weights b(w);
-  pk_pipe<P::kSums, PF>([&](int i) { return P::sum_operand(X, at, i); }, [&](int i, const auto& a) { P::sum(acc, a, b, i); });
+  typename P::Weights b;
+  b.set(w);
+  pk_pipe<P::kSums, PF, 0x6>([&](auto i) { return P::sum_operand(X, at, i); }, [&](auto i, const auto& a) { P::sum(acc, a, b, i); }, [](auto) {});
 }
 
 // ax += X^T wx, ay += Y^T wy
@@ -305,9 +352,15 @@ __device__ __forceinline__ void pk_accumulate2(at_f16 (&ax)[DT / 32], PkLds X, c
                                                const PkLane<T, DT>& at) {
   using P = PkProducts<T, DT>;
   constexpr int N = P::kSums;
-  const typename P::Weights bx(wx), by(wy);
-  pk_pipe<2 * N, PF>([&](int i) { return P::sum_operand(i < N ? X : Y, at, i % N); },
-                     [&](int i, const auto& a) { P::sum(i < N ? ax : ay, a, i < N ? bx : by, i % N); });
+  typename P::Weights bx, by;
+  bx.set(wx);
+  by.set(wy);
+  pk_pipe<2 * N, PF, 0x6>([&](auto i) { return P::sum_operand(i < N ? X : Y, at, i % N); },
+                     [&](auto i, const auto& a) {
+                       if constexpr (i < N) P::sum(ax, a, bx, i);
+                       else P::sum(ay, a, by, i - N);
+                     },
+                     [](auto) {});
 }
 
 typedef __bf16 pk_bf16 __attribute__((ext_vector_type(16)));
@@ -320,48 +373,45 @@ __device__ __forceinline__ void pk_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Writes acc * f (f: of the lane's row) as rows of T: through the wave's LDS scratch, so that each lane
-// stores 16 bytes and the wave whole rows. `row(r)`: the address of own row r of the wave's 32, or null.
-// REST: what the rounding to T leaves of them instead.
+// Writes acc * f (f: of the lane's row) as rows of T: through the wave's LDS scratch, half a tile of the same
+// layout, so that each lane stores 16 bytes and the wave whole rows. `row(r)`: the address of own row r of the
+// wave's 32, or null. REST: what the rounding to T leaves of them instead.
 template <typename T, int DT, bool REST = false, typename R>
-__device__ __forceinline__ void pk_store(const at_f16 (&acc)[DT / 32], float f, T* scratch, int dim, int lane, R&& row) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T)), LD = DT + E, C = DT / E;
-  static_assert(32 * LD * sizeof(T) <= PkTile<T, DT>::BYTES, "the scratch fits a tile");
+__device__ __forceinline__ void pk_store(const at_f16 (&acc)[DT / 32], float f, unsigned char* scratch, int dim, int lane, R&& row) {
+  using Tile = PkTile<T, DT>;
   const int grp = lane >> 5, col = lane & 31;
+  unsigned char* mine = scratch + col * Tile::ROW;
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) {
     at_f16 v = acc[nd] * f;
     if constexpr (REST) v -= __builtin_convertvector(__builtin_convertvector(v, pk_bf16), at_f16);
-    if constexpr (sizeof(T) == 2) {
-      uint16_t* t = reinterpret_cast<uint16_t*>(scratch) + col * LD + 32 * nd + 4 * grp;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint4 u = __builtin_bit_cast(uint4, at_bf8_regs(v, 8 * s));
-        *reinterpret_cast<uint2*>(t + 16 * s) = uint2{u.x, u.y};
-        *reinterpret_cast<uint2*>(t + 16 * s + 8) = uint2{u.z, u.w};
-      }
-    } else {
-      float* t = scratch + col * LD + 32 * nd + 4 * grp;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) *reinterpret_cast<at_f4*>(t + 8 * c) = at_f4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+    for (int c = 0; c < 4; ++c) {  // channels 32 nd + 8 c + 4 grp .. + 3
+      const at_f4 x = {v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(mine + (((4 * nd + c) ^ Tile::swizzle(col)) << 4) + 8 * grp) = __builtin_bit_cast(uint2, __builtin_convertvector(x, pk_bf4));
+      else
+        *reinterpret_cast<at_f4*>(mine + (((8 * nd + 2 * c + grp) ^ Tile::swizzle(col)) << 4)) = x;
     }
   }
   pk_wave_sync();
+  constexpr int C = DT / Tile::E;
 #pragma unroll 2
   for (int k = 0; k < C / 2; ++k) {
-    const int idx = lane + 64 * k, r = idx / C, ch = E * (idx - r * C);
+    const int idx = lane + 64 * k, r = idx / C, c = idx - r * C;
     T* to = row(r);
-    if (to != nullptr && ch < dim) *reinterpret_cast<uint4*>(to + ch) = *reinterpret_cast<const uint4*>(scratch + r * LD + ch);
+    if (to != nullptr && c * Tile::E < dim)
+      *reinterpret_cast<uint4*>(to + c * Tile::E) = *reinterpret_cast<const uint4*>(scratch + r * Tile::ROW + ((c ^ Tile::swizzle(r)) << 4));
   }
   pk_wave_sync();
 }
 
 // Rows of zeros: own rows [r0, r1) of the matrix, `row(r)` their addresses, by the whole workgroup.
-template <typename T, int NT, typename R>
+template <typename T, typename R>
 __device__ __forceinline__ void pk_zero_rows(int r0, int r1, int dim, R&& row) {
   constexpr int E = 16 / static_cast<int>(sizeof(T));
   const int c = dim / E;
-  for (int idx = threadIdx.x; idx < (r1 - r0) * c; idx += NT) {
+  for (int idx = threadIdx.x; idx < (r1 - r0) * c; idx += 64 * kPkWaves) {
     const int r = idx / c;
     *reinterpret_cast<uint4*>(row(r0 + r) + E * (idx - r * c)) = uint4{0u, 0u, 0u, 0u};
   }
@@ -379,47 +429,64 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t pk_buffer(const void* p, int b
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
 }
 
-// The transfers of one 64-row tile by the workgroup's 256 threads: piece u is row u / CPR, slot u % CPR,
+// The workgroup's barrier, with the wave's transfers into LDS landed and its LDS reads done.
+__device__ __forceinline__ void pk_barrier() {
+  wait_vmem();
+  __syncthreads();
+}
+
+// The transfers of one 64-row tile by the workgroup: piece u is row u / CPR, slot u % CPR,
 // which holds the row's chunk slot ^ swizzle(row). A thread's pieces are kStep rows apart. Row strides are
 // below 2^22 elements (the host's check), so a tile's offsets fit 31 bits.
 template <typename T, int DT>
 struct PkStream {
   using Tile = PkTile<T, DT>;
-  static constexpr int kStep = 256 / Tile::CPR, NV = kPkChunk / kStep;
+  static constexpr int kStep = 64 * kPkWaves / Tile::CPR, NV = kPkChunk / kStep;
+  static_assert(kStep * NV == kPkChunk, "whole pieces");
   static __device__ __forceinline__ void transfer(__amdgpu_buffer_rsrc_t src, int offset, unsigned char* lds, int v) {
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (MSDA_LDS void*)(lds + (256 * v + 64 * wave) * 16), 16, offset, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (MSDA_LDS void*)(lds + 64 * (kPkWaves * v + wave) * 16), 16, offset, 0, 0, 0);
   }
   // row and channel of piece v of thread t
   static __device__ __forceinline__ int row(int t, int v) { return t / Tile::CPR + kStep * v; }
   static __device__ __forceinline__ int channel(int t, int v) { return Tile::E * ((t % Tile::CPR) ^ Tile::swizzle(row(t, v))); }
-  // rows [first, first + 64) of a tensor whose row r is base + r stride; rows from `end` on are zeros
-  static __device__ __forceinline__ void load(unsigned char* lds, const T* base, int64_t stride, int first, int end, int dim) {
-    const int st = static_cast<int>(stride) * static_cast<int>(sizeof(T));
-    const __amdgpu_buffer_rsrc_t src = pk_buffer(base + first * stride, min(end - first, kPkChunk) * st);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int t = static_cast<int>(threadIdx.x), ch = channel(t, v);
-      transfer(src, dim == Tile::DP || ch < dim ? row(t, v) * st + ch * static_cast<int>(sizeof(T)) : kPkFar, lds, v);
+  // Rows [first, first + 64) of two tensors (row r at base + r stride), rows from `end` on as zeros (all of them
+  // when there is no such tile), into two tiles: 2 NV pieces, which are issued one at a time between other
+  // work. A piece keeps the CU's address unit busy for 16 clocks, and the waves that issue theirs together wait
+  // for one another: together at the start of a chunk they took 480 of the forward's 3,300 clocks a chunk.
+  struct Pair {
+    __amdgpu_buffer_rsrc_t x, y;
+    unsigned char* lx;
+    unsigned char* ly;
+    int sx, sy, dim;
+    __device__ __forceinline__ Pair(unsigned char* to_x, const T* bx, int64_t stride_x, unsigned char* to_y, const T* by, int64_t stride_y, int first,
+                                    int end, int d)
+        : lx(to_x), ly(to_y), sx(static_cast<int>(stride_x * static_cast<int>(sizeof(T)))), sy(static_cast<int>(stride_y * static_cast<int>(sizeof(T)))), dim(d) {
+      // (by hand: the compiler takes a clamp to the vector unit, and a buffer in vector registers to a loop)
+      const int rows = __builtin_amdgcn_readfirstlane(min(max(end - first, 0), kPkChunk));
+      x = pk_buffer(bx + first * stride_x, rows * sx);
+      y = pk_buffer(by + first * stride_y, rows * sy);
     }
-  }
+    template <int I>
+    __device__ __forceinline__ void piece() const {
+      constexpr int v = I % NV;
+      const int t = static_cast<int>(threadIdx.x), ch = channel(t, v);
+      const int o = dim == Tile::DP || ch < dim ? row(t, v) * (I < NV ? sx : sy) + ch * static_cast<int>(sizeof(T)) : kPkFar;
+      transfer(I < NV ? x : y, o, I < NV ? lx : ly, v);
+    }
+    __device__ __forceinline__ void all() const {
+      pk_for<2 * NV>([&](auto i) { piece<i>(); });
+    }
+  };
 };
 
-// The rows r = t G + g of a key head's queries, in chunks of at most 64: whole tokens while 64 rows hold one
-// (then a row's place in its chunk gives its token and head whatever the chunk), 64 rows otherwise.
+// The rows r = t G + g of a key head's queries (G <= 64), in chunks of whole tokens, at most 64 rows: a row's
+// place in its chunk gives its token and head whatever the chunk.
 struct PkRows {
-  int group, tokens, rows;   // tokens of a chunk (0: not whole ones), its rows
-  uint32_t magic;            // x / group = x magic >> 16 for x < 64, group <= 64 (x (magic group - 2^16) < 2^16)
-  __device__ __forceinline__ explicit PkRows(int g) : group(g) {
-    tokens = g <= kPkChunk ? kPkChunk / g : 0;
-    rows = tokens != 0 ? tokens * g : kPkChunk;
-    magic = tokens != 0 ? (65536 + g - 1) / g : 0;
-  }
-  // token and head of row x of a chunk whose first row has head g0 (0 in chunks of whole tokens)
-  __device__ __forceinline__ int token(int x, int g0) const {
-    return tokens != 0 ? static_cast<int>((static_cast<uint32_t>(x) * magic) >> 16) : (g0 + x >= group ? 1 : 0);
-  }
-  __device__ __forceinline__ int head(int x, int g0, int token) const { return g0 + x - token * group; }
+  int group, tokens;  // tokens of a chunk
+  uint32_t magic;     // x / group = x magic >> 16 for x < 64: x (magic group - 2^16) < 2^16
+  __device__ __forceinline__ explicit PkRows(int g) : group(g), tokens(kPkChunk / g), magic((65536 + g - 1) / g) {}
+  __device__ __forceinline__ int token(int x) const { return static_cast<int>((static_cast<uint32_t>(x) * magic) >> 16); }
 };
 
 // ---- queries on their own side: forward and dq -------------------------------------------------
@@ -431,14 +498,14 @@ struct PkQueries {
   int rows, r0;     // rows of the sequence's matrix, first of the workgroup's
   int64_t k_first;  // first key row
   int m, shift;     // keys; a row of token t sees the keys below min(m, t + shift + 1)
-  __device__ PkQueries(const PackParams& p, int lane) {
+  __device__ PkQueries(const PackParams& p, int splits, int lane) {
     // key heads fastest: with 8 of them each stays on one XCD, whose L2 then holds its keys; the last
     // tiles, which see the most keys of a causal sequence, first
     const int b = static_cast<int>(blockIdx.x), rest = b / p.kv_heads;
     kv_head = b - rest * p.kv_heads;
-    const int slot = p.slots - 1 - rest / p.splits;
-    split = rest % p.splits;
-    w = pk_place<kPkTile>(p.q_offsets, p.sequences, p.q_rows, p.group, slot, lane);
+    const int slot = p.slots - 1 - rest / splits;
+    split = rest % splits;
+    w = pk_place(p.q_offsets, p.sequences, p.q_rows, p.group, slot, lane);
     rows = w.own * p.group;
     r0 = w.tile * kPkTile;
     k_first = 0;
@@ -483,97 +550,169 @@ __device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lim, int grp) {
 // reference score m and sum l. m starts at the first chunk's maximum (whose weight, the largest of a short
 // row, is then 1 and rounds to itself) and moves when a chunk's exceeds it by 2^8.
 template <typename T, int DT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_fwd_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 : 2) : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
-  __shared__ __align__(16) unsigned char K0[Tile::BYTES], V0[Tile::BYTES], K1[Tile::BYTES], V1[Tile::BYTES];
+  using Stream = PkStream<T, DT>;
+  // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
+  __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, lane);
+  const PkQueries w(p, p.splits, lane);
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* out = static_cast<T*>(p.out);
+  const int end = w.w.seq < 0 ? 0 : w.seen(p, r1 - 1), chunks = (end + kPkChunk - 1) / kPkChunk;  // that the workgroup sees
+  const int parts = min(max((chunks + p.part - 1) / p.part, 1), p.splits);
+  if (w.split >= parts) return;
+  if (p.splits > 1 && w.split == 0)  // one part writes its rows itself
+    for (int r = w.r0 + static_cast<int>(threadIdx.x); r < r1; r += 64 * kPkWaves) p.part_n[w.stat(p, r)] = parts;
   if (w.w.seq < 0) {
-    if (p.splits == 1) {
-      pk_zero_rows<T, 256>(w.r0, r1, p.dim, [&](int r) { return w.row(p, out, kPkO, r); });
-    } else {
-      for (int r = w.r0 + static_cast<int>(threadIdx.x); r < r1; r += 256)
-        *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(w.split) * p.q_rows * p.heads + w.stat(p, r)) * 2) = float2{0.0f, 0.0f};
-    }
+    pk_zero_rows<T>(w.r0, r1, p.dim, [&](int r) { return w.row(p, out, kPkO, r); });
     return;
   }
   const int wr0 = w.r0 + 32 * wave, ri = wr0 + col;
   const bool valid = ri < w.rows;
   const int lim = valid ? w.seen(p, ri) : 0;
-  const int end = w.seen(p, r1 - 1);                                          // keys that the workgroup sees
-  const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;   // the wave
-  const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                   // every row of the wave
-  int c0 = 0, c1 = (end + kPkChunk - 1) / kPkChunk;
-  if (p.splits > 1) {
-    const int per = (c1 + p.splits - 1) / p.splits;
-    c0 = min(c1, w.split * per);
-    c1 = min(c1, c0 + per);
-  }
+  const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;  // keys that the wave sees
+  const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                  // that every row of it sees
+  const int per = (chunks + parts - 1) / parts, c0 = w.split * per, c1 = min(chunks, c0 + per);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
   const T* kp = static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
   const T* vp = static_cast<const T*>(p.v) + w.k_first * p.st[kPkV][0] + w.kv_head * p.st[kPkV][1];
-  float m = 0.0f, l = 0.0f;
+  float m = 0.0f, l = 0.0f;  // l: of the lane's half of the keys
+  bool fresh = true;         // no key seen yet
   at_f16 o[DT / 32];
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) o[nd] = at_zero16();
 
-  auto stage = [&](unsigned char* K, unsigned char* V, int c) {
-    PkStream<T, DT>::load(K, kp, p.st[kPkK][0], c * kPkChunk, w.m, p.dim);
-    PkStream<T, DT>::load(V, vp, p.st[kPkV][0], c * kPkChunk, w.m, p.dim);
+  using Pair = typename Stream::Pair;
+  auto tile = [&](unsigned char* K, unsigned char* V, int c) {  // behind the last: zeros, which nothing reads
+    return Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < c1 ? w.m : 0, p.dim);
   };
-  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c) {
+  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    if (k0 >= wend) return;
+    if (k0 >= wend) {
+      next.all();
+      return;
+    }
     at_f16 s0 = at_zero16(), s1 = at_zero16();
-    pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
-    if (k0 + kPkChunk > wfull) {
-      pk_mask(s0, k0, lim, grp);
-      pk_mask(s1, k0 + 32, lim, grp);
-    }
-    float bm = -INFINITY;
+    if constexpr (sizeof(T) == 2) {
+      // Phases of KS products: scores of keys 0 .. 31, of 32 .. 63 beside the softmax of the first, sums of
+      // the first beside the softmax of the second, sums of the second. The vector work fits beside the
+      // products of one wave; a CU's other workgroup fills the rest.
+      using P = PkProducts<T, DT>;
+      constexpr int KS = P::kScores, HA = KS >= 4 ? KS / 2 - 1 : 1, HB = KS - 1 - HA;  // steps up to the maximum, behind it
+      float bm, alpha = 1.0f;
+      // step t of the softmax of block x, whose keys start at k: x = scale2 s - m and its maximum, m moved if it
+      // has to, weights and their sum (a lane sums its half of the keys until the end)
+      auto soft = [&](at_f16& x, int k, auto step) {
+        constexpr int t = decltype(step)::value, first = HB > 0 ? HA + 1 : HA, parts = HB > 0 ? HB : 1;
+        if constexpr (t == 1) {
+          if (k + 32 > wfull) pk_mask(x, k, lim, grp);
+          bm = -INFINITY;
+        }
+        if constexpr (t >= 1 && t <= HA) {
+          constexpr int lo = 16 * (t - 1) / HA, hi = 16 * t / HA;
+          pk_for<hi - lo>([&](auto i) {
+            x[lo + i] = fmaf(x[lo + i], p.scale2, -m);
+            bm = fmaxf(bm, x[lo + i]);
+          });
+        }
+        if constexpr (t == HA) {
+          bm = at_max_halves(bm);
+          const bool move = bm > kAtLazy || (fresh && bm != -INFINITY);
+          if (__any(move)) {
+            const float d = move ? bm : 0.0f, a = fresh ? 0.0f : at_exp2(-d);
+            alpha *= a;
+            m += d;
+            l *= a;
+            x -= d;
+            fresh = fresh && !move;
+          }
+        }
+        if constexpr (t >= first) {
+          constexpr int lo = 16 * (t - first) / parts, hi = 16 * (t - first + 1) / parts;
+          pk_for<hi - lo>([&](auto i) {
+            x[lo + i] = at_exp2(x[lo + i]);
+            l += x[lo + i];
+          });
+        }
+      };
+      auto rescale = [&] {  // between phases: the sums of a phase belong to one m
+        if (__any(alpha != 1.0f)) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bm = fmaxf(bm, fmaxf(s0[i], s1[i]));
-    bm = at_max_halves(bm) * p.scale2;
-    if (bm != -INFINITY && (bm > m + kAtLazy || l == 0.0f)) {
-      const float alpha = l == 0.0f ? 0.0f : at_exp2(m - bm);
-      m = bm;
-      l *= alpha;
+          for (int nd = 0; nd < DT / 32; ++nd) o[nd] *= alpha;
+          alpha = 1.0f;
+        }
+      };
+      typename P::Weights w0, w1;
+      pk_pipe<4 * KS, PF>(
+          [&](auto i) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (b < 2) return P::row_operand(K + b * 32 * Tile::ROW, at, t);
+            else return P::sum_operand(V + (b - 2) * 32 * Tile::ROW, at, t);
+          },
+          [&](auto i, const auto& a) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (b == 0) P::score(s0, a, q, t);
+            if constexpr (b == 1) P::score(s1, a, q, t);
+            if constexpr (b == 2) P::sum(o, a, w0, t);
+            if constexpr (b == 3) P::sum(o, a, w1, t);
+          },
+          [&](auto i) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (i < 2 * Stream::NV) next.template piece<i>();
+            if constexpr (b == 1) soft(s0, k0, PkInt<t>{});
+            if constexpr (b == 2) soft(s1, k0 + 32, PkInt<t>{});
+            if constexpr ((b == 1 || b == 2) && t == KS - 1) {
+              rescale();
+              if constexpr (b == 1) w0.set(s0);
+              else w1.set(s1);
+            }
+          });
+    } else {
+      next.all();
+      pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
+      if (k0 + kPkChunk > wfull) {
+        pk_mask(s0, k0, lim, grp);
+        pk_mask(s1, k0 + 32, lim, grp);
+      }
+      float bm = -INFINITY;
 #pragma unroll
-      for (int nd = 0; nd < DT / 32; ++nd) o[nd] *= alpha;
-    }
-    float rs = 0.0f;
+      for (int i = 0; i < 16; ++i) bm = fmaxf(bm, fmaxf(s0[i], s1[i]));
+      bm = at_max_halves(bm) * p.scale2;
+      if (bm != -INFINITY && (bm > m + kAtLazy || fresh)) {
+        const float alpha = fresh ? 0.0f : at_exp2(m - bm);
+        m = bm;
+        l *= alpha;
+        fresh = false;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s0[i] = at_exp2(fmaf(s0[i], p.scale2, -m));
-      s1[i] = at_exp2(fmaf(s1[i], p.scale2, -m));
-      rs += s0[i] + s1[i];
+        for (int nd = 0; nd < DT / 32; ++nd) o[nd] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s0[i] = at_exp2(fmaf(s0[i], p.scale2, -m));
+        s1[i] = at_exp2(fmaf(s1[i], p.scale2, -m));
+        l += s0[i] + s1[i];
+      }
+      pk_accumulate2<T, DT, PF>(o, V, s0, o, V + 32 * Tile::ROW, s1, at);
     }
-    l += at_sum_halves(rs);
-    pk_accumulate2<T, DT, PF>(o, V, s0, o, V + 32 * Tile::ROW, s1, at);
   };
-  if (c0 < c1) stage(K0, V0, c0);
+  if (c0 < c1) tile(X0, Y0, c0).all();
   for (int c = c0; c < c1; c += 2) {
-    wait_vmem();
-    __syncthreads();  // tile c is there, and every wave is done with tile c - 1
-    if (c + 1 < c1) stage(K1, V1, c + 1);
-    chunk(K0, V0, c);
+    pk_barrier();  // tile c is there, and every wave is done with tile c - 1
+    chunk(X0, Y0, c, tile(X1, Y1, c + 1));
     if (c + 1 >= c1) break;
-    wait_vmem();
-    __syncthreads();
-    if (c + 2 < c1) stage(K0, V0, c + 2);
-    chunk(K1, V1, c + 1);
+    pk_barrier();
+    chunk(X1, Y1, c + 1, tile(X0, Y0, c + 2));
   }
-  __syncthreads();  // the tiles hold the waves' scratch from here
-  unsigned char* const tiles[4] = {K0, V0, K1, V1};
-  T* scratch = reinterpret_cast<T*>(wave == 0 ? tiles[0] : wave == 1 ? tiles[1] : wave == 2 ? tiles[2] : tiles[3]);
-  if (p.splits > 1) {  // sums as they are: registers hold 4 consecutive channels of the lane's row
+  l = at_sum_halves(l);
+  pk_barrier();  // the tiles hold the waves' scratch from here
+  unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
+  if (parts > 1) {  // sums as they are: registers hold 4 consecutive channels of the lane's row
     if (!valid) return;
     const int64_t part = static_cast<int64_t>(w.split) * p.q_rows * p.heads + w.stat(p, ri);
     float* po = p.part_o + part * p.dim;
@@ -608,30 +747,45 @@ __device__ __forceinline__ void pk_put4(T* to, at_f4 v) {
   }
 }
 
-// The split forward's parts joined: one row (token, head) to a wave's quarter, 16 lanes a row.
-template <typename T>
+// The split forward's parts joined, LPR lanes a row (token, head): each lane weighs some parts, then sums four
+// channels at a time over all of them.
+template <typename T, int LPR>
 __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
-  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.heads, row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 15;
+  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.heads, row = static_cast<int64_t>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
+  const int lane = threadIdx.x % LPR;
+  const int parts = row < rows ? min(p.part_n[row], p.splits) : 0;
+  float2 ml[kPkMostParts / LPR];  // of parts lane, lane + LPR, ..
   float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
-    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+#pragma unroll
+  for (int i = 0; i < kPkMostParts / LPR; ++i) {
+    const int s = lane + LPR * i;
+    ml[i] = s < parts ? *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2) : float2{0.0f, 0.0f};
+    if (ml[i].y != 0.0f) m = fmaxf(m, ml[i].x);
   }
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
-    if (ml.y != 0.0f) l += ml.y * at_exp2(ml.x - m);
+#pragma unroll
+  for (int x = LPR / 2; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x, LPR));
+#pragma unroll
+  for (int i = 0; i < kPkMostParts / LPR; ++i) {
+    ml[i].x = ml[i].y != 0.0f ? at_exp2(ml[i].x - m) : 0.0f;  // the part's weight
+    l += ml[i].y * ml[i].x;
   }
+#pragma unroll
+  for (int x = LPR / 2; x > 0; x /= 2) l += __shfl_xor(l, x, LPR);
+  if (parts <= 1) return;  // written already
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t tok = row / p.heads, h = row - tok * p.heads;
   T* out = static_cast<T*>(p.out) + tok * p.st[kPkO][0] + h * p.st[kPkO][1];
-  for (int ch = 4 * lane; ch < p.dim; ch += 64) {
+  for (int ch = 4 * lane; ch < p.dim + 4 * (LPR - 1); ch += 4 * LPR) {  // every lane takes part in the shuffles
+    const bool mine = ch < p.dim;
     at_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
-      if (ml.y != 0.0f) a += *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch) * at_exp2(ml.x - m);
-    }
+#pragma unroll
+    for (int i = 0; i < kPkMostParts / LPR; ++i)
+#pragma unroll 4
+      for (int s = LPR * i; s < min(parts, LPR * (i + 1)); ++s) {
+        const float w = __shfl(ml[i].x, s - LPR * i, LPR);
+        if (mine && w != 0.0f) a += *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch) * w;
+      }
+    if (!mine) continue;
     a *= inv;
     pk_put4(out + ch, a);
     if constexpr (sizeof(T) == 2)
@@ -644,18 +798,20 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
 
 // dq, and delta into the statistics for the key side (alone when gq is null).
 template <typename T, int DT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_q_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
-  __shared__ __align__(16) unsigned char K0[Tile::BYTES], V0[Tile::BYTES], K1[Tile::BYTES], V1[Tile::BYTES];
+  using Stream = PkStream<T, DT>;
+  // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
+  __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, lane);
+  const PkQueries w(p, 1, lane);
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* gq = static_cast<T*>(p.gq);
   if (w.w.seq < 0) {
-    if (gq != nullptr) pk_zero_rows<T, 256>(w.r0, r1, p.dim, [&](int r) { return w.row(p, gq, kPkGQ, r); });
+    if (gq != nullptr) pk_zero_rows<T>(w.r0, r1, p.dim, [&](int r) { return w.row(p, gq, kPkGQ, r); });
     return;
   }
   const int wr0 = w.r0 + 32 * wave, ri = wr0 + col, rc = min(ri, w.rows - 1);
@@ -698,43 +854,88 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_q_kernel(c
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) dq[nd] = at_zero16();
 
-  auto stage = [&](unsigned char* K, unsigned char* V, int c) {
-    PkStream<T, DT>::load(K, kp, p.st[kPkK][0], c * kPkChunk, w.m, p.dim);
-    PkStream<T, DT>::load(V, vp, p.st[kPkV][0], c * kPkChunk, w.m, p.dim);
+  using Pair = typename Stream::Pair;
+  auto tile = [&](unsigned char* K, unsigned char* V, int c) {  // behind the last: zeros, which nothing reads
+    return Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < chunks ? w.m : 0, p.dim);
   };
-  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c) {
+  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    if (k0 >= wend) return;
-#pragma unroll 1
-    for (int h = 0; h < kPkChunk; h += 32) {
+    if (k0 >= wend) {
+      next.all();
+      return;
+    }
+    if constexpr (bf) {
+      // Phases of KS products: S, dP beside the weights, of the first 32 keys and of the second (beside ds of the
+      // first), then their sums (beside ds of the second).
+      using P = PkProducts<T, DT>;
+      constexpr int KS = P::kScores;
+      at_f16 sa = at_zero16(), sb = at_zero16(), da = at_zero16(), db = at_zero16();
+      typename P::Weights wa, wb;
       PkLane<T, DT> now = at;  // as in pk_bwd_kv_kernel
       asm volatile("" : "+v"(now.row), "+v"(now.tr));
-      at_f16 s = at_zero16(), dp = at_zero16();
-      pk_scores2<T, DT, PF>(s, K + h * Tile::ROW, q, dp, V + h * Tile::ROW, go, now);
+      auto weigh = [&](at_f16& s, auto t) { pk_beside<KS, t>([&](int i) { s[i] = at_exp2(fmaf(s[i], p.scale2, -m)); }); };
+      auto slope = [&](at_f16& s, const at_f16& d, typename P::Weights& w, int k, auto t) {
+        pk_beside<KS, t>([&](int i) { s[i] *= d[i] - delta; });
+        if constexpr (t == KS - 1) {
+          if (k + 32 > wfull) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = at_exp2(bf ? fmaf(s[i], p.scale2, -m) : fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
-      if (k0 + h + 32 > wfull) {
+            for (int i = 0; i < 16; ++i) s[i] = k + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+          }
+          w.set(s);
+        }
+      };
+      pk_pipe<6 * KS, PF>(
+          [&](auto i) {
+            constexpr int b = i / KS, t = i % KS;
+            const PkLds X = (b == 1 || b == 3 ? V : K) + (b == 2 || b == 3 || b == 5 ? 32 * Tile::ROW : 0);
+            if constexpr (b < 4) return P::row_operand(X, now, t);
+            else return P::sum_operand(X, now, t);
+          },
+          [&](auto i, const auto& a) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (b == 0) P::score(sa, a, q, t);
+            if constexpr (b == 1) P::score(da, a, go, t);
+            if constexpr (b == 2) P::score(sb, a, q, t);
+            if constexpr (b == 3) P::score(db, a, go, t);
+            if constexpr (b == 4) P::sum(dq, a, wa, t);
+            if constexpr (b == 5) P::sum(dq, a, wb, t);
+          },
+          [&](auto i) {
+            constexpr int b = i / KS;
+            constexpr PkInt<i % KS> t{};
+            if constexpr (i < 2 * Stream::NV) next.template piece<i>();
+            if constexpr (b == 1) weigh(sa, t);
+            if constexpr (b == 2) slope(sa, da, wa, k0, t);
+            if constexpr (b == 3) weigh(sb, t);
+            if constexpr (b == 4) slope(sb, db, wb, k0 + 32, t);
+          });
+    } else {
+      next.all();
+#pragma unroll 1
+      for (int h = 0; h < kPkChunk; h += 32) {
+        at_f16 s = at_zero16(), dp = at_zero16();
+        pk_scores2<T, DT, PF>(s, K + h * Tile::ROW, q, dp, V + h * Tile::ROW, go, at);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+        for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
+        if (k0 + h + 32 > wfull) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+        }
+        pk_accumulate<T, DT, PF>(dq, K + h * Tile::ROW, s, at);
       }
-      pk_accumulate<T, DT, PF>(dq, K + h * Tile::ROW, s, now);
     }
   };
-  if (chunks > 0) stage(K0, V0, 0);
+  if (chunks > 0) tile(X0, Y0, 0).all();
   for (int c = 0; c < chunks; c += 2) {
-    wait_vmem();
-    __syncthreads();
-    if (c + 1 < chunks) stage(K1, V1, c + 1);
-    chunk(K0, V0, c);
+    pk_barrier();
+    chunk(X0, Y0, c, tile(X1, Y1, c + 1));
     if (c + 1 >= chunks) break;
-    wait_vmem();
-    __syncthreads();
-    if (c + 2 < chunks) stage(K0, V0, c + 2);
-    chunk(K1, V1, c + 1);
+    pk_barrier();
+    chunk(X1, Y1, c + 1, tile(X0, Y0, c + 2));
   }
-  __syncthreads();
-  T* scratch = reinterpret_cast<T*>(wave == 0 ? K0 : wave == 1 ? V0 : wave == 2 ? K1 : V1);
+  pk_barrier();
+  unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
   pk_store<T, DT>(dq, p.scale, scratch, p.dim, lane,
                   [&](int r) { return wr0 + r < w.rows ? w.row(p, gq, kPkGQ, wr0 + r) : static_cast<T*>(nullptr); });
 }
@@ -746,15 +947,15 @@ struct PkKeys {
   int kv_head, part;
   int b0, b1;            // keys of the tile, in the sequence's range
   int m, n, q_first;     // keys and queries of the sequence, its first query row
-  int rows, shift;
-  int first, chunks;     // the first token that sees a key of the tile; chunks of rows (token and head) from there
+  int shift;
+  int first, chunks;     // the first token that sees a key of the tile; chunks of tokens from there
   int parts;             // workgroups that share them
-  __device__ PkKeys(const PackParams& p, const PkRows& walk, int lane) {
-    // key heads fastest (PkQueries); the first tiles, which the most queries of a causal sequence see, first
-    const int b = static_cast<int>(blockIdx.x), rest = b / p.kv_heads;
-    kv_head = b - rest * p.kv_heads;
-    part = rest % p.splits;
-    w = pk_place<kPkTile>(p.k_offsets, p.sequences, p.k_rows, 1, rest / p.splits, lane);
+  // b: tile and key head (fastest, as in PkQueries; the first tiles, which the most queries of a causal sequence
+  // see, first)
+  __device__ PkKeys(const PackParams& p, const PkRows& walk, int lane, int b, int part_) : part(part_) {
+    const int slot = b / p.kv_heads;
+    kv_head = b - slot * p.kv_heads;
+    w = pk_place(p.k_offsets, p.sequences, p.k_rows, 1, slot, lane);
     b0 = w.tile * kPkTile;
     b1 = min(b0 + kPkTile, w.own);
     m = n = q_first = 0;
@@ -763,11 +964,10 @@ struct PkKeys {
       q_first = min(max(p.q_offsets[w.seq], 0), p.q_rows);
       n = min(max(p.q_offsets[w.seq + 1], q_first), p.q_rows) - q_first;
     }
-    rows = n * p.group;
     shift = m - n;
     first = p.causal ? min(max(b0 - shift, 0), n) : 0;
-    chunks = b0 < m ? (rows - first * p.group + walk.rows - 1) / walk.rows : 0;
-    parts = min(max(chunks / kPkLeastPart, 1), p.splits);
+    chunks = b0 < m ? (n - first + walk.tokens - 1) / walk.tokens : 0;
+    parts = min(max((chunks + kPkPart - 1) / kPkPart, 1), p.splits);
   }
   template <typename T>
   __device__ T* row(const PackParams& p, T* base, int t, int j) const {
@@ -783,29 +983,35 @@ struct PkKeys {
 // head's group) that see them, 64 at a time. A tile that many rows see is shared by several workgroups,
 // whose sums pk_join_kv_kernel adds in their order.
 template <typename T, int DT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_kv_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
-  __shared__ __align__(16) unsigned char Q0[Tile::BYTES], G0[Tile::BYTES], Q1[Tile::BYTES], G1[Tile::BYTES];
+  // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
+  __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
   // of the tile's rows: the numbers that its scores and dP start from (bf16), or m, log2 l and delta (f32);
   // the keys that the row sees
   __shared__ __align__(16) float row_s[2][kPkChunk], row_d[2][kPkChunk], row_l[2][sizeof(T) == 2 ? 4 : kPkChunk];
   __shared__ __align__(16) int row_lim[2][kPkChunk];
   constexpr bool bf = sizeof(T) == 2;
-  constexpr int PF = bf ? 3 : 2;
+  constexpr int PF = bf && DT != 64 && DT != 128 ? 3 : 2;
+  // At 128 channels k, v, dk and dv take 192 of a wave's 256 registers. The last KEEP pieces of v wait in LDS: in
+  // registers the compiler spilled them, and each reload from scratch memory waited for the tile in flight.
+  constexpr int KEEP = bf && DT == 128 ? 3 : 0;
+  __shared__ __align__(16) unsigned char kept_rows[KEEP > 0 ? KEEP * kPkWaves * 1024 : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
-  const PkLane<T, DT> at(lane);
   const PkRows walk(p.group);
-  const PkKeys w(p, walk, lane);
+  // the parts of a tile are a grid of tiles apart: the first parts of all tiles start before any second
+  const int tiles = static_cast<int>(gridDim.x) / p.splits, my_part = static_cast<int>(blockIdx.x) / tiles;
+  const PkKeys w(p, walk, lane, static_cast<int>(blockIdx.x) - my_part * tiles, my_part);
   if (w.b0 >= w.w.own || w.part >= w.parts) return;
   T* gk = static_cast<T*>(p.gk);
   T* gv = static_cast<T*>(p.gv);
   if (w.chunks <= 0) {
-    if (gk != nullptr) pk_zero_rows<T, 256>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gk, kPkGK, j); });
-    if (gv != nullptr) pk_zero_rows<T, 256>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gv, kPkGV, j); });
+    if (gk != nullptr) pk_zero_rows<T>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gk, kPkGK, j); });
+    if (gv != nullptr) pk_zero_rows<T>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gv, kPkGV, j); });
     return;
   }
-  const int m = w.m, shift = w.shift, rows = w.rows;
+  const int m = w.m, shift = w.shift;
   const int wb0 = w.b0 + 32 * wave;
   PkRow<T, DT> k, v;
   {
@@ -813,6 +1019,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
     k.load(w.row(p, static_cast<const T*>(p.k), kPkK, min(kj, m - 1)), kj < m, p.dim, grp);
     v.load(w.row(p, static_cast<const T*>(p.v), kPkV, min(kj, m - 1)), kj < m, p.dim, grp);
   }
+  if constexpr (KEEP > 0)  // of this lane, so no barrier
+    for (int j = 0; j < KEEP; ++j) *reinterpret_cast<at_bf8*>(kept_rows + threadIdx.x * 16 + j * kPkWaves * 1024) = v.x[DT / 16 - KEEP + j];
   const T* qp = static_cast<const T*>(p.q) + w.q_first * p.st[kPkQ][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkQ][1];
   const T* gp = static_cast<const T*>(p.go) + w.q_first * p.st[kPkGO][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkGO][1];
   const float* sp = p.stats + 4 * (static_cast<int64_t>(w.q_first) * p.heads + w.kv_head * p.group);
@@ -821,29 +1029,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) dk[nd] = dv[nd] = at_zero16();
 
-  // Chunk c: its first row, and that row's token and head
-  auto place = [&](int c, int& r0, int& t0, int& g0) {
-    r0 = w.first * p.group + c * walk.rows;
-    t0 = walk.tokens != 0 ? w.first + c * walk.tokens : r0 / p.group;
-    g0 = walk.tokens != 0 ? 0 : r0 - t0 * p.group;
-  };
+  const int sq[2] = {static_cast<int>(p.st[kPkQ][0] * static_cast<int>(sizeof(T))), static_cast<int>(p.st[kPkQ][1] * static_cast<int>(sizeof(T)))};
+  const int sg[2] = {static_cast<int>(p.st[kPkGO][0] * static_cast<int>(sizeof(T))), static_cast<int>(p.st[kPkGO][1] * static_cast<int>(sizeof(T)))};
   // Tile c into Q, G and the row arrays `buf`: the rows' numbers by one wave each, a row a lane.
   auto stage = [&](unsigned char* Q, unsigned char* G, int buf, int c) {
-    int r0, t0, g0;
-    place(c, r0, t0, g0);
-    const int count = min(walk.rows, rows - r0);
-    constexpr int E = sizeof(T);
+    const int t0 = w.first + c * walk.tokens, count = min(walk.tokens, w.n - t0) * p.group;
     int thread = threadIdx.x;
     asm volatile("" : "+v"(thread));  // the pieces' offsets are formed anew (as in block)
     const __amdgpu_buffer_rsrc_t qs = pk_buffer(qp + t0 * p.st[kPkQ][0], kPkFar), gs = pk_buffer(gp + t0 * p.st[kPkGO][0], kPkFar);
 #pragma unroll
     for (int v = 0; v < Stream::NV; ++v) {
-      const int x = Stream::row(thread, v), t = walk.token(x, g0), g = walk.head(x, g0, t), ch = Stream::channel(thread, v);
+      const int x = Stream::row(thread, v), t = walk.token(x), g = x - t * p.group, ch = Stream::channel(thread, v);
       const bool ok = x < count && (p.dim == Tile::DP || ch < p.dim);
-      Stream::transfer(qs, ok ? (t * static_cast<int>(p.st[kPkQ][0]) + g * static_cast<int>(p.st[kPkQ][1]) + ch) * E : kPkFar, Q, v);
-      Stream::transfer(gs, ok ? (t * static_cast<int>(p.st[kPkGO][0]) + g * static_cast<int>(p.st[kPkGO][1]) + ch) * E : kPkFar, G, v);
+      Stream::transfer(qs, ok ? t * sq[0] + g * sq[1] + ch * static_cast<int>(sizeof(T)) : kPkFar, Q, v);
+      Stream::transfer(gs, ok ? t * sg[0] + g * sg[1] + ch * static_cast<int>(sizeof(T)) : kPkFar, G, v);
     }
-    const int x = thread & 63, t = walk.token(x, g0), g = walk.head(x, g0, t), o = x < count ? (t * p.heads + g) * 16 : kPkFar;
+    const int x = thread & 63, t = walk.token(x), g = x - t * p.group, o = x < count ? (t * p.heads + g) * 16 : kPkFar;
     const __amdgpu_buffer_rsrc_t ss = pk_buffer(sp + 4 * static_cast<int64_t>(t0) * p.heads, kPkFar);
     if (wave == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_s[buf]), 4, o + (bf ? 12 : 0), 0, 0, 0);
     if (wave == 1) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_d[buf]), 4, o + 8, 0, 0, 0);
@@ -851,29 +1052,82 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
     if (wave == 3) row_lim[buf][x] = x >= count ? 0 : p.causal ? min(max(t0 + t + shift + 1, 0), m) : m;
   };
   // One 32-row block; `all`: every row sees every key of the wave.
-  auto block = [&](bool all, PkLds Q, PkLds G, const float* rs, const float* rd, const float* rl, const int* lims) {
-    // formed anew in each step: kept over the loop, the offsets' dozen registers spill at 128 channels
-    PkLane<T, DT> now = at;
+  auto block = [&](bool all, PkLds Q, PkLds G, int h, const float* rs, const float* rd, const float* rl, const int* lims) {
+    // All that a lane's place gives is formed anew in each block, the operands' offsets in each phase: kept, they spill
+    // at 128 channels.
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, grp = lane >> 5, col = lane & 31;
+    PkLane<T, DT> now(lane);
+    now.row += h * Tile::ROW;
+    now.tr += h * Tile::ROW;
     asm volatile("" : "+v"(now.row), "+v"(now.tr));
+    // bf16: the matrix units start from the rows' numbers
+    auto start = [&](at_f16& x, const float* numbers) {
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const at_f4 a = bf ? *reinterpret_cast<const at_f4*>(numbers + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * c4 + j] = a[j];
+      }
+    };
+    uint32_t kept = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((MSDA_LDS unsigned char*)(kept_rows))) + thread * 16;
+    asm volatile("" : "+v"(kept));  // one register: the arrays' addresses do not fit an LDS instruction's offset
     at_f16 s, dp;
+    start(s, rs);
+    if (!bf) start(dp, rd);
+    using P = PkProducts<T, DT>;
+    const int kj = wb0 + col;
+    auto unseen = [&](at_f16& x) {  // pairs that are not seen weigh nothing
+      if (all) return;
 #pragma unroll
-    for (int c4 = 0; c4 < 4; ++c4) {  // bf16: the matrix units start from the rows' numbers
-      const at_f4 a = bf ? *reinterpret_cast<const at_f4*>(rs + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
-      const at_f4 b = bf ? *reinterpret_cast<const at_f4*>(rd + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[4 * c4 + j] = a[j];
-        dp[4 * c4 + j] = b[j];
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
+        x[4 * c4] = kj < lm.x ? x[4 * c4] : 0.0f;
+        x[4 * c4 + 1] = kj < lm.y ? x[4 * c4 + 1] : 0.0f;
+        x[4 * c4 + 2] = kj < lm.z ? x[4 * c4 + 2] : 0.0f;
+        x[4 * c4 + 3] = kj < lm.w ? x[4 * c4 + 3] : 0.0f;
       }
-    }
-    pk_scores2<T, DT, PF>(s, Q, k, dp, G, v, now);
+    };
     if constexpr (bf) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = at_exp2(s[i] * p.scale2);
-        dp[i] *= s[i];
-      }
+      // Phases of KS products: S, dP beside the weights, dv beside ds, dk.
+      constexpr int KS = P::kScores;
+      typename P::Weights w, ds;
+      at_bf8 last[KEEP > 0 ? KEEP : 1];
+      pk_pipe<4 * KS, PF>(
+          [&](auto i) {
+            constexpr int b = i / KS, t = i % KS;
+            const PkLds X = b == 0 || b == 3 ? Q : G;
+            if constexpr (t == 0) asm volatile("" : "+v"(now.row), "+v"(now.tr));
+            if constexpr (b < 2) return P::row_operand(X, now, t);
+            else return P::sum_operand(X, now, t);
+          },
+          [&](auto i, const auto& a) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (b == 0) P::score(s, a, k, t);
+            if constexpr (b == 1 && t < KS - KEEP) P::score(dp, a, v, t);
+            if constexpr (b == 1 && t >= KS - KEEP) P::score(dp, a, last[t - (KS - KEEP)]);
+            if constexpr (b == 2) P::sum(dv, a, w, t);
+            if constexpr (b == 3) P::sum(dk, a, ds, t);
+          },
+          [&](auto i) {
+            constexpr int b = i / KS, t = i % KS;
+            if constexpr (i == KS - 1) start(dp, rd);
+            if constexpr (KEEP > 0 && b == 1 && t + 2 >= KS - KEEP && t + 2 < KS)
+              last[t + 2 - (KS - KEEP)] = *reinterpret_cast<const MSDA_LDS at_bf8*>(reinterpret_cast<PkLds>(static_cast<uintptr_t>(kept)) + (t + 2 - (KS - KEEP)) * kPkWaves * 1024);
+            if constexpr (b == 1) pk_beside<KS, t>([&](int j) { s[j] = at_exp2(s[j] * p.scale2); });
+            if constexpr (b == 1 && t == KS - 1) {
+              unseen(s);
+              w.set(s);
+            }
+            if constexpr (b == 2) pk_beside<KS, t>([&](int j) { dp[j] *= s[j]; });
+            if constexpr (b == 2 && t == KS - 1) {
+              unseen(dp);
+              ds.set(dp);
+            }
+          });
     } else {
+      pk_scores2<T, DT, PF>(s, Q, k, dp, G, v, now);
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
         const int a = 8 * c4 + 4 * grp;
@@ -886,47 +1140,32 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
           dp[i] = s[i] * (dp[i] - dd[j]);
         }
       }
+      unseen(s);
+      unseen(dp);
+      pk_accumulate2<T, DT, PF>(dv, G, s, dk, Q, dp, now);
     }
-    if (!all) {
-      const int kj = wb0 + col;
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {
-        const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
-        const int lim[4] = {lm.x, lm.y, lm.z, lm.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * c4 + j;
-          s[i] = kj < lim[j] ? s[i] : 0.0f;
-          dp[i] = kj < lim[j] ? dp[i] : 0.0f;
-        }
-      }
-    }
-    pk_accumulate2<T, DT, PF>(dv, G, s, dk, Q, dp, now);
   };
   auto chunk = [&](const unsigned char* Qb, const unsigned char* Gb, int buf, int c) {
     PkLds Q = (PkLds)(Qb), G = (PkLds)(Gb);
-    int r0, t0, g0;
-    place(c, r0, t0, g0);
-    const int r1 = min(r0 + walk.rows, rows), t1 = walk.tokens != 0 ? min(t0 + walk.tokens, w.n) : (r1 - 1) / p.group + 1;
+    const int t0 = w.first + c * walk.tokens, t1 = min(t0 + walk.tokens, w.n), count = (t1 - t0) * p.group;
     if (wb0 >= m || (p.causal && t1 + shift <= wb0)) return;
     // every row sees every key of the wave
-    const bool full = r0 + kPkChunk == r1 && wb0 + 32 <= m && (!p.causal || t0 + shift >= wb0 + 31);
+    const bool full = __builtin_amdgcn_readfirstlane(count == kPkChunk && wb0 + 32 <= m && (!p.causal || t0 + shift >= wb0 + 31)) != 0;
 #pragma unroll 1
-    for (int h = 0; h < r1 - r0; h += 32)
-      block(full, Q + h * Tile::ROW, G + h * Tile::ROW, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h);
+    for (int h = 0; h < count; h += 32)
+      block(full, Q, G, h, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h);
   };
-  if (c0 < c1) stage(Q0, G0, 0, c0);
+  if (c0 < c1) stage(X0, Y0, 0, c0);
   for (int c = c0; c < c1; c += 2) {
-    wait_vmem();
-    __syncthreads();
-    if (c + 1 < c1) stage(Q1, G1, 1, c + 1);
-    chunk(Q0, G0, 0, c);
+    pk_barrier();
+    if (c + 1 < c1) stage(X1, Y1, 1, c + 1);
+    chunk(X0, Y0, 0, c);
     if (c + 1 >= c1) break;
-    wait_vmem();
-    __syncthreads();
-    if (c + 2 < c1) stage(Q0, G0, 0, c + 2);
-    chunk(Q1, G1, 1, c + 1);
+    pk_barrier();
+    if (c + 2 < c1) stage(X0, Y0, 0, c + 2);
+    chunk(X1, Y1, 1, c + 1);
   }
+  pk_barrier();
   if (w.parts > 1) {
     const int kj = wb0 + col;
     if (kj >= w.b1) return;
@@ -943,8 +1182,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
       }
     return;
   }
-  __syncthreads();
-  T* scratch = reinterpret_cast<T*>(wave == 0 ? Q0 : wave == 1 ? G0 : wave == 2 ? Q1 : G1);
+  unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
   // keys from m on (rows of the range behind the sequence's keys) hold zeros: their scores never counted
   if (gk != nullptr)
     pk_store<T, DT>(dk, p.scale, scratch, p.dim, lane, [&](int r) { return wb0 + r < w.b1 ? w.row(p, gk, kPkGK, wb0 + r) : static_cast<T*>(nullptr); });
@@ -952,22 +1190,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) pk_bwd_kv_kernel(
     pk_store<T, DT>(dv, 1.0f, scratch, p.dim, lane, [&](int r) { return wb0 + r < w.b1 ? w.row(p, gv, kPkGV, wb0 + r) : static_cast<T*>(nullptr); });
 }
 
-// The sums of a tile's parts, in their order (the grid of pk_bwd_kv_kernel with one part).
+// The sums of a tile's parts, in their order: kPkJoin workgroups a tile, of all key heads (which have as many parts).
 template <typename T>
 __global__ void __launch_bounds__(256) pk_join_kv_kernel(const PackParams p) {
-  PackParams one = p;
-  one.splits = 1;
-  const PkKeys w(one, PkRows(p.group), threadIdx.x & 63);
-  const int parts = min(max(w.chunks / kPkLeastPart, 1), p.splits);
-  if (w.b0 >= w.w.own || parts == 1) return;
-  const int pieces = p.dim / 4;
-  for (int i = threadIdx.x; i < 2 * (w.b1 - w.b0) * pieces; i += 256) {
-    const int which = i & 1, key = w.b0 + (i >> 1) / pieces, ch = 4 * ((i >> 1) % pieces);
+  const int tile = static_cast<int>(blockIdx.x) / kPkJoin, share = kPkTile / kPkJoin;
+  PkKeys w(p, PkRows(p.group), threadIdx.x & 63, tile * p.kv_heads, 0);
+  if (w.parts == 1) return;
+  const int first = w.b0 + share * (static_cast<int>(blockIdx.x) % kPkJoin), keys = min(share, w.b1 - first), pieces = p.dim / 4;
+  for (int i = threadIdx.x; i < 2 * keys * p.kv_heads * pieces; i += 256) {
+    const int r = i / pieces, ch = 4 * (i - r * pieces), row = r >> 1, which = r & 1, key = row / p.kv_heads;
+    w.kv_head = row - key * p.kv_heads;
     T* base = static_cast<T*>(which == 0 ? p.gk : p.gv);
     if (base == nullptr) continue;
     at_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < parts; ++s) a += *reinterpret_cast<const at_f4*>(p.part_kv + w.part_row(p, 2 * s + which, key) * p.dim + ch);
-    pk_put4(w.row(p, base, which == 0 ? kPkGK : kPkGV, key) + ch, which == 0 ? a * p.scale : a);
+#pragma unroll 4
+    for (int s = 0; s < w.parts; ++s) a += *reinterpret_cast<const at_f4*>(p.part_kv + w.part_row(p, 2 * s + which, first + key) * p.dim + ch);
+    pk_put4(w.row(p, base, which == 0 ? kPkGK : kPkGV, first + key) + ch, which == 0 ? a * p.scale : a);
   }
 }
 

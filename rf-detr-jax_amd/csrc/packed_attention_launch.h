@@ -12,7 +12,7 @@ template <typename K>
 int pk_launch(K kernel, int64_t grid, const msda::PackParams& p, hipStream_t st, const char* what) {
   if (grid >= (int64_t{1} << 31)) return fail(MSDA_ERR_UNSUPPORTED, "packed attention: too many workgroups");
   if (grid == 0) return MSDA_OK;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * msda::kPkWaves), 0, st, p);
   return check_launch(what);
 }
 
@@ -20,22 +20,22 @@ template <typename T, int DT>
 int pk_fwd(const msda::PackParams& p, hipStream_t st) {
   const int rc = pk_launch(msda::pk_fwd_kernel<T, DT>, static_cast<int64_t>(p.slots) * p.splits * p.kv_heads, p, st, "packed attention forward");
   if (rc != MSDA_OK || p.splits == 1) return rc;
-  return pk_launch(msda::pk_join_kernel<T>, (static_cast<int64_t>(p.q_rows) * p.heads + 15) / 16, p, st, "packed attention forward (join)");
+  constexpr int LPR = DT <= 64 ? 16 : 32;
+  return pk_launch(msda::pk_join_kernel<T, LPR>, (static_cast<int64_t>(p.q_rows) * p.heads + 256 / LPR - 1) / (256 / LPR), p, st,
+                   "packed attention forward (join)");
 }
 
 // q_slots, k_slots: tiles of the queries' and of the keys' side; p.splits: parts of a key tile
 template <typename T, int DT>
 int pk_bwd(msda::PackParams p, int q_slots, int k_slots, hipStream_t st) {
-  msda::PackParams q = p;
-  q.slots = q_slots;
-  q.splits = 1;
-  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT>, static_cast<int64_t>(q_slots) * p.kv_heads, q, st, "packed attention backward (queries)");
+  p.slots = q_slots;
+  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT>, static_cast<int64_t>(q_slots) * p.kv_heads, p, st, "packed attention backward (queries)");
   if (rc != MSDA_OK || (p.gk == nullptr && p.gv == nullptr)) return rc;
   p.slots = k_slots;
   rc = pk_launch(msda::pk_bwd_kv_kernel<T, DT>, static_cast<int64_t>(k_slots) * p.splits * p.kv_heads, p, st,
                  "packed attention backward (keys, values)");
   if (rc != MSDA_OK || p.splits == 1) return rc;
-  return pk_launch(msda::pk_join_kv_kernel<T>, static_cast<int64_t>(k_slots) * p.kv_heads, p, st, "packed attention backward (join)");
+  return pk_launch(msda::pk_join_kv_kernel<T>, static_cast<int64_t>(k_slots) * msda::kPkJoin, p, st, "packed attention backward (join)");
 }
 
 template <typename T>
