@@ -444,14 +444,16 @@ int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float
  * for more rows than it holds). Query t of a sequence sees its keys j < m, with `causal` those with
  * j <= t + m - n: the last query sees every key, so one new token over a cache of m keys is n = 1.
  *   out = softmax(scale q k^T over the seen keys) v, 0 where no key is seen.
- * A pair that is not seen takes no part, whatever its rows hold. Rows of out and of the gradients that
+ * A pair that is not seen takes no part, whatever its rows hold (infinities and NaN too). Rows of out and of the gradients that
  * belong to no sequence, and of grad_k and grad_v from the m-th of a sequence on, are written as zeros.
  * Offsets and lengths are clamped to the tensors' rows: others than rising ones give unspecified
  * values, never an access out of bounds.
  *
  * head_dim: a multiple of 8, at most 128. `strides` holds the element strides (row, head) of each
  * tensor; channels are contiguous, and rows start on 16-byte boundaries (bases, and strides in bytes, are
- * multiples of 16), head_dim to 2^22 elements apart, a row's heads within 2^23 elements. scale > 0. q_rows * heads / kv_heads and k_rows below 2^31 less 128 rows a sequence.
+ * multiples of 16), head_dim to 2^22 elements apart, q's and grad_out's heads of a key head within
+ * 2^27 elements. At most 64 query heads to a key head. scale: 2^-64 to 2^64. q_rows * heads / kv_heads and k_rows below 2^31 less 128
+ * rows a sequence.
  * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
  * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them and uses entries 2
  * and 3 between its kernels. May be NULL in a forward whose backward is not wanted.

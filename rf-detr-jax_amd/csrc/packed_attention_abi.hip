@@ -97,10 +97,12 @@ int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
     if (strides[i] < 0 || strides[i] % e != 0)
       return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: stride %d (%lld) must be a non-negative multiple of 16 bytes", i,
                   static_cast<long long>(strides[i]));
-  for (int i = 0; i < ntensors; ++i)  // a tile's byte offsets are formed in 31 bits, its end from its rows
+  // A tile's byte offsets are formed in 31 bits, its end from its rows: 64 rows, in the backward those of a group's heads
+  const int64_t group = s.heads == 0 ? 1 : s.heads / s.kv_heads;
+  for (int i = 0; i < ntensors; ++i)
     if (strides[2 * i] != 0 || strides[2 * i + 1] != 0)
-      if (strides[2 * i] < s.head_dim || strides[2 * i] >= (int64_t{1} << 22) || strides[2 * i + 1] * s.heads >= (int64_t{1} << 23))
-        return fail(MSDA_ERR_UNSUPPORTED, "packed attention: strides %lld, %lld of tensor %d: rows must lie head_dim to 2^22 elements apart, a row's heads within 2^23",
+      if (strides[2 * i] < s.head_dim || strides[2 * i] >= (int64_t{1} << 22) || ((i == 0 || i == 4) && strides[2 * i + 1] >= (int64_t{1} << 27) / group))
+        return fail(MSDA_ERR_UNSUPPORTED, "packed attention: strides %lld, %lld of tensor %d: rows must lie head_dim to 2^22 elements apart, the heads of a group within 2^27",
                     static_cast<long long>(strides[2 * i]), static_cast<long long>(strides[2 * i + 1]), i);
   return MSDA_OK;
 }
@@ -128,7 +130,8 @@ msda::PackParams pk_params(const PackShape& s, const int32_t* q_offsets, const i
 }
 
 int pk_scale(float scale) {
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: scale %g must be positive and finite", static_cast<double>(scale));
+  // (the backward divides by it)
+  if (!(scale >= 0x1p-64f && scale <= 0x1p64f)) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: scale %g must lie from 2^-64 to 2^64", static_cast<double>(scale));
   return MSDA_OK;
 }
 

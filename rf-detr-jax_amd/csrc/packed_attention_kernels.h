@@ -437,7 +437,7 @@ __device__ __forceinline__ void pk_barrier() {
 
 // The transfers of one 64-row tile by the workgroup: piece u is row u / CPR, slot u % CPR,
 // which holds the row's chunk slot ^ swizzle(row). A thread's pieces are kStep rows apart. Row strides are
-// below 2^22 elements (the host's check), so a tile's offsets fit 31 bits.
+// below 2^22 elements, a group's heads within 2^27 (the host's checks), so a tile's offsets fit 31 bits.
 template <typename T, int DT>
 struct PkStream {
   using Tile = PkTile<T, DT>;
@@ -479,6 +479,52 @@ struct PkStream {
     }
   };
 };
+
+// A causal chunk that not every row of the workgroup sees whole: the weights of its unseen pairs are zeros, and
+// zero times an infinity or NaN of an unseen row would reach the sums. So such a tile is searched first (one
+// round of 16-byte reads and a barrier, for the chunks on the diagonal alone), values that are no finite numbers
+// become zeros, and the rows that held some are marked in `bad`, for those who see them.
+typedef uint16_t pk_u2 __attribute__((ext_vector_type(2)));
+template <typename T, int DT>
+__device__ __forceinline__ void pk_settle(unsigned char* tile, uint32_t* bad) {
+  using Tile = PkTile<T, DT>;
+  constexpr bool bf = sizeof(T) == 2;
+  constexpr int N = Tile::BYTES / (16 * 64 * kPkWaves);
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // addresses formed here, not kept in registers from before the loop
+  uint4* mine = reinterpret_cast<uint4*>(tile) + thread;
+  // the largest magnitude, as an integer: of the upper and of the lower halves in bf16
+  uint32_t most = 0;
+  auto larger = [](uint32_t a, uint32_t b) {
+    if constexpr (bf) return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pk_u2, a), __builtin_bit_cast(pk_u2, b)));
+    else return max(a, b);
+  };
+  constexpr uint32_t kMagnitude = bf ? 0x7fff7fffu : 0x7fffffffu;
+#pragma unroll 1  // (unrolled, the key side's kernel spills at 128 channels: 277 us for 264 over 8,848 tokens of 16 heads)
+  for (int v = 0; v < N; ++v) {
+    const uint4 x = mine[64 * kPkWaves * v];
+    most = larger(larger(larger(most, x.x & kMagnitude), larger(x.y & kMagnitude, x.z & kMagnitude)), x.w & kMagnitude);
+  }
+  if (most < 0x7f800000u && (!bf || (most & 0xffffu) < 0x7f80u)) return;
+#pragma unroll 1
+  for (int v = 0; v < N; ++v) {
+    const int r = (thread + 64 * kPkWaves * v) / Tile::CPR;
+    auto settled = [](uint32_t w) {
+      if ((w & 0x7f800000u) == 0x7f800000u) w &= bf ? 0xffffu : 0u;
+      if (bf && (w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+      return w;
+    };
+    const uint4 x = mine[64 * kPkWaves * v], y = {settled(x.x), settled(x.y), settled(x.z), settled(x.w)};
+    if (x.x == y.x && x.y == y.y && x.z == y.z && x.w == y.w) continue;
+    mine[64 * kPkWaves * v] = y;
+    atomicOr(bad + (r >> 5), 1u << (r & 31));
+  }
+}
+__device__ __forceinline__ uint64_t pk_settled(const uint32_t* bad) {
+  __syncthreads();
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bad[1])))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bad[0])));
+}
 
 // The rows r = t G + g of a key head's queries (G <= 64), in chunks of whole tokens, at most 64 rows: a row's
 // place in its chunk gives its token and head whatever the chunk.
@@ -555,6 +601,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
   __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
+  __shared__ uint32_t bad[2][2];  // pk_settle's rows of a chunk, by turns
+  if (threadIdx.x < 4) bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
@@ -576,6 +624,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   const int lim = valid ? w.seen(p, ri) : 0;
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;  // keys that the wave sees
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                  // that every row of it sees
+  const int all = w.seen(p, w.r0);                                           // that every row of the workgroup sees
   const int per = (chunks + parts - 1) / parts, c0 = w.split * per, c1 = min(chunks, c0 + per);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
@@ -591,9 +640,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   auto tile = [&](unsigned char* K, unsigned char* V, int c) {  // behind the last: zeros, which nothing reads
     return Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < c1 ? w.m : 0, p.dim);
   };
-  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c, const Pair& next) {
+  bool sick = false;  // pk_settle found some
+  auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
+    if (min(k0 + kPkChunk, w.m) > all) {
+      if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
+      pk_settle<T, DT>(Vb, bad[turn]);
+      sick = sick || pk_settled(bad[turn]) != 0;
+    }
     if (k0 >= wend) {
       next.all();
       return;
@@ -704,10 +759,26 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   if (c0 < c1) tile(X0, Y0, c0).all();
   for (int c = c0; c < c1; c += 2) {
     pk_barrier();  // tile c is there, and every wave is done with tile c - 1
-    chunk(X0, Y0, c, tile(X1, Y1, c + 1));
+    chunk(X0, Y0, 0, c, tile(X1, Y1, c + 1));
     if (c + 1 >= c1) break;
     pk_barrier();
-    chunk(X1, Y1, c + 1, tile(X0, Y0, c + 2));
+    chunk(X1, Y1, 1, c + 1, tile(X0, Y0, c + 2));
+  }
+  if (sick) {  // infinities and NaN of those chunks for the rows that see them
+#pragma unroll 1
+    for (int j = max(all / kPkChunk, c0) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
+#pragma unroll
+      for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int ch = 32 * nd + 8 * (i >> 2) + 4 * grp + (i & 3);
+          float x = 0.0f;
+          if (ch < p.dim) {
+            if constexpr (sizeof(T) == 2) x = bf16_to_f32(vp[j * p.st[kPkV][0] + ch]);
+            else x = vp[j * p.st[kPkV][0] + ch];
+          }
+          if (x - x != 0.0f) o[nd][i] += x;
+        }
   }
   l = at_sum_halves(l);
   pk_barrier();  // the tiles hold the waves' scratch from here
@@ -803,6 +874,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
   __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
+  __shared__ uint32_t bad[2][2];  // pk_settle's rows of a chunk, by turns
+  if (threadIdx.x < 4) bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
@@ -820,6 +893,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   const int end = w.seen(p, r1 - 1);
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;
+  const int all = w.seen(p, w.r0);  // keys that every row of the workgroup sees
   const int chunks = (end + kPkChunk - 1) / kPkChunk;
   PkRow<T, DT> q, go;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, rc), valid, p.dim, grp);
@@ -858,9 +932,16 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   auto tile = [&](unsigned char* K, unsigned char* V, int c) {  // behind the last: zeros, which nothing reads
     return Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < chunks ? w.m : 0, p.dim);
   };
-  auto chunk = [&](const unsigned char* Kb, const unsigned char* Vb, int c, const Pair& next) {
+  float factor = p.scale;  // NaN: the row sees a key that is not finite
+  auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
+    if (min(k0 + kPkChunk, w.m) > all) {
+      if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
+      pk_settle<T, DT>(Kb, bad[turn]);
+      const uint64_t sick = pk_settled(bad[turn]);
+      if (sick != 0 && k0 + static_cast<int>(__builtin_ctzll(sick)) < lim) factor = NAN;
+    }
     if (k0 >= wend) {
       next.all();
       return;
@@ -929,14 +1010,14 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   if (chunks > 0) tile(X0, Y0, 0).all();
   for (int c = 0; c < chunks; c += 2) {
     pk_barrier();
-    chunk(X0, Y0, c, tile(X1, Y1, c + 1));
+    chunk(X0, Y0, 0, c, tile(X1, Y1, c + 1));
     if (c + 1 >= chunks) break;
     pk_barrier();
-    chunk(X1, Y1, c + 1, tile(X0, Y0, c + 2));
+    chunk(X1, Y1, 1, c + 1, tile(X0, Y0, c + 2));
   }
   pk_barrier();
   unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
-  pk_store<T, DT>(dq, p.scale, scratch, p.dim, lane,
+  pk_store<T, DT>(dq, factor, scratch, p.dim, lane,
                   [&](int r) { return wr0 + r < w.rows ? w.row(p, gq, kPkGQ, wr0 + r) : static_cast<T*>(nullptr); });
 }
 
@@ -988,6 +1069,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
   __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
+  __shared__ uint32_t bad[2][2];  // pk_settle's rows of a chunk, by turns
+  if (threadIdx.x < 4) bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   // of the tile's rows: the numbers that its scores and dP start from (bf16), or m, log2 l and delta (f32);
   // the keys that the row sees
   __shared__ __align__(16) float row_s[2][kPkChunk], row_d[2][kPkChunk], row_l[2][sizeof(T) == 2 ? 4 : kPkChunk];
@@ -1145,6 +1228,17 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       pk_accumulate2<T, DT, PF>(dv, G, s, dk, Q, dp, now);
     }
   };
+  bool spoilt = false;  // the lane's key is seen by a row that is not finite
+  auto settle = [&](unsigned char* Q, unsigned char* G, int buf, int c) {
+    const int t0 = w.first + c * walk.tokens;
+    if (!p.causal || t0 + shift >= min(w.b1, m) - 1) return;  // every row sees every key
+    if (threadIdx.x < 2) bad[buf ^ 1][threadIdx.x] = 0;
+    pk_settle<T, DT>(Q, bad[buf]);
+    pk_settle<T, DT>(G, bad[buf]);
+    const uint64_t sick = pk_settled(bad[buf]);
+    // rows see more keys the later they come
+    if (sick != 0) spoilt = spoilt || wb0 + col < row_lim[buf][63 - static_cast<int>(__builtin_clzll(sick))];
+  };
   auto chunk = [&](const unsigned char* Qb, const unsigned char* Gb, int buf, int c) {
     PkLds Q = (PkLds)(Qb), G = (PkLds)(Gb);
     const int t0 = w.first + c * walk.tokens, t1 = min(t0 + walk.tokens, w.n), count = (t1 - t0) * p.group;
@@ -1158,14 +1252,27 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   if (c0 < c1) stage(X0, Y0, 0, c0);
   for (int c = c0; c < c1; c += 2) {
     pk_barrier();
+    settle(X0, Y0, 0, c);
     if (c + 1 < c1) stage(X1, Y1, 1, c + 1);
     chunk(X0, Y0, 0, c);
     if (c + 1 >= c1) break;
     pk_barrier();
+    settle(X1, Y1, 1, c + 1);
     if (c + 2 < c1) stage(X0, Y0, 0, c + 2);
     chunk(X1, Y1, 1, c + 1);
   }
   pk_barrier();
+  if (__any(spoilt || wb0 + col >= m)) {  // keys from m on (rows of the range behind the sequence's keys) get zeros
+    const float none = spoilt ? NAN : 0.0f;
+    const bool keep = !spoilt && wb0 + col < m;
+#pragma unroll
+    for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        dk[nd][i] = keep ? dk[nd][i] : none;
+        dv[nd][i] = keep ? dv[nd][i] : none;
+      }
+  }
   if (w.parts > 1) {
     const int kj = wb0 + col;
     if (kj >= w.b1) return;
@@ -1183,7 +1290,6 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     return;
   }
   unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
-  // keys from m on (rows of the range behind the sequence's keys) hold zeros: their scores never counted
   if (gk != nullptr)
     pk_store<T, DT>(dk, p.scale, scratch, p.dim, lane, [&](int r) { return wb0 + r < w.b1 ? w.row(p, gk, kPkGK, wb0 + r) : static_cast<T*>(nullptr); });
   if (gv != nullptr)

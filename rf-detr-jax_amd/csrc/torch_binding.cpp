@@ -540,7 +540,7 @@ variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
   variable_list defined;
   for (const Tensor& g : grads)
-    if (g.defined()) defined.push_back(g);
+    if (g.defined()) defined.push_back(g.requires_grad_(true));  // (the node is kept only where an input has one)
   if (defined.empty()) return grads;
   const auto node = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate the gradients of ") + what,
                                                                     static_cast<int64_t>(defined.size()));
@@ -558,11 +558,13 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
-// [rows, heads, D] as the packed kernels read it: channels contiguous, rows on 16-byte boundaries and apart
-bool packed_rows(const Tensor& t) {
+// [rows, heads, D] as the packed kernels read it: channels contiguous, rows on 16-byte boundaries and apart, the
+// heads of a group (queries and their cotangents) within 2^27 elements
+bool packed_rows(const Tensor& t, int64_t group = 1) {
   const int64_t step = 16 / t.element_size();
   return t.dim() == 3 && t.stride(2) == 1 && t.stride(0) % step == 0 && t.stride(1) % step == 0 && t.stride(0) >= t.size(2) &&
-         t.stride(0) < (int64_t{1} << 22) && t.stride(1) * t.size(1) < (int64_t{1} << 22) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+         t.stride(0) < (int64_t{1} << 22) && (group == 1 || t.stride(1) < (int64_t{1} << 27) / group) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
 struct Packed {  // one call's sizes
@@ -609,8 +611,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const at::ScalarType type = grads[0].scalar_type();
-    const auto rows = [&](const Tensor& t) {
-      return t.defined() && t.is_cuda() && t.scalar_type() == type && packed_rows(t) ? t : aligned(restored(t, type));
+    const auto rows = [&](const Tensor& t) {  // 64 query heads share a key head at most
+      return t.defined() && t.is_cuda() && t.scalar_type() == type && packed_rows(t, 64) ? t : aligned(restored(t, type));
     };
     const Tensor q = rows(saved[0]), k = rows(saved[1]), v = rows(saved[2]), out = aligned(restored(saved[3], type));
     const Tensor rest = saved[4].defined() ? aligned(restored(saved[4], type)) : Tensor();
@@ -618,7 +620,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     const Tensor key_lengths = saved[8].defined() ? restored(saved[8], at::kInt) : Tensor(), g = rows(grads[0]);
     saved_as(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && q.sizes() == g.sizes() && out.sizes() == q.sizes() &&
              (!rest.defined() || rest.sizes() == q.sizes()) && stats.sizes().equals({q.size(0), q.size(1), 4}) && k.size(2) == q.size(2) &&
-             q.size(1) % k.size(1) == 0 && offsets.dim() == 1 && offsets.numel() >= 1 && key_offsets.sizes() == offsets.sizes() &&
+             k.size(1) != 0 && q.size(1) % k.size(1) == 0 && offsets.dim() == 1 && offsets.numel() >= 1 && key_offsets.sizes() == offsets.sizes() &&
              (!key_lengths.defined() || (key_lengths.dim() == 1 && key_lengths.numel() == offsets.numel() - 1)));
     for (const Tensor* t : {&k, &v, &out, &rest, &stats, &offsets, &key_offsets, &key_lengths, &g})
       saved_as(!t->defined() || t->device() == q.device());
@@ -658,18 +660,19 @@ py::object packed_attention(const py::handle& q, const py::handle& k, const py::
     return py::none();
   if (!value_type(*a) || a->dim() != 3) return py::none();
   for (const Tensor* t : {a, b, c}) {
-    if (t->scalar_type() != a->scalar_type() || t->device() != a->device() || !packed_rows(*t)) return py::none();
+    if (t->scalar_type() != a->scalar_type() || t->device() != a->device() || !packed_rows(*t, t == a ? 64 : 1)) return py::none();
     for (int64_t n : t->sizes())
       if (n >= (int64_t{1} << 31)) return py::none();
   }
-  if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || a->size(1) % b->size(1) != 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
+  if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || b->size(1) == 0 || a->size(1) % b->size(1) != 0 || a->size(1) > 64 * b->size(1) ||
+      a->size(2) == 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
     return py::none();
   for (const Tensor* t : {o, ko, kl})
     if (t != nullptr && (t->dim() != 1 || t->scalar_type() != at::kInt || t->device() != a->device() || !t->is_contiguous())) return py::none();
   if (ko->numel() != o->numel() || (kl != nullptr && kl->numel() != o->numel() - 1)) return py::none();
   if (!scale.is_none() && !PyFloat_CheckExact(scale.ptr())) return py::none();
   const double s = scale.is_none() ? 1.0 / std::sqrt(static_cast<double>(a->size(2))) : PyFloat_AS_DOUBLE(scale.ptr());
-  if (!(s > 0.0) || !std::isfinite(static_cast<float>(s)) || static_cast<float>(s) == 0.0f) return py::none();
+  if (!(s >= 0x1p-64 && s <= 0x1p64)) return py::none();
   const Packed p(*a, *b, *o, causal, s);
   if (!wants_grad({a, b, c})) return py::cast(packed_forward(*a, *b, *c, *o, *ko, kl != nullptr ? *kl : Tensor(), p, false)[0]);
   return py::cast(PackedAttention::apply(*a, *b, *c, *o, *ko, kl != nullptr ? std::optional<Tensor>(*kl) : std::nullopt, p));

@@ -32,10 +32,11 @@ def _stream(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def _rows16(t):
-    """``t`` as the kernels read it: channels contiguous, rows on 16-byte boundaries and apart (a copy where they are not)."""
+def _rows16(t, group=1):
+    """``t`` as the kernels read it: channels contiguous, rows on 16-byte boundaries and apart, the heads of a group
+    within 2^27 elements (a copy where they are not)."""
     step, (row, head, channel) = 16 // t.element_size(), t.stride()
-    if channel != 1 or row % step or head % step or t.data_ptr() % 16 or not t.shape[2] <= row < 1 << 22 or head * t.shape[1] >= 1 << 22:
+    if channel != 1 or row % step or head % step or t.data_ptr() % 16 or not t.shape[2] <= row < 1 << 22 or (group > 1 and head * group >= 1 << 27):
         t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
     return t
 
@@ -58,6 +59,8 @@ def _check(q, k, v):
             raise TypeError(f"attention dtype {t.dtype} is not supported (float32 or bfloat16)")
         if t.dim() != 3:
             raise ValueError(f"{name} must be [rows, heads, D], got {tuple(t.shape)}")
+        if max(t.shape) >= 1 << 31:
+            raise ValueError(f"{name} is too large: {tuple(t.shape)}")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k and v must be of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     if k.device != q.device or v.device != q.device:
@@ -66,6 +69,8 @@ def _check(q, k, v):
         raise ValueError(f"q [T, H, D] and k, v [S, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.shape[1] and (k.shape[1] == 0 or q.shape[1] % k.shape[1]):
         raise ValueError(f"{q.shape[1]} query heads do not divide into {k.shape[1]} key heads")
+    if q.shape[1] > 64 * k.shape[1]:
+        raise ValueError(f"at most 64 query heads may share a key head, got {q.shape[1]} and {k.shape[1]}")
     if q.shape[2] % 8 or not 8 <= q.shape[2] <= 128:
         raise ValueError(f"head_dim must be a multiple of 8 up to 128, got {q.shape[2]}")
 
@@ -87,8 +92,8 @@ class _Sequences:
 
 def _scale(scale, head_dim):
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        raise ValueError(f"scale must lie from 2^-64 to 2^64, got {scale}")
     return scale
 
 
@@ -138,7 +143,7 @@ def packed_attention_forward(q, k, v, offsets, key_offsets=None, key_lengths=Non
     left, ``[T, H, D]`` (else None)."""
     _check(q, k, v)
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
-    out, rest, stats = _forward(*(_rows16(t) for t in (q, k, v)), seq, causal, _scale(scale, q.shape[2]), True)
+    out, rest, stats = _forward(_rows16(q, 64), _rows16(k), _rows16(v), seq, causal, _scale(scale, q.shape[2]), True)
     return out, (stats, rest)
 
 
@@ -154,7 +159,7 @@ def packed_attention_backward(q, k, v, out, saved, grad_out, offsets, key_offset
         raise ValueError("out, its statistics and grad_out must be on the queries' device")
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
     # hooks on saved tensors may hand back other types and layouts: as the kernels read them
-    q, k, v, out, grad_out = (_rows16(t.to(q.dtype)) for t in (q, k, v, out, grad_out))
+    q, k, v, out, grad_out = (_rows16(t.to(q.dtype), 64) for t in (q, k, v, out, grad_out))
     if rest is not None:
         out, rest = out.contiguous(), rest.to(q.dtype).contiguous()  # of the same strides
     stats = stats.to(torch.float32).contiguous()
@@ -168,7 +173,7 @@ class _PackedAttention(torch.autograd.Function):
         seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
         scale = _scale(scale, q.shape[2])
         needs = any(ctx.needs_input_grad[:3])
-        q, k, v = (_rows16(t) for t in (q, k, v))
+        q, k, v = _rows16(q, 64), _rows16(k), _rows16(v)
         out, rest, stats = _forward(q, k, v, seq, causal, scale, needs)
         if needs:
             ctx.save_for_backward(q, k, v, out, rest, stats, offsets, key_offsets, key_lengths)
@@ -190,8 +195,8 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
 
     Args:
         q: ``[T, H, D]``, the queries of all sequences behind one another. ``D`` is a multiple of 8 up to 128.
-        k, v: ``[S, Hk, D]``; query head ``h`` reads key head ``h // (H // Hk)``. All three may be views with
-            larger row and head strides (slices of one projection).
+        k, v: ``[S, Hk, D]``; query head ``h`` reads key head ``h // (H // Hk)``, which at most 64 share. All three
+            may be views with larger row and head strides (slices of one projection).
         offsets: int32 ``[N + 1]`` on the same GPU: sequence ``i`` holds the queries ``offsets[i]`` to
             ``offsets[i + 1] - 1`` (none, one or many).
         key_offsets: the same for its keys; ``offsets`` when None.
@@ -199,10 +204,12 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
             for more); all of them when None.
         causal: query ``t`` of ``n`` sees the keys ``j <= t + m - n`` of ``m``, so that the last query sees every
             key; False: every key of its sequence.
-        scale: of the scores, positive; ``D ** -0.5`` when None.
+        scale: of the scores, from ``2 ** -64`` to ``2 ** 64``; ``D ** -0.5`` when None.
 
     A query that sees no key gives zeros. Rows of the result, and of the gradients, outside every sequence are
-    zeros. Pairs that are not seen take no part, whatever their rows hold. Offsets must rise and lie within the
+    zeros. Pairs that are not seen take no part, whatever their rows hold (infinities and NaN too; a key that is not
+    finite makes the gradients of the queries that see it NaN, a query that is not, or its cotangent, those of the keys
+    it sees). Offsets must rise and lie within the
     rows; they are not read back, and wrong ones give unspecified values.
 
     Raises:

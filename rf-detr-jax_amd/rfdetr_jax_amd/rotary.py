@@ -111,6 +111,8 @@ def rotary_embed(q, k, positions, sections, base=10000.0, shared_frequencies=Fal
             raise TypeError(f"{name} dtype {t.dtype} is not supported (float32 or bfloat16)")
         if t.dim() < 2:
             raise ValueError(f"{name} must be [..., heads, D], got {tuple(t.shape)}")
+        if t.numel() >= (1 << 31) * max(t.shape[-1] * t.shape[-2], 1):
+            raise ValueError(f"{name} holds too many tokens: {tuple(t.shape)}")
     if k is not None and (k.dtype != q.dtype or k.device != q.device):
         raise TypeError(f"q and k must be of one type and on one device, got {q.dtype} on {q.device} and {k.dtype} on {k.device}")
     if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):

@@ -313,3 +313,174 @@ def test_rotary_prompt_and_tokens(dtype):
     got = packed_attention(nq, *cache, _int([0, 1, 2]), starts, _int(lengths))
     at = last.cpu().numpy()
     _within(got, PA.attention(*arrays[:3], seqs)[at], bound[0][at], "token by token")
+
+
+#        queries, keys, heads, key heads, head dim; the key and the query that are spoilt
+SPOILT = {
+    "square": (150, 150, 4, 2, 64, 100, 20),
+    "tile_edge": (192, 192, 1, 1, 32, 127, 64),
+    "one_key_head": (200, 230, 8, 1, 128, 200, 11),
+    "odd_group": (90, 300, 6, 2, 40, 280, 3),
+    "over_a_cache": (9, 2100, 4, 1, 128, 2095, 2),  # the keys are split
+    "last": (65, 65, 2, 2, 96, 64, 64),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")], ids=["nan", "inf", "minus_inf"])
+@pytest.mark.parametrize("name", sorted(SPOILT))
+def test_unseen_pairs_take_no_part_whatever_they_hold(name, value, dtype):
+    """Rows that do not see a value that is no finite number keep their results to the bit, those that see it do not."""
+    n, m, h, hk, d, key, query = SPOILT[name]
+    _note(f"packed attention unseen {name} {value} {dtype}")
+    shift = m - n
+    off, koff = [0, n, n + 30], [0, m, m + 30]
+    q, k, v, g = _normal(21, dtype, (n + 30, h, d), (m + 30, hk, d), (m + 30, hk, d), (n + 30, h, d))
+    args = (_int(off), _int(koff))
+    clean = _run(q, k, v, g, *args)
+    _compare(q, k, v, g, clean, PA.sequences(off, koff), True)
+    sees = max(key - shift, 0)  # the first query that sees the key
+
+    bad_v = v.clone()
+    bad_v[key, :, 5] = value
+    out, gq, gk, gv = _run(q, k, bad_v, g, *args)
+    others = [c for c in range(d) if c != 5]
+    assert torch.equal(out[:sees], clean[0][:sees]) and torch.equal(out[n:], clean[0][n:])
+    assert torch.equal(out[sees:n, :, others], clean[0][sees:n, :, others])
+    assert not torch.isfinite(out[sees:n, :, 5]).any()
+    assert torch.equal(gq[:sees], clean[1][:sees]) and torch.equal(gq[n:], clean[1][n:])
+    assert torch.equal(gk[m:], clean[2][m:]) and torch.equal(gv[m:], clean[3][m:])
+    assert torch.isnan(gq[sees:n]).any()
+
+    bad_k = k.clone()
+    bad_k[key, :, 5] = value
+    out, gq, gk, gv = _run(q, bad_k, v, g, *args)
+    for x, c, first, last in ((out, clean[0], sees, n), (gq, clean[1], sees, n), (gk, clean[2], m, m), (gv, clean[3], m, m)):
+        if first < last:
+            assert torch.equal(x[:first], c[:first])
+        assert torch.equal(x[last:], c[last:])
+    assert torch.isnan(gq[sees:n]).any()
+
+    unseen = query + shift + 1  # the first key that the query does not see
+    for which in range(2):
+        q2, g2 = q.clone(), g.clone()
+        (q2, g2)[which][query, :, 7] = value
+        out, gq, gk, gv = _run(q2, k, v, g2, *args)
+        for x, c in ((out, clean[0]), (gq, clean[1])):
+            assert torch.equal(x[:query], c[:query]) and torch.equal(x[query + 1:], c[query + 1:])
+        for x, c in ((gk, clean[2]), (gv, clean[3])):
+            assert torch.equal(x[unseen:], c[unseen:])
+        assert not torch.isfinite(gk[:unseen]).all() and not torch.isfinite(gq[query]).all()
+
+
+@TYPES
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+def test_keys_behind_the_length_get_zeros_where_queries_are_not_finite(causal, dtype):
+    off, koff, lengths = [0, 40], [0, 100], [70]
+    q, k, v, g = _normal(22, dtype, (40, 2, 128), (100, 2, 128), (100, 2, 128), (40, 2, 128))
+    for which in range(2):
+        q2, g2 = q.clone(), g.clone()
+        (q2, g2)[which][3] = float("nan")
+        _, _, gk, gv = _run(q2, k, v, g2, _int(off), _int(koff), _int(lengths), causal=causal)
+        assert not gk[70:].any() and not gv[70:].any()
+        assert torch.isnan(gk[:33]).all()
+
+
+#      lengths, keys, heads, key heads, head dim
+WIDE = {
+    "thousands": ([int(i * 7919 % 4) for i in range(5000)], None, 2, 1, 8),
+    "sixty_four_to_a_head": ([40, 3], [50, 3], 64, 1, 64),
+    "thirty_three_to_a_head": ([30, 66], None, 66, 2, 32),
+    "one_token_in_many": ([0] * 100 + [1] + [0] * 100, [0] * 100 + [333] + [0] * 100, 64, 2, 128),
+    "long_keys": ([130, 2], [4000, 3000], 2, 1, 128),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("name", sorted(WIDE))
+def test_many_sequences_wide_groups_and_long_keys(name, dtype):
+    lengths, keys, h, hk, d = WIDE[name]
+    keys = lengths if keys is None else keys
+    _note(f"packed attention {name} {dtype}")
+    off, koff = np.cumsum([0, *lengths]), np.cumsum([0, *keys])
+    q, k, v, g = _normal(23, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d), (off[-1], h, d))
+    for causal in (False, True):
+        got = _run(q, k, v, g, _int(off), _int(koff), causal=causal)
+        _compare(q, k, v, g, got, PA.sequences(off, koff), causal)
+
+
+@TYPES
+def test_rows_far_apart(dtype):
+    """A cache whose rows lie beyond 2^31 elements, and heads in front of the rows (head-major), without a copy."""
+    h, hk, d, stride, fill = 4, 2, 64, 1 << 14, [90, 300]
+    first = [(1 << 31) // stride + 5, (1 << 31) // stride + 400]
+    rows = first[1] + 400
+    store = torch.empty(rows * stride, dtype=dtype, device=_dev())
+    k, v = (store.view(rows, stride)[:, at:at + hk * d].unflatten(1, (hk, d)) for at in (0, hk * d))
+    koff, off = [*first, rows], [0, 90, 95]
+    small = _normal(24, dtype, (rows - first[0], hk, d), (rows - first[0], hk, d), (95, h, d), (95, h, d))
+    k[first[0]:], v[first[0]:] = small[:2]
+    q, g = small[2:]
+    out, saved = packed_attention_forward(q, k, v, _int(off), _int(koff), _int(fill))
+    grads = packed_attention_backward(q, k, v, out, saved, g, _int(off), _int(koff), _int(fill))
+    near = [0, first[1] - first[0], rows - first[0]]
+    tail = (out, grads[0], *(x[first[0]:] for x in grads[1:]))
+    assert not any(x[:first[0]].any() for x in grads[1:])
+    _compare(q, *small[:2], g, tail, PA.sequences(off, near, fill), True)
+    major = store.view(-1)[:2 * hk * (1 << 29)].view(2, hk, -1, d)  # a head lies 2^29 elements behind the one before
+    kk, vv = (x.transpose(0, 1)[-400:] for x in major)
+    kk.copy_(small[0][:400]), vv.copy_(small[1][:400])
+    got = packed_attention_forward(q, kk, vv, _int(off), _int([0, 90, 400]), _int([90, 300]))[0]
+    want = packed_attention_forward(q, small[0][:400], small[1][:400], _int(off), _int([0, 90, 400]), _int([90, 300]))[0]
+    assert torch.equal(got, want)
+
+
+@TYPES
+def test_both_ways_in_give_the_same_bits(dtype):
+    """The C++ function and the Python one, which takes what the first does not; 64-bit offsets."""
+    from rfdetr_jax_amd.packed_attention import _PackedAttention
+
+    off, koff, lengths = [0, 33, 150], [0, 100, 260], [70, 160]
+    q, k, v, g = _normal(25, dtype, (150, 4, 64), (260, 2, 64), (260, 2, 64), (150, 4, 64))
+    args = (_int(off), _int(koff), _int(lengths))
+    want = _run(q, k, v, g, *args, scale=0.3)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = _PackedAttention.apply(*leaves, *args, True, 0.3)
+    got = (out, *torch.autograd.grad(out, leaves, g))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = _run(q, k, v, g, *(x.long() for x in args), scale=0.3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_gradients_are_not_differentiable_again():
+    from rfdetr_jax_amd.packed_attention import _PackedAttention
+
+    q, k, v, g = (x.requires_grad_(True) for x in _normal(26, torch.float32, (10, 2, 32), (10, 1, 32), (10, 1, 32), (10, 2, 32)))
+    for call in (packed_attention, lambda *a: _PackedAttention.apply(*a, None, None, True, None)):
+        (grad,) = torch.autograd.grad(call(q, k, v, _int([0, 10])), [q], g, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            torch.autograd.grad(grad.sum(), [q])
+
+
+def test_front_end_refusals():
+    d = _dev()
+    q, k, off = torch.zeros(6, 4, 32, device=d), torch.zeros(6, 2, 32, device=d), _int([0, 6])
+    for args, error, text in (
+            ((q.double(), k.double(), k.double(), off), TypeError, "not supported"), ((q, k.bfloat16(), k, off), TypeError, "one type"),
+            ((q[0], k, k, off), ValueError, "rows, heads, D"), ((q, k, k[:5], off), ValueError, "expected"), ((q, k[..., :16], k[..., :16], off), ValueError, "expected"),
+            ((q[:, :3], k, k, off), ValueError, "divide"), ((q, k[:, :0], k[:, :0], off), ValueError, "divide"),
+            ((q.repeat(1, 33, 1), k, k, off), ValueError, "share"), ((q[..., :12], k[..., :12], k[..., :12], off), ValueError, "head_dim"),
+            ((q.repeat(1, 1, 5), k.repeat(1, 1, 5), k.repeat(1, 1, 5), off), ValueError, "head_dim"), ((q[..., :0], k[..., :0], k[..., :0], off), ValueError, "head_dim"),
+            ((q, k, k, off.float()), TypeError, "int32"), ((q, k, k, off[None]), ValueError, "offsets"), ((q, k, k, off[:0]), ValueError, "offsets"),
+            ((q, k, k, off, _int([0, 3, 6])), ValueError, "key_offsets"), ((q, k, k, off, None, _int([1, 2])), ValueError, "key_lengths"),
+            ((q, k, k, off.cpu()), ValueError, "cpu"), ((q, k, k, off, None, _int([6]).cpu()), ValueError, "cpu"), ((q, k.cpu(), k, off), RuntimeError, "no CPU path"),
+            ((q, k, k, off, None, None, True, 0.0), ValueError, "scale"), ((q, k, k, off, None, None, True, float("nan")), ValueError, "scale"),
+            ((q, k, k, off, None, None, True, 1e-30), ValueError, "scale")):
+        with pytest.raises(error, match=text):
+            packed_attention(*args)
+        with pytest.raises(error, match=text):
+            packed_attention_forward(*args)
+    out, saved = packed_attention_forward(q, k, k, off)
+    for bad in ((out[:5], saved, q), (out, (saved[0][:, :2], None), q), (out, saved, q[:, :2]), (out, saved, q.cpu())):
+        with pytest.raises(ValueError):
+            packed_attention_backward(q, k, k, *bad, off)

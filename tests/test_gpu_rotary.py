@@ -149,3 +149,20 @@ def test_in_a_graph(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+def test_refusals_and_second_derivatives():
+    q, pos = torch.randn(6, 2, 32, device=_dev()), torch.zeros(6, 2, dtype=torch.int32, device=_dev())
+    for args, error, text in (
+            ((q.double(), None, pos, (8, 8)), TypeError, "not supported"), ((q[0, 0], None, pos, (8, 8)), ValueError, "heads, D"),
+            ((q, q.bfloat16(), pos, (8, 8)), TypeError, "one type"), ((q, q[:5], pos, (8, 8)), ValueError, "expected"), ((q, q[..., :16], pos, (4, 4)), ValueError, "expected"),
+            ((q, q, pos.to(torch.int16), (8, 8)), TypeError, "int32"), ((q, q, pos.cpu(), (8, 8)), ValueError, "cpu"), ((q, q, pos, (8, 8, 1)), ValueError, "positions"),
+            ((q, q, pos, ()), ValueError, "sections"), ((q, q, pos, (8, 0)), ValueError, "sections"), ((q, q, pos, (8, 9)), ValueError, "pairs"),
+            ((q[..., :31], None, pos, (8, 7)), ValueError, "even"), ((q, q, pos, (8, 8), 0.0), ValueError, "base"), ((q, q, pos, (8, 8), float("inf")), ValueError, "base"),
+            ((q.cpu(), None, pos, (8, 8)), RuntimeError, "no CPU path")):
+        with pytest.raises(error, match=text):
+            rotary_embed(*args)
+    leaf, g = q.clone().requires_grad_(True), torch.randn_like(q).requires_grad_(True)
+    (grad,) = torch.autograd.grad(rotary_embed(leaf, None, pos, (8, 8)), [leaf], g, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        torch.autograd.grad(grad.sum(), [leaf])

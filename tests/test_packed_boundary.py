@@ -47,8 +47,9 @@ INVALID, UNSUPPORTED = _native.ERR_INVALID_ARGUMENT, _native.ERR_UNSUPPORTED
     ({"qo": None}, INVALID, "offsets"), ({"ko": None}, INVALID, "offsets"), ({"v": ODD}, INVALID, "16 bytes"), ({"stats": ODD}, INVALID, "16 bytes"),
     ({"kl": ctypes.c_void_p((1 << 20) + 2)}, INVALID, "4 bytes"), ({"strides": _i64(*([260, 64] * 8))}, INVALID, "stride"),
     ({"strides": _i64(*([-256, 64] * 8))}, INVALID, "stride"), ({"strides": _i64(*([56, 64] * 8))}, UNSUPPORTED, "apart"),
-    ({"strides": _i64(*([1 << 22, 64] * 8))}, UNSUPPORTED, "apart"), ({"strides": _i64(*([256, 1 << 21] * 8))}, UNSUPPORTED, "apart"),
-    ({"rest": ODD}, INVALID, "16 bytes"),
+    ({"strides": _i64(*([1 << 22, 64] * 8))}, UNSUPPORTED, "apart"), ({"strides": _i64(*([256, 1 << 26] * 8))}, UNSUPPORTED, "apart"),
+    ({"rest": ODD}, INVALID, "16 bytes"), ({"h": 130, "hk": 2}, UNSUPPORTED, "key head"), ({"scale": 2.0 ** -65}, INVALID, "scale"),
+    ({"scale": 2.0 ** 65}, INVALID, "scale"),
 ])
 def test_attention_refusals(direction, change, code, text):
     rc, msg = _attention(direction, **change)
