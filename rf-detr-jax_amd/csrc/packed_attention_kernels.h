@@ -11,12 +11,11 @@
 // keys serves all of them, a new token of every head fills one tile, and dk and dv are summed over the
 // heads inside one workgroup (no atomics, one order).
 //
-// Finding the tile. The tiles of BM rows lie in slots: segment s (the rows before the first sequence,
-// the sequences, the rows behind the last) takes the slots from floor(first row / BM) + s on, which are
-// at least ceil(rows / BM) many. So the grid is rows / BM + segments, known without the lengths, and a
-// workgroup finds its segment by a search over the offsets alone: no length is read back by the host
-// and no launch prepares a table. Offsets are clamped to the tensors' rows: wrong ones give wrong values
-// and no access out of bounds. Rows outside every sequence are written as zeros.
+// Finding the tile. The segments (the rows before the first sequence, the sequences, the rows behind the
+// last) of some rows have at most rows / 128 + segments tiles of 128 rows, so the grid is known without the
+// lengths, and a workgroup finds its tile by adding up the segments' tiles (pk_place): no length is read back
+// by the host and no launch prepares a table. Offsets are clamped to the tensors' rows: wrong ones give
+// wrong values and no access out of bounds. Rows outside every sequence are written as zeros.
 //
 // Layouts of the products as in attention_kernels.h: scores are formed transposed (streamed rows x own
 // rows), a lane owns one own row (its softmax statistics stay in the lane), and the weights in their
@@ -78,11 +77,11 @@ __device__ __align__(16) const uint32_t pk_zeros[4] = {0u, 0u, 0u, 0u};
 
 // ---- the workgroup's place ---------------------------------------------------------------------
 
-// First row of segment s, 0 <= s <= sequences + 2, clamped to the tensor.
+// First row of segment s, 0 <= s <= sequences + 2, clamped to the tensor (a load without a branch, so that several
+// are under way together).
 __device__ __forceinline__ int pk_bound(const int32_t* offsets, int s, int sequences, int rows) {
-  if (s == 0) return 0;
-  if (s >= sequences + 2) return rows;
-  return min(max(offsets[s - 1], 0), rows);
+  const int x = min(max(offsets[min(max(s - 1, 0), sequences)], 0), rows);
+  return s == 0 ? 0 : s >= sequences + 2 ? rows : x;
 }
 
 struct PkPlace {
@@ -92,26 +91,124 @@ struct PkPlace {
   int tile;        // tile of the segment
 };
 
-// The segment of `slot` (the wave searches 64 segments at a time): the last one that starts at or
-// before it. `unit`: rows of a tile's matrix to a row of the tensor.
-__device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequences, int rows, int unit, int slot, int lane) {
-  int lo = 0, hi = sequences + 2;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-    const bool at = s < hi && static_cast<int>(static_cast<uint32_t>(pk_bound(offsets, s, sequences, rows)) * unit / kPkTile) + s <= slot;
-    const int n = max(1, static_cast<int>(__popcll(__ballot(at))));
-    lo += (n - 1) * step;
-    hi = min(hi, lo + step);
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int pk_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // within rows of 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15's to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31's to the upper half
+  return x;
+}
+
+constexpr int kPkCounted = 1024;  // segments whose tiles a wave counts
+
+// Tile, or unit of a tile's work, of workgroup `index` of a grid: by number, or from the last one on. `unit`: rows of
+// a tile's matrix to a row of the tensor. No rows (own = 0) for the grid's tiles that do not exist.
+// Up to kPkCounted segments the wave adds up all segments' units, count(s, rows) of segment s, and w.tile is the
+// unit's number in its segment. So the units that do not exist are the grid's last. That matters: the hardware
+// hands workgroups to its shader engines in turn whether they end at once or not, and with empty ones among
+// them (sequences of 128 rows: every second one) half of the CUs stood idle: forward of 128 times 128 queries over
+// 1,024 keys, 8 heads, 173 us for 140 in bf16 at 128 channels, 540 for 287 in f32 at 64.
+// Of more segments it searches, 64 at a time, among `slots` tiles, with segment s at tile floor(first row / 128) + s,
+// behind which it has room for ceil(rows / 128).
+template <bool LAST_FIRST, typename Count>
+__device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequences, int rows, int unit, int index, int slots, int lane, Count&& count) {
+  const int segments = sequences + 2;
+  PkPlace w{-1, 0, 0, 0};
+  int s;
+  if (segments <= kPkCounted) {
+    const int per = (segments + 63) / 64;
+    auto units = [&](int s) {
+      const int n = pk_bound(offsets, s + 1, sequences, rows) - pk_bound(offsets, s, sequences, rows), units = count(s, max(n, 1));
+      return s >= segments || n <= 0 ? 0 : units;
+    };
+    int mine = 0;
+    for (int i = 0; i < per; ++i) mine += units(lane * per + i);
+    int end = pk_scan(mine);
+    const int total = __builtin_amdgcn_readlane(end, 63), t = LAST_FIRST ? total - 1 - index : index;
+    if (t < 0 || t >= total) return w;
+    int at = static_cast<int>(__popcll(__ballot(end <= t))), base = __builtin_amdgcn_readlane(end - mine, at);
+    s = at * per;
+    if (per > 1) {
+      mine = lane < per ? units(s + lane) : 0;
+      end = base + pk_scan(mine);
+      at = static_cast<int>(__popcll(__ballot(end <= t)));
+      base = __builtin_amdgcn_readlane(end - mine, at);
+      s += at;
+    }
+    w.tile = t - base;
+  } else {
+    const int slot = LAST_FIRST ? slots - 1 - index : index;
+    int lo = 0, hi = segments;
+    auto at = [&](int s) { return static_cast<int>(static_cast<uint32_t>(pk_bound(offsets, s, sequences, rows)) * unit / kPkTile) + s; };
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, x = lo + lane * step;
+      const int n = max(1, static_cast<int>(__popcll(__ballot(x < hi && at(x) <= slot))));
+      lo += (n - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    s = __builtin_amdgcn_readfirstlane(lo);
+    w.tile = slot - at(s);
+    if (w.tile < 0) return PkPlace{-1, 0, 0, 0};  // only where the offsets fall
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  PkPlace w;
-  w.first = pk_bound(offsets, lo, sequences, rows);
-  w.own = max(0, pk_bound(offsets, lo + 1, sequences, rows) - w.first);
-  w.seq = lo >= 1 && lo <= sequences ? lo - 1 : -1;
-  w.tile = slot - (static_cast<int>(static_cast<uint32_t>(w.first) * unit / kPkTile) + lo);
-  if (w.tile < 0) w.tile = w.own = 0;  // only where the offsets fall
+  w.first = pk_bound(offsets, s, sequences, rows);
+  w.own = max(0, pk_bound(offsets, s + 1, sequences, rows) - w.first);
+  w.seq = s >= 1 && s <= sequences ? s - 1 : -1;
   return w;
 }
+
+// The place in line of number `index` of `count`: every second round is walked backwards. Workgroups go to the 8
+// XCDs, and there to 4 shader engines, in turn, R tiles to a round; a causal sequence's tiles fall by size, and
+// walked in one direction the first of them would get the largest of every round.
+__device__ __forceinline__ int pk_line(int index, int count, int kv_heads) {
+  const int shift = 5 - min(5, static_cast<int>(__builtin_ctz(kv_heads))), round = index >> shift;
+  if ((round & 1) == 0 || (round + 1) << shift > count) return index;
+  return (2 * round + 1 << shift) - 1 - index;
+}
+
+__device__ __forceinline__ int pk_tiles(int rows, int unit) { return static_cast<int>((static_cast<uint32_t>(rows) * unit + (kPkTile - 1)) / kPkTile); }
+
+// The keys of sequence `seq`: first row and number.
+struct PkRange {
+  int first, count;
+  __device__ __forceinline__ PkRange(const PackParams& p, int seq) {
+    first = min(max(p.k_offsets[seq], 0), p.k_rows);
+    const int end = min(max(p.k_offsets[seq + 1], first), p.k_rows);
+    count = p.k_lengths != nullptr ? min(max(p.k_lengths[seq], 0), end - first) : end - first;
+  }
+};
+
+// The split forward: how many workgroups share tile i of a sequence of n queries and m keys. At least p.part chunks
+// of keys each (more where a long sequence would make more parts than p.splits); a causal sequence's
+// tiles see 2 / G chunks more from one to the next, so every `step` tiles make one part more, from the first tile
+// that sees a key on, and the parts of the first x tiles have a closed form. With c chunks seen by the last tile
+// and the tile sizes' roundings it has fewer than 1 + (c + 2) / part parts, at most room + 2 = p.splits.
+struct PkParts {
+  int first, from, step;
+  __device__ __forceinline__ PkParts(const PackParams& p, int n, int m) {
+    const int shift = m - n, most = (m + kPkChunk - 1) / kPkChunk, room = p.splits - 2;  // most: chunks that the last tile sees
+    const int part = most <= p.part * room ? p.part : (most + room - 1) / room;
+    int chunks = most;  // that the first tile with keys sees
+    from = 0;
+    step = 1 << 30;
+    if (p.causal && n * p.group > kPkTile) {
+      from = shift < 0 ? -shift * p.group / kPkTile : 0;
+      step = (part * p.group + 1) / 2;
+      const int token = (min((from + 1) * kPkTile, n * p.group) - 1) / p.group;
+      chunks = (min(max(token + shift + 1, 0), m) + kPkChunk - 1) / kPkChunk;
+    }
+    first = max((chunks + part - 1) / part, 1);
+  }
+  __device__ __forceinline__ int of(int tile) const { return tile - from < step ? first : first + (tile - from) / step; }
+  __device__ __forceinline__ int before(int x) const {
+    const int y = max(x - from, 0);
+    if (y <= step) return x * first;
+    const int q = y / step;
+    return x * first + q * (q - 1) / 2 * step + q * (y - q * step);
+  }
+};
 
 // ---- operands ----------------------------------------------------------------------------------
 
@@ -540,27 +637,55 @@ struct PkRows {
 struct PkQueries {
   PkPlace w;
   int kv_head;      // key head
-  int split;
-  int rows, r0;     // rows of the sequence's matrix, first of the workgroup's
+  int split, parts; // the workgroup's part of the tile's keys, of so many (forward)
+  int rows, r0;     // rows of the sequence's matrix, first of the workgroup's; none: no work
   int64_t k_first;  // first key row
   int m, shift;     // keys; a row of token t sees the keys below min(m, t + shift + 1)
-  __device__ PkQueries(const PackParams& p, int splits, int lane) {
+  template <bool SPLIT>
+  __device__ PkQueries(const PackParams& p, int lane, std::bool_constant<SPLIT>) {
     // key heads fastest: with 8 of them each stays on one XCD, whose L2 then holds its keys; the last
     // tiles, which see the most keys of a causal sequence, first
     const int b = static_cast<int>(blockIdx.x), rest = b / p.kv_heads;
     kv_head = b - rest * p.kv_heads;
-    const int slot = p.slots - 1 - rest / splits;
-    split = rest % splits;
-    w = pk_place(p.q_offsets, p.sequences, p.q_rows, p.group, slot, lane);
+    parts = 1;
+    split = 0;
+    const bool counted = p.sequences + 2 <= kPkCounted, shared = SPLIT && p.splits > 1;
+    if (!shared) {
+      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, pk_line(rest, p.slots, p.kv_heads), p.slots, lane, [&](int, int n) { return pk_tiles(n, p.group); });
+    } else {
+      split = counted ? 0 : rest / p.slots;
+      const int line = pk_line(rest - split * p.slots, counted ? p.slots * p.splits : p.slots, p.kv_heads);
+      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, line, p.slots, lane, [&](int s, int n) {
+        const int tiles = pk_tiles(n, p.group);
+        const PkRange keys(p, min(max(s - 1, 0), p.sequences - 1));
+        return s >= 1 && s <= p.sequences ? PkParts(p, n, keys.count).before(tiles) : tiles;
+      });
+    }
     rows = w.own * p.group;
-    r0 = w.tile * kPkTile;
     k_first = 0;
     m = 0;
-    if (w.seq >= 0) {
-      const int a = min(max(p.k_offsets[w.seq], 0), p.k_rows), b2 = min(max(p.k_offsets[w.seq + 1], a), p.k_rows);
-      k_first = a;
-      m = p.k_lengths != nullptr ? min(max(p.k_lengths[w.seq], 0), b2 - a) : b2 - a;
+    if (w.seq >= 0 && w.own > 0) {
+      const PkRange keys(p, w.seq);
+      k_first = keys.first;
+      m = keys.count;
+      if (shared) {
+        const PkParts all(p, w.own, m);
+        if (counted) {  // the tile of the sequence's part w.tile: the last one before which no more parts lie
+          int lo = 0, hi = pk_tiles(w.own, p.group);
+          while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64, x = lo + lane * step;
+            const int n = static_cast<int>(__popcll(__ballot(x < hi && all.before(x) <= w.tile)));
+            lo += (n - 1) * step;
+            hi = min(hi, lo + step);
+          }
+          split = w.tile - all.before(lo);
+          w.tile = lo;
+        }
+        parts = all.of(w.tile);
+      }
     }
+    if (split >= parts) rows = 0;
+    r0 = w.tile * kPkTile;
     shift = m - w.own;
   }
   __device__ int seen(const PackParams& p, int r) const { return p.causal ? min(max(r / p.group + shift + 1, 0), m) : m; }
@@ -606,13 +731,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, p.splits, lane);
+  const PkQueries w(p, lane, std::true_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* out = static_cast<T*>(p.out);
   const int end = w.w.seq < 0 ? 0 : w.seen(p, r1 - 1), chunks = (end + kPkChunk - 1) / kPkChunk;  // that the workgroup sees
-  const int parts = min(max((chunks + p.part - 1) / p.part, 1), p.splits);
-  if (w.split >= parts) return;
+  const int parts = w.parts;
   if (p.splits > 1 && w.split == 0)  // one part writes its rows itself
     for (int r = w.r0 + static_cast<int>(threadIdx.x); r < r1; r += 64 * kPkWaves) p.part_n[w.stat(p, r)] = parts;
   if (w.w.seq < 0) {
@@ -879,7 +1003,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, 1, lane);
+  const PkQueries w(p, lane, std::false_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* gq = static_cast<T*>(p.gq);
@@ -1036,7 +1160,7 @@ struct PkKeys {
   __device__ PkKeys(const PackParams& p, const PkRows& walk, int lane, int b, int part_) : part(part_) {
     const int slot = b / p.kv_heads;
     kv_head = b - slot * p.kv_heads;
-    w = pk_place(p.k_offsets, p.sequences, p.k_rows, 1, slot, lane);
+    w = pk_place<false>(p.k_offsets, p.sequences, p.k_rows, 1, pk_line(slot, p.slots, p.kv_heads), p.slots, lane, [](int, int n) { return pk_tiles(n, 1); });
     b0 = w.tile * kPkTile;
     b1 = min(b0 + kPkTile, w.own);
     m = n = q_first = 0;
