@@ -463,6 +463,9 @@ __device__ __forceinline__ void pk_accumulate2(at_f16 (&ax)[DT / 32], PkLds X, c
 typedef __bf16 pk_bf16 __attribute__((ext_vector_type(16)));
 typedef __bf16 pk_bf4 __attribute__((ext_vector_type(4)));
 
+// What the rounding to bf16 leaves.
+__device__ __forceinline__ at_f16 pk_rest(const at_f16& x) { return x - __builtin_convertvector(__builtin_convertvector(x, pk_bf16), at_f16); }
+
 // A wave's LDS accesses are in order; this keeps the compiler from exchanging them.
 __device__ __forceinline__ void pk_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -481,7 +484,7 @@ __device__ __forceinline__ void pk_store(const at_f16 (&acc)[DT / 32], float f, 
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) {
     at_f16 v = acc[nd] * f;
-    if constexpr (REST) v -= __builtin_convertvector(__builtin_convertvector(v, pk_bf16), at_f16);
+    if constexpr (REST) v = pk_rest(v);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {  // channels 32 nd + 8 c + 4 grp .. + 3
       const at_f4 x = {v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
@@ -721,7 +724,7 @@ __device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lim, int grp) {
 // reference score m and sum l. m starts at the first chunk's maximum (whose weight, the largest of a short
 // row, is then 1 and rounds to itself) and moves when a chunk's exceeds it by 2^8.
 template <typename T, int DT>
-__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 : 2) : 1) pk_fwd_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 : DT <= 64 ? 3 : 2) : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
@@ -749,6 +752,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;  // keys that the wave sees
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                  // that every row of it sees
   const int all = w.seen(p, w.r0);                                           // that every row of the workgroup sees
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk;
   const int per = (chunks + parts - 1) / parts, c0 = w.split * per, c1 = min(chunks, c0 + per);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
@@ -820,10 +824,11 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
           });
         }
       };
-      auto rescale = [&] {  // between phases: the sums of a phase belong to one m
+      auto rescale = [&](auto phase) {  // between phases: the sums of a phase belong to one m
         if (__any(alpha != 1.0f)) {
 #pragma unroll
           for (int nd = 0; nd < DT / 32; ++nd) o[nd] *= alpha;
+          if constexpr (phase == 2) s0 *= alpha;  // (for the rounding's rest below)
           alpha = 1.0f;
         }
       };
@@ -847,11 +852,16 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 4 
             if constexpr (b == 1) soft(s0, k0, PkInt<t>{});
             if constexpr (b == 2) soft(s1, k0 + 32, PkInt<t>{});
             if constexpr ((b == 1 || b == 2) && t == KS - 1) {
-              rescale();
+              rescale(PkInt<b>{});
               if constexpr (b == 1) w0.set(s0);
               else w1.set(s1);
             }
           });
+      // Rows of fewer than 64 keys: what the rounding of the weights left, too. The rounding's errors do not average
+      // out over few keys, and delta, from the output, carries them into every ds of the row, where they are as large
+      // as those of ds's own rounding. (60 calls of 1 to 8 sequences of 1 to 600 rows: 7 of 240 results were more than
+      // 1.5 times as far off as the exact ones rounded, with this and the same for dq 1.)
+      if (k0 == 0 && few) pk_accumulate2<T, DT, 2>(o, V, pk_rest(s0), o, V + 32 * Tile::ROW, pk_rest(s1), at);
     } else {
       next.all();
       pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
@@ -1018,6 +1028,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;
   const int all = w.seen(p, w.r0);  // keys that every row of the workgroup sees
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk;
   const int chunks = (end + kPkChunk - 1) / kPkChunk;
   PkRow<T, DT> q, go;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, rc), valid, p.dim, grp);
@@ -1115,6 +1126,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
             if constexpr (b == 3) weigh(sb, t);
             if constexpr (b == 4) slope(sb, db, wb, k0 + 32, t);
           });
+      if (k0 == 0 && few)  // as in the forward: of ds
+        pk_accumulate2<T, DT, 2>(dq, K, pk_rest(sa), dq, K + 32 * Tile::ROW, pk_rest(sb), now);
     } else {
       next.all();
 #pragma unroll 1
