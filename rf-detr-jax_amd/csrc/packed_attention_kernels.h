@@ -105,7 +105,8 @@ __device__ __forceinline__ int pk_scan(int x) {
 constexpr int kPkCounted = 1024;  // segments whose tiles a wave counts
 
 // Tile, or unit of a tile's work, of workgroup `index` of a grid: by number, or from the last one on. `unit`: rows of
-// a tile's matrix to a row of the tensor. No rows (own = 0) for the grid's tiles that do not exist.
+// a tile's matrix to a row of the tensor; `alike`: units are of about one size, so no order is better. No rows
+// (own = 0) for the grid's tiles that do not exist.
 // Up to kPkCounted segments the wave adds up all segments' units, count(s, rows) of segment s, and w.tile is the
 // unit's number in its segment. So the units that do not exist are the grid's last. That matters: the hardware
 // hands workgroups to its shader engines in turn whether they end at once or not, and with empty ones among
@@ -114,7 +115,8 @@ constexpr int kPkCounted = 1024;  // segments whose tiles a wave counts
 // Of more segments it searches, 64 at a time, among `slots` tiles, with segment s at tile floor(first row / 128) + s,
 // behind which it has room for ceil(rows / 128).
 template <bool LAST_FIRST, typename Count>
-__device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequences, int rows, int unit, int index, int slots, int lane, Count&& count) {
+__device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequences, int rows, int unit, int index, int slots, int lane, bool alike,
+                                            Count&& count) {
   const int segments = sequences + 2;
   PkPlace w{-1, 0, 0, 0};
   int s;
@@ -124,21 +126,35 @@ __device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequence
       const int n = pk_bound(offsets, s + 1, sequences, rows) - pk_bound(offsets, s, sequences, rows), units = count(s, max(n, 1));
       return s >= segments || n <= 0 ? 0 : units;
     };
-    int mine = 0;
-    for (int i = 0; i < per; ++i) mine += units(lane * per + i);
-    int end = pk_scan(mine);
-    const int total = __builtin_amdgcn_readlane(end, 63), t = LAST_FIRST ? total - 1 - index : index;
-    if (t < 0 || t >= total) return w;
-    int at = static_cast<int>(__popcll(__ballot(end <= t))), base = __builtin_amdgcn_readlane(end - mine, at);
-    s = at * per;
-    if (per > 1) {
-      mine = lane < per ? units(s + lane) : 0;
-      end = base + pk_scan(mine);
-      at = static_cast<int>(__popcll(__ballot(end <= t)));
-      base = __builtin_amdgcn_readlane(end - mine, at);
-      s += at;
+    if (per == 1 && !alike) {  // the longest segment first: the work of its tiles sets the time if they start last
+      const int mine = units(lane), length = lane >= segments ? 0 : pk_bound(offsets, lane + 1, sequences, rows) - pk_bound(offsets, lane, sequences, rows);
+      int base = 0;
+      for (int j = 0; j < segments; ++j) {
+        const int other = __builtin_amdgcn_readlane(length, j), more = __builtin_amdgcn_readlane(mine, j);
+        base += other > length || (other == length && j < lane) ? more : 0;
+      }
+      const uint64_t here = __ballot(base <= index && index < base + mine);
+      if (here == 0) return w;
+      s = static_cast<int>(__builtin_ctzll(here));
+      w.tile = index - __builtin_amdgcn_readlane(base, s);
+      if (LAST_FIRST) w.tile = __builtin_amdgcn_readlane(mine, s) - 1 - w.tile;
+    } else {
+      int mine = 0;
+      for (int i = 0; i < per; ++i) mine += units(lane * per + i);
+      int end = pk_scan(mine);
+      const int total = __builtin_amdgcn_readlane(end, 63), t = LAST_FIRST ? total - 1 - index : index;
+      if (t < 0 || t >= total) return w;
+      int at = static_cast<int>(__popcll(__ballot(end <= t))), base = __builtin_amdgcn_readlane(end - mine, at);
+      s = at * per;
+      if (per > 1) {
+        mine = lane < per ? units(s + lane) : 0;
+        end = base + pk_scan(mine);
+        at = static_cast<int>(__popcll(__ballot(end <= t)));
+        base = __builtin_amdgcn_readlane(end - mine, at);
+        s += at;
+      }
+      w.tile = t - base;
     }
-    w.tile = t - base;
   } else {
     const int slot = LAST_FIRST ? slots - 1 - index : index;
     int lo = 0, hi = segments;
@@ -654,11 +670,11 @@ struct PkQueries {
     split = 0;
     const bool counted = p.sequences + 2 <= kPkCounted, shared = SPLIT && p.splits > 1;
     if (!shared) {
-      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, pk_line(rest, p.slots, p.kv_heads), p.slots, lane, [&](int, int n) { return pk_tiles(n, p.group); });
+      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, pk_line(rest, p.slots, p.kv_heads), p.slots, lane, false, [&](int, int n) { return pk_tiles(n, p.group); });
     } else {
       split = counted ? 0 : rest / p.slots;
       const int line = pk_line(rest - split * p.slots, counted ? p.slots * p.splits : p.slots, p.kv_heads);
-      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, line, p.slots, lane, [&](int s, int n) {
+      w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, line, p.slots, lane, true, [&](int s, int n) {
         const int tiles = pk_tiles(n, p.group);
         const PkRange keys(p, min(max(s - 1, 0), p.sequences - 1));
         return s >= 1 && s <= p.sequences ? PkParts(p, n, keys.count).before(tiles) : tiles;
@@ -1173,7 +1189,7 @@ struct PkKeys {
   __device__ PkKeys(const PackParams& p, const PkRows& walk, int lane, int b, int part_) : part(part_) {
     const int slot = b / p.kv_heads;
     kv_head = b - slot * p.kv_heads;
-    w = pk_place<false>(p.k_offsets, p.sequences, p.k_rows, 1, pk_line(slot, p.slots, p.kv_heads), p.slots, lane, [](int, int n) { return pk_tiles(n, 1); });
+    w = pk_place<false>(p.k_offsets, p.sequences, p.k_rows, 1, pk_line(slot, p.slots, p.kv_heads), p.slots, lane, false, [](int, int n) { return pk_tiles(n, 1); });
     b0 = w.tile * kPkTile;
     b1 = min(b0 + kPkTile, w.own);
     m = n = q_first = 0;
@@ -1220,9 +1236,10 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   __shared__ __align__(16) unsigned char kept_rows[KEEP > 0 ? KEEP * kPkWaves * 1024 : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkRows walk(p.group);
-  // the parts of a tile are a grid of tiles apart: the first parts of all tiles start before any second
-  const int tiles = static_cast<int>(gridDim.x) / p.splits, my_part = static_cast<int>(blockIdx.x) / tiles;
-  const PkKeys w(p, walk, lane, static_cast<int>(blockIdx.x) - my_part * tiles, my_part);
+  // the parts of a tile are a grid of tiles apart, the last of all tiles first: of shared tiles all parts are full,
+  // those of one part, down to a few rows, come last and even out
+  const int tiles = static_cast<int>(gridDim.x) / p.splits, turn = static_cast<int>(blockIdx.x) / tiles;
+  const PkKeys w(p, walk, lane, static_cast<int>(blockIdx.x) - turn * tiles, p.splits - 1 - turn);
   if (w.b0 >= w.w.own || w.part >= w.parts) return;
   T* gk = static_cast<T*>(p.gk);
   T* gv = static_cast<T*>(p.gv);
