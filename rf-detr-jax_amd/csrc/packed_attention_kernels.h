@@ -104,7 +104,7 @@ __device__ __forceinline__ int pk_scan(int x) {
 
 constexpr int kPkCounted = 1024;  // segments whose tiles a wave counts
 
-// Tile, or unit of a tile's work, of workgroup `index` of a grid: by number, or from the last one on. `unit`: rows of
+// Tile, or unit of a tile's work, of workgroup `index` of a grid. LAST_FIRST: a segment's last one first. `unit`: rows of
 // a tile's matrix to a row of the tensor; `alike`: units are of about one size, so no order is better. No rows
 // (own = 0) for the grid's tiles that do not exist.
 // Up to kPkCounted segments the wave adds up all segments' units, count(s, rows) of segment s, and w.tile is the

@@ -484,3 +484,20 @@ def test_front_end_refusals():
     for bad in ((out[:5], saved, q), (out, (saved[0][:, :2], None), q), (out, saved, q[:, :2]), (out, saved, q.cpu())):
         with pytest.raises(ValueError):
             packed_attention_backward(q, k, k, *bad, off)
+
+
+@TYPES
+@pytest.mark.parametrize("count", [61, 62, 63, 126, 1021, 1022, 1023])
+def test_numbers_of_sequences_where_the_search_changes(count, dtype):
+    """64 segments of rows fit a wave, 1,024 are counted, more are searched; equal lengths, none and longer ones among them."""
+    lengths = [i * 7 % 5 if i % 11 else 0 for i in range(count)]
+    lengths[count // 2] = 140
+    off = np.cumsum([0, *lengths])
+    q, k, v, g = _normal(27, dtype, (off[-1], 2, 32), (off[-1], 1, 32), (off[-1], 1, 32), (off[-1], 2, 32))
+    got = _run(q, k, v, g, _int(off))
+    _compare(q, k, v, g, got, PA.sequences(off), True)
+    fill = [n + 100 + i % 37 for i, n in enumerate(lengths)]  # few rows, split keys
+    koff = np.cumsum([0, *(m + 3 for m in fill)])
+    k, v = _normal(28, dtype, (koff[-1], 1, 32), (koff[-1], 1, 32))
+    out = packed_attention(q, k, v, _int(off), _int(koff), _int(fill))
+    _compare(q, k, v, torch.zeros_like(q), (out,), PA.sequences(off, koff, fill), True)
