@@ -25,12 +25,12 @@ int pk_shape(const PackShape& s) {
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: negative extent");
   if (s.head_dim < 8 || s.head_dim > 128 || s.head_dim % 8 != 0)
     return fail(MSDA_ERR_UNSUPPORTED, "packed attention: head_dim %d (multiples of 8 up to 128 supported)", s.head_dim);
-  if (s.heads != 0 && (s.kv_heads == 0 || s.heads % s.kv_heads != 0))
+  if (s.heads == 0 || s.kv_heads == 0 || s.heads % s.kv_heads != 0)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: %d heads do not divide into %d key heads", s.heads, s.kv_heads);
-  if (s.heads != 0 && s.heads / s.kv_heads > msda::kPkChunk)
+  if (s.heads / s.kv_heads > msda::kPkChunk)
     return fail(MSDA_ERR_UNSUPPORTED, "packed attention: %d query heads to a key head (at most %d)", s.heads / s.kv_heads, msda::kPkChunk);
   // row numbers of a key head's matrix, tiles included, are formed in 32 bits
-  const int64_t group = s.heads == 0 ? 1 : s.heads / s.kv_heads, tiles = (static_cast<int64_t>(s.sequences) + 3) * msda::kPkTile;
+  const int64_t group = s.heads / s.kv_heads, tiles = (static_cast<int64_t>(s.sequences) + 3) * msda::kPkTile;
   if (s.q_rows * group + tiles >= (int64_t{1} << 31) || s.k_rows + tiles >= (int64_t{1} << 31))
     return fail(MSDA_ERR_UNSUPPORTED, "packed attention: too many rows");
   return MSDA_OK;
@@ -45,7 +45,7 @@ struct PackSplit {
 
 PackSplit pk_split(const PackShape& s) {
   const PackSplit none{1, 1 << 30};
-  if (s.heads == 0 || s.sequences == 0) return none;
+  if (s.sequences == 0) return none;
   const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads);
   const int64_t tiles = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
   const int64_t chunks = (s.k_rows / s.sequences + msda::kPkChunk - 1) / msda::kPkChunk;  // of an average sequence
@@ -80,7 +80,7 @@ int64_t pk_fwd_workspace(const PackShape& s) {
 // that makes more than kMost parts, or the tiles alone are several rounds of workgroups).
 int pk_parts(const PackShape& s) {
   constexpr int64_t kWant = 2048, kMost = 8;
-  if (s.heads == 0 || s.sequences == 0 || s.k_rows == 0) return 1;
+  if (s.sequences == 0 || s.k_rows == 0) return 1;
   const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
   // The rows of one sequence, if it is 4 times the average: a longer one takes longer parts, and batches of short
   // sequences start no second kernel (4 us).
@@ -103,7 +103,7 @@ int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
       return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: stride %d (%lld) must be a non-negative multiple of 16 bytes", i,
                   static_cast<long long>(strides[i]));
   // A tile's byte offsets are formed in 31 bits, its end from its rows: 64 rows, in the backward those of a group's heads
-  const int64_t group = s.heads == 0 ? 1 : s.heads / s.kv_heads;
+  const int64_t group = s.heads / s.kv_heads;
   for (int i = 0; i < ntensors; ++i)
     if (strides[2 * i] != 0 || strides[2 * i + 1] != 0)
       if (strides[2 * i] < s.head_dim || strides[2 * i] >= (int64_t{1} << 22) || ((i == 0 || i == 4) && strides[2 * i + 1] >= (int64_t{1} << 27) / group))
@@ -173,7 +173,7 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
   if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 4)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
-  if (q_rows == 0 || heads == 0) return MSDA_OK;
+  if (q_rows == 0) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if (q == nullptr || out == nullptr || (k_rows != 0 && (k == nullptr || v == nullptr)))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: NULL tensor pointer");
@@ -211,7 +211,7 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
   if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 8)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
-  if (heads == 0 || (grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
+  if ((grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: NULL tensor pointer");

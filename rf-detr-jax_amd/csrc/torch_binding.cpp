@@ -664,7 +664,7 @@ py::object packed_attention(const py::handle& q, const py::handle& k, const py::
     for (int64_t n : t->sizes())
       if (n >= (int64_t{1} << 31)) return py::none();
   }
-  if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || b->size(1) == 0 || a->size(1) % b->size(1) != 0 || a->size(1) > 64 * b->size(1) ||
+  if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || a->size(1) == 0 || b->size(1) == 0 || a->size(1) % b->size(1) != 0 || a->size(1) > 64 * b->size(1) ||
       a->size(2) == 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
     return py::none();
   for (const Tensor* t : {o, ko, kl})

@@ -67,7 +67,7 @@ def _check(q, k, v):
         raise ValueError(f"q, k and v must be on one device, got {q.device}, {k.device}, {v.device}")
     if k.shape != v.shape or k.shape[2] != q.shape[2]:
         raise ValueError(f"q [T, H, D] and k, v [S, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.shape[1] and (k.shape[1] == 0 or q.shape[1] % k.shape[1]):
+    if q.shape[1] == 0 or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{q.shape[1]} query heads do not divide into {k.shape[1]} key heads")
     if q.shape[1] > 64 * k.shape[1]:
         raise ValueError(f"at most 64 query heads may share a key head, got {q.shape[1]} and {k.shape[1]}")

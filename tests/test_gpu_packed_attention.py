@@ -468,7 +468,7 @@ def test_front_end_refusals():
     for args, error, text in (
             ((q.double(), k.double(), k.double(), off), TypeError, "not supported"), ((q, k.bfloat16(), k, off), TypeError, "one type"),
             ((q[0], k, k, off), ValueError, "rows, heads, D"), ((q, k, k[:5], off), ValueError, "expected"), ((q, k[..., :16], k[..., :16], off), ValueError, "expected"),
-            ((q[:, :3], k, k, off), ValueError, "divide"), ((q, k[:, :0], k[:, :0], off), ValueError, "divide"),
+            ((q[:, :3], k, k, off), ValueError, "divide"), ((q, k[:, :0], k[:, :0], off), ValueError, "divide"), ((q[:, :0], k, k, off), ValueError, "divide"),
             ((q.repeat(1, 33, 1), k, k, off), ValueError, "share"), ((q[..., :12], k[..., :12], k[..., :12], off), ValueError, "head_dim"),
             ((q.repeat(1, 1, 5), k.repeat(1, 1, 5), k.repeat(1, 1, 5), off), ValueError, "head_dim"), ((q[..., :0], k[..., :0], k[..., :0], off), ValueError, "head_dim"),
             ((q, k, k, off.float()), TypeError, "int32"), ((q, k, k, off[None]), ValueError, "offsets"), ((q, k, k, off[:0]), ValueError, "offsets"),

@@ -41,6 +41,7 @@ INVALID, UNSUPPORTED = _native.ERR_INVALID_ARGUMENT, _native.ERR_UNSUPPORTED
 @pytest.mark.parametrize("change, code, text", [
     ({"dtype": 2}, UNSUPPORTED, "dtype"), ({"n": -1}, INVALID, "negative"), ({"t": -4}, INVALID, "negative"), ({"d": 60}, UNSUPPORTED, "head_dim"),
     ({"d": 136}, UNSUPPORTED, "head_dim"), ({"d": 0}, UNSUPPORTED, "head_dim"), ({"h": 5}, INVALID, "divide"), ({"hk": 0}, INVALID, "divide"),
+    ({"h": 0}, INVALID, "divide"), ({"h": 0, "hk": 0}, INVALID, "divide"),
     ({"t": 2 ** 31 - 1}, UNSUPPORTED, "rows"), ({"s": 2 ** 31 - 1}, UNSUPPORTED, "rows"), ({"n": 2 ** 25}, UNSUPPORTED, "rows"),
     ({"scale": 0.0}, INVALID, "scale"), ({"scale": -1.0}, INVALID, "scale"), ({"scale": float("nan")}, INVALID, "scale"),
     ({"scale": float("inf")}, INVALID, "scale"), ({"q": None}, INVALID, "NULL"), ({"k": None}, INVALID, "NULL"), ({"out": None}, INVALID, "NULL"),
