@@ -598,8 +598,9 @@ struct PkStream {
 
 // A causal chunk that not every row of the workgroup sees whole: the weights of its unseen pairs are zeros, and
 // zero times an infinity or NaN of an unseen row would reach the sums. So such a tile is searched first (one
-// round of 16-byte reads and a barrier, for the chunks on the diagonal alone), values that are no finite numbers
-// become zeros, and the rows that held some are marked in `bad`, for those who see them.
+// round of 16-byte reads and a barrier, for the chunks on the diagonal alone, and the forward's first in bf16
+// where rows of fewer than 64 keys take the weights' rest), values that are no finite numbers become zeros, and
+// the rows that held some are marked in `bad`, for those who see them.
 typedef uint16_t pk_u2 __attribute__((ext_vector_type(2)));
 template <typename T, int DT>
 __device__ __forceinline__ void pk_settle(unsigned char* tile, uint32_t* bad) {
@@ -788,7 +789,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    if (min(k0 + kPkChunk, w.m) > all) {
+    // (the rest of a weight is 0 or of either sign: an infinity times it would be NaN, or the other infinity)
+    if (min(k0 + kPkChunk, w.m) > all || (sizeof(T) == 2 && k0 == 0 && all < kPkChunk)) {
       if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
       pk_settle<T, DT>(Vb, bad[turn]);
       sick = sick || pk_settled(bad[turn]) != 0;

@@ -501,3 +501,51 @@ def test_numbers_of_sequences_where_the_search_changes(count, dtype):
     k, v = _normal(28, dtype, (koff[-1], 1, 32), (koff[-1], 1, 32))
     out = packed_attention(q, k, v, _int(off), _int(koff), _int(fill))
     _compare(q, k, v, torch.zeros_like(q), (out,), PA.sequences(off, koff, fill), True)
+
+
+#        queries, keys, heads, key heads, head dim, causal; the key that is spoilt
+SEEN = {
+    "short": (40, 40, 2, 1, 64, False, 11),
+    "one_token": (1, 63, 8, 2, 128, True, 20),
+    "one_key": (5, 1, 2, 2, 32, False, 0),
+    "two_tiles": (150, 63, 4, 4, 32, False, 62),
+    "causal": (63, 63, 4, 2, 64, True, 0),
+    "chunk": (7, 50, 4, 1, 40, True, 30),
+    "short_rows_of_a_long_prompt": (200, 200, 2, 2, 96, True, 5),
+    "whole_tile": (70, 64, 2, 1, 128, False, 40),
+    "long": (30, 300, 4, 2, 64, False, 299),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("name", sorted(SEEN))
+def test_infinities_of_seen_values_come_out_as_they_are(name, dtype):
+    """Every weight of these rows is above 0, so an infinity in a channel of a value gives that infinity where it is seen,
+    both signs together and NaN give NaN; the other channels, and the rows that do not see it, keep their bits."""
+    n, m, h, hk, d, causal, key = SEEN[name]
+    _note(f"packed attention seen infinities {name} {dtype}")
+    q, k, v = _normal(29, dtype, (n + 9, h, d), (m + 9, hk, d), (m + 9, hk, d))
+    args = (_int([0, n, n + 9]), _int([0, m, m + 9]), None, causal)
+    clean = packed_attention(q, k, v, *args)
+    assert torch.isfinite(clean).all()
+    sees = max(key - (m - n), 0) if causal else 0
+    bad = v.clone()
+    bad[key, :, 3], bad[key, :, 4], bad[key, :, d - 1] = float("inf"), -float("inf"), float("nan")
+    wrong = [3, 4, d - 1]
+    if m > 1:  # a second key, seen by fewer or more rows: both signs in one channel
+        other = key - 1 if key else 1
+        bad[key, :, 6], bad[other, :, 6] = float("inf"), -float("inf")
+        wrong.append(6)
+    out = packed_attention(q, k, bad, *args)
+    last = max(key, other if m > 1 else 0)
+    first = sees if m == 1 or not causal else min(sees, max(other - (m - n), 0))
+    both = sees if m == 1 or not causal else max(last - (m - n), 0)
+    rest = [c for c in range(d) if c not in wrong]
+    assert torch.equal(out[:first], clean[:first]) and torch.equal(out[n:], clean[n:])
+    assert torch.equal(out[:n, :, rest], clean[:n, :, rest])
+    for at, value in ((3, float("inf")), (4, -float("inf"))):
+        assert torch.equal(out[sees:n, :, at], torch.full_like(out[sees:n, :, at], value))
+        assert torch.equal(out[:sees, :, at], clean[:sees, :, at])
+    assert torch.isnan(out[sees:n, :, d - 1]).all()
+    if m > 1:
+        assert torch.isnan(out[both:n, :, 6]).all()
