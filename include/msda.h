@@ -455,8 +455,7 @@ int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float
  * 2^27 elements. At most 64 query heads to a key head. scale: 2^-64 to 2^64. q_rows * heads / kv_heads and k_rows below 2^31 less 128
  * rows a sequence.
  * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
- * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them and uses entries 2
- * and 3 between its kernels. May be NULL in a forward whose backward is not wanted.
+ * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them. May be NULL in a forward whose backward is not wanted.
  * out_rest: NULL, or for bf16 a tensor of out's strides: the forward writes what out's rounding left, the
  * backward reads out + out_rest for rowsum(grad_out * out), whose error is then that of f32 sums.
  * Sums, softmax and statistics are f32; bf16 products run on bf16 matrix instructions, with the softmax
@@ -481,7 +480,8 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
 
 /*
  * Backward of msda_packed_attention_fwd for the cotangent grad_out: grad_q, grad_k, grad_v (each may be
- * NULL to skip it). out, out_rest and stats are the forward's (stats entries 2 and 3 are overwritten).
+ * NULL to skip it). out, out_rest and stats are the forward's. Entries 2 and 3 of stats are overwritten: two calls
+ * with one stats have to come one behind the other (msda_packed_attention_bwd_const otherwise).
  * strides: [8 tensors: q, k, v, out, grad_out, grad_q, grad_k, grad_v][2].
  */
 int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
@@ -490,6 +490,17 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
                               const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads,
                               int kv_heads, int head_dim, const int64_t* strides, int causal, float scale,
                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same with stats left as they are. row_numbers: [q_rows * heads][4] f32, 16-byte aligned, which the call
+ * uses between its kernels (NULL when neither grad_k nor grad_v is wanted).
+ */
+int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                                    const float* stats, float* row_numbers, const void* grad_out, int dtype,
+                                    void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets,
+                                    const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows,
+                                    int k_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
+                                    int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- Rotary positions on several axes -------------------------------------------------------
  * Rotates channel pairs of queries and keys by angles that grow with the token's position on each of

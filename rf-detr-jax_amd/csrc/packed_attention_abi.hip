@@ -203,20 +203,22 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_fwd<msda::bf16_t>(p, st) : msda_host::dispatch_pk_fwd<float>(p, st);
 }
 
-int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, float* stats,
-                              const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
-                              const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
-                              const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* stats,
+                                    float* row_numbers, const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
+                                    const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows,
+                                    int heads, int kv_heads, int head_dim, const int64_t* strides, int causal, float scale, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
   if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 8)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
   if ((grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
-  if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)))
+  if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)) ||
+      (q_rows != 0 && row_numbers == nullptr && (grad_k != nullptr || grad_v != nullptr)))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: NULL tensor pointer");
   if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) || !aligned_to(out_rest, 16) || !aligned_to(stats, 16) ||
-      !aligned_to(grad_out, 16) || !aligned_to(grad_q, 16) || !aligned_to(grad_k, 16) || !aligned_to(grad_v, 16))
+      !aligned_to(row_numbers, 16) || !aligned_to(grad_out, 16) || !aligned_to(grad_q, 16) || !aligned_to(grad_k, 16) || !aligned_to(grad_v, 16))
     return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: tensors must be aligned to 16 bytes");
   static const int order[8] = {msda::kPkQ, msda::kPkK, msda::kPkV, msda::kPkO, msda::kPkGO, msda::kPkGQ, msda::kPkGK, msda::kPkGV};
   msda::PackParams p = pk_params(s, q_offsets, k_offsets, k_lengths, strides, 8, order, causal, scale);
@@ -229,7 +231,8 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
   p.gq = grad_q;
   p.gk = grad_k;
   p.gv = grad_v;
-  p.stats = stats;
+  p.stats = const_cast<float*>(stats);  // (the backward reads it)
+  p.numbers = grad_k != nullptr || grad_v != nullptr ? row_numbers : nullptr;
   if (grad_k != nullptr || grad_v != nullptr) p.splits = pk_parts(s);
   if (p.splits > 1) {
     const int64_t need = pk_bwd_workspace(s);
@@ -242,6 +245,14 @@ int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_bwd<msda::bf16_t>(p, q_slots, k_slots, st)
                                   : msda_host::dispatch_pk_bwd<float>(p, q_slots, k_slots, st);
+}
+
+int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, float* stats,
+                              const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets, const int32_t* k_offsets,
+                              const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim,
+                              const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  return msda_packed_attention_bwd_const(q, k, v, out, out_rest, stats, stats, grad_out, dtype, grad_q, grad_k, grad_v, q_offsets, k_offsets, k_lengths,
+                                         sequences, q_rows, k_rows, heads, kv_heads, head_dim, strides, causal, scale, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

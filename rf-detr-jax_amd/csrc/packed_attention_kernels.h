@@ -49,7 +49,9 @@ struct PackParams {
   void* gq;  // backward outputs (each may be null)
   void* gk;
   void* gv;
-  float* stats;  // [q_rows * heads][4]: m, log2 l (forward); two numbers of the backward (pk_bwd_q_kernel); row (token, head)
+  float* stats;    // [q_rows * heads][4]: m, log2 l (forward; the backward reads them); row (token, head)
+  float* numbers;  // backward: the same and two numbers more (pk_bwd_q_kernel), for the key side; stats itself, or a
+                   // buffer of the call; null when neither gk nor gv is wanted
   const int32_t* q_offsets;  // [sequences + 1]
   const int32_t* k_offsets;  // [sequences + 1]
   const int32_t* k_lengths;  // [sequences], or null: all rows of a sequence's range
@@ -1019,7 +1021,7 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
     *reinterpret_cast<float2*>(p.stats + 4 * row) = pk_stats(m, l);
 }
 
-// dq, and delta into the statistics for the key side (alone when gq is null).
+// dq, and the rows' numbers for the key side (alone when gq is null).
 template <typename T, int DT>
 __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_q_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
@@ -1065,12 +1067,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       }
     }
     delta = at_sum_halves(delta);
-    float* st = p.stats + 4 * w.stat(p, rc);
-    m = st[0];
-    ll = st[1];
+    const int64_t row = 4 * w.stat(p, rc);
+    m = p.stats[row];
+    ll = p.stats[row + 1];
     // for the key side: delta; bf16: -delta and -(m + log2 l) / scale2, which its sums start from (the weight is
     // 2^(scale2 s) then; the number is rounded at its own size, 2^-24 of it)
-    if (valid && grp == 0) *reinterpret_cast<float2*>(st + 2) = sizeof(T) == 2 ? float2{-delta, -(m + ll) / p.scale2} : float2{delta, 0.0f};
+    if (p.numbers != nullptr && valid && grp == 0)
+      *reinterpret_cast<at_f4*>(p.numbers + row) = sizeof(T) == 2 ? at_f4{m, ll, -delta, -(m + ll) / p.scale2} : at_f4{m, ll, delta, 0.0f};
   }
   if (gq == nullptr) return;
   constexpr bool bf = sizeof(T) == 2;
@@ -1262,7 +1265,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     for (int j = 0; j < KEEP; ++j) *reinterpret_cast<at_bf8*>(kept_rows + threadIdx.x * 16 + j * kPkWaves * 1024) = v.x[DT / 16 - KEEP + j];
   const T* qp = static_cast<const T*>(p.q) + w.q_first * p.st[kPkQ][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkQ][1];
   const T* gp = static_cast<const T*>(p.go) + w.q_first * p.st[kPkGO][0] + static_cast<int64_t>(w.kv_head) * p.group * p.st[kPkGO][1];
-  const float* sp = p.stats + 4 * (static_cast<int64_t>(w.q_first) * p.heads + w.kv_head * p.group);
+  const float* sp = p.numbers + 4 * (static_cast<int64_t>(w.q_first) * p.heads + w.kv_head * p.group);
   const int per = (w.chunks + w.parts - 1) / w.parts, c0 = w.part * per, c1 = min(w.chunks, c0 + per);
   at_f16 dk[DT / 32], dv[DT / 32];
 #pragma unroll

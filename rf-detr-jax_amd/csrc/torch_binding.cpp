@@ -52,7 +52,7 @@ struct Library {
   decltype(&msda_attention_fwd) attention_fwd;
   decltype(&msda_attention_bwd) attention_bwd;
   decltype(&msda_packed_attention_fwd) packed_fwd;
-  decltype(&msda_packed_attention_bwd) packed_bwd;
+  decltype(&msda_packed_attention_bwd_const) packed_bwd;
   decltype(&msda_packed_attention_fwd_workspace_size) packed_fwd_workspace_size;
   decltype(&msda_packed_attention_bwd_workspace_size) packed_bwd_workspace_size;
   decltype(&msda_rotary) rotary;
@@ -80,7 +80,7 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_attention_fwd", lib.attention_fwd);
   get("msda_attention_bwd", lib.attention_bwd);
   get("msda_packed_attention_fwd", lib.packed_fwd);
-  get("msda_packed_attention_bwd", lib.packed_bwd);
+  get("msda_packed_attention_bwd_const", lib.packed_bwd);
   get("msda_packed_attention_fwd_workspace_size", lib.packed_fwd_workspace_size);
   get("msda_packed_attention_bwd_workspace_size", lib.packed_bwd_workspace_size);
   get("msda_rotary", lib.rotary);
@@ -627,6 +627,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     const Packed p(q, k, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
     const auto like = [](bool wanted, const Tensor& t) { return wanted ? at::empty(t.sizes(), t.options()) : Tensor(); };
     Tensor gq = like(ctx->needs_input_grad(0), q), gk = like(ctx->needs_input_grad(1), k), gv = like(ctx->needs_input_grad(2), v), ws;
+    // what the kernels hand on: other calls may read the statistics
+    const Tensor numbers = like(gk.defined() || gv.defined(), stats);
     const int64_t bytes = gk.defined() || gv.defined()
                               ? lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim)
                               : 0;
@@ -640,7 +642,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         st[2 * i + 1] = t[i]->stride(1);
       }
     launch(q, [&](void* stream) {
-      return lib.packed_bwd(ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), fptr(stats), ptr(g), code(q), ptr(gq), ptr(gk), ptr(gv), iptr(offsets),
+      return lib.packed_bwd(ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), fptr(stats), fptr(numbers), ptr(g), code(q), ptr(gq), ptr(gk), ptr(gv), iptr(offsets),
                             iptr(key_offsets), iptr(key_lengths), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale,
                             ptr(ws), bytes, stream);
     });

@@ -60,6 +60,7 @@ SIGNATURES = {
     "msda_packed_attention_bwd_workspace_size": ([_I] * 7, _I64),
     "msda_packed_attention_fwd": ([_P, _P, _P, _I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
     "msda_packed_attention_bwd": ([_P] * 7 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
+    "msda_packed_attention_bwd_const": ([_P] * 8 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
     "msda_rotary": ([_P] * 4 + [_I, _P] + [_I] * 5 + [_P] * 3 + [_I, ctypes.c_double] + [_I] * 3 + [_P], _I),
     # include/msda_probe.h
     "msda_probe_lds_read": ([_P, _I, _I, _P], _I),

@@ -8,7 +8,7 @@
   autograd.
 
 The lengths stay on the GPU: nothing is read back, so a call can be captured into a graph and replayed
-with other lengths. Both directions run in HIP kernels (``msda_packed_attention_fwd`` / ``_bwd``). There is
+with other lengths. Both directions run in HIP kernels (``msda_packed_attention_fwd`` / ``_bwd_const``). There is
 no CPU path. No counterpart in the reference.
 """
 
@@ -130,9 +130,11 @@ def _backward(q, k, v, out, rest, stats, grad_out, seq, causal, scale, needs):
         nbytes = lib.msda_packed_attention_bwd_workspace_size(code, *dims) if needs[1] or needs[2] else 0
         _native.check(min(nbytes, 0))
         ws = _native.workspace(nbytes, q.device) if nbytes else None
-        rc = lib.msda_packed_attention_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(stats), _ptr(grad_out), code,
-                                           *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), *dims,
-                                           _strides((q, k, v, out, grad_out, *grads)), int(causal), scale, _ptr(ws), nbytes, _stream(q.device))
+        numbers = torch.empty_like(stats) if needs[1] or needs[2] else None  # what the kernels hand on: other calls may read stats
+        rc = lib.msda_packed_attention_bwd_const(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(stats), _ptr(numbers), _ptr(grad_out), code,
+                                                 *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), *dims,
+                                                 _strides((q, k, v, out, grad_out, *grads)), int(causal), scale, _ptr(ws), nbytes,
+                                                 _stream(q.device))
     _native.check(rc)
     return grads
 
@@ -150,7 +152,7 @@ def packed_attention_forward(q, k, v, offsets, key_offsets=None, key_lengths=Non
 def packed_attention_backward(q, k, v, out, saved, grad_out, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None,
                               needs=(True, True, True)):
     """``(grad_q, grad_k, grad_v)``, contiguous, for the cotangent ``grad_out`` of ``out``; ``out`` and
-    ``saved`` as :func:`packed_attention_forward` gave them. None where ``needs`` says so."""
+    ``saved`` as :func:`packed_attention_forward` gave them, which are only read. None where ``needs`` says so."""
     _check(q, k, v)
     stats, rest = saved
     if any(t.shape != q.shape for t in (out, grad_out, *(() if rest is None else (rest,)))) or tuple(stats.shape) != (*q.shape[:2], 4):

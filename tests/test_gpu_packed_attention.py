@@ -549,3 +549,30 @@ def test_infinities_of_seen_values_come_out_as_they_are(name, dtype):
     assert torch.isnan(out[sees:n, :, d - 1]).all()
     if m > 1:
         assert torch.isnan(out[both:n, :, 6]).all()
+
+
+@TYPES
+def test_backward_leaves_what_the_forward_saved(dtype):
+    """The statistics and the rest are read alone: one forward serves several cotangents, on two streams at once, too."""
+    off = _int([0, 300, 513, 600])
+    q, k, v, g, g2 = _normal(30, dtype, (600, 8, 64), (600, 2, 64), (600, 2, 64), (600, 8, 64), (600, 8, 64))
+    out, (stats, rest) = packed_attention_forward(q, k, v, off)
+    stats[..., 2:] = 7.0  # (no part of the statistics)
+    before = [None if x is None else x.clone() for x in (out, stats, rest)]
+    want = [packed_attention_backward(q, k, v, out, (stats, rest), x, off) for x in (g, g2)]
+    for x, y in zip((out, stats, rest), before):
+        assert (x is None and y is None) or torch.equal(x, y)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for x, s in zip((g, g2), streams):
+            with torch.cuda.stream(s):
+                got.append(packed_attention_backward(q, k, v, out, (stats, rest), x, off))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    # the autograd function: one graph, two cotangents
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = packed_attention(*leaves, off)
+    got = [torch.autograd.grad(out, leaves, x, retain_graph=True) for x in (g, g2, g)]
+    assert all(torch.equal(a, b) for x, y in zip(got, (*want, want[0])) for a, b in zip(x, y))

@@ -113,3 +113,21 @@ def test_front_end_refuses_cpu_tensors_and_other_types():
         packed_attention(x, x, x, off)
     with pytest.raises(RuntimeError, match="no CPU path"):
         rotary_embed(x, x, torch.zeros(4, 1, dtype=torch.int32), (16,))
+
+
+def test_attention_backward_with_row_numbers_of_its_own():
+    lib, strides = _native.lib(), _i64(*([256, 64] * 8))
+
+    def call(numbers, **kw):
+        a = dict(stats=PTR, go=PTR, gq=PTR, gk=PTR, gv=PTR, scale=0.125, d=64)
+        a.update(kw)
+        rc = lib.msda_packed_attention_bwd_const(PTR, PTR, PTR, PTR, None, a["stats"], numbers, a["go"], 1, a["gq"], a["gk"], a["gv"], PTR, PTR, None,
+                                                 1, 4, 4, 4, 2, a["d"], strides, 1, a["scale"], None, 0, None)
+        return rc, lib.msda_last_error().decode()
+
+    for numbers, change, code, text in ((None, {}, INVALID, "NULL"), (None, {"gq": None, "gk": None}, INVALID, "NULL"), (ODD, {}, INVALID, "16 bytes"),
+                                        (PTR, {"stats": None}, INVALID, "NULL"), (PTR, {"go": None}, INVALID, "NULL"), (PTR, {"scale": 0.0}, INVALID, "scale"),
+                                        (PTR, {"d": 60}, UNSUPPORTED, "head_dim")):
+        rc, msg = call(numbers, **change)
+        assert rc == code and text in msg, (rc, msg)
+    assert call(None, gq=None, gk=None, gv=None)[0] == 0
