@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       // products of one wave; a CU's other workgroup fills the rest.
       using P = PkProducts<T, DT>;
       constexpr int KS = P::kScores, HA = KS >= 4 ? KS / 2 - 1 : 1, HB = KS - 1 - HA;  // steps up to the maximum, behind it
-      float bm, alpha = 1.0f;
+      float bm, alpha = 1.0f, late = 1.0f;  // late: what scales the first half's weights after their rounding
       // step t of the softmax of block x, whose keys start at k: x = scale2 s - m and its maximum, m moved if it
       // has to, weights and their sum (a lane sums its half of the keys until the end)
       auto soft = [&](at_f16& x, int k, auto step) {
@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
         if (__any(alpha != 1.0f)) {
 #pragma unroll
           for (int nd = 0; nd < DT / 32; ++nd) o[nd] *= alpha;
-          if constexpr (phase == 2) s0 *= alpha;  // (for the rounding's rest below)
+          if constexpr (phase == 2) late = alpha;
           alpha = 1.0f;
         }
       };
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       // out over few keys, and delta, from the output, carries them into every ds of the row, where they are as large
       // as those of ds's own rounding. (60 calls of 1 to 8 sequences of 1 to 600 rows: 7 of 240 results were more than
       // 1.5 times as far off as the exact ones rounded, with this and the same for dq 1.)
-      if (k0 == 0 && few) pk_accumulate2<T, DT, 2>(o, V, pk_rest(s0), o, V + 32 * Tile::ROW, pk_rest(s1), at);
+      if (k0 == 0 && few) pk_accumulate2<T, DT, 2>(o, V, pk_rest(s0) * late, o, V + 32 * Tile::ROW, pk_rest(s1), at);
     } else {
       next.all();
       pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);

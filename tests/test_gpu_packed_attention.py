@@ -576,3 +576,22 @@ def test_backward_leaves_what_the_forward_saved(dtype):
     out = packed_attention(*leaves, off)
     got = [torch.autograd.grad(out, leaves, x, retain_graph=True) for x in (g, g2, g)]
     assert all(torch.equal(a, b) for x, y in zip(got, (*want, want[0])) for a, b in zip(x, y))
+
+
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("late", [False, True], ids=["level", "late_maximum"])
+def test_short_bf16_rows_keep_what_the_weights_rounding_left(late, causal):
+    """Rows of fewer than 64 keys. A weight is the sum of two bf16 numbers, off by half a step of half a step (2^-16 of it);
+    the result rounds once. With a late maximum the last keys outweigh the first 32, whose values are as much
+    larger, by 2^11: the rest of those weights is scaled with them."""
+    n, d = 60, 64
+    q, k, v = _normal(31, torch.bfloat16, (n, 4, d), (n, 2, d), (n, 2, d))
+    if late:
+        q[..., 0], k[..., 0] = 8, 0
+        k[32:, :, 0] = 8  # 8 of a score: 11.5 of its log2
+        v[:32] *= 2.0 ** 11
+    out = packed_attention(q, k, v, _int([0, n]), causal=causal)
+    arrays, seqs = [_np(x) for x in (q, k, v)], PA.sequences([0, n])
+    want = PA.attention(*arrays, seqs, causal)
+    bound = PA.bounds(*arrays, np.zeros_like(arrays[0]), seqs, 2.0 ** -16, causal)[0]
+    _within(out, want, (1 + 2.0 ** -8) * bound + 2.0 ** -8 * np.abs(want), "out")
