@@ -95,7 +95,8 @@ int64_t pk_bwd_workspace(const PackShape& s) {
   return parts == 1 ? 0 : static_cast<int64_t>(parts) * 2 * s.k_rows * s.kv_heads * s.head_dim * 4;
 }
 
-int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
+template <int ntensors>
+int pk_strides(const PackShape& s, const int64_t* strides, const void* const (&tensors)[ntensors]) {
   if (strides == nullptr) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: NULL strides");
   const int64_t e = s.dtype == MSDA_DTYPE_BF16 ? 8 : 4;
   for (int i = 0; i < 2 * ntensors; ++i)
@@ -105,7 +106,7 @@ int pk_strides(const PackShape& s, const int64_t* strides, int ntensors) {
   // A tile's byte offsets are formed in 31 bits, its end from its rows: 64 rows, in the backward those of a group's heads
   const int64_t group = s.heads / s.kv_heads;
   for (int i = 0; i < ntensors; ++i)
-    if (strides[2 * i] != 0 || strides[2 * i + 1] != 0)
+    if (tensors[i] != nullptr || strides[2 * i] != 0 || strides[2 * i + 1] != 0)
       if (strides[2 * i] < s.head_dim || strides[2 * i] >= (int64_t{1} << 22) || ((i == 0 || i == 4) && strides[2 * i + 1] >= (int64_t{1} << 27) / group))
         return fail(MSDA_ERR_UNSUPPORTED, "packed attention: strides %lld, %lld of tensor %d: rows must lie head_dim to 2^22 elements apart, the heads of a group within 2^27",
                     static_cast<long long>(strides[2 * i]), static_cast<long long>(strides[2 * i + 1]), i);
@@ -172,7 +173,7 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
-  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 4)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides<4>(s, strides, {q, k, v, out})) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
   if (q_rows == 0) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if (q == nullptr || out == nullptr || (k_rows != 0 && (k == nullptr || v == nullptr)))
@@ -211,7 +212,9 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
-  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides(s, strides, 8)) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides<8>(s, strides, {q, k, v, out, grad_out, grad_q, grad_k, grad_v})) != MSDA_OK ||
+      (rc = pk_scale(scale)) != MSDA_OK)
+    return rc;
   if ((grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if ((q_rows != 0 && (q == nullptr || out == nullptr || stats == nullptr || grad_out == nullptr)) || (k_rows != 0 && (k == nullptr || v == nullptr)) ||

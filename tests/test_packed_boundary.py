@@ -131,3 +131,16 @@ def test_attention_backward_with_row_numbers_of_its_own():
         rc, msg = call(numbers, **change)
         assert rc == code and text in msg, (rc, msg)
     assert call(None, gq=None, gk=None, gv=None)[0] == 0
+
+
+@pytest.mark.parametrize("direction", ["fwd", "bwd"])
+def test_rows_on_top_of_each_other_are_refused(direction):
+    """Strides of 0 stand for a tensor that is not there: a gradient that is not wanted."""
+    tensors = 4 if direction == "fwd" else 8
+    for i in range(tensors):
+        strides = [256, 64] * tensors
+        strides[2 * i:2 * i + 2] = [0, 0]
+        rc, msg = _attention(direction, strides=_i64(*strides))
+        assert rc == UNSUPPORTED and "apart" in msg, (i, rc, msg)
+    if direction == "bwd":
+        assert _attention(direction, strides=_i64(*([256, 64] * 5 + [0, 0] * 3)), gq=None, gk=None, gv=None)[0] == 0
