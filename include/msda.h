@@ -452,7 +452,7 @@ int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float
  * head_dim: a multiple of 8, at most 128. `strides` holds the element strides (row, head) of each
  * tensor (0, 0 for one that is NULL); channels are contiguous, and rows start on 16-byte boundaries (bases, and strides in bytes, are
  * multiples of 16), head_dim to 2^22 elements apart, q's and grad_out's heads of a key head within
- * 2^27 elements. At most 64 query heads to a key head. scale: 2^-64 to 2^64. q_rows * heads / kv_heads and k_rows below 2^31 less 128
+ * 2^27 elements. At most 64 query heads to a key head; backward: fewer than 2^21 key heads. scale: 2^-64 to 2^64. q_rows * heads / kv_heads and k_rows below 2^31 less 128
  * rows a sequence.
  * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
  * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them. May be NULL in a forward whose backward is not wanted.

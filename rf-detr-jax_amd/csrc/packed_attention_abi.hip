@@ -36,6 +36,14 @@ int pk_shape(const PackShape& s) {
   return MSDA_OK;
 }
 
+int pk_bwd_shape(const PackShape& s) {
+  const int rc = pk_shape(s);
+  if (rc != MSDA_OK) return rc;
+  // The key side forms the byte offsets of a tile's row numbers in 31 bits: at most 64 / group tokens of `heads` times 16 bytes.
+  if (s.kv_heads >= 1 << 21) return fail(MSDA_ERR_UNSUPPORTED, "packed attention backward: %d key heads (fewer than 2^21 supported)", s.kv_heads);
+  return MSDA_OK;
+}
+
 // The forward's split of the keys over workgroups: how many at most share a tile of rows, and the chunks of 64 keys
 // that make one worth it. The lengths are not known here, only their sums; a workgroup finds its tile's number
 // of parts from the length (PkParts).
@@ -162,7 +170,7 @@ int64_t msda_packed_attention_fwd_workspace_size(int dtype, int sequences, int q
 int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
-  const int rc = pk_shape(s);
+  const int rc = pk_bwd_shape(s);
   return rc != MSDA_OK ? rc : pk_bwd_workspace(s);
 }
 
@@ -212,7 +220,7 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
-  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides<8>(s, strides, {q, k, v, out, grad_out, grad_q, grad_k, grad_v})) != MSDA_OK ||
+  if ((rc = pk_bwd_shape(s)) != MSDA_OK || (rc = pk_strides<8>(s, strides, {q, k, v, out, grad_out, grad_q, grad_k, grad_v})) != MSDA_OK ||
       (rc = pk_scale(scale)) != MSDA_OK)
     return rc;
   if ((grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;

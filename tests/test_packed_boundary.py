@@ -144,3 +144,10 @@ def test_rows_on_top_of_each_other_are_refused(direction):
         assert rc == UNSUPPORTED and "apart" in msg, (i, rc, msg)
     if direction == "bwd":
         assert _attention(direction, strides=_i64(*([256, 64] * 5 + [0, 0] * 3)), gq=None, gk=None, gv=None)[0] == 0
+
+
+def test_key_heads_whose_row_numbers_pass_31_bits_are_refused():
+    """A tile's numbers lie up to 64 rows of all heads apart, 16 bytes each: 2^21 key heads head-major, whatever the group."""
+    for hk, group in ((1 << 21, 1), (1 << 21, 2), (1 << 24, 1)):
+        rc, msg = _attention("bwd", t=64, s=64, h=hk * group, hk=hk, d=8, strides=_i64(*([8, 512] * 8)))
+        assert rc == UNSUPPORTED and "key heads" in msg, (rc, msg)
