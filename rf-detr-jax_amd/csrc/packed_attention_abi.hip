@@ -13,9 +13,9 @@ namespace {
 using msda_host::aligned_to;
 using msda_host::fail;
 
-struct PackShape {
-  int dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim;
-};
+using msda::PackShape;
+using msda::PackSplit;
+using msda::pk_split;
 
 int64_t slots_of(int64_t rows, int sequences) { return rows / msda::kPkTile + sequences + 2; }
 
@@ -42,39 +42,6 @@ int pk_bwd_shape(const PackShape& s) {
   // The key side forms the byte offsets of a tile's row numbers in 31 bits: at most 64 / group tokens of `heads` times 16 bytes.
   if (s.kv_heads >= 1 << 21) return fail(MSDA_ERR_UNSUPPORTED, "packed attention backward: %d key heads (fewer than 2^21 supported)", s.kv_heads);
   return MSDA_OK;
-}
-
-// The forward's split of the keys over workgroups: how many at most share a tile of rows, and the chunks of 64 keys
-// that make one worth it. The lengths are not known here, only their sums; a workgroup finds its tile's number
-// of parts from the length (PkParts).
-struct PackSplit {
-  int most, part;
-};
-
-PackSplit pk_split(const PackShape& s) {
-  const PackSplit none{1, 1 << 30};
-  if (s.sequences == 0) return none;
-  const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads);
-  const int64_t tiles = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
-  const int64_t chunks = (s.k_rows / s.sequences + msda::kPkChunk - 1) / msda::kPkChunk;  // of an average sequence
-  if (tiles == 0) return none;
-  // The work in parts that even out over the CUs: in bf16 one to each of the two workgroups that a CU holds; in f32,
-  // whose products one workgroup alone keeps busy, 8 to a CU. One sequence of 6,000 tokens, 8 heads, causal (376 tiles,
-  // the last of 94 chunks), us a call: bf16, 128 channels 131 with a workgroup a tile, 107 in 512 parts, 114 in
-  // 2048; f32, 64 channels 532, 432 and 360. (Batches whose tiles even out by themselves pay for it: 512 tiles of 16
-  // chunks in f32 175 us for 145.)
-  const bool bf = s.dtype == MSDA_DTYPE_BF16;
-  const int64_t wanted = bf ? 512 : 2048, even = (tiles * chunks + wanted - 1) / wanted;
-  // Few rows to a tile (new tokens over caches): a part's own cost is small against its keys, so calls of any size
-  // are split, because the longest cache would set their time. Full tiles: a part writes and the join reads 128
-  // rows of f32 sums, the time of about 6 chunks of keys at 128 channels in bf16; in f32 (300 keys, 32 channels) parts of
-  // 2 chunks cost 41 us for 31.
-  const bool few = rows <= int64_t{32} * s.sequences;
-  const int64_t part = few ? std::clamp<int64_t>(even, 2, 16) : std::max<int64_t>(even, bf ? 6 : 8);
-  if (chunks <= part) return none;
-  // An average sequence's parts, for full tiles twice those (a longer one's are longer)
-  const int64_t most = std::min<int64_t>((few ? 1 : 2) * ((chunks + part - 1) / part), msda::kPkMostParts - 2);
-  return PackSplit{static_cast<int>(most) + 2, static_cast<int>(part)};  // (PkParts: room for two more)
 }
 
 // Bytes of the split forward's parts: f32 sums, (m, l) of every row and part, the rows' numbers of parts.

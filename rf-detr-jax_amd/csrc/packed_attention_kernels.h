@@ -33,6 +33,7 @@
 
 #include "attention_common.h"
 #include "msda_kernels.h"  // bf16_t, wait_vmem
+#include "packed_attention_parts.h"
 
 namespace msda {
 
@@ -68,10 +69,6 @@ struct PackParams {
   float scale2;  // scale log2(e)
 };
 
-constexpr int kPkWaves = 4;              // of a workgroup
-constexpr int kPkTile = 32 * kPkWaves;   // own rows of a workgroup: 32 a wave
-constexpr int kPkChunk = 64;             // streamed rows of a tile
-constexpr int kPkMostParts = 64;  // of a forward tile's keys
 constexpr int kPkPart = 32;  // chunks of a workgroup on the key side, unless that makes more parts than the host gave room for
 constexpr int kPkJoin = 32;   // workgroups that join a key tile's parts
 
@@ -195,36 +192,6 @@ struct PkRange {
     first = min(max(p.k_offsets[seq], 0), p.k_rows);
     const int end = min(max(p.k_offsets[seq + 1], first), p.k_rows);
     count = p.k_lengths != nullptr ? min(max(p.k_lengths[seq], 0), end - first) : end - first;
-  }
-};
-
-// The split forward: how many workgroups share tile i of a sequence of n queries and m keys. At least p.part chunks
-// of keys each (more where a long sequence would make more parts than p.splits); a causal sequence's
-// tiles see 2 / G chunks more from one to the next, so every `step` tiles make one part more, from the first tile
-// that sees a key on, and the parts of the first x tiles have a closed form. With c chunks seen by the last tile
-// and the tile sizes' roundings it has fewer than 1 + (c + 2) / part parts, at most room + 2 = p.splits.
-struct PkParts {
-  int first, from, step;
-  __device__ __forceinline__ PkParts(const PackParams& p, int n, int m) {
-    const int shift = m - n, most = (m + kPkChunk - 1) / kPkChunk, room = p.splits - 2;  // most: chunks that the last tile sees
-    const int part = most <= p.part * room ? p.part : (most + room - 1) / room;
-    int chunks = most;  // that the first tile with keys sees
-    from = 0;
-    step = 1 << 30;
-    if (p.causal && n * p.group > kPkTile) {
-      from = shift < 0 ? -shift * p.group / kPkTile : 0;
-      step = (part * p.group + 1) / 2;
-      const int token = (min((from + 1) * kPkTile, n * p.group) - 1) / p.group;
-      chunks = (min(max(token + shift + 1, 0), m) + kPkChunk - 1) / kPkChunk;
-    }
-    first = max((chunks + part - 1) / part, 1);
-  }
-  __device__ __forceinline__ int of(int tile) const { return tile - from < step ? first : first + (tile - from) / step; }
-  __device__ __forceinline__ int before(int x) const {
-    const int y = max(x - from, 0);
-    if (y <= step) return x * first;
-    const int q = y / step;
-    return x * first + q * (q - 1) / 2 * step + q * (y - q * step);
   }
 };
 
@@ -680,7 +647,7 @@ struct PkQueries {
       w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, line, p.slots, lane, true, [&](int s, int n) {
         const int tiles = pk_tiles(n, p.group);
         const PkRange keys(p, min(max(s - 1, 0), p.sequences - 1));
-        return s >= 1 && s <= p.sequences ? PkParts(p, n, keys.count).before(tiles) : tiles;
+        return s >= 1 && s <= p.sequences ? PkParts(p.splits, p.part, p.causal != 0, p.group, n, keys.count).before(tiles) : tiles;
       });
     }
     rows = w.own * p.group;
@@ -691,7 +658,7 @@ struct PkQueries {
       k_first = keys.first;
       m = keys.count;
       if (shared) {
-        const PkParts all(p, w.own, m);
+        const PkParts all(p.splits, p.part, p.causal != 0, p.group, w.own, m);
         if (counted) {  // the tile of the sequence's part w.tile: the last one before which no more parts lie
           int lo = 0, hi = pk_tiles(w.own, p.group);
           while (hi - lo > 1) {

@@ -30,7 +30,7 @@ SOURCES = [os.path.join(CSRC, f) for f in ("msda_abi.hip", "msda_fwd_f32.hip", "
                                            "packed_attention_bwd_bf16.hip", "rotary_abi.hip", "probe_abi.hip")]
 HEADERS = [os.path.join(CSRC, f) for f in ("msda_kernels.h", "msda_band_kernels.h", "msda_gather_kernels.h", "msda_fused_bwd_kernels.h", "msda_launch.h", "grid_sample_kernels.h",
                                            "value_proj_kernels.h", "value_proj_mfma_kernels.h", "attention_common.h", "attention_kernels.h",
-                                           "attention_split_kernels.h", "packed_attention_kernels.h", "packed_attention_launch.h",
+                                           "attention_split_kernels.h", "packed_attention_kernels.h", "packed_attention_launch.h", "packed_attention_parts.h",
                                            "rotary_kernels.h")] + [
     os.path.join(INCLUDE, "msda.h"), os.path.join(INCLUDE, "msda_probe.h")]
 BUILD_DIR = os.path.join(ROOT, "_build")

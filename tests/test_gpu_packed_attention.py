@@ -595,3 +595,30 @@ def test_short_bf16_rows_keep_what_the_weights_rounding_left(late, causal):
     want = PA.attention(*arrays, seqs, causal)
     bound = PA.bounds(*arrays, np.zeros_like(arrays[0]), seqs, 2.0 ** -16, causal)[0]
     _within(out, want, (1 + 2.0 ** -8) * bound + 2.0 ** -8 * np.abs(want), "out")
+
+
+#      lengths, keys, heads, key heads, head dim: the numbers of parts of a sequence's tiles grow
+GROWING = {
+    "prompts": ([1500, 400, 33], None, 8, 8, 64),
+    "group_of_three": ([1100, 700], None, 6, 2, 32),
+    "fewer_keys": ([1500, 900], [1100, 900], 4, 4, 40),  # tiles without keys in front
+    "more_keys": ([900, 640, 2], [1700, 700, 500], 2, 2, 128),
+    "seventy_tiles": ([4250], None, 2, 1, 32),
+    "seventy_sequences": ([300 + i * 397 % 500 for i in range(70)], None, 1, 1, 32),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("name", sorted(GROWING))
+def test_tiles_with_more_parts_the_more_keys_they_see(name, dtype):
+    from rfdetr_jax_amd import _native
+
+    lengths, keys, h, hk, d = GROWING[name]
+    keys = lengths if keys is None else keys
+    _note(f"packed attention parts {name} {dtype}")
+    off, koff = np.cumsum([0, *lengths]), np.cumsum([0, *keys])
+    code = _native.DTYPE_BF16 if dtype == torch.bfloat16 else _native.DTYPE_F32
+    assert _native.lib().msda_packed_attention_fwd_workspace_size(code, len(lengths), off[-1], koff[-1], h, hk, d) > 0
+    q, k, v, g = _normal(32, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d), (off[-1], h, d))
+    got = _run(q, k, v, g, _int(off), _int(koff))
+    _compare(q, k, v, g, got, PA.sequences(off, koff), True)
