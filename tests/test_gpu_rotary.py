@@ -166,3 +166,35 @@ def test_refusals_and_second_derivatives():
     (grad,) = torch.autograd.grad(rotary_embed(leaf, None, pos, (8, 8)), [leaf], g, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate"):
         torch.autograd.grad(grad.sum(), [leaf])
+
+
+@TYPES
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "neighbours"])
+def test_int64_positions_past_32_bits_against_oracle(interleaved, dtype):
+    """Positions of 2^33 to 2^36 of either sign, whose low 32 bits are other positions. Beside the usual bound an angle is
+    off by its f64 steps: a frequency base ** -e is formed from a rounded exponent, e ln(base) < 9.3, so that two ways to
+    it differ by 4 roundings of at most 9.3 and 8 of 1, less than 2^6 times 2^-53; that relative error of an angle
+    moves a channel by |angle| 2^-47 of |u| + |w|. At 2^36 it is 2^-11, at the low 32 bits' angle or the other sign
+    of the order of 1."""
+    sections = (8, 12, 12)
+    q, k, gq, gk = _normal(6, dtype, (150, 2, 64), (150, 1, 64), (150, 2, 64), (150, 1, 64))
+    rng = np.random.default_rng(7)
+    pos = (rng.choice([-1, 1], (150, 3)) * np.exp2(rng.uniform(33, 36, (150, 3)))).astype(np.int64)
+    p = torch.from_numpy(pos).to(_dev())
+    for shared in (False, True):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k)]
+        outs = rotary_embed(*leaves, p, sections, shared_frequencies=shared, interleaved=interleaved)
+        grads = torch.autograd.grad(outs, leaves, (gq, gk))
+        angle = np.abs(RO.angles(pos, sections, shared=shared))[:, None]
+        for got, x, sign in ((outs[0], q, 1.0), (outs[1], k, 1.0), (grads[0], gq, -1.0), (grads[1], gk, -1.0)):
+            x64 = _np(x)
+            want = RO.rotate(x64, pos, sections, 10000.0, shared, interleaved, sign)
+            a, b = (slice(0, 64, 2), slice(1, 64, 2)) if interleaved else (slice(0, 32), slice(32, 64))
+            reach = np.abs(x64[..., a]) + np.abs(x64[..., b])
+            for s in (a, b):
+                bound = HALF_STEP[dtype] * np.abs(want[..., s]) + (8 * 2.0 ** -24 + angle * 2.0 ** -47) * reach
+                assert (np.abs(_np(got)[..., s] - want[..., s]) <= bound * (1 + HALF_STEP[dtype])).all()
+            # positions cut to 32 bits, or of the other sign, are far outside
+            for wrong in (pos.astype(np.int32), -pos):
+                other = RO.rotate(x64, wrong, sections, 10000.0, shared, interleaved, sign)
+                assert np.abs(_np(got) - other).max() > 0.5
