@@ -153,6 +153,8 @@ __device__ __forceinline__ PkPlace pk_place(const int32_t* offsets, int sequence
         s += at;
       }
       w.tile = t - base;
+      // Offsets that rise have fewer units than the grid. Of ones that fall and rise again the sum may pass 32 bits.
+      if (at > 63 || static_cast<uint32_t>(w.tile) >= static_cast<uint32_t>(__builtin_amdgcn_readlane(mine, at & 63))) return PkPlace{-1, 0, 0, 0};
     }
   } else {
     const int slot = LAST_FIRST ? slots - 1 - index : index;

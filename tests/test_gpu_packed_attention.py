@@ -622,3 +622,20 @@ def test_tiles_with_more_parts_the_more_keys_they_see(name, dtype):
     q, k, v, g = _normal(32, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d), (off[-1], h, d))
     got = _run(q, k, v, g, _int(off), _int(koff))
     _compare(q, k, v, g, got, PA.sequences(off, koff), True)
+
+
+def test_offsets_that_fall_and_rise_over_many_rows_stay_in_bounds():
+    """A thousand sequences over the same 25 million rows of 64 heads: the sum of their tiles passes 32 bits. The call ends, and
+    a right one behind it is right."""
+    rows = 25_000_000
+    q = torch.empty(rows, 64, 8, dtype=torch.bfloat16, device=_dev())
+    k = torch.zeros(1, 1, 8, dtype=torch.bfloat16, device=_dev())
+    off = _int([0 if i % 2 == 0 else rows for i in range(1001)])
+    out = packed_attention(q, k, k, off, torch.zeros_like(off), causal=False)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape
+    del q, out
+    torch.cuda.empty_cache()
+    off = [0, 100, 150]
+    q, k, v, g = _normal(33, torch.bfloat16, (150, 4, 32), (150, 2, 32), (150, 2, 32), (150, 4, 32))
+    _compare(q, k, v, g, _run(q, k, v, g, _int(off)), PA.sequences(off), True)
