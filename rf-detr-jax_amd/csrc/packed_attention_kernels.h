@@ -569,9 +569,8 @@ struct PkStream {
 
 // A causal chunk that not every row of the workgroup sees whole: the weights of its unseen pairs are zeros, and
 // zero times an infinity or NaN of an unseen row would reach the sums. So such a tile is searched first (one
-// round of 16-byte reads and a barrier, for the chunks on the diagonal alone, and the forward's first in bf16
-// where rows of fewer than 64 keys take the weights' rest), values that are no finite numbers become zeros, and
-// the rows that held some are marked in `bad`, for those who see them.
+// round of 16-byte reads and a barrier, for the chunks on the diagonal alone), values that are no finite numbers
+// become zeros, and the rows that held some are marked in `bad`, for those who see them.
 typedef uint16_t pk_u2 __attribute__((ext_vector_type(2)));
 template <typename T, int DT>
 __device__ __forceinline__ void pk_settle(unsigned char* tile, uint32_t* bad) {
@@ -740,7 +739,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;  // keys that the wave sees
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                  // that every row of it sees
   const int all = w.seen(p, w.r0);                                           // that every row of the workgroup sees
-  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk;
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = w.rows <= 32;
   const int per = (chunks + parts - 1) / parts, c0 = w.split * per, c1 = min(chunks, c0 + per);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
@@ -760,8 +759,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    // (the rest of a weight is 0 or of either sign: an infinity times it would be NaN, or the other infinity)
-    if (min(k0 + kPkChunk, w.m) > all || (sizeof(T) == 2 && k0 == 0 && all < kPkChunk)) {
+    if (min(k0 + kPkChunk, w.m) > all) {
       if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
       pk_settle<T, DT>(Vb, bad[turn]);
       sick = sick || pk_settled(bad[turn]) != 0;
@@ -846,11 +844,14 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
               else w1.set(s1);
             }
           });
-      // Rows of fewer than 64 keys: what the rounding of the weights left, too. The rounding's errors do not average
-      // out over few keys, and delta, from the output, carries them into every ds of the row, where they are as large
-      // as those of ds's own rounding. (60 calls of 1 to 8 sequences of 1 to 600 rows: 7 of 240 results were more than
-      // 1.5 times as far off as the exact ones rounded, with this and the same for dq 1.)
-      if (k0 == 0 && few) pk_accumulate2<T, DT, 2>(o, V, pk_rest(s0) * late, o, V + 32 * Tile::ROW, pk_rest(s1), at);
+      // Rows of fewer than 64 keys, and sequences whose rows one wave holds: what the rounding of the weights left, too.
+      // The rounding's errors do not average out over few keys, and delta, from the output, carries them into every ds
+      // of the row, where they are as large as those of ds's own rounding. (60 calls of 1 to 8 sequences of 1 to 600
+      // rows: 7 of 240 results were more than 1.5 times as far off as the exact ones rounded, with this and the same
+      // for dq 1.) New tokens over caches are bound by the loads: 64 of them, 128 channels, are 1.00 times as far off as
+      // the exact results rounded where it was 1.38, in 121 us for 116. For rows of every kind the products are half as
+      // many again: 16,000 tokens of prompts 897 us for 631, to 1.00 from 1.2 to 1.4.
+      if ((k0 == 0 && few) || narrow) pk_accumulate2<T, DT, 2>(o, V, pk_rest(s0) * late, o, V + 32 * Tile::ROW, pk_rest(s1), at);
     } else {
       next.all();
       pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
@@ -887,9 +888,23 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     pk_barrier();
     chunk(X1, Y1, 1, c + 1, tile(X0, Y0, c + 2));
   }
-  if (sick) {  // infinities and NaN of those chunks for the rows that see them
+  // Infinities and NaN of values: those that pk_settle took out, for the rows that see them, and those that the rest of a
+  // weight, 0 or of either sign, made NaN. Where a row sees some in a channel, their sum is the result.
+  bool odd = false;
+  if constexpr (sizeof(T) == 2)
+    if (few || narrow) {
+#pragma unroll
+      for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) odd = odd || o[nd][i] != o[nd][i];
+      odd = __any(odd);
+    }
+  if (sick || odd) {
+    at_f16 y[DT / 32];
+#pragma unroll
+    for (int nd = 0; nd < DT / 32; ++nd) y[nd] = at_zero16();
 #pragma unroll 1
-    for (int j = max(all / kPkChunk, c0) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
+    for (int j = (odd ? c0 : max(all / kPkChunk, c0)) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
 #pragma unroll
       for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
@@ -900,8 +915,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
             if constexpr (sizeof(T) == 2) x = bf16_to_f32(vp[j * p.st[kPkV][0] + ch]);
             else x = vp[j * p.st[kPkV][0] + ch];
           }
-          if (x - x != 0.0f) o[nd][i] += x;
+          if (x - x != 0.0f) y[nd][i] += x;
         }
+#pragma unroll
+    for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[nd][i] = y[nd][i] != 0.0f ? y[nd][i] : o[nd][i];
   }
   l = at_sum_halves(l);
   pk_barrier();  // the tiles hold the waves' scratch from here

@@ -514,6 +514,9 @@ SEEN = {
     "short_rows_of_a_long_prompt": (200, 200, 2, 2, 96, True, 5),
     "whole_tile": (70, 64, 2, 1, 128, False, 40),
     "long": (30, 300, 4, 2, 64, False, 299),
+    "token_over_a_cache": (1, 2000, 8, 1, 128, True, 1234),  # the keys are split
+    "chunk_over_a_cache": (7, 500, 4, 1, 64, True, 498),
+    "many_rows": (40, 500, 4, 1, 64, True, 300),
 }
 
 
@@ -639,3 +642,19 @@ def test_offsets_that_fall_and_rise_over_many_rows_stay_in_bounds():
     off = [0, 100, 150]
     q, k, v, g = _normal(33, torch.bfloat16, (150, 4, 32), (150, 2, 32), (150, 2, 32), (150, 4, 32))
     _compare(q, k, v, g, _run(q, k, v, g, _int(off)), PA.sequences(off), True)
+
+
+@pytest.mark.parametrize("d", [40, 64, 128])
+def test_new_bf16_tokens_keep_what_the_weights_rounding_left(d):
+    """Sequences of at most 32 rows over caches of any length, split or not: the two bf16 numbers of a weight, as for short
+    rows."""
+    lengths, keys = [1, 3, 4, 2], [2000, 700, 100, 1300]
+    off, koff = np.cumsum([0, *lengths]), np.cumsum([0, *keys])
+    q, k, v = _normal(34, torch.bfloat16, (off[-1], 8, d), (koff[-1], 1, d), (koff[-1], 1, d))
+    seqs = PA.sequences(off, koff)
+    for factor in (1, 4):  # sums of many keys, and rows that a few of them make
+        out = packed_attention(q * factor, k, v, _int(off), _int(koff))
+        arrays = [_np(x) for x in (q * factor, k, v)]
+        want = PA.attention(*arrays, seqs)
+        bound = PA.bounds(*arrays, np.zeros_like(arrays[0]), seqs, 2.0 ** -16)[0]
+        _within(out, want, (1 + 2.0 ** -8) * bound + 2.0 ** -8 * np.abs(want), "out")
