@@ -452,21 +452,27 @@ int msda_attention_dropout_keep(int batch, int groups, int heads, int len, float
  * head_dim: a multiple of 8, at most 128. `strides` holds the element strides (row, head) of each
  * tensor (0, 0 for one that is NULL); channels are contiguous, and rows start on 16-byte boundaries (bases, and strides in bytes, are
  * multiples of 16), head_dim to 2^22 elements apart, q's and grad_out's heads of a key head within
- * 2^27 elements. At most 64 query heads to a key head; backward: fewer than 2^21 key heads. scale: 2^-64 to 2^64. q_rows * heads / kv_heads and k_rows below 2^31 less 128
- * rows a sequence.
+ * 2^27 elements. At most 64 query heads to a key head; backward: fewer than 2^21 key heads. scale: 2^-64 to 2^64.
+ * q_rows * heads / kv_heads and k_rows below 2^31 less 128 rows a sequence.
  * stats: [q_rows * heads][4] f32, 16-byte aligned: the forward writes entries 0 and 1 (their sum is log2
  * of the row's sum of 2^(scale2 q.k), scale2 = scale log2(e)), the backward reads them. May be NULL in a forward whose backward is not wanted.
  * out_rest: NULL, or for bf16 a tensor of out's strides: the forward writes what out's rounding left, the
  * backward reads out + out_rest for rowsum(grad_out * out), whose error is then that of f32 sums.
- * Sums, softmax and statistics are f32; bf16 products run on bf16 matrix instructions, with the softmax
- * weights and their gradients rounded to bf16, f32 products on f32 ones. No result depends on an order of
- * atomics.
+ * Sums, softmax and statistics are f32; f32 products run on f32 matrix instructions, bf16 ones on bf16 matrix
+ * instructions, with the softmax weights and their gradients rounded to bf16. The weights of out keep two bf16
+ * numbers where a sequence's queries times heads / kv_heads are at most 32, and, as grad_q's gradients of
+ * weights, where a row sees fewer than 64 keys. No result depends on an order of atomics.
  */
 
 /*
- * Device workspaces in bytes (functions of the shape only), or a negative code: partial sums of forward
- * calls with so few query rows that the keys of a sequence are split over several workgroups, and of
- * backward calls with so few key tiles that the rows seeing one are; else 0.
+ * Device workspaces in bytes (functions of the shape only), or a negative code; 0 where nothing is split.
+ * Forward: partial sums of calls whose keys are split over several workgroups, because few query rows (of
+ * which there are at most 32 a sequence on average) stand over long ranges of keys, or because the tiles of
+ * 128 rows do not fill the CUs evenly (prompts, too: one f32 sequence of 4,096 tokens, 8 heads, 128 channels,
+ * 307 MB for an output of 17). (parts (head_dim + 2) + 1) q_rows heads 4 with parts <= 64.
+ * Backward: partial sums of grad_k and grad_v where there are so few key tiles that the rows seeing one are
+ * split: parts 2 k_rows kv_heads head_dim 4 with parts <= 8, room for all rows though few tiles may have
+ * parts: up to 16 times the two gradients in bf16, 8 times in f32.
  */
 int64_t msda_packed_attention_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);
 int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim);

@@ -110,7 +110,10 @@ constexpr int kPkCounted = 1024;  // segments whose tiles a wave counts
 // unit's number in its segment. So the units that do not exist are the grid's last. That matters: the hardware
 // hands workgroups to its shader engines in turn whether they end at once or not, and with empty ones among
 // them (sequences of 128 rows: every second one) half of the CUs stood idle: forward of 128 times 128 queries over
-// 1,024 keys, 8 heads, 173 us for 140 in bf16 at 128 channels, 540 for 287 in f32 at 64.
+// 1,024 keys, 8 heads, 173 us for 140 in bf16 at 128 channels, 540 for 287 in f32 at 64. The counting has its price,
+// the loads of 2 segments / 64 offsets a lane, one behind the other, and the sorting of up to 64 segments another: 128
+// tokens each that see themselves, 8 heads, bf16 at 64 channels, 62 sequences 17.7 us, 63 10.0, 1,022 267, and 1,023,
+// searched, 96.
 // Of more segments it searches, 64 at a time, among `slots` tiles, with segment s at tile floor(first row / 128) + s,
 // behind which it has room for ceil(rows / 128).
 template <bool LAST_FIRST, typename Count>
@@ -1224,7 +1227,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   constexpr bool bf = sizeof(T) == 2;
   constexpr int PF = bf && DT != 64 && DT != 128 ? 3 : 2;
   // At 128 channels k, v, dk and dv take 192 of a wave's 256 registers. The last KEEP pieces of v wait in LDS: in
-  // registers the compiler spilled them, and each reload from scratch memory waited for the tile in flight.
+  // registers the compiler spilled them, and each reload from scratch memory waited for the tile in flight. Three
+  // registers of other values are spilled still, two of them read back in the loop, behind a chunk's products.
   constexpr int KEEP = bf && DT == 128 ? 3 : 0;
   __shared__ __align__(16) unsigned char kept_rows[KEEP > 0 ? KEEP * kPkWaves * 1024 : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;

@@ -34,17 +34,20 @@ inline PackSplit pk_split(const PackShape& s) {
   const int64_t tiles = std::min<int64_t>(rows, rows / kPkTile + s.sequences) * s.kv_heads;
   const int64_t chunks = (s.k_rows / s.sequences + kPkChunk - 1) / kPkChunk;  // of an average sequence
   if (tiles == 0) return none;
-  // The work in parts that even out over the CUs: in bf16 one to each of the two workgroups that a CU holds; in f32,
-  // whose products one workgroup alone keeps busy, 8 to a CU. One sequence of 6,000 tokens, 8 heads, causal (376 tiles,
+  // The work in parts that even out over the CUs: in bf16 one to each of the two workgroups that a CU holds, in f32 8
+  // to a CU. The chunks counted here are those of the keys' room, not of their lengths, so there may be fewer parts with
+  // work than wanted (3 caches of 16,384 rows, 30,022 keys in them: 380 for 512). One sequence of 6,000 tokens, 8 heads, causal (376 tiles,
   // the last of 94 chunks), us a call: bf16, 128 channels 131 with a workgroup a tile, 107 in 512 parts, 114 in
   // 2048; f32, 64 channels 532, 432 and 360. (Batches whose tiles even out by themselves pay for it: 512 tiles of 16
   // chunks in f32 175 us for 145.)
   const bool bf = s.dtype == MSDA_DTYPE_BF16;
   const int64_t wanted = bf ? 512 : 2048, even = (tiles * chunks + wanted - 1) / wanted;
-  // Few rows to a tile (new tokens over caches): a part's own cost is small against its keys, so calls of any size
-  // are split, because the longest cache would set their time. Full tiles: a part writes and the join reads 128
+  // Few rows to a tile on average (new tokens over caches): a part's own cost is small against its keys, so a call of
+  // any size is split, because the longest cache would set its time. Full tiles: a part writes and the join reads 128
   // rows of f32 sums, the time of about 6 chunks of keys at 128 channels in bf16; in f32 (300 keys, 32 channels) parts of
-  // 2 chunks cost 41 us for 31.
+  // 2 chunks cost 41 us for 31. The choice is one for the whole batch: a chunk of 512 tokens (32 heads) among 63 single
+  // ones over caches of up to 8,000 keys makes the average row count large, nothing is split, and the longest cache
+  // does set the time: 238 us, where 64 single tokens take 121.
   const bool few = rows <= int64_t{32} * s.sequences;
   const int64_t part = few ? std::clamp<int64_t>(even, 2, 16) : std::max<int64_t>(even, bf ? 6 : 8);
   if (chunks <= part) return none;

@@ -208,6 +208,12 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
             key; False: every key of its sequence.
         scale: of the scores, from ``2 ** -64`` to ``2 ** 64``; ``D ** -0.5`` when None.
 
+    Sums, softmax and statistics are float32. Of bfloat16 inputs the softmax weights and their gradients are rounded to
+    bfloat16 for the matrix products: results lie 1.2 to 1.5 times as far from the exact ones as these rounded;
+    new tokens (a sequence's tokens times ``H / Hk`` up to 32) keep their weights in two bfloat16 numbers. Float32
+    inputs are float32 throughout. Calls whose work does not fill the GPU evenly take a workspace of partial sums, in
+    float32 prompts up to some hundred MB (``msda_packed_attention_fwd_workspace_size``).
+
     A query that sees no key gives zeros. Rows of the result, and of the gradients, outside every sequence are
     zeros. Pairs that are not seen take no part, whatever their rows hold (infinities and NaN too; a key that is not
     finite makes the gradients of the queries that see it NaN, a query that is not, or its cotangent, those of the keys

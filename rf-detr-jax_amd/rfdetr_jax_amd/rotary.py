@@ -91,7 +91,7 @@ def rotary_embed(q, k, positions, sections, base=10000.0, shared_frequencies=Fal
             each axis its own.
         interleaved: pair ``i`` is the channels ``(2 i, 2 i + 1)``; False: ``(i, i + n)``.
 
-    Differentiable in ``q`` and ``k`` (the rotation back). Products are float32, rounded once.
+    Differentiable in ``q`` and ``k`` (the rotation back), not in ``positions``, which get no gradient. Products are float32, rounded once.
 
     Raises:
         ValueError: shapes, devices or sizes that do not fit.
