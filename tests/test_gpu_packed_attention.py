@@ -658,3 +658,29 @@ def test_new_bf16_tokens_keep_what_the_weights_rounding_left(d):
         want = PA.attention(*arrays, seqs)
         bound = PA.bounds(*arrays, np.zeros_like(arrays[0]), seqs, 2.0 ** -16)[0]
         _within(out, want, (1 + 2.0 ** -8) * bound + 2.0 ** -8 * np.abs(want), "out")
+
+
+@TYPES
+def test_c_entry_that_keeps_its_numbers_in_the_statistics(dtype):
+    """msda_packed_attention_bwd gives the bits of the torch functions, which call the entry with a buffer, and leaves the
+    statistics' first two entries, so that a second call behind it gives them again."""
+    import ctypes
+
+    from rfdetr_jax_amd import _native
+
+    off = _int([0, 70, 200])
+    q, k, v, g = _normal(35, dtype, (200, 4, 64), (200, 2, 64), (200, 2, 64), (200, 4, 64))
+    out, (stats, rest) = packed_attention_forward(q, k, v, off)
+    want = packed_attention_backward(q, k, v, out, (stats, rest), g, off)
+    lib, code, dims = _native.lib(), _native.DTYPE_BF16 if dtype == torch.bfloat16 else _native.DTYPE_F32, (2, 200, 200, 4, 2, 64)
+    nbytes = lib.msda_packed_attention_bwd_workspace_size(code, *dims)
+    ws = _native.workspace(nbytes, q.device)
+    ptr = [ctypes.c_void_p(None if x is None else x.data_ptr()) for x in (q, k, v, out, rest, stats, g, off, ws)]
+    for _ in range(2):
+        grads = [torch.full_like(x, float("nan")) for x in (q, k, v)]
+        strides = (ctypes.c_int64 * 16)(*(s for x in (q, k, v, out, g, *grads) for s in x.stride()[:2]))
+        rc = lib.msda_packed_attention_bwd(*ptr[:7], code, *(ctypes.c_void_p(x.data_ptr()) for x in grads), ptr[7], ptr[7], None, *dims, strides, 1,
+                                           64 ** -0.5, ptr[8], nbytes, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        _native.check(rc)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
