@@ -508,6 +508,45 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
                                     int k_rows, int heads, int kv_heads, int head_dim, const int64_t* strides,
                                     int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Attention over packed sequences with shaped scores. Query t of a sequence stands at the place t + m - n among its
+ * keys. Its score for key j is
+ *   x = cap tanh(scale q.k / cap) - slopes[head] |place - j|
+ * (without cap: scale q.k), and it sees the keys with |place - j| < window and, where causal, j <= place or
+ * j < prefix_lengths[sequence]; everything else is as above, stats included (log2 of the sum of 2^(x log2(e))).
+ * cap: 0 (none) or 2^-32 to 2^32. window: 0 (none) or the number of places. slopes: [heads] f32, device memory, finite,
+ * or NULL. prefix_lengths: [sequences] int32, device memory, or NULL; only with causal (a sequence's first keys, which
+ * all its queries see: a prompt or an image before a text; 0 and less: none).
+ * shape NULL: the calls above. A window makes keys, tiles and the work that lie outside it go away.
+ * Backward: msda_packed_attention_bwd_const's arguments. slopes have no gradient.
+ * Workspaces: as above, with the window (0: none).
+ */
+typedef struct msda_score_shape {
+  float cap;
+  int window;
+  const float* slopes;
+  const int32_t* prefix_lengths;
+} msda_score_shape;
+
+int64_t msda_packed_attention_shaped_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                                                        int head_dim, int window);
+int64_t msda_packed_attention_shaped_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                                                        int head_dim, int window);
+
+int msda_packed_attention_shaped_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest,
+                                     float* stats, const int32_t* q_offsets, const int32_t* k_offsets,
+                                     const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads,
+                                     int kv_heads, int head_dim, const int64_t* strides, int causal, float scale,
+                                     const msda_score_shape* shape, void* workspace, int64_t workspace_bytes, void* stream);
+
+int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                                     const float* stats, float* row_numbers, const void* grad_out, int dtype,
+                                     void* grad_q, void* grad_k, void* grad_v, const int32_t* q_offsets,
+                                     const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows,
+                                     int k_rows, int heads, int kv_heads, int head_dim, const int64_t* strides, int causal,
+                                     float scale, const msda_score_shape* shape, void* workspace, int64_t workspace_bytes,
+                                     void* stream);
+
 /* ---- Rotary positions on several axes -------------------------------------------------------
  * Rotates channel pairs of queries and keys by angles that grow with the token's position on each of
  * `axes` axes (time, height, width, ...). No counterpart in the reference.

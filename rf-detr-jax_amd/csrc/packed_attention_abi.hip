@@ -44,29 +44,33 @@ int pk_bwd_shape(const PackShape& s) {
   return MSDA_OK;
 }
 
+// The window of the scores; the largest int where there is none.
+int pk_window(const msda_score_shape* shape) { return shape == nullptr || shape->window == 0 ? 0x7fffffff : shape->window; }
+
 // Bytes of the split forward's parts: f32 sums, (m, l) of every row and part, the rows' numbers of parts.
-int64_t pk_fwd_workspace(const PackShape& s) {
-  const int64_t parts = pk_split(s).most, rows = static_cast<int64_t>(s.q_rows) * s.heads;
+int64_t pk_fwd_workspace(const PackShape& s, int window) {
+  const int64_t parts = pk_split(s, window).most, rows = static_cast<int64_t>(s.q_rows) * s.heads;
   return parts == 1 ? 0 : (parts * (s.head_dim + 2) + 1) * rows * 4;
 }
 
 // The number of workgroups that may share a tile of keys in the backward: a causal sequence's first keys are
 // seen by all its rows, so with few tiles the longest one sets the time. A part is kPkPart chunks (more where
 // that makes more than kMost parts, or the tiles alone are several rounds of workgroups).
-int pk_parts(const PackShape& s) {
+int pk_parts(const PackShape& s, int window) {
   constexpr int64_t kWant = 2048, kMost = 8;
   if (s.sequences == 0 || s.k_rows == 0) return 1;
   const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
   // The rows of one sequence, if it is 4 times the average: a longer one takes longer parts, and batches of short
   // sequences start no second kernel (4 us).
-  const int64_t rows = std::min<int64_t>(s.q_rows, 4 * (static_cast<int64_t>(s.q_rows) / s.sequences + 1));
+  // No more than a window's see a tile.
+  const int64_t rows = std::min<int64_t>({s.q_rows, 4 * (static_cast<int64_t>(s.q_rows) / s.sequences + 1), msda::pk_in_window(window)});
   const int64_t chunks = rows * (s.heads / s.kv_heads) / msda::kPkChunk;
   return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, (chunks + msda::kPkPart - 1) / msda::kPkPart, kMost})));
 }
 
 // Bytes of the parts' f32 sums of dk and dv.
-int64_t pk_bwd_workspace(const PackShape& s) {
-  const int parts = pk_parts(s);
+int64_t pk_bwd_workspace(const PackShape& s, int window) {
+  const int parts = pk_parts(s, window);
   return parts == 1 ? 0 : static_cast<int64_t>(parts) * 2 * s.k_rows * s.kv_heads * s.head_dim * 4;
 }
 
@@ -123,6 +127,59 @@ int pk_offsets(const int32_t* q_offsets, const int32_t* k_offsets, const int32_t
   return MSDA_OK;
 }
 
+int pk_check_shape(const msda_score_shape* shape, int causal) {
+  if (shape == nullptr) return MSDA_OK;
+  if (shape->cap != 0.0f && !(shape->cap >= 0x1p-32f && shape->cap <= 0x1p32f))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: cap %g must be 0 or lie from 2^-32 to 2^32", static_cast<double>(shape->cap));
+  if (shape->window < 0) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: window %d", shape->window);
+  if (shape->prefix_lengths != nullptr && !causal) return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: prefix lengths without causal");
+  if (!aligned_to(shape->slopes, 4) || !aligned_to(shape->prefix_lengths, 4))
+    return fail(MSDA_ERR_INVALID_ARGUMENT, "packed attention: slopes and prefix lengths must be aligned to 4 bytes");
+  return MSDA_OK;
+}
+
+// Fills in the shape; the kernels that it needs (enum PackShaped), 0 for the plain ones.
+int pk_set_shape(msda::PackParams& p, const msda_score_shape* shape) {
+  p.window = pk_window(shape);
+  if (shape == nullptr) return 0;
+  int mod = shape->window != 0 || shape->prefix_lengths != nullptr ? msda::kPkRanges : 0;
+  p.prefix = shape->prefix_lengths;
+  if (shape->slopes != nullptr) {
+    mod |= msda::kPkRanges | msda::kPkSlope;
+    p.slopes = shape->slopes;
+  }
+  if (shape->cap != 0.0f) {
+    mod |= msda::kPkRanges | msda::kPkCap;
+    const double cap = shape->cap, inner = static_cast<double>(p.scale) / cap;
+    p.inner = static_cast<float>(inner);
+    p.cap2 = static_cast<float>(1.4426950408889634 * cap);
+    p.bend = static_cast<float>(2.0 * 1.4426950408889634 * inner);
+  }
+  return mod;
+}
+
+template <typename T>
+int pk_run_fwd(const msda::PackParams& p, int mod, hipStream_t st) {
+  switch (mod) {
+    case 0: return msda_host::dispatch_pk_fwd<T, 0>(p, st);
+    case 4: return msda_host::dispatch_pk_fwd<T, 4>(p, st);
+    case 5: return msda_host::dispatch_pk_fwd<T, 5>(p, st);
+    case 6: return msda_host::dispatch_pk_fwd<T, 6>(p, st);
+    default: return msda_host::dispatch_pk_fwd<T, 7>(p, st);
+  }
+}
+
+template <typename T>
+int pk_run_bwd(const msda::PackParams& p, int mod, int q_slots, int k_slots, hipStream_t st) {
+  switch (mod) {
+    case 0: return msda_host::dispatch_pk_bwd<T, 0>(p, q_slots, k_slots, st);
+    case 4: return msda_host::dispatch_pk_bwd<T, 4>(p, q_slots, k_slots, st);
+    case 5: return msda_host::dispatch_pk_bwd<T, 5>(p, q_slots, k_slots, st);
+    case 6: return msda_host::dispatch_pk_bwd<T, 6>(p, q_slots, k_slots, st);
+    default: return msda_host::dispatch_pk_bwd<T, 7>(p, q_slots, k_slots, st);
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -131,24 +188,44 @@ int64_t msda_packed_attention_fwd_workspace_size(int dtype, int sequences, int q
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   const int rc = pk_shape(s);
-  return rc != MSDA_OK ? rc : pk_fwd_workspace(s);
+  return rc != MSDA_OK ? rc : pk_fwd_workspace(s, 0x7fffffff);
 }
 
 int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   const int rc = pk_bwd_shape(s);
-  return rc != MSDA_OK ? rc : pk_bwd_workspace(s);
+  return rc != MSDA_OK ? rc : pk_bwd_workspace(s, 0x7fffffff);
 }
 
-int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest, float* stats,
-                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
-                              int head_dim, const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes,
-                              void* stream) {
+int64_t msda_packed_attention_shaped_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim, int window) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  const msda_score_shape shape{0.0f, window, nullptr, nullptr};
+  int rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_check_shape(&shape, 1)) != MSDA_OK) return rc;
+  return pk_fwd_workspace(s, pk_window(&shape));
+}
+
+int64_t msda_packed_attention_shaped_bwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim, int window) {
+  msda_host::clear_error();
+  const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
+  const msda_score_shape shape{0.0f, window, nullptr, nullptr};
+  int rc;
+  if ((rc = pk_bwd_shape(s)) != MSDA_OK || (rc = pk_check_shape(&shape, 1)) != MSDA_OK) return rc;
+  return pk_bwd_workspace(s, pk_window(&shape));
+}
+
+int msda_packed_attention_shaped_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest, float* stats,
+                                     const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                                     int head_dim, const int64_t* strides, int causal, float scale, const msda_score_shape* shape,
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
-  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides<4>(s, strides, {q, k, v, out})) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK) return rc;
+  if ((rc = pk_shape(s)) != MSDA_OK || (rc = pk_strides<4>(s, strides, {q, k, v, out})) != MSDA_OK || (rc = pk_scale(scale)) != MSDA_OK ||
+      (rc = pk_check_shape(shape, causal)) != MSDA_OK)
+    return rc;
   if (q_rows == 0) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
   if (q == nullptr || out == nullptr || (k_rows != 0 && (k == nullptr || v == nullptr)))
@@ -164,11 +241,12 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
   p.rest = dtype == MSDA_DTYPE_BF16 ? out_rest : nullptr;
   p.stats = stats;
   p.slots = static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
-  const PackSplit split = pk_split(s);
+  const int mod = pk_set_shape(p, shape);
+  const PackSplit split = pk_split(s, p.window);
   p.splits = split.most;
   p.part = split.part;
   if (p.splits > 1) {
-    const int64_t need = pk_fwd_workspace(s);
+    const int64_t need = pk_fwd_workspace(s, p.window);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_fwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
     p.part_o = static_cast<float*>(workspace);
@@ -176,19 +254,27 @@ int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int d
     p.part_n = reinterpret_cast<int32_t*>(p.part_ml + static_cast<int64_t>(p.splits) * q_rows * heads * 2);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_fwd<msda::bf16_t>(p, st) : msda_host::dispatch_pk_fwd<float>(p, st);
+  return dtype == MSDA_DTYPE_BF16 ? pk_run_fwd<msda::bf16_t>(p, mod, st) : pk_run_fwd<float>(p, mod, st);
 }
 
-int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* stats,
-                                    float* row_numbers, const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
-                                    const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows,
-                                    int heads, int kv_heads, int head_dim, const int64_t* strides, int causal, float scale, void* workspace,
-                                    int64_t workspace_bytes, void* stream) {
+int msda_packed_attention_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest, float* stats,
+                              const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                              int head_dim, const int64_t* strides, int causal, float scale, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  return msda_packed_attention_shaped_fwd(q, k, v, dtype, out, out_rest, stats, q_offsets, k_offsets, k_lengths, sequences, q_rows, k_rows, heads, kv_heads,
+                                          head_dim, strides, causal, scale, nullptr, workspace, workspace_bytes, stream);
+}
+
+int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* stats,
+                                     float* row_numbers, const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
+                                     const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows,
+                                     int heads, int kv_heads, int head_dim, const int64_t* strides, int causal, float scale, const msda_score_shape* shape,
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   int rc;
   if ((rc = pk_bwd_shape(s)) != MSDA_OK || (rc = pk_strides<8>(s, strides, {q, k, v, out, grad_out, grad_q, grad_k, grad_v})) != MSDA_OK ||
-      (rc = pk_scale(scale)) != MSDA_OK)
+      (rc = pk_scale(scale)) != MSDA_OK || (rc = pk_check_shape(shape, causal)) != MSDA_OK)
     return rc;
   if ((grad_q == nullptr && grad_k == nullptr && grad_v == nullptr) || (q_rows == 0 && k_rows == 0)) return MSDA_OK;
   if ((rc = pk_offsets(q_offsets, k_offsets, k_lengths)) != MSDA_OK) return rc;
@@ -211,9 +297,10 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
   p.gv = grad_v;
   p.stats = const_cast<float*>(stats);  // (the backward reads it)
   p.numbers = grad_k != nullptr || grad_v != nullptr ? row_numbers : nullptr;
-  if (grad_k != nullptr || grad_v != nullptr) p.splits = pk_parts(s);
+  const int mod = pk_set_shape(p, shape);
+  if (grad_k != nullptr || grad_v != nullptr) p.splits = pk_parts(s, p.window);
   if (p.splits > 1) {
-    const int64_t need = pk_bwd_workspace(s);
+    const int64_t need = pk_bwd_workspace(s, p.window);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
     p.part_kv = static_cast<float*>(workspace);
@@ -221,8 +308,16 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
   const int q_slots = q_rows == 0 ? 0 : static_cast<int>(slots_of(static_cast<int64_t>(q_rows) * p.group, sequences));
   const int k_slots = k_rows == 0 ? 0 : static_cast<int>(slots_of(k_rows, sequences));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == MSDA_DTYPE_BF16 ? msda_host::dispatch_pk_bwd<msda::bf16_t>(p, q_slots, k_slots, st)
-                                  : msda_host::dispatch_pk_bwd<float>(p, q_slots, k_slots, st);
+  return dtype == MSDA_DTYPE_BF16 ? pk_run_bwd<msda::bf16_t>(p, mod, q_slots, k_slots, st) : pk_run_bwd<float>(p, mod, q_slots, k_slots, st);
+}
+
+int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* stats,
+                                    float* row_numbers, const void* grad_out, int dtype, void* grad_q, void* grad_k, void* grad_v,
+                                    const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows,
+                                    int heads, int kv_heads, int head_dim, const int64_t* strides, int causal, float scale, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  return msda_packed_attention_shaped_bwd(q, k, v, out, out_rest, stats, row_numbers, grad_out, dtype, grad_q, grad_k, grad_v, q_offsets, k_offsets, k_lengths,
+                                          sequences, q_rows, k_rows, heads, kv_heads, head_dim, strides, causal, scale, nullptr, workspace, workspace_bytes, stream);
 }
 
 int msda_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, float* stats,

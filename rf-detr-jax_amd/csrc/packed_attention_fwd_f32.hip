@@ -1,6 +1,7 @@
 // packed_attention_fwd_f32.hip — the packed-sequence attention's forward kernels for f32 tensors.
+#define MSDA_PK_INSTANTIATE
 #include "packed_attention_launch.h"
 
 namespace msda_host {
-template int dispatch_pk_fwd<float>(const msda::PackParams&, hipStream_t);
+MSDA_PK_FWD(float, 0);
 }  // namespace msda_host

@@ -67,7 +67,16 @@ struct PackParams {
   int slots;     // tiles of the kernel's own side
   float scale;   // of the scores
   float scale2;  // scale log2(e)
+  // shaped scores (PackShaped)
+  const float* slopes;    // [heads], or null
+  const int32_t* prefix;  // [sequences], or null
+  int window;             // keys at this distance and farther are not seen
+  float inner, cap2, bend;  // scale / cap, cap log2(e), 2 log2(e) scale / cap
 };
+
+// What a kernel of shaped scores does besides the ranges [lo, hi) of keys that a query sees; 0: the plain kernels,
+// whose ranges begin at 0.
+enum PackShaped { kPkRanges = 4, kPkCap = 1, kPkSlope = 2 };
 
 constexpr int kPkPart = 32;  // chunks of a workgroup on the key side, unless that makes more parts than the host gave room for
 constexpr int kPkJoin = 32;   // workgroups that join a key tile's parts
@@ -198,6 +207,52 @@ struct PkRange {
     const int end = min(max(p.k_offsets[seq + 1], first), p.k_rows);
     count = p.k_lengths != nullptr ? min(max(p.k_lengths[seq], 0), end - first) : end - first;
   }
+};
+
+// ---- shaped scores -----------------------------------------------------------------------------
+//
+// A query stands at the place t + m - n among its sequence's keys. With y = scale q.k / cap the score is
+//   x = cap tanh(y) - slope |place - j|,  and d x / d (scale q.k) = 1 - tanh(y)^2,
+// over the keys with |place - j| < window and (not causal, or j <= place, or j < prefix): one range [lo, hi), whose
+// ends rise with the query, so that tiles, waves and rows skip and mask keys as the causal kernels do.
+
+__device__ __forceinline__ int pk_lo(const PackParams& p, int place) { return place < p.window ? 0 : place - p.window + 1; }
+__device__ __forceinline__ int pk_hi(const PackParams& p, int place, int prefix, int m) {
+  const int reach = place > m - p.window ? m : place + p.window;
+  return max(min(p.causal ? max(place + 1, min(prefix, reach)) : reach, m), 0);
+}
+
+// tanh(y) = y P(y^2) up to kPkNear, to 7e-7 of itself for bf16 (whose weights are rounded to 2^-8 of themselves) and
+// 8e-8 for f32: 6 instructions, none of them transcendental, where 1 - 2 / (1 + e^2y) takes two of those (16 clocks
+// each for 4) and, near 0, only keeps 6e-8 of 1. Farther out that one is used. Both coefficients by least squares,
+// reweighted towards the smallest largest relative error.
+template <typename T>
+constexpr float kPkNear = sizeof(T) == 2 ? 0.75f : 0.625f;
+template <typename T>
+__device__ __forceinline__ float pk_near(float y) {
+  const float u = y * y;
+  if constexpr (sizeof(T) == 2) return y * fmaf(fmaf(fmaf(fmaf(0x1.ad73b8p-7f, u, -0x1.9be082p-5f), u, 0x1.0fbbc6p-3f), u, -0x1.554bbap-2f), u, 1.0f);
+  else return y * fmaf(fmaf(fmaf(fmaf(fmaf(-0x1.75e1ccp-8f, u, 0x1.52269ap-6f), u, -0x1.b83c5ap-5f), u, 0x1.110726p-3f), u, -0x1.555532p-2f), u, 1.0f);
+}
+template <typename T>
+__device__ __forceinline__ float pk_bent(const PackParams& p, float s) {  // of any score
+  const float y = s * p.inner, far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + at_exp2(s * p.bend)), 1.0f);
+  return fabsf(y) < kPkNear<T> ? pk_near<T>(y) : far;
+}
+// Some score of the wave's block lies beyond kPkNear (NaN does not).
+template <typename T>
+__device__ __forceinline__ bool pk_far(const PackParams& p, const at_f16& s) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
+  return __any(most * p.inner >= kPkNear<T>);
+}
+
+// One row's bias: of the key that lies `ahead` of the lane's first key of a block.
+struct PkBias {
+  float slope;  // -slope log2(e)
+  float first;  // the first key's number less the row's place
+  __device__ __forceinline__ float add(float x, int ahead) const { return fmaf(slope, fabsf(first + static_cast<float>(ahead)), x); }
 };
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -627,13 +682,15 @@ struct PkRows {
 
 // ---- queries on their own side: forward and dq -------------------------------------------------
 
+template <int MOD>
 struct PkQueries {
   PkPlace w;
   int kv_head;      // key head
   int split, parts; // the workgroup's part of the tile's keys, of so many (forward)
   int rows, r0;     // rows of the sequence's matrix, first of the workgroup's; none: no work
   int64_t k_first;  // first key row
-  int m, shift;     // keys; a row of token t sees the keys below min(m, t + shift + 1)
+  int m, shift;     // keys; a row of token t stands at place t + shift, and sees the keys up to there
+  int prefix;
   template <bool SPLIT>
   __device__ PkQueries(const PackParams& p, int lane, std::bool_constant<SPLIT>) {
     // key heads fastest: with 8 of them each stays on one XCD, whose L2 then holds its keys; the last
@@ -651,18 +708,20 @@ struct PkQueries {
       w = pk_place<true>(p.q_offsets, p.sequences, p.q_rows, p.group, line, p.slots, lane, true, [&](int s, int n) {
         const int tiles = pk_tiles(n, p.group);
         const PkRange keys(p, min(max(s - 1, 0), p.sequences - 1));
-        return s >= 1 && s <= p.sequences ? PkParts(p.splits, p.part, p.causal != 0, p.group, n, keys.count).before(tiles) : tiles;
+        return s >= 1 && s <= p.sequences ? parts_of(p, n, keys.count).before(tiles) : tiles;
       });
     }
     rows = w.own * p.group;
     k_first = 0;
     m = 0;
+    prefix = 0;
     if (w.seq >= 0 && w.own > 0) {
+      if (MOD != 0 && p.prefix != nullptr) prefix = p.prefix[w.seq];
       const PkRange keys(p, w.seq);
       k_first = keys.first;
       m = keys.count;
       if (shared) {
-        const PkParts all(p.splits, p.part, p.causal != 0, p.group, w.own, m);
+        const PkParts all = parts_of(p, w.own, m);
         if (counted) {  // the tile of the sequence's part w.tile: the last one before which no more parts lie
           int lo = 0, hi = pk_tiles(w.own, p.group);
           while (hi - lo > 1) {
@@ -681,7 +740,21 @@ struct PkQueries {
     r0 = w.tile * kPkTile;
     shift = m - w.own;
   }
-  __device__ int seen(const PackParams& p, int r) const { return p.causal ? min(max(r / p.group + shift + 1, 0), m) : m; }
+  // Parts of the tiles of n queries over m keys. Inside a window every tile sees about as many keys.
+  static __device__ __forceinline__ PkParts parts_of(const PackParams& p, int n, int m) {
+    if (MOD != 0 && p.window < m) return PkParts(p.splits, p.part, false, p.group, n, min(m, pk_in_window(p.window)));
+    return PkParts(p.splits, p.part, p.causal != 0, p.group, n, m);
+  }
+  // A row sees the keys from(r) .. seen(r) - 1.
+  __device__ int seen(const PackParams& p, int r) const {
+    if constexpr (MOD != 0) return pk_hi(p, r / p.group + shift, prefix, m);
+    return p.causal ? min(max(r / p.group + shift + 1, 0), m) : m;
+  }
+  __device__ int from(const PackParams& p, int r) const { return MOD != 0 ? pk_lo(p, r / p.group + shift) : 0; }
+  __device__ PkBias bias(const PackParams& p, int r, int grp) const {
+    const int tok = r / p.group;
+    return PkBias{p.slopes[kv_head * p.group + r - tok * p.group] * -1.44269504f, static_cast<float>(4 * grp - (tok + shift))};
+  }
   template <typename T>
   __device__ T* row(const PackParams& p, T* base, int t, int r) const {
     const int tok = r / p.group, g = r - tok * p.group;
@@ -710,10 +783,16 @@ __device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lim, int grp) {
   for (int i = 0; i < 16; ++i) s[i] = k0 + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : -INFINITY;
 }
 
+// The same for keys that are not among the `span` from lo on.
+__device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lo, int span, int grp) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = static_cast<uint32_t>(k0 + 8 * (i >> 2) + 4 * grp + (i & 3) - lo) < static_cast<uint32_t>(span) ? s[i] : -INFINITY;
+}
+
 // Forward. A workgroup takes 128 rows and walks over the keys that they see, 64 at a time, with a running
 // reference score m and sum l. m starts at the first chunk's maximum (whose weight, the largest of a short
 // row, is then 1 and rounds to itself) and moves when a chunk's exceeds it by 2^8.
-template <typename T, int DT>
+template <typename T, int DT, int MOD>
 __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 : DT <= 64 ? 3 : 2) : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
@@ -724,11 +803,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, lane, std::true_type());
+  const PkQueries<MOD> w(p, lane, std::true_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* out = static_cast<T*>(p.out);
-  const int end = w.w.seq < 0 ? 0 : w.seen(p, r1 - 1), chunks = (end + kPkChunk - 1) / kPkChunk;  // that the workgroup sees
+  const int end = w.w.seq < 0 ? 0 : w.seen(p, r1 - 1);
+  const int cb = w.w.seq < 0 ? 0 : w.from(p, w.r0) / kPkChunk;  // the first chunk that the workgroup sees
+  const int chunks = max((end + kPkChunk - 1) / kPkChunk - cb, 0);
   const int parts = w.parts;
   if (p.splits > 1 && w.split == 0)  // one part writes its rows itself
     for (int r = w.r0 + static_cast<int>(threadIdx.x); r < r1; r += 64 * kPkWaves) p.part_n[w.stat(p, r)] = parts;
@@ -742,8 +823,14 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;  // keys that the wave sees
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;                  // that every row of it sees
   const int all = w.seen(p, w.r0);                                           // that every row of the workgroup sees
-  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = w.rows <= 32;
-  const int per = (chunks + parts - 1) / parts, c0 = w.split * per, c1 = min(chunks, c0 + per);
+  // with ranges: the lane's, from lo on; what every row of the wave, of the workgroup sees begins at wlo, alo
+  const int lo = MOD != 0 && valid ? w.from(p, ri) : 0, span = max(lim - lo, 0);
+  const int wbegin = MOD != 0 && wr0 < w.rows ? w.from(p, wr0) : 0;
+  const int wlo = MOD != 0 && wr0 < w.rows ? w.from(p, min(wr0 + 31, w.rows - 1)) : 0, alo = MOD != 0 ? w.from(p, r1 - 1) : 0;
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = w.rows <= 32 || (MOD != 0 && p.window < kPkChunk);
+  const int per = (chunks + parts - 1) / parts, c0 = cb + w.split * per, c1 = min(cb + chunks, c0 + per);
+  PkBias bias{0.0f, 0.0f};
+  if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, min(ri, w.rows - 1), grp);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
   const T* kp = static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
@@ -762,12 +849,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    if (min(k0 + kPkChunk, w.m) > all) {
-      if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
+    if (MOD != 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;  // settled chunks at both ends of the range, others between them
+    if (min(k0 + kPkChunk, w.m) > all || (MOD != 0 && k0 < alo)) {
+      if (MOD == 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
       pk_settle<T, DT>(Vb, bad[turn]);
       sick = sick || pk_settled(bad[turn]) != 0;
     }
-    if (k0 >= wend) {
+    if (k0 >= wend || (MOD != 0 && k0 + kPkChunk <= wbegin)) {
       next.all();
       return;
     }
@@ -778,21 +866,43 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       // products of one wave; a CU's other workgroup fills the rest.
       using P = PkProducts<T, DT>;
       constexpr int KS = P::kScores, HA = KS >= 4 ? KS / 2 - 1 : 1, HB = KS - 1 - HA;  // steps up to the maximum, behind it
+      bool far = false;
       float bm, alpha = 1.0f, late = 1.0f;  // late: what scales the first half's weights after their rounding
       // step t of the softmax of block x, whose keys start at k: x = scale2 s - m and its maximum, m moved if it
       // has to, weights and their sum (a lane sums its half of the keys until the end)
       auto soft = [&](at_f16& x, int k, auto step) {
         constexpr int t = decltype(step)::value, first = HB > 0 ? HA + 1 : HA, parts = HB > 0 ? HB : 1;
         if constexpr (t == 1) {
-          if (k + 32 > wfull) pk_mask(x, k, lim, grp);
+          if constexpr (MOD == 0) {
+            if (k + 32 > wfull) pk_mask(x, k, lim, grp);
+          }
+          if constexpr ((MOD & kPkCap) != 0) far = pk_far<T>(p, x);
           bm = -INFINITY;
         }
         if constexpr (t >= 1 && t <= HA) {
-          constexpr int lo = 16 * (t - 1) / HA, hi = 16 * t / HA;
-          pk_for<hi - lo>([&](auto i) {
-            x[lo + i] = fmaf(x[lo + i], p.scale2, -m);
-            bm = fmaxf(bm, x[lo + i]);
-          });
+          constexpr int i0 = 16 * (t - 1) / HA, i1 = 16 * t / HA;
+          if constexpr (MOD == 0) {
+            pk_for<i1 - i0>([&](auto i) {
+              x[i0 + i] = fmaf(x[i0 + i], p.scale2, -m);
+              bm = fmaxf(bm, x[i0 + i]);
+            });
+          } else {
+            float to = -m;
+            PkBias b = bias;
+            if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
+            auto shape = [&](int i, float bent) {
+              x[i] = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, to) : fmaf(x[i], p.scale2, to);
+              if constexpr ((MOD & kPkSlope) != 0) x[i] = b.add(x[i], 8 * (i >> 2) + (i & 3));
+            };
+            if ((MOD & kPkCap) != 0 && far) pk_for<i1 - i0>([&](auto i) { shape(i0 + i, pk_bent<T>(p, x[i0 + i])); });
+            else pk_for<i1 - i0>([&](auto i) { shape(i0 + i, pk_near<T>(x[i0 + i] * p.inner)); });
+            if (k + 32 > wfull || k < wlo)
+              pk_for<i1 - i0>([&](auto j) {
+                constexpr int i = i0 + j;
+                x[i] = static_cast<uint32_t>(k + 8 * (i >> 2) + 4 * grp + (i & 3) - lo) < static_cast<uint32_t>(span) ? x[i] : -INFINITY;
+              });
+            pk_for<i1 - i0>([&](auto i) { bm = fmaxf(bm, x[i0 + i]); });
+          }
         }
         if constexpr (t == HA) {
           bm = at_max_halves(bm);
@@ -858,14 +968,33 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     } else {
       next.all();
       pk_scores2<T, DT, PF>(s0, K, q, s1, K + 32 * Tile::ROW, q, at);
-      if (k0 + kPkChunk > wfull) {
-        pk_mask(s0, k0, lim, grp);
-        pk_mask(s1, k0 + 32, lim, grp);
+      if constexpr (MOD == 0) {
+        if (k0 + kPkChunk > wfull) {
+          pk_mask(s0, k0, lim, grp);
+          pk_mask(s1, k0 + 32, lim, grp);
+        }
+      } else {
+        PkBias b = bias;
+        if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s0[i] = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s0[i]) * p.cap2 : s0[i] * p.scale2;
+          s1[i] = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s1[i]) * p.cap2 : s1[i] * p.scale2;
+          if constexpr ((MOD & kPkSlope) != 0) {
+            s0[i] = b.add(s0[i], 8 * (i >> 2) + (i & 3));
+            s1[i] = b.add(s1[i], 32 + 8 * (i >> 2) + (i & 3));
+          }
+        }
+        if (k0 + kPkChunk > wfull || k0 < wlo) {
+          pk_mask(s0, k0, lo, span, grp);
+          pk_mask(s1, k0 + 32, lo, span, grp);
+        }
       }
       float bm = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) bm = fmaxf(bm, fmaxf(s0[i], s1[i]));
-      bm = at_max_halves(bm) * p.scale2;
+      bm = at_max_halves(bm);
+      if constexpr (MOD == 0) bm *= p.scale2;
       if (bm != -INFINITY && (bm > m + kAtLazy || fresh)) {
         const float alpha = fresh ? 0.0f : at_exp2(m - bm);
         m = bm;
@@ -876,8 +1005,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s0[i] = at_exp2(fmaf(s0[i], p.scale2, -m));
-        s1[i] = at_exp2(fmaf(s1[i], p.scale2, -m));
+        s0[i] = at_exp2(MOD != 0 ? s0[i] - m : fmaf(s0[i], p.scale2, -m));
+        s1[i] = at_exp2(MOD != 0 ? s1[i] - m : fmaf(s1[i], p.scale2, -m));
         l += s0[i] + s1[i];
       }
       pk_accumulate2<T, DT, PF>(o, V, s0, o, V + 32 * Tile::ROW, s1, at);
@@ -907,7 +1036,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd) y[nd] = at_zero16();
 #pragma unroll 1
-    for (int j = (odd ? c0 : max(all / kPkChunk, c0)) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
+    for (int j = MOD != 0 ? max(c0 * kPkChunk, lo) : (odd ? c0 : max(all / kPkChunk, c0)) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
 #pragma unroll
       for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
@@ -1013,7 +1142,7 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
 }
 
 // dq, and the rows' numbers for the key side (alone when gq is null).
-template <typename T, int DT>
+template <typename T, int DT, int MOD>
 __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_q_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
@@ -1024,7 +1153,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries w(p, lane, std::false_type());
+  const PkQueries<MOD> w(p, lane, std::false_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* gq = static_cast<T*>(p.gq);
@@ -1039,8 +1168,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   const int wend = wr0 < w.rows ? w.seen(p, min(wr0 + 31, w.rows - 1)) : 0;
   const int wfull = wr0 + 31 < w.rows ? w.seen(p, wr0) : 0;
   const int all = w.seen(p, w.r0);  // keys that every row of the workgroup sees
-  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk;
-  const int chunks = (end + kPkChunk - 1) / kPkChunk;
+  const int lo = MOD != 0 && valid ? w.from(p, ri) : 0, span = max(lim - lo, 0);  // as in the forward
+  const int wbegin = MOD != 0 && wr0 < w.rows ? w.from(p, wr0) : 0;
+  const int wlo = MOD != 0 && wr0 < w.rows ? w.from(p, min(wr0 + 31, w.rows - 1)) : 0, alo = MOD != 0 ? w.from(p, r1 - 1) : 0;
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = MOD != 0 && p.window < kPkChunk;
+  const int cb = w.from(p, w.r0) / kPkChunk, chunks = (end + kPkChunk - 1) / kPkChunk;
+  PkBias bias{0.0f, 0.0f};
+  if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, rc, grp);
   PkRow<T, DT> q, go;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, rc), valid, p.dim, grp);
   go.load(w.row(p, static_cast<const T*>(p.go), kPkGO, rc), valid, p.dim, grp);
@@ -1064,7 +1198,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     // for the key side: delta; bf16: -delta and -(m + log2 l) / scale2, which its sums start from (the weight is
     // 2^(scale2 s) then; the number is rounded at its own size, 2^-24 of it)
     if (p.numbers != nullptr && valid && grp == 0)
-      *reinterpret_cast<at_f4*>(p.numbers + row) = sizeof(T) == 2 ? at_f4{m, ll, -delta, -(m + ll) / p.scale2} : at_f4{m, ll, delta, 0.0f};
+      *reinterpret_cast<at_f4*>(p.numbers + row) = sizeof(T) == 2 ? at_f4{m, ll, -delta, (MOD & kPkCap) != 0 ? -(m + ll) : -(m + ll) / p.scale2} : at_f4{m, ll, delta, 0.0f};
   }
   if (gq == nullptr) return;
   constexpr bool bf = sizeof(T) == 2;
@@ -1083,13 +1217,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
-    if (min(k0 + kPkChunk, w.m) > all) {
-      if (threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
+    if (MOD != 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;  // settled chunks at both ends of the range, others between them
+    if (min(k0 + kPkChunk, w.m) > all || (MOD != 0 && k0 < alo)) {
+      if (MOD == 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
       pk_settle<T, DT>(Kb, bad[turn]);
-      const uint64_t sick = pk_settled(bad[turn]);
+      uint64_t sick = pk_settled(bad[turn]);
+      if constexpr (MOD != 0) sick = sick != 0 && lo - k0 < kPkChunk ? sick >> max(lo - k0, 0) << max(lo - k0, 0) : 0;
       if (sick != 0 && k0 + static_cast<int>(__builtin_ctzll(sick)) < lim) factor = NAN;
     }
-    if (k0 >= wend) {
+    if (k0 >= wend || (MOD != 0 && k0 + kPkChunk <= wbegin)) {
       next.all();
       return;
     }
@@ -1102,13 +1238,35 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       typename P::Weights wa, wb;
       PkLane<T, DT> now = at;  // as in pk_bwd_kv_kernel
       asm volatile("" : "+v"(now.row), "+v"(now.tr));
-      auto weigh = [&](at_f16& s, auto t) { pk_beside<KS, t>([&](int i) { s[i] = at_exp2(fmaf(s[i], p.scale2, -m)); }); };
+      bool far = false;
+      // MOD: weights, times the slope of the cap
+      auto weigh = [&](at_f16& s, int k, auto t) {
+        if constexpr (MOD == 0) {
+          pk_beside<KS, t>([&](int i) { s[i] = at_exp2(fmaf(s[i], p.scale2, -m)); });
+        } else {
+          if constexpr ((MOD & kPkCap) != 0 && t == 1) far = pk_far<T>(p, s);
+          PkBias b = bias;
+          if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
+          auto shape = [&](int i, float bent) {
+            float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, -m) : fmaf(s[i], p.scale2, -m);
+            if constexpr ((MOD & kPkSlope) != 0) x = b.add(x, 8 * (i >> 2) + (i & 3));
+            s[i] = at_exp2(x);
+            if constexpr ((MOD & kPkCap) != 0) s[i] *= fmaf(-bent, bent, 1.0f);
+          };
+          if ((MOD & kPkCap) != 0 && far) pk_beside<KS, t>([&](int i) { shape(i, pk_bent<T>(p, s[i])); });
+          else pk_beside<KS, t>([&](int i) { shape(i, pk_near<T>(s[i] * p.inner)); });
+        }
+      };
       auto slope = [&](at_f16& s, const at_f16& d, typename P::Weights& w, int k, auto t) {
         pk_beside<KS, t>([&](int i) { s[i] *= d[i] - delta; });
         if constexpr (t == KS - 1) {
-          if (k + 32 > wfull) {
+          if (MOD == 0 && k + 32 > wfull) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = k + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+          }
+          if (MOD != 0 && (k + 32 > wfull || k < wlo)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = static_cast<uint32_t>(k + 8 * (i >> 2) + 4 * grp + (i & 3) - lo) < static_cast<uint32_t>(span) ? s[i] : 0.0f;
           }
           w.set(s);
         }
@@ -1133,12 +1291,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
             constexpr int b = i / KS;
             constexpr PkInt<i % KS> t{};
             if constexpr (i < 2 * Stream::NV) next.template piece<i>();
-            if constexpr (b == 1) weigh(sa, t);
+            if constexpr (b == 1) weigh(sa, k0, t);
             if constexpr (b == 2) slope(sa, da, wa, k0, t);
-            if constexpr (b == 3) weigh(sb, t);
+            if constexpr (b == 3) weigh(sb, k0 + 32, t);
             if constexpr (b == 4) slope(sb, db, wb, k0 + 32, t);
           });
-      if (k0 == 0 && few)  // as in the forward: of ds
+      if ((k0 == 0 && few) || narrow)  // as in the forward: of ds
         pk_accumulate2<T, DT, 2>(dq, K, pk_rest(sa), dq, K + 32 * Tile::ROW, pk_rest(sb), now);
     } else {
       next.all();
@@ -1146,18 +1304,35 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       for (int h = 0; h < kPkChunk; h += 32) {
         at_f16 s = at_zero16(), dp = at_zero16();
         pk_scores2<T, DT, PF>(s, K + h * Tile::ROW, q, dp, V + h * Tile::ROW, go, at);
+        if constexpr (MOD == 0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
-        if (k0 + h + 32 > wfull) {
+          for (int i = 0; i < 16; ++i) s[i] = at_exp2(fmaf(s[i], p.scale2, -m) - ll) * (dp[i] - delta);
+          if (k0 + h + 32 > wfull) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+            for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
+          }
+        } else {
+          PkBias b = bias;
+          if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k0 + h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float bent = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s[i]) : 0.0f;
+            float x = (MOD & kPkCap) != 0 ? bent * p.cap2 : s[i] * p.scale2;
+            if constexpr ((MOD & kPkSlope) != 0) x = b.add(x, 8 * (i >> 2) + (i & 3));
+            s[i] = at_exp2((x - m) - ll) * (dp[i] - delta);
+            if constexpr ((MOD & kPkCap) != 0) s[i] *= fmaf(-bent, bent, 1.0f);
+          }
+          if (k0 + h + 32 > wfull || k0 + h < wlo) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = static_cast<uint32_t>(k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) - lo) < static_cast<uint32_t>(span) ? s[i] : 0.0f;
+          }
         }
         pk_accumulate<T, DT, PF>(dq, K + h * Tile::ROW, s, at);
       }
     }
   };
-  if (chunks > 0) tile(X0, Y0, 0).all();
-  for (int c = 0; c < chunks; c += 2) {
+  if (cb < chunks) tile(X0, Y0, cb).all();
+  for (int c = cb; c < chunks; c += 2) {
     pk_barrier();
     chunk(X0, Y0, 0, c, tile(X1, Y1, c + 1));
     if (c + 1 >= chunks) break;
@@ -1172,12 +1347,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
 
 // ---- keys on their own side: dk and dv ---------------------------------------------------------
 
+template <bool RANGES>
 struct PkKeys {
   PkPlace w;
   int kv_head, part;
   int b0, b1;            // keys of the tile, in the sequence's range
   int m, n, q_first;     // keys and queries of the sequence, its first query row
-  int shift;
+  int shift, prefix;
   int first, chunks;     // the first token that sees a key of the tile; chunks of tokens from there
   int parts;             // workgroups that share them
   // b: tile and key head (fastest, as in PkQueries; the first tiles, which the most queries of a causal sequence
@@ -1196,13 +1372,25 @@ struct PkKeys {
     }
     shift = m - n;
     first = p.causal ? min(max(b0 - shift, 0), n) : 0;
-    chunks = b0 < m ? (n - first + walk.tokens - 1) / walk.tokens : 0;
+    int end = n;
+    prefix = 0;
+    if constexpr (RANGES) {
+      // lo and hi rise with the token: those with hi > b0 and lo < the tile's end
+      if (p.prefix != nullptr && w.seq >= 0) prefix = p.prefix[w.seq];
+      const int64_t reach = static_cast<int64_t>(b0) - p.window + 1 - shift;
+      if (!p.causal || prefix > b0) first = static_cast<int>(min(max(reach, static_cast<int64_t>(0)), static_cast<int64_t>(first)));
+      if (!p.causal) first = static_cast<int>(min(max(reach, static_cast<int64_t>(0)), static_cast<int64_t>(n)));
+      end = static_cast<int>(min(max(static_cast<int64_t>(min(b1, m)) - 1 + p.window - shift, static_cast<int64_t>(first)), static_cast<int64_t>(n)));
+    }
+    chunks = b0 < m ? (end - first + walk.tokens - 1) / walk.tokens : 0;
     parts = min(max((chunks + kPkPart - 1) / kPkPart, 1), p.splits);
   }
   template <typename T>
   __device__ T* row(const PackParams& p, T* base, int t, int j) const {
     return base + (static_cast<int64_t>(w.first) + j) * p.st[t][0] + kv_head * p.st[t][1];
   }
+  __device__ int hi(const PackParams& p, int t) const { return pk_hi(p, t + shift, prefix, m); }
+  __device__ int lo(const PackParams& p, int t) const { return pk_lo(p, t + shift); }
   // row of the parts' sums of key j
   __device__ int64_t part_row(const PackParams& p, int which, int j) const {
     return (static_cast<int64_t>(which) * p.k_rows + w.first + j) * p.kv_heads + kv_head;
@@ -1212,7 +1400,7 @@ struct PkKeys {
 // A workgroup takes 128 keys, 32 a wave in registers, and walks over the rows (tokens and heads of the key
 // head's group) that see them, 64 at a time. A tile that many rows see is shared by several workgroups,
 // whose sums pk_join_kv_kernel adds in their order.
-template <typename T, int DT>
+template <typename T, int DT, int MOD>
 __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_kv_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
@@ -1224,6 +1412,9 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   // the keys that the row sees
   __shared__ __align__(16) float row_s[2][kPkChunk], row_d[2][kPkChunk], row_l[2][sizeof(T) == 2 ? 4 : kPkChunk];
   __shared__ __align__(16) int row_lim[2][kPkChunk];
+  // MOD: the first of these keys, the row's place less the tile's first key, and its slope, which the head gives
+  __shared__ __align__(16) int row_lo[2][MOD != 0 ? kPkChunk : 4];
+  __shared__ __align__(16) float row_place[2][(MOD & kPkSlope) != 0 ? kPkChunk : 4], row_slope[(MOD & kPkSlope) != 0 ? kPkChunk : 4];
   constexpr bool bf = sizeof(T) == 2;
   constexpr int PF = bf && DT != 64 && DT != 128 ? 3 : 2;
   // At 128 channels k, v, dk and dv take 192 of a wave's 256 registers. The last KEEP pieces of v wait in LDS: in
@@ -1236,7 +1427,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   // the parts of a tile are a grid of tiles apart, the last of all tiles first: of shared tiles all parts are full,
   // those of one part, down to a few rows, come last and even out
   const int tiles = static_cast<int>(gridDim.x) / p.splits, turn = static_cast<int>(blockIdx.x) / tiles;
-  const PkKeys w(p, walk, lane, static_cast<int>(blockIdx.x) - turn * tiles, p.splits - 1 - turn);
+  const PkKeys<MOD != 0> w(p, walk, lane, static_cast<int>(blockIdx.x) - turn * tiles, p.splits - 1 - turn);
   if (w.b0 >= w.w.own || w.part >= w.parts) return;
   T* gk = static_cast<T*>(p.gk);
   T* gv = static_cast<T*>(p.gv);
@@ -1245,8 +1436,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     if (gv != nullptr) pk_zero_rows<T>(w.b0, w.b1, p.dim, [&](int j) { return w.row(p, gv, kPkGV, j); });
     return;
   }
-  const int m = w.m, shift = w.shift;
+  const int m = w.m, shift = w.shift, wb = w.b0;
   const int wb0 = w.b0 + 32 * wave;
+  if constexpr ((MOD & kPkSlope) != 0)  // before the first barrier
+    if (threadIdx.x < kPkChunk) {
+      const int g = static_cast<int>(threadIdx.x) - walk.token(threadIdx.x) * p.group;
+      row_slope[threadIdx.x] = p.slopes[w.kv_head * p.group + g] * -1.44269504f;
+    }
   PkRow<T, DT> k, v;
   {
     const int kj = wb0 + col;
@@ -1283,10 +1479,17 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     if (wave == 0) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_s[buf]), 4, o + (bf ? 12 : 0), 0, 0, 0);
     if (wave == 1) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_d[buf]), 4, o + 8, 0, 0, 0);
     if (wave == 2 && !bf) __builtin_amdgcn_raw_ptr_buffer_load_lds(ss, (MSDA_LDS void*)(row_l[buf]), 4, o + 4, 0, 0, 0);
-    if (wave == 3) row_lim[buf][x] = x >= count ? 0 : p.causal ? min(max(t0 + t + shift + 1, 0), m) : m;
+    if constexpr (MOD == 0) {
+      if (wave == 3) row_lim[buf][x] = x >= count ? 0 : p.causal ? min(max(t0 + t + shift + 1, 0), m) : m;
+    } else if (wave == 3) {
+      row_lim[buf][x] = x >= count ? 0 : w.hi(p, t0 + t);
+      row_lo[buf][x] = w.lo(p, t0 + t);
+      if constexpr ((MOD & kPkSlope) != 0) row_place[buf][x] = static_cast<float>(t0 + t + shift - w.b0);
+    }
   };
   // One 32-row block; `all`: every row sees every key of the wave.
-  auto block = [&](bool all, PkLds Q, PkLds G, int h, const float* rs, const float* rd, const float* rl, const int* lims) {
+  auto block = [&](bool all, PkLds Q, PkLds G, int h, const float* rs, const float* rd, const float* rl, const int* lims, const int* los, const float* places,
+                   const float* slopes) {
     // All that a lane's place gives is formed anew in each block, the operands' offsets in each phase: kept, they spill
     // at 128 channels.
     int thread = threadIdx.x;
@@ -1297,10 +1500,10 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     now.tr += h * Tile::ROW;
     asm volatile("" : "+v"(now.row), "+v"(now.tr));
     // bf16: the matrix units start from the rows' numbers
-    auto start = [&](at_f16& x, const float* numbers) {
+    auto start = [&](at_f16& x, const float* numbers, bool zero) {
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
-        const at_f4 a = bf ? *reinterpret_cast<const at_f4*>(numbers + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        const at_f4 a = !zero ? *reinterpret_cast<const at_f4*>(numbers + 8 * c4 + 4 * grp) : at_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[4 * c4 + j] = a[j];
       }
@@ -1308,12 +1511,23 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     uint32_t kept = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((MSDA_LDS unsigned char*)(kept_rows))) + thread * 16;
     asm volatile("" : "+v"(kept));  // one register: the arrays' addresses do not fit an LDS instruction's offset
     at_f16 s, dp;
-    start(s, rs);
-    if (!bf) start(dp, rd);
+    start(s, rs, !bf || (MOD & kPkCap) != 0);
+    if (!bf) start(dp, rd, true);
     using P = PkProducts<T, DT>;
     const int kj = wb0 + col;
     auto unseen = [&](at_f16& x) {  // pairs that are not seen weigh nothing
       if (all) return;
+      if constexpr (MOD != 0) {
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp), lf = *reinterpret_cast<const int4*>(los + 8 * c4 + 4 * grp);
+          x[4 * c4] = kj < lm.x && kj >= lf.x ? x[4 * c4] : 0.0f;
+          x[4 * c4 + 1] = kj < lm.y && kj >= lf.y ? x[4 * c4 + 1] : 0.0f;
+          x[4 * c4 + 2] = kj < lm.z && kj >= lf.z ? x[4 * c4 + 2] : 0.0f;
+          x[4 * c4 + 3] = kj < lm.w && kj >= lf.w ? x[4 * c4 + 3] : 0.0f;
+        }
+        return;
+      }
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
         const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
@@ -1327,6 +1541,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       // Phases of KS products: S, dP beside the weights, dv beside ds, dk.
       constexpr int KS = P::kScores;
       typename P::Weights w, ds;
+      bool far = false;
+      at_f16 bend;  // the slopes of the cap
       at_bf8 last[KEEP > 0 ? KEEP : 1];
       pk_pipe<4 * KS, PF>(
           [&](auto i) {
@@ -1346,13 +1562,27 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
           },
           [&](auto i) {
             constexpr int b = i / KS, t = i % KS;
-            if constexpr (i == KS - 1) start(dp, rd);
+            if constexpr (i == KS - 1) start(dp, rd, false);
             if constexpr (KEEP > 0 && b == 1 && t + 2 >= KS - KEEP && t + 2 < KS)
               last[t + 2 - (KS - KEEP)] = *reinterpret_cast<const MSDA_LDS at_bf8*>(reinterpret_cast<PkLds>(static_cast<uintptr_t>(kept)) + (t + 2 - (KS - KEEP)) * kPkWaves * 1024);
-            if constexpr (b == 1) pk_beside<KS, t>([&](int j) { s[j] = at_exp2(s[j] * p.scale2); });
+            if constexpr (b == 1 && MOD == 0) pk_beside<KS, t>([&](int j) { s[j] = at_exp2(s[j] * p.scale2); });
+            if constexpr (b == 1 && MOD != 0) {
+              if constexpr ((MOD & kPkCap) != 0 && t == 1) far = pk_far<T>(p, s);
+              // register j, its row's number (with the cap; else the products started from it) and bias
+              auto shape = [&](int j, float bent) {
+                const int row = 8 * (j >> 2) + 4 * grp + (j & 3);
+                float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, rs[row]) : s[j] * p.scale2;
+                if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[row], fabsf(places[row] - static_cast<float>(kj - static_cast<int>(wb))), x);
+                s[j] = at_exp2(x);
+                if constexpr ((MOD & kPkCap) != 0) bend[j] = fmaf(-bent, bent, 1.0f);
+              };
+              if ((MOD & kPkCap) != 0 && far) pk_beside<KS, t>([&](int j) { shape(j, pk_bent<T>(p, s[j])); });
+              else pk_beside<KS, t>([&](int j) { shape(j, pk_near<T>(s[j] * p.inner)); });
+            }
             if constexpr (b == 1 && t == KS - 1) {
               unseen(s);
               w.set(s);
+              if constexpr ((MOD & kPkCap) != 0) s *= bend;
             }
             if constexpr (b == 2) pk_beside<KS, t>([&](int j) { dp[j] *= s[j]; });
             if constexpr (b == 2 && t == KS - 1) {
@@ -1370,8 +1600,17 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = 4 * c4 + j;
-          s[i] = at_exp2(fmaf(s[i], p.scale2, -mm[j]) - ll[j]);
-          dp[i] = s[i] * (dp[i] - dd[j]);
+          if constexpr (MOD == 0) {
+            s[i] = at_exp2(fmaf(s[i], p.scale2, -mm[j]) - ll[j]);
+            dp[i] = s[i] * (dp[i] - dd[j]);
+          } else {
+            const float bent = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s[i]) : 0.0f;
+            float x = (MOD & kPkCap) != 0 ? bent * p.cap2 : s[i] * p.scale2;
+            if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[a + j], fabsf(places[a + j] - static_cast<float>(kj - wb)), x);
+            s[i] = at_exp2((x - mm[j]) - ll[j]);
+            dp[i] = s[i] * (dp[i] - dd[j]);
+            if constexpr ((MOD & kPkCap) != 0) dp[i] *= fmaf(-bent, bent, 1.0f);
+          }
         }
       }
       unseen(s);
@@ -1382,23 +1621,42 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   bool spoilt = false;  // the lane's key is seen by a row that is not finite
   auto settle = [&](unsigned char* Q, unsigned char* G, int buf, int c) {
     const int t0 = w.first + c * walk.tokens;
-    if (!p.causal || t0 + shift >= min(w.b1, m) - 1) return;  // every row sees every key
-    if (threadIdx.x < 2) bad[buf ^ 1][threadIdx.x] = 0;
+    if (MOD != 0 && threadIdx.x < 2) bad[buf ^ 1][threadIdx.x] = 0;
+    if constexpr (MOD == 0) {
+      if (!p.causal || t0 + shift >= min(w.b1, m) - 1) return;  // every row sees every key
+    } else if (w.hi(p, t0) >= min(w.b1, m) && w.lo(p, min(t0 + walk.tokens, w.n) - 1) <= w.b0) {
+      return;
+    }
+    if (MOD == 0 && threadIdx.x < 2) bad[buf ^ 1][threadIdx.x] = 0;
     pk_settle<T, DT>(Q, bad[buf]);
     pk_settle<T, DT>(G, bad[buf]);
     const uint64_t sick = pk_settled(bad[buf]);
+    if constexpr (MOD != 0) {
+      for (uint64_t left = sick; left != 0; left &= left - 1) {
+        const int x = static_cast<int>(__builtin_ctzll(left));
+        spoilt = spoilt || (wb0 + col < row_lim[buf][x] && wb0 + col >= row_lo[buf][x]);
+      }
+      return;
+    }
     // rows see more keys the later they come
     if (sick != 0) spoilt = spoilt || wb0 + col < row_lim[buf][63 - static_cast<int>(__builtin_clzll(sick))];
   };
   auto chunk = [&](const unsigned char* Qb, const unsigned char* Gb, int buf, int c) {
     PkLds Q = (PkLds)(Qb), G = (PkLds)(Gb);
     const int t0 = w.first + c * walk.tokens, t1 = min(t0 + walk.tokens, w.n), count = (t1 - t0) * p.group;
-    if (wb0 >= m || (p.causal && t1 + shift <= wb0)) return;
-    // every row sees every key of the wave
-    const bool full = __builtin_amdgcn_readfirstlane(count == kPkChunk && wb0 + 32 <= m && (!p.causal || t0 + shift >= wb0 + 31)) != 0;
+    bool seen;  // every row sees every key of the wave
+    if constexpr (MOD == 0) {
+      if (wb0 >= m || (p.causal && t1 + shift <= wb0)) return;
+      seen = count == kPkChunk && wb0 + 32 <= m && (!p.causal || t0 + shift >= wb0 + 31);
+    } else {
+      if (wb0 >= m || w.hi(p, t1 - 1) <= wb0 || w.lo(p, t0) >= wb0 + 32) return;
+      seen = count == kPkChunk && wb0 + 32 <= m && w.hi(p, t0) >= wb0 + 32 && w.lo(p, t1 - 1) <= wb0;
+    }
+    const bool full = __builtin_amdgcn_readfirstlane(seen) != 0;
 #pragma unroll 1
     for (int h = 0; h < count; h += 32)
-      block(full, Q, G, h, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h);
+      block(full, Q, G, h, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h, row_lo[buf] + (MOD != 0 ? h : 0),
+            row_place[buf] + ((MOD & kPkSlope) != 0 ? h : 0), row_slope + ((MOD & kPkSlope) != 0 ? h : 0));
   };
   if (c0 < c1) stage(X0, Y0, 0, c0);
   for (int c = c0; c < c1; c += 2) {
@@ -1448,10 +1706,10 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
 }
 
 // The sums of a tile's parts, in their order: kPkJoin workgroups a tile, of all key heads (which have as many parts).
-template <typename T>
+template <typename T, bool RANGES>
 __global__ void __launch_bounds__(256) pk_join_kv_kernel(const PackParams p) {
   const int tile = static_cast<int>(blockIdx.x) / kPkJoin, share = kPkTile / kPkJoin;
-  PkKeys w(p, PkRows(p.group), threadIdx.x & 63, tile * p.kv_heads, 0);
+  PkKeys<RANGES> w(p, PkRows(p.group), threadIdx.x & 63, tile * p.kv_heads, 0);
   if (w.parts == 1) return;
   const int first = w.b0 + share * (static_cast<int>(blockIdx.x) % kPkJoin), keys = min(share, w.b1 - first), pieces = p.dim / 4;
   for (int i = threadIdx.x; i < 2 * keys * p.kv_heads * pieces; i += 256) {

@@ -16,9 +16,9 @@ int pk_launch(K kernel, int64_t grid, const msda::PackParams& p, hipStream_t st,
   return check_launch(what);
 }
 
-template <typename T, int DT>
+template <typename T, int DT, int MOD>
 int pk_fwd(const msda::PackParams& p, hipStream_t st) {
-  const int rc = pk_launch(msda::pk_fwd_kernel<T, DT>, static_cast<int64_t>(p.slots) * p.splits * p.kv_heads, p, st, "packed attention forward");
+  const int rc = pk_launch(msda::pk_fwd_kernel<T, DT, MOD>, static_cast<int64_t>(p.slots) * p.splits * p.kv_heads, p, st, "packed attention forward");
   if (rc != MSDA_OK || p.splits == 1) return rc;
   constexpr int LPR = DT <= 64 ? 16 : 32;
   return pk_launch(msda::pk_join_kernel<T, LPR>, (static_cast<int64_t>(p.q_rows) * p.heads + 256 / LPR - 1) / (256 / LPR), p, st,
@@ -26,38 +26,53 @@ int pk_fwd(const msda::PackParams& p, hipStream_t st) {
 }
 
 // q_slots, k_slots: tiles of the queries' and of the keys' side; p.splits: parts of a key tile
-template <typename T, int DT>
+template <typename T, int DT, int MOD>
 int pk_bwd(msda::PackParams p, int q_slots, int k_slots, hipStream_t st) {
   p.slots = q_slots;
-  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT>, static_cast<int64_t>(q_slots) * p.kv_heads, p, st, "packed attention backward (queries)");
+  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT, MOD>, static_cast<int64_t>(q_slots) * p.kv_heads, p, st, "packed attention backward (queries)");
   if (rc != MSDA_OK || (p.gk == nullptr && p.gv == nullptr)) return rc;
   p.slots = k_slots;
-  rc = pk_launch(msda::pk_bwd_kv_kernel<T, DT>, static_cast<int64_t>(k_slots) * p.splits * p.kv_heads, p, st,
+  rc = pk_launch(msda::pk_bwd_kv_kernel<T, DT, MOD>, static_cast<int64_t>(k_slots) * p.splits * p.kv_heads, p, st,
                  "packed attention backward (keys, values)");
   if (rc != MSDA_OK || p.splits == 1) return rc;
-  return pk_launch(msda::pk_join_kv_kernel<T>, static_cast<int64_t>(k_slots) * msda::kPkJoin, p, st, "packed attention backward (join)");
+  return pk_launch(msda::pk_join_kv_kernel<T, MOD != 0>, static_cast<int64_t>(k_slots) * msda::kPkJoin, p, st, "packed attention backward (join)");
 }
 
-template <typename T>
+// MOD: 0, or the kernels of shaped scores (enum PackShaped)
+template <typename T, int MOD>
 int dispatch_pk_fwd(const msda::PackParams& p, hipStream_t st) {
-  if (p.dim <= 32) return pk_fwd<T, 32>(p, st);
-  if (p.dim <= 64) return pk_fwd<T, 64>(p, st);
-  if (p.dim <= 96) return pk_fwd<T, 96>(p, st);
-  return pk_fwd<T, 128>(p, st);
+  if (p.dim <= 32) return pk_fwd<T, 32, MOD>(p, st);
+  if (p.dim <= 64) return pk_fwd<T, 64, MOD>(p, st);
+  if (p.dim <= 96) return pk_fwd<T, 96, MOD>(p, st);
+  return pk_fwd<T, 128, MOD>(p, st);
 }
 
-template <typename T>
+template <typename T, int MOD>
 int dispatch_pk_bwd(const msda::PackParams& p, int q_slots, int k_slots, hipStream_t st) {
-  if (p.dim <= 32) return pk_bwd<T, 32>(p, q_slots, k_slots, st);
-  if (p.dim <= 64) return pk_bwd<T, 64>(p, q_slots, k_slots, st);
-  if (p.dim <= 96) return pk_bwd<T, 96>(p, q_slots, k_slots, st);
-  return pk_bwd<T, 128>(p, q_slots, k_slots, st);
+  if (p.dim <= 32) return pk_bwd<T, 32, MOD>(p, q_slots, k_slots, st);
+  if (p.dim <= 64) return pk_bwd<T, 64, MOD>(p, q_slots, k_slots, st);
+  if (p.dim <= 96) return pk_bwd<T, 96, MOD>(p, q_slots, k_slots, st);
+  return pk_bwd<T, 128, MOD>(p, q_slots, k_slots, st);
 }
 
-// Instantiated in packed_attention_{fwd,bwd}_{f32,bf16}.hip.
-extern template int dispatch_pk_fwd<float>(const msda::PackParams&, hipStream_t);
-extern template int dispatch_pk_fwd<msda::bf16_t>(const msda::PackParams&, hipStream_t);
-extern template int dispatch_pk_bwd<float>(const msda::PackParams&, int, int, hipStream_t);
-extern template int dispatch_pk_bwd<msda::bf16_t>(const msda::PackParams&, int, int, hipStream_t);
+// Instantiated in packed_attention_{fwd,bwd}_{f32,bf16}.hip and packed_attention_shaped_{fwd,bwd}_*.hip.
+#define MSDA_PK_FWD(T, MOD) template int dispatch_pk_fwd<T, MOD>(const msda::PackParams&, hipStream_t)
+#define MSDA_PK_BWD(T, MOD) template int dispatch_pk_bwd<T, MOD>(const msda::PackParams&, int, int, hipStream_t)
+#ifndef MSDA_PK_INSTANTIATE
+#define MSDA_PK_EXTERN(T) \
+  extern MSDA_PK_FWD(T, 0); \
+  extern MSDA_PK_FWD(T, 4); \
+  extern MSDA_PK_FWD(T, 5); \
+  extern MSDA_PK_FWD(T, 6); \
+  extern MSDA_PK_FWD(T, 7); \
+  extern MSDA_PK_BWD(T, 0); \
+  extern MSDA_PK_BWD(T, 4); \
+  extern MSDA_PK_BWD(T, 5); \
+  extern MSDA_PK_BWD(T, 6); \
+  extern MSDA_PK_BWD(T, 7)
+MSDA_PK_EXTERN(float);
+MSDA_PK_EXTERN(msda::bf16_t);
+#undef MSDA_PK_EXTERN
+#endif
 
 }  // namespace msda_host

@@ -27,12 +27,16 @@ struct PackSplit {
   int most, part;
 };
 
-inline PackSplit pk_split(const PackShape& s) {
+// Keys that a tile of queries sees inside a window, at most.
+constexpr int pk_in_window(int window) { return window > (1 << 30) ? window : window + kPkTile; }
+
+// `window`: of shaped scores; the largest int where there is none.
+inline PackSplit pk_split(const PackShape& s, int window = 0x7fffffff) {
   const PackSplit none{1, 1 << 30};
   if (s.sequences == 0) return none;
   const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads);
   const int64_t tiles = std::min<int64_t>(rows, rows / kPkTile + s.sequences) * s.kv_heads;
-  const int64_t chunks = (s.k_rows / s.sequences + kPkChunk - 1) / kPkChunk;  // of an average sequence
+  const int64_t chunks = (std::min(s.k_rows / s.sequences, pk_in_window(window)) + kPkChunk - 1) / kPkChunk;  // of an average sequence
   if (tiles == 0) return none;
   // The work in parts that even out over the CUs: in bf16 one to each of the two workgroups that a CU holds, in f32 8
   // to a CU. The chunks counted here are those of the keys' room, not of their lengths, so there may be fewer parts with

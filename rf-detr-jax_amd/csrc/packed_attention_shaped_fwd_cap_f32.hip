@@ -1,0 +1,8 @@
+// packed_attention_shaped_fwd_cap_f32.hip — the forward kernels of shaped scores with a cap for f32 tensors.
+#define MSDA_PK_INSTANTIATE
+#include "packed_attention_launch.h"
+
+namespace msda_host {
+MSDA_PK_FWD(float, 5);
+MSDA_PK_FWD(float, 7);
+}  // namespace msda_host

@@ -51,10 +51,10 @@ struct Library {
   decltype(&msda_value_proj_bwd_workspace_size) value_proj_bwd_workspace_size;
   decltype(&msda_attention_fwd) attention_fwd;
   decltype(&msda_attention_bwd) attention_bwd;
-  decltype(&msda_packed_attention_fwd) packed_fwd;
-  decltype(&msda_packed_attention_bwd_const) packed_bwd;
-  decltype(&msda_packed_attention_fwd_workspace_size) packed_fwd_workspace_size;
-  decltype(&msda_packed_attention_bwd_workspace_size) packed_bwd_workspace_size;
+  decltype(&msda_packed_attention_shaped_fwd) packed_fwd;
+  decltype(&msda_packed_attention_shaped_bwd) packed_bwd;
+  decltype(&msda_packed_attention_shaped_fwd_workspace_size) packed_fwd_workspace_size;
+  decltype(&msda_packed_attention_shaped_bwd_workspace_size) packed_bwd_workspace_size;
   decltype(&msda_rotary) rotary;
 };
 
@@ -79,10 +79,10 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_value_proj_bwd_workspace_size", lib.value_proj_bwd_workspace_size);
   get("msda_attention_fwd", lib.attention_fwd);
   get("msda_attention_bwd", lib.attention_bwd);
-  get("msda_packed_attention_fwd", lib.packed_fwd);
-  get("msda_packed_attention_bwd_const", lib.packed_bwd);
-  get("msda_packed_attention_fwd_workspace_size", lib.packed_fwd_workspace_size);
-  get("msda_packed_attention_bwd_workspace_size", lib.packed_bwd_workspace_size);
+  get("msda_packed_attention_shaped_fwd", lib.packed_fwd);
+  get("msda_packed_attention_shaped_bwd", lib.packed_bwd);
+  get("msda_packed_attention_shaped_fwd_workspace_size", lib.packed_fwd_workspace_size);
+  get("msda_packed_attention_shaped_bwd_workspace_size", lib.packed_bwd_workspace_size);
   get("msda_rotary", lib.rotary);
   check_status = py::object(check).release().ptr();
   parameter_type = reinterpret_cast<PyTypeObject*>(py::object(parameter).release().ptr());
@@ -571,13 +571,19 @@ struct Packed {  // one call's sizes
   int sequences, q_rows, k_rows, heads, kv_heads, dim;
   bool causal;
   float scale;
-  Packed(const Tensor& q, const Tensor& k, const Tensor& offsets, bool c, double s)
+  float cap;           // 0: none
+  int window;          // 0: none
+  Tensor slopes, prefix;  // or undefined
+  Packed(const Tensor& q, const Tensor& k, const Tensor& offsets, bool c, double s, double cap_, int64_t window_, const Tensor& slopes_, const Tensor& prefix_)
       : sequences(static_cast<int>(offsets.numel() - 1)), q_rows(static_cast<int>(q.size(0))), k_rows(static_cast<int>(k.size(0))),
         heads(static_cast<int>(q.size(1))), kv_heads(static_cast<int>(k.size(1))), dim(static_cast<int>(q.size(2))), causal(c),
-        scale(static_cast<float>(s)) {}
+        scale(static_cast<float>(s)), cap(static_cast<float>(cap_)), window(static_cast<int>(window_)), slopes(slopes_), prefix(prefix_) {}
+  msda_score_shape shape() const;
 };
 
 const int32_t* iptr(const Tensor& t) { return static_cast<const int32_t*>(ptr(t)); }
+
+msda_score_shape Packed::shape() const { return {cap, window, static_cast<const float*>(ptr(slopes)), iptr(prefix)}; }
 
 // (out, what its rounding left, statistics); the last two as the backward needs them
 std::array<Tensor, 3> packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& key_offsets,
@@ -587,13 +593,14 @@ std::array<Tensor, 3> packed_forward(const Tensor& q, const Tensor& k, const Ten
     if (q.scalar_type() == at::kBFloat16) rest = at::empty(q.sizes(), q.options());
     stats = at::empty({q.size(0), q.size(1), 4}, q.options().dtype(at::kFloat));
   }
-  const int64_t bytes = lib.packed_fwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim);
+  const int64_t bytes = lib.packed_fwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, p.window);
   check(bytes);
   if (bytes != 0) ws = workspace(bytes, q);
   const int64_t st[8] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1)};
+  const msda_score_shape shape = p.shape();
   launch(q, [&](void* stream) {
     return lib.packed_fwd(ptr(q), ptr(k), ptr(v), code(q), ptr(out), ptr(rest), fptr(stats), iptr(offsets), iptr(key_offsets), iptr(key_lengths),
-                          p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale, ptr(ws), bytes, stream);
+                          p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale, &shape, ptr(ws), bytes, stream);
   });
   return {out, rest, stats};
 }
@@ -602,9 +609,11 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, const Tensor& key_offsets,
                         const std::optional<Tensor>& key_lengths, const Packed& p) {
     const auto [out, rest, stats] = packed_forward(q, k, v, offsets, key_offsets, key_lengths.value_or(Tensor()), p, true);
-    ctx->save_for_backward({q, k, v, out, rest, stats, offsets, key_offsets, key_lengths.value_or(Tensor())});
+    ctx->save_for_backward({q, k, v, out, rest, stats, offsets, key_offsets, key_lengths.value_or(Tensor()), p.slopes, p.prefix});
     ctx->saved_data["causal"] = p.causal;
     ctx->saved_data["scale"] = static_cast<double>(p.scale);
+    ctx->saved_data["cap"] = static_cast<double>(p.cap);
+    ctx->saved_data["window"] = static_cast<int64_t>(p.window);
     return out;
   }
 
@@ -622,15 +631,19 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
              (!rest.defined() || rest.sizes() == q.sizes()) && stats.sizes().equals({q.size(0), q.size(1), 4}) && k.size(2) == q.size(2) &&
              k.size(1) != 0 && q.size(1) % k.size(1) == 0 && offsets.dim() == 1 && offsets.numel() >= 1 && key_offsets.sizes() == offsets.sizes() &&
              (!key_lengths.defined() || (key_lengths.dim() == 1 && key_lengths.numel() == offsets.numel() - 1)));
-    for (const Tensor* t : {&k, &v, &out, &rest, &stats, &offsets, &key_offsets, &key_lengths, &g})
+    const Tensor slopes = saved[9].defined() ? restored(saved[9], at::kFloat) : Tensor(), prefix = saved[10].defined() ? restored(saved[10], at::kInt) : Tensor();
+    saved_as((!slopes.defined() || slopes.sizes().equals({q.size(1)})) && (!prefix.defined() || prefix.sizes().equals({offsets.numel() - 1})));
+    for (const Tensor* t : {&k, &v, &out, &rest, &stats, &offsets, &key_offsets, &key_lengths, &slopes, &prefix, &g})
       saved_as(!t->defined() || t->device() == q.device());
-    const Packed p(q, k, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    const Packed p(q, k, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(),
+                   ctx->saved_data["window"].toInt(), slopes, prefix);
+    const msda_score_shape shape = p.shape();
     const auto like = [](bool wanted, const Tensor& t) { return wanted ? at::empty(t.sizes(), t.options()) : Tensor(); };
     Tensor gq = like(ctx->needs_input_grad(0), q), gk = like(ctx->needs_input_grad(1), k), gv = like(ctx->needs_input_grad(2), v), ws;
     // what the kernels hand on: other calls may read the statistics
     const Tensor numbers = like(gk.defined() || gv.defined(), stats);
     const int64_t bytes = gk.defined() || gv.defined()
-                              ? lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim)
+                              ? lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, p.window)
                               : 0;
     check(bytes);
     if (bytes != 0) ws = workspace(bytes, q);
@@ -644,7 +657,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     launch(q, [&](void* stream) {
       return lib.packed_bwd(ptr(q), ptr(k), ptr(v), ptr(out), ptr(rest), fptr(stats), fptr(numbers), ptr(g), code(q), ptr(gq), ptr(gk), ptr(gv), iptr(offsets),
                             iptr(key_offsets), iptr(key_lengths), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, st, p.causal, p.scale,
-                            ptr(ws), bytes, stream);
+                            &shape, ptr(ws), bytes, stream);
     });
     return once({gq, gk, gv, Tensor(), Tensor(), Tensor(), Tensor()}, "packed_attention");
   }
@@ -653,12 +666,14 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
 };
 
-// q [T, H, D], k and v [S, Hk, D]; scale: a Python float, or None
+// q [T, H, D], k and v [S, Hk, D]; scale, cap: a Python float, or None; window: a Python int, or None
 py::object packed_attention(const py::handle& q, const py::handle& k, const py::handle& v, const py::handle& offsets, const py::handle& key_offsets,
-                            const py::handle& key_lengths, bool causal, const py::handle& scale) {
-  const Tensor *a, *b, *c, *o, *ko, *kl = nullptr;
+                            const py::handle& key_lengths, bool causal, const py::handle& scale, const py::handle& cap, const py::handle& slopes,
+                            const py::handle& window, const py::handle& prefix_lengths) {
+  const Tensor *a, *b, *c, *o, *ko, *kl = nullptr, *sl = nullptr, *pl = nullptr;
   if (!ordinary_state() || (a = plain(q)) == nullptr || (b = plain(k)) == nullptr || (c = plain(v)) == nullptr || (o = plain(offsets)) == nullptr ||
-      (ko = key_offsets.is_none() ? o : plain(key_offsets)) == nullptr || (!key_lengths.is_none() && (kl = plain(key_lengths)) == nullptr))
+      (ko = key_offsets.is_none() ? o : plain(key_offsets)) == nullptr || (!key_lengths.is_none() && (kl = plain(key_lengths)) == nullptr) ||
+      (!slopes.is_none() && (sl = plain(slopes)) == nullptr) || (!prefix_lengths.is_none() && (pl = plain(prefix_lengths)) == nullptr))
     return py::none();
   if (!value_type(*a) || a->dim() != 3) return py::none();
   for (const Tensor* t : {a, b, c}) {
@@ -669,13 +684,24 @@ py::object packed_attention(const py::handle& q, const py::handle& k, const py::
   if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || a->size(1) == 0 || b->size(1) == 0 || a->size(1) % b->size(1) != 0 || a->size(1) > 64 * b->size(1) ||
       a->size(2) == 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
     return py::none();
-  for (const Tensor* t : {o, ko, kl})
+  if (sl != nullptr && (sl->dim() != 1 || sl->size(0) != a->size(1) || !f32(*sl) || sl->device() != a->device() || !sl->is_contiguous() || sl->requires_grad()))
+    return py::none();
+  if (pl != nullptr && (!causal || pl->numel() != o->numel() - 1)) return py::none();
+  for (const Tensor* t : {o, ko, kl, pl})
     if (t != nullptr && (t->dim() != 1 || t->scalar_type() != at::kInt || t->device() != a->device() || !t->is_contiguous())) return py::none();
   if (ko->numel() != o->numel() || (kl != nullptr && kl->numel() != o->numel() - 1)) return py::none();
   if (!scale.is_none() && !PyFloat_CheckExact(scale.ptr())) return py::none();
   const double s = scale.is_none() ? 1.0 / std::sqrt(static_cast<double>(a->size(2))) : PyFloat_AS_DOUBLE(scale.ptr());
   if (!(s >= 0x1p-64 && s <= 0x1p64)) return py::none();
-  const Packed p(*a, *b, *o, causal, s);
+  if ((!cap.is_none() && !PyFloat_CheckExact(cap.ptr())) || (!window.is_none() && !PyLong_CheckExact(window.ptr()))) return py::none();
+  const double top = cap.is_none() ? 0.0 : PyFloat_AS_DOUBLE(cap.ptr());
+  if (!cap.is_none() && !(top >= 0x1p-32 && top <= 0x1p32)) return py::none();
+  const int64_t reach = window.is_none() ? 0 : PyLong_AsLongLong(window.ptr());
+  if (!window.is_none() && (reach < 1 || reach >= (int64_t{1} << 31))) {
+    PyErr_Clear();
+    return py::none();
+  }
+  const Packed p(*a, *b, *o, causal, s, top, reach, sl != nullptr ? *sl : Tensor(), pl != nullptr ? *pl : Tensor());
   if (!wants_grad({a, b, c})) return py::cast(packed_forward(*a, *b, *c, *o, *ko, kl != nullptr ? *kl : Tensor(), p, false)[0]);
   return py::cast(PackedAttention::apply(*a, *b, *c, *o, *ko, kl != nullptr ? std::optional<Tensor>(*kl) : std::nullopt, p));
 }

@@ -26,6 +26,12 @@ ERR_UNSUPPORTED = -2
 ERR_LAUNCH = -3
 ERR_DEVICE = -4
 
+class ScoreShape(ctypes.Structure):
+    """msda_score_shape."""
+
+    _fields_ = [("cap", ctypes.c_float), ("window", ctypes.c_int), ("slopes", ctypes.c_void_p), ("prefix_lengths", ctypes.c_void_p)]
+
+
 #: Every function include/msda.h declares, with its ctypes signature.
 _I = ctypes.c_int
 _P = ctypes.c_void_p
@@ -61,6 +67,10 @@ SIGNATURES = {
     "msda_packed_attention_fwd": ([_P, _P, _P, _I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
     "msda_packed_attention_bwd": ([_P] * 7 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
     "msda_packed_attention_bwd_const": ([_P] * 8 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _I64, _P], _I),
+    "msda_packed_attention_shaped_fwd_workspace_size": ([_I] * 8, _I64),
+    "msda_packed_attention_shaped_bwd_workspace_size": ([_I] * 8, _I64),
+    "msda_packed_attention_shaped_fwd": ([_P, _P, _P, _I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _P, _I64, _P], _I),
+    "msda_packed_attention_shaped_bwd": ([_P] * 8 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _P, _I64, _P], _I),
     "msda_rotary": ([_P] * 4 + [_I, _P] + [_I] * 5 + [_P] * 3 + [_I, ctypes.c_double] + [_I] * 3 + [_P], _I),
     # include/msda_probe.h
     "msda_probe_lds_read": ([_P, _I, _I, _P], _I),

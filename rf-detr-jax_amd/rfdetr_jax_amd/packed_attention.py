@@ -4,12 +4,14 @@
   behind one another, ``H`` a multiple of ``Hk`` (each key head serves ``H / Hk`` query heads), causal or
   not, differentiable in q, k and v. With ``key_lengths`` the keys are a cache with room for more rows than
   it holds, and the queries its newest tokens (one each, or a chunk of a prompt).
+  Scores may be capped by a tanh, fall with the distance of query and key, and end at a window; a prefix of a causal
+  sequence may be seen by all its queries.
 * :func:`packed_attention_forward` / :func:`packed_attention_backward` — the two directions without
   autograd.
 
 The lengths stay on the GPU: nothing is read back, so a call can be captured into a graph and replayed
-with other lengths. Both directions run in HIP kernels (``msda_packed_attention_fwd`` / ``_bwd_const``). There is
-no CPU path. No counterpart in the reference.
+with other lengths. Both directions run in HIP kernels (``msda_packed_attention_fwd`` / ``_bwd_const``, shaped scores
+in ``msda_packed_attention_shaped_fwd`` / ``_bwd``). There is no CPU path. No counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -97,6 +99,37 @@ def _scale(scale, head_dim):
     return scale
 
 
+class _Shape:
+    """What the scores of one call are besides ``scale q.k``."""
+
+    def __init__(self, cap, slopes, window, prefix_lengths, causal, heads, sequences, device):
+        self.cap = 0.0 if cap is None else float(cap)
+        if cap is not None and not 2.0 ** -32 <= self.cap <= 2.0 ** 32:
+            raise ValueError(f"cap must lie from 2^-32 to 2^32, got {cap}")
+        if window is not None and (int(window) != window or not 1 <= window < 1 << 31):
+            raise ValueError(f"window must be a positive whole number, got {window}")
+        self.window = 0 if window is None else int(window)
+        if slopes is not None:
+            if slopes.dtype != torch.float32:
+                raise TypeError(f"slopes must be float32, got {slopes.dtype}")
+            if tuple(slopes.shape) != (heads,):
+                raise ValueError(f"slopes must be [{heads}], got {tuple(slopes.shape)}")
+            if slopes.device != device:
+                raise ValueError(f"slopes are on {slopes.device}, the queries on {device}")
+            if slopes.requires_grad and torch.is_grad_enabled():
+                raise ValueError("slopes get no gradient: pass them detached")
+            slopes = slopes.detach().contiguous()
+        self.slopes = slopes
+        if prefix_lengths is not None:
+            if not causal:
+                raise ValueError("prefix_lengths belong to causal attention: without causal every query sees every key")
+            prefix_lengths = _int32(prefix_lengths, (sequences,), "prefix_lengths", device)
+        self.prefix = prefix_lengths
+
+    def pointer(self):
+        return ctypes.byref(_native.ScoreShape(self.cap, self.window, _ptr(self.slopes), _ptr(self.prefix)))
+
+
 def _strides(tensors):
     flat = []
     for t in tensors:
@@ -104,7 +137,7 @@ def _strides(tensors):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _forward(q, k, v, seq, causal, scale, backward):
+def _forward(q, k, v, seq, causal, scale, shape, backward):
     """``(out, rest, stats)``; with ``backward`` what it needs: what out's rounding left (bfloat16) and statistics."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     rest = torch.empty_like(out) if backward and q.dtype == torch.bfloat16 else None
@@ -112,45 +145,47 @@ def _forward(q, k, v, seq, causal, scale, backward):
     lib, code = _native.lib(), _DTYPES[q.dtype]
     dims = (seq.count, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
     with torch.cuda.device(q.device):
-        nbytes = lib.msda_packed_attention_fwd_workspace_size(code, *dims)
+        nbytes = lib.msda_packed_attention_shaped_fwd_workspace_size(code, *dims, shape.window)
         _native.check(min(nbytes, 0))
         ws = _native.workspace(nbytes, q.device) if nbytes else None
-        rc = lib.msda_packed_attention_fwd(_ptr(q), _ptr(k), _ptr(v), code, _ptr(out), _ptr(rest), _ptr(stats), _ptr(seq.q), _ptr(seq.k),
-                                           _ptr(seq.lengths), *dims, _strides((q, k, v, out)), int(causal), scale, _ptr(ws), nbytes,
-                                           _stream(q.device))
+        rc = lib.msda_packed_attention_shaped_fwd(_ptr(q), _ptr(k), _ptr(v), code, _ptr(out), _ptr(rest), _ptr(stats), _ptr(seq.q), _ptr(seq.k),
+                                                  _ptr(seq.lengths), *dims, _strides((q, k, v, out)), int(causal), scale, shape.pointer(),
+                                                  _ptr(ws), nbytes, _stream(q.device))
     _native.check(rc)
     return out, rest, stats
 
 
-def _backward(q, k, v, out, rest, stats, grad_out, seq, causal, scale, needs):
+def _backward(q, k, v, out, rest, stats, grad_out, seq, causal, scale, shape, needs):
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None for t, need in zip((q, k, v), needs)]
     lib, code = _native.lib(), _DTYPES[q.dtype]
     dims = (seq.count, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
     with torch.cuda.device(q.device):
-        nbytes = lib.msda_packed_attention_bwd_workspace_size(code, *dims) if needs[1] or needs[2] else 0
+        nbytes = lib.msda_packed_attention_shaped_bwd_workspace_size(code, *dims, shape.window) if needs[1] or needs[2] else 0
         _native.check(min(nbytes, 0))
         ws = _native.workspace(nbytes, q.device) if nbytes else None
         numbers = torch.empty_like(stats) if needs[1] or needs[2] else None  # what the kernels hand on: other calls may read stats
-        rc = lib.msda_packed_attention_bwd_const(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(stats), _ptr(numbers), _ptr(grad_out), code,
-                                                 *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), *dims,
-                                                 _strides((q, k, v, out, grad_out, *grads)), int(causal), scale, _ptr(ws), nbytes,
-                                                 _stream(q.device))
+        rc = lib.msda_packed_attention_shaped_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(stats), _ptr(numbers), _ptr(grad_out), code,
+                                                  *(_ptr(g) for g in grads), _ptr(seq.q), _ptr(seq.k), _ptr(seq.lengths), *dims,
+                                                  _strides((q, k, v, out, grad_out, *grads)), int(causal), scale, shape.pointer(), _ptr(ws),
+                                                  nbytes, _stream(q.device))
     _native.check(rc)
     return grads
 
 
-def packed_attention_forward(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None):
+def packed_attention_forward(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None, *, cap=None, slopes=None,
+                             window=None, prefix_lengths=None):
     """``(out, saved)`` of :func:`packed_attention`'s arguments, without autograd; ``saved`` is for
     :func:`packed_attention_backward`: the statistics ``[T, H, 4]``, and for bfloat16 what the rounding of ``out``
     left, ``[T, H, D]`` (else None)."""
     _check(q, k, v)
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
-    out, rest, stats = _forward(_rows16(q, 64), _rows16(k), _rows16(v), seq, causal, _scale(scale, q.shape[2]), True)
+    shape = _Shape(cap, slopes, window, prefix_lengths, causal, q.shape[1], seq.count, q.device)
+    out, rest, stats = _forward(_rows16(q, 64), _rows16(k), _rows16(v), seq, causal, _scale(scale, q.shape[2]), shape, True)
     return out, (stats, rest)
 
 
 def packed_attention_backward(q, k, v, out, saved, grad_out, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None,
-                              needs=(True, True, True)):
+                              needs=(True, True, True), *, cap=None, slopes=None, window=None, prefix_lengths=None):
     """``(grad_q, grad_k, grad_v)``, contiguous, for the cotangent ``grad_out`` of ``out``; ``out`` and
     ``saved`` as :func:`packed_attention_forward` gave them, which are only read. None where ``needs`` says so."""
     _check(q, k, v)
@@ -160,39 +195,43 @@ def packed_attention_backward(q, k, v, out, saved, grad_out, offsets, key_offset
     if any(t.device != q.device for t in (out, grad_out, stats, *(() if rest is None else (rest,)))):
         raise ValueError("out, its statistics and grad_out must be on the queries' device")
     seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
+    shape = _Shape(cap, slopes, window, prefix_lengths, causal, q.shape[1], seq.count, q.device)
     # hooks on saved tensors may hand back other types and layouts: as the kernels read them
     q, k, v, out, grad_out = (_rows16(t.to(q.dtype), 64) for t in (q, k, v, out, grad_out))
     if rest is not None:
         out, rest = out.contiguous(), rest.to(q.dtype).contiguous()  # of the same strides
     stats = stats.to(torch.float32).contiguous()
-    return tuple(_backward(q, k, v, out, rest, stats, grad_out, seq, causal, _scale(scale, q.shape[2]), needs))
+    return tuple(_backward(q, k, v, out, rest, stats, grad_out, seq, causal, _scale(scale, q.shape[2]), shape, needs))
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, offsets, key_offsets, key_lengths, causal, scale):
+    def forward(ctx, q, k, v, offsets, key_offsets, key_lengths, causal, scale, cap=None, slopes=None, window=None, prefix_lengths=None):
         _check(q, k, v)
         seq = _Sequences(q, k, offsets, key_offsets, key_lengths)
+        shape = _Shape(cap, slopes, window, prefix_lengths, causal, q.shape[1], seq.count, q.device)
         scale = _scale(scale, q.shape[2])
         needs = any(ctx.needs_input_grad[:3])
         q, k, v = _rows16(q, 64), _rows16(k), _rows16(v)
-        out, rest, stats = _forward(q, k, v, seq, causal, scale, needs)
+        out, rest, stats = _forward(q, k, v, seq, causal, scale, shape, needs)
         if needs:
-            ctx.save_for_backward(q, k, v, out, rest, stats, offsets, key_offsets, key_lengths)
-            ctx.causal, ctx.scale = causal, scale
+            ctx.save_for_backward(q, k, v, out, rest, stats, offsets, key_offsets, key_lengths, slopes, prefix_lengths)
+            ctx.causal, ctx.scale, ctx.cap, ctx.window = causal, scale, cap, window
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, rest, stats, offsets, key_offsets, key_lengths = ctx.saved_tensors
+        q, k, v, out, rest, stats, offsets, key_offsets, key_lengths, slopes, prefix_lengths = ctx.saved_tensors
         q, k, v = (t.to(grad_out.dtype) for t in (q, k, v))
         grads = packed_attention_backward(q, k, v, out, (stats, rest), grad_out, offsets, key_offsets, key_lengths, ctx.causal, ctx.scale,
-                                          ctx.needs_input_grad[:3])
-        return (*grads, None, None, None, None, None)
+                                          ctx.needs_input_grad[:3], cap=ctx.cap, slopes=None if slopes is None else slopes.float(), window=ctx.window,
+                                          prefix_lengths=prefix_lengths)
+        return (*grads, *[None] * 9)
 
 
-def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None):
+def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=True, scale=None, *, cap=None, slopes=None, window=None,
+                     prefix_lengths=None):
     """Softmax attention of packed sequences: ``[T, H, D]`` in ``q``'s type (float32 or bfloat16).
 
     Args:
@@ -207,6 +246,15 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
         causal: query ``t`` of ``n`` sees the keys ``j <= t + m - n`` of ``m``, so that the last query sees every
             key; False: every key of its sequence.
         scale: of the scores, from ``2 ** -64`` to ``2 ** 64``; ``D ** -0.5`` when None.
+        cap: a score ``s = scale q.k`` becomes ``cap tanh(s / cap)``; from ``2 ** -32`` to ``2 ** 32``.
+        slopes: float32 ``[H]`` on the same GPU: behind the cap, head ``h``'s scores fall by ``slopes[h]`` for each place
+            between query and key, ``|t + m - n - j|``. Finite; they get no gradient.
+        window: keys at this distance and farther are not seen, on either side (1: a query's own place alone). What lies
+            outside costs nothing.
+        prefix_lengths: int32 ``[N]``, with ``causal``: the first so many keys of a sequence are seen by all its queries,
+            the ones before them too (an image or a prompt before a text). A window bounds these, too.
+
+    Documents that must not see each other are sequences of their own.
 
     Sums, softmax and statistics are float32. Of bfloat16 inputs the softmax weights and their gradients are rounded to
     bfloat16 for the matrix products: results lie 1.2 to 1.5 times as far from the exact ones as these rounded;
@@ -225,7 +273,7 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
         TypeError: types other than the above.
         RuntimeError: tensors that are not on a GPU.
     """
-    out = _native.binding().packed_attention(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale)
+    out = _native.binding().packed_attention(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale, cap, slopes, window, prefix_lengths)
     if out is not None:
         return out
-    return _PackedAttention.apply(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale)
+    return _PackedAttention.apply(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale, cap, slopes, window, prefix_lengths)
