@@ -571,6 +571,30 @@ int msda_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtyp
                 const int64_t* strides, const int64_t* position_strides, const int32_t* sections, int axes,
                 double base, int shared_frequencies, int interleaved, int inverse, void* stream);
 
+/* ---- Norms of queries and keys with rotary positions ----------------------------------------
+ * Each head of each token, a row x of head_dim channels, becomes R [x r w] with r = 1 / sqrt(mean(x^2) + eps), w the
+ * head's weight ([head_dim], the same for all heads of q, of k; NULL: ones) and R the rotation of msda_rotary, whose
+ * arguments the others are. Queries and keys take one launch. No counterpart in the reference.
+ *   weight_type: enum msda_dtype of the weights and of their gradients, f32 or bf16.
+ *   strides: element strides (token, head), forward of q, q_out, k, k_out [4][2]; backward of q, grad_q_out, grad_q, k,
+ *   grad_k_out, grad_k [6][2]. An output may be its input.
+ * eps: 2^-126 to 2^126. Sums are f32, results rounded once.
+ * Backward, for the cotangents of q_out and k_out: grad_q, grad_k and the weights' gradients (each may be NULL), the last
+ * as sums over all tokens and heads in a fixed order, which take the workspace (NULL without them).
+ */
+int msda_norm_rotary_fwd(const void* q, void* q_out, const void* k, void* k_out, int dtype, const void* q_weight, const void* k_weight,
+                         int weight_type, const void* positions, int position_type, int tokens, int heads, int kv_heads, int head_dim,
+                         const int64_t* strides, const int64_t* position_strides, const int32_t* sections, int axes, double base,
+                         int shared_frequencies, int interleaved, double eps, void* stream);
+
+int64_t msda_norm_rotary_bwd_workspace_size(int tokens, int head_dim);
+
+int msda_norm_rotary_bwd(const void* q, const void* grad_q_out, void* grad_q, const void* k, const void* grad_k_out, void* grad_k, int dtype,
+                         const void* q_weight, const void* k_weight, void* grad_q_weight, void* grad_k_weight, int weight_type,
+                         const void* positions, int position_type, int tokens, int heads, int kv_heads, int head_dim,
+                         const int64_t* strides, const int64_t* position_strides, const int32_t* sections, int axes, double base,
+                         int shared_frequencies, int interleaved, double eps, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

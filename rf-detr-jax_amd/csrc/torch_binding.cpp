@@ -56,6 +56,9 @@ struct Library {
   decltype(&msda_packed_attention_shaped_fwd_workspace_size) packed_fwd_workspace_size;
   decltype(&msda_packed_attention_shaped_bwd_workspace_size) packed_bwd_workspace_size;
   decltype(&msda_rotary) rotary;
+  decltype(&msda_norm_rotary_fwd) norm_rotary_fwd;
+  decltype(&msda_norm_rotary_bwd) norm_rotary_bwd;
+  decltype(&msda_norm_rotary_bwd_workspace_size) norm_rotary_bwd_workspace_size;
 };
 
 Library lib;
@@ -84,6 +87,9 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_packed_attention_shaped_fwd_workspace_size", lib.packed_fwd_workspace_size);
   get("msda_packed_attention_shaped_bwd_workspace_size", lib.packed_bwd_workspace_size);
   get("msda_rotary", lib.rotary);
+  get("msda_norm_rotary_fwd", lib.norm_rotary_fwd);
+  get("msda_norm_rotary_bwd", lib.norm_rotary_bwd);
+  get("msda_norm_rotary_bwd_workspace_size", lib.norm_rotary_bwd_workspace_size);
   check_status = py::object(check).release().ptr();
   parameter_type = reinterpret_cast<PyTypeObject*>(py::object(parameter).release().ptr());
 }
@@ -767,42 +773,196 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 };
 
-// q [T, H, D], k [T, Hk, D] or None, positions [T, A]; sections: a tuple of Python ints
-py::object rotary(const py::handle& q, const py::handle& k, const py::handle& positions, const py::handle& sections, const py::handle& base, bool shared,
-                  bool interleaved) {
-  const Tensor *a, *b = nullptr, *p;
-  if (!ordinary_state() || (a = plain(q)) == nullptr || (!k.is_none() && (b = plain(k)) == nullptr) || (p = plain(positions)) == nullptr ||
-      !PyTuple_CheckExact(sections.ptr()) || !PyFloat_CheckExact(base.ptr()))
-    return py::none();
+// The plan and the checks of an ordinary call: q [T, H, D], k [T, Hk, D] or null, positions [T, A]; sections: a tuple of
+// Python ints.
+std::optional<RotaryPlan> rotary_plan(const Tensor* a, const Tensor* b, const Tensor* p, const py::handle& sections, const py::handle& base, bool shared,
+                                      bool interleaved) {
+  if (!PyTuple_CheckExact(sections.ptr()) || !PyFloat_CheckExact(base.ptr())) return std::nullopt;
   RotaryPlan plan{{}, PyFloat_AS_DOUBLE(base.ptr()), shared, interleaved};
   int64_t pairs = 0;
   for (const py::handle& n : py::reinterpret_borrow<py::tuple>(sections)) {
-    if (!PyLong_CheckExact(n.ptr())) return py::none();
+    if (!PyLong_CheckExact(n.ptr())) return std::nullopt;
     const int64_t x = PyLong_AsLongLong(n.ptr());
     if (x < 1 || x > 128) {
       PyErr_Clear();
-      return py::none();
+      return std::nullopt;
     }
     plan.sections.push_back(x);
     pairs += x;
   }
-  if (plan.sections.empty() || plan.sections.size() > 8 || !(plan.base > 0.0) || !std::isfinite(plan.base)) return py::none();
-  if (a->dim() != 3 || !value_type(*a) || a->stride(2) != 1 || a->size(2) % 2 != 0 || a->size(2) > 256 || 2 * pairs > a->size(2)) return py::none();
+  if (plan.sections.empty() || plan.sections.size() > 8 || !(plan.base > 0.0) || !std::isfinite(plan.base)) return std::nullopt;
+  if (a->dim() != 3 || !value_type(*a) || a->stride(2) != 1 || a->size(2) % 2 != 0 || a->size(2) > 256 || 2 * pairs > a->size(2)) return std::nullopt;
   if (b != nullptr && (b->dim() != 3 || b->scalar_type() != a->scalar_type() || b->device() != a->device() || b->stride(2) != 1 ||
                        b->size(0) != a->size(0) || b->size(2) != a->size(2)))
-    return py::none();
+    return std::nullopt;
   for (const Tensor* t : {a, b})
-    if (t != nullptr && (t->size(0) >= (int64_t{1} << 31) || t->size(1) > (1 << 15))) return py::none();
+    if (t != nullptr && (t->size(0) >= (int64_t{1} << 31) || t->size(1) > (1 << 15))) return std::nullopt;
   const auto type = p->scalar_type();
   if (p->dim() != 2 || p->size(0) != a->size(0) || p->size(1) != static_cast<int64_t>(plan.sections.size()) || p->device() != a->device() ||
       (type != at::kInt && type != at::kLong && type != at::kFloat))
-    return py::none();
+    return std::nullopt;
+  return plan;
+}
+
+// q [T, H, D], k [T, Hk, D] or None, positions [T, A]
+py::object rotary(const py::handle& q, const py::handle& k, const py::handle& positions, const py::handle& sections, const py::handle& base, bool shared,
+                  bool interleaved) {
+  const Tensor *a, *b = nullptr, *p;
+  if (!ordinary_state() || (a = plain(q)) == nullptr || (!k.is_none() && (b = plain(k)) == nullptr) || (p = plain(positions)) == nullptr) return py::none();
+  const auto found = rotary_plan(a, b, p, sections, base, shared, interleaved);
+  if (!found) return py::none();
+  const RotaryPlan& plan = *found;
   if (!wants_grad({a, b})) {
     const auto out = rotated(*a, b != nullptr ? *b : Tensor(), *p, plan, false);
     if (b == nullptr) return py::cast(out[0]);
     return py::make_tuple(out[0], out[1]);
   }
   const auto out = Rotary::apply(*a, b != nullptr ? std::optional<Tensor>(*b) : std::nullopt, *p, plan);
+  if (b == nullptr) return py::cast(out[0]);
+  return py::make_tuple(out[0], out[1]);
+}
+
+// ---- norms of queries and keys with rotary positions ------------------------------------------
+
+struct NormPlan {
+  RotaryPlan rotary;
+  double eps;
+};
+
+// What both directions pass behind the tensors; strides of `n` tensors, tokens from `like`.
+struct NormCall {
+  int64_t st[12] = {}, ps[2];
+  int32_t sections[8];
+  int position_type, tokens, heads, kv_heads, dim, axes;
+  NormCall(std::initializer_list<const Tensor*> tensors, const Tensor& q, const Tensor& k, const Tensor& positions, const NormPlan& plan) {
+    int i = 0;
+    for (const Tensor* t : tensors) {
+      if (t->defined()) {
+        st[i] = t->stride(0);
+        st[i + 1] = t->stride(1);
+      }
+      i += 2;
+    }
+    ps[0] = positions.stride(0);
+    ps[1] = positions.stride(1);
+    axes = static_cast<int>(plan.rotary.sections.size());
+    for (int j = 0; j < axes; ++j) sections[j] = static_cast<int32_t>(plan.rotary.sections[j]);
+    position_type = positions.scalar_type() == at::kInt ? MSDA_POSITION_I32 : positions.scalar_type() == at::kLong ? MSDA_POSITION_I64 : MSDA_POSITION_F32;
+    const Tensor& like = q.defined() ? q : k;
+    tokens = static_cast<int>(like.size(0));
+    heads = q.defined() ? static_cast<int>(q.size(1)) : 0;
+    kv_heads = k.defined() ? static_cast<int>(k.size(1)) : 0;
+    dim = static_cast<int>(like.size(2));
+  }
+};
+
+int weight_type(const Tensor& a, const Tensor& b) {
+  return a.defined() ? code(a) : b.defined() ? code(b) : MSDA_DTYPE_F32;
+}
+
+std::array<Tensor, 2> normed(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& positions, const NormPlan& plan) {
+  std::array<Tensor, 2> out = {at::empty(q.sizes(), q.options()), k.defined() ? at::empty(k.sizes(), k.options()) : Tensor()};
+  const NormCall c({&q, &out[0], &k, &out[1]}, q, k, positions, plan);
+  launch(q, [&](void* stream) {
+    return lib.norm_rotary_fwd(ptr(q), ptr(out[0]), ptr(k), ptr(out[1]), code(q), ptr(qw), ptr(kw), weight_type(qw, kw), ptr(positions), c.position_type,
+                               c.tokens, c.heads, c.kv_heads, c.dim, c.st, c.ps, c.sections, c.axes, plan.rotary.base, plan.rotary.shared,
+                               plan.rotary.interleaved, plan.eps, stream);
+  });
+  return out;
+}
+
+struct NormRotary : torch::autograd::Function<NormRotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const std::optional<Tensor>& qw,
+                               const std::optional<Tensor>& kw, const Tensor& positions, const NormPlan& plan) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k.value_or(Tensor()), qw.value_or(Tensor()), kw.value_or(Tensor()), positions});
+    ctx->saved_data["sections"] = plan.rotary.sections;
+    ctx->saved_data["base"] = plan.rotary.base;
+    ctx->saved_data["shared"] = plan.rotary.shared;
+    ctx->saved_data["interleaved"] = plan.rotary.interleaved;
+    ctx->saved_data["eps"] = plan.eps;
+    ctx->saved_data["position_type"] = static_cast<int64_t>(positions.scalar_type());
+    ctx->saved_data["type"] = static_cast<int64_t>(q.scalar_type());
+    ctx->saved_data["weight_type"] = static_cast<int64_t>(qw ? qw->scalar_type() : kw ? kw->scalar_type() : at::kFloat);
+    const auto out = normed(q, k.value_or(Tensor()), qw.value_or(Tensor()), kw.value_or(Tensor()), positions, plan);
+    if (!k) return {out[0]};
+    return {out[0], out[1]};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const NormPlan plan{{ctx->saved_data["sections"].toIntVector(), ctx->saved_data["base"].toDouble(), ctx->saved_data["shared"].toBool(),
+                         ctx->saved_data["interleaved"].toBool()},
+                        ctx->saved_data["eps"].toDouble()};
+    const auto saved = ctx->get_saved_variables();
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), wtype = static_cast<at::ScalarType>(ctx->saved_data["weight_type"].toInt());
+    const Tensor positions = restored(saved[4], static_cast<at::ScalarType>(ctx->saved_data["position_type"].toInt()));
+    variable_list out(6);
+    Tensor x[2], g[2], w[2], gx[2], gw[2];
+    const Tensor* like = nullptr;
+    const auto rows = [](const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); };
+    for (int i = 0; i < 2; ++i) {
+      if (static_cast<size_t>(i) >= grads.size() || !grads[i].defined() || !saved[i].defined()) continue;  // no gradient of its own, nor its weight's
+      x[i] = saved[i].is_cuda() && saved[i].scalar_type() == type && saved[i].dim() == 3 ? rows(saved[i]) : restored(saved[i], type);
+      g[i] = rows(grads[i].to(type));
+      if (saved[2 + i].defined()) w[i] = restored(saved[2 + i], wtype);
+      saved_as(x[i].dim() == 3 && x[i].sizes() == g[i].sizes() && (!w[i].defined() || w[i].sizes().equals({x[i].size(2)})) && x[i].device() == g[i].device() &&
+               (!w[i].defined() || w[i].device() == x[i].device()) && positions.device() == x[i].device());
+      if (like == nullptr) like = &x[i];
+    }
+    if (like == nullptr) return out;
+    // needs_input_grad counts the tensors that were given
+    int edge = 0;
+    const bool given[4] = {true, saved[1].defined(), saved[2].defined(), saved[3].defined()};
+    bool needs[4];
+    for (int i = 0; i < 4; ++i) needs[i] = given[i] && ctx->needs_input_grad(edge++);
+    for (int i = 0; i < 2; ++i) {
+      gx[i] = x[i].defined() && needs[i] ? at::empty(x[i].sizes(), x[i].options()) : Tensor();
+      if (w[i].defined() && needs[2 + i]) gw[i] = at::empty(w[i].sizes(), w[i].options());
+    }
+    saved_as(positions.dim() == 2 && positions.size(0) == like->size(0) && positions.size(1) == static_cast<int64_t>(plan.rotary.sections.size()));
+    const NormCall c({&x[0], &g[0], &gx[0], &x[1], &g[1], &gx[1]}, x[0], x[1], positions, plan);
+    Tensor ws;
+    int64_t bytes = 0;
+    if (gw[0].defined() || gw[1].defined()) {
+      bytes = lib.norm_rotary_bwd_workspace_size(c.tokens, c.dim);
+      check(bytes);
+      ws = workspace(bytes, *like);
+    }
+    launch(*like, [&](void* stream) {
+      return lib.norm_rotary_bwd(ptr(x[0]), ptr(g[0]), ptr(gx[0]), ptr(x[1]), ptr(g[1]), ptr(gx[1]), code(*like), ptr(w[0]), ptr(w[1]), ptr(gw[0]), ptr(gw[1]),
+                                 weight_type(w[0], w[1]), ptr(positions), c.position_type, c.tokens, c.heads, c.kv_heads, c.dim, c.st, c.ps, c.sections, c.axes,
+                                 plan.rotary.base, plan.rotary.shared, plan.rotary.interleaved, plan.eps, ptr(ws), bytes, stream);
+    });
+    for (int i = 0; i < 2; ++i) {
+      out[i] = gx[i];
+      out[2 + i] = gw[i];
+    }
+    return once(out, "norm_rotary_embed");
+  }
+};
+
+// q [T, H, D], k [T, Hk, D] or None, weights [D] or None, positions [T, A]
+py::object norm_rotary(const py::handle& q, const py::handle& k, const py::handle& q_weight, const py::handle& k_weight, const py::handle& positions,
+                       const py::handle& sections, const py::handle& base, bool shared, bool interleaved, const py::handle& eps) {
+  const Tensor *a, *b = nullptr, *p, *w[2] = {};
+  if (!ordinary_state() || (a = plain(q)) == nullptr || (!k.is_none() && (b = plain(k)) == nullptr) || (p = plain(positions)) == nullptr ||
+      (!q_weight.is_none() && (w[0] = plain(q_weight)) == nullptr) || (!k_weight.is_none() && (b == nullptr || (w[1] = plain(k_weight)) == nullptr)) ||
+      !PyFloat_CheckExact(eps.ptr()))
+    return py::none();
+  const auto found = rotary_plan(a, b, p, sections, base, shared, interleaved);
+  if (!found) return py::none();
+  const NormPlan plan{*found, PyFloat_AS_DOUBLE(eps.ptr())};
+  if (!(plan.eps >= 0x1p-126 && plan.eps <= 0x1p126)) return py::none();
+  for (const Tensor* t : w)
+    if (t != nullptr && (t->dim() != 1 || t->size(0) != a->size(2) || !value_type(*t) || t->device() != a->device() || !t->is_contiguous())) return py::none();
+  if (w[0] != nullptr && w[1] != nullptr && w[0]->scalar_type() != w[1]->scalar_type()) return py::none();
+  const auto maybe = [](const Tensor* t) { return t != nullptr ? std::optional<Tensor>(*t) : std::nullopt; };
+  if (!wants_grad({a, b, w[0], w[1]})) {
+    const auto out = normed(*a, maybe(b).value_or(Tensor()), maybe(w[0]).value_or(Tensor()), maybe(w[1]).value_or(Tensor()), *p, plan);
+    if (b == nullptr) return py::cast(out[0]);
+    return py::make_tuple(out[0], out[1]);
+  }
+  const auto out = NormRotary::apply(*a, maybe(b), maybe(w[0]), maybe(w[1]), *p, plan);
   if (b == nullptr) return py::cast(out[0]);
   return py::make_tuple(out[0], out[1]);
 }
@@ -827,4 +987,5 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("attention", &attention);
   m.def("packed_attention", &packed_attention);
   m.def("rotary", &rotary);
+  m.def("norm_rotary", &norm_rotary);
 }

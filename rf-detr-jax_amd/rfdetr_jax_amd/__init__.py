@@ -7,8 +7,8 @@ backed by hand-written HIP kernels through the C ABI in include/msda.h. Also the
 kernels, the segmentation head's point sampling (``bilinear_grid_sample``, ``point_sample``), and the
 decoder's grouped self-attention (``MultiheadAttention``, ``scaled_dot_product_attention``,
 layers.py:54-99, :491-548). Beside it, without a counterpart in the reference, attention over packed
-sequences of different lengths with grouped heads (``packed_attention``) and rotary positions on several
-axes (``rotary_embed``).
+sequences of different lengths with grouped heads (``packed_attention``), rotary positions on several axes
+(``rotary_embed``), and these with a norm of every head in the same pass (``norm_rotary_embed``).
 """
 
 from .attention import (
@@ -19,6 +19,7 @@ from .attention import (
     scaled_dot_product_attention,
 )
 from .grid_sample import bilinear_grid_sample, point_sample
+from .norm_rotary import norm_rotary_embed
 from .ops import (
     SAMPLERS,
     ms_deform_attn,
@@ -50,6 +51,7 @@ __all__ = [
     "ms_deform_attn_fused",
     "ms_deform_attn_fused_backward",
     "ms_deform_attn_fused_forward",
+    "norm_rotary_embed",
     "packed_attention",
     "packed_attention_backward",
     "packed_attention_forward",
