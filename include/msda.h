@@ -547,6 +547,46 @@ int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v
                                      float scale, const msda_score_shape* shape, void* workspace, int64_t workspace_bytes,
                                      void* stream);
 
+/* ---- A cache of keys and values in 4 bits ----------------------------------------------------
+ * For serving: rows of keys and values held in 4.25 bits a channel, the calls that write and read rows, and attention
+ * over them. No counterpart in the reference.
+ *   codes  (keys, values)                [kv_heads, rows, 16 B] bytes, B = ceil(head_dim / 32), 16-byte aligned
+ *   scales (key_scales, value_scales)    [kv_heads, rows, B] bytes
+ * 32 channels of a row are a block with one power of two 2^e, held as e + 127; a channel is 4 bits, the first of two in
+ * the lower half of their byte: a sign (8) and the code of {0, 1/2, 1, 3/2, 2, 3, 4, 6} times 2^e. Writing takes the least
+ * e with every magnitude within 7 2^e, from -120 to 125, and the nearest value for each channel, the even code between
+ * two. A block that holds an infinity or NaN reads as NaN (scale 255). Channels behind head_dim are zeros.
+ *
+ * Sequences as above: sequence i's keys are the rows from k_offsets[i] on, as many as k_lengths[i] says (NULL: all before
+ * k_offsets[i + 1]), and its tokens q_offsets[i] .. q_offsets[i + 1] - 1 are the newest of them: its last token is its
+ * last key. msda_cache4_write puts the tokens' keys and values there (k_lengths counts them already),
+ * msda_cache4_read gives the values that the rows there stand for, in dtype (exact in both). Tokens of no sequence, and
+ * those older than its keys, are not written, and read as zeros; other rows of the cache stay as they are. Sequences whose
+ * rows overlap write over each other in no order. k, v: [tokens, kv_heads, head_dim], strides [2][2] in elements (token,
+ * head), channels contiguous, rows on 16-byte boundaries.
+ *
+ * msda_cache4_attention: msda_packed_attention_shaped_fwd over the cache (shape NULL: plain scores), without statistics;
+ * strides of q and out [2][2]. Every value of the cache is a bf16 number exactly; with bf16 queries weights and out are
+ * rounded as there (two bf16 numbers a weight for sequences of few rows), f32 queries are f32 throughout. The workspace
+ * holds partial sums, as there; its size is 0 where nothing is split.
+ */
+int msda_cache4_write(const void* k, const void* v, int dtype, uint8_t* keys, uint8_t* key_scales, uint8_t* values,
+                      uint8_t* value_scales, const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
+                      int sequences, int tokens, int rows, int kv_heads, int head_dim, const int64_t* strides, void* stream);
+
+int msda_cache4_read(const uint8_t* keys, const uint8_t* key_scales, const uint8_t* values, const uint8_t* value_scales,
+                     void* k, void* v, int dtype, const int32_t* q_offsets, const int32_t* k_offsets, const int32_t* k_lengths,
+                     int sequences, int tokens, int rows, int kv_heads, int head_dim, const int64_t* strides, void* stream);
+
+int64_t msda_cache4_attention_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads,
+                                             int head_dim, int window);
+
+int msda_cache4_attention(const void* q, int dtype, void* out, const uint8_t* keys, const uint8_t* key_scales,
+                          const uint8_t* values, const uint8_t* value_scales, const int32_t* q_offsets,
+                          const int32_t* k_offsets, const int32_t* k_lengths, int sequences, int q_rows, int k_rows, int heads,
+                          int kv_heads, int head_dim, const int64_t* strides, int causal, float scale,
+                          const msda_score_shape* shape, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Rotary positions on several axes -------------------------------------------------------
  * Rotates channel pairs of queries and keys by angles that grow with the token's position on each of
  * `axes` axes (time, height, width, ...). No counterpart in the reference.

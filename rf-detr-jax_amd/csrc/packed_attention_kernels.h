@@ -32,6 +32,7 @@
 #include <utility>
 
 #include "attention_common.h"
+#include "cache4_common.h"
 #include "msda_kernels.h"  // bf16_t, wait_vmem
 #include "packed_attention_parts.h"
 
@@ -72,6 +73,9 @@ struct PackParams {
   const int32_t* prefix;  // [sequences], or null
   int window;             // keys at this distance and farther are not seen
   float inner, cap2, bend;  // scale / cap, cap log2(e), 2 log2(e) scale / cap
+  // a cache in 4 bits (cache4_kernels.h): k and v are its codes
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
 };
 
 // What a kernel of shaped scores does besides the ranges [lo, hi) of keys that a query sees; 0: the plain kernels,
@@ -612,6 +616,8 @@ struct PkStream {
       x = pk_buffer(bx + first * stride_x, rows * sx);
       y = pk_buffer(by + first * stride_y, rows * sy);
     }
+    static constexpr int kPieces = 2 * NV;
+    __device__ __forceinline__ void finish() const {}
     template <int I>
     __device__ __forceinline__ void piece() const {
       constexpr int v = I % NV;
@@ -623,6 +629,72 @@ struct PkStream {
       pk_for<2 * NV>([&](auto i) { piece<i>(); });
     }
   };
+};
+
+// The same of a cache in 4 bits: a thread takes a quarter of one row of keys and of values, DT / 4 channels, loads its codes
+// and scales before the products of a chunk and writes them behind these, as T, where the transfers of Pair would have
+// put them. A row is DT / 2 bytes of codes and DT / 32 of scales.
+template <typename T, int DT>
+struct PkCachePair {
+  using Tile = PkTile<T, DT>;
+  static constexpr int N = DT / 32, kPieces = 2;
+  static_assert(4 * kPkChunk == 64 * kPkWaves, "a quarter of a row to a thread");
+  unsigned char* to[2];
+  const uint8_t* codes[2];
+  const uint8_t* scales[2];
+  int row, end;
+  uint32_t c[2][N], s[2][DT == 96 ? 2 : 1];
+  __device__ __forceinline__ PkCachePair(unsigned char* x, unsigned char* y, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
+                                         int first, int rows)
+      : to{x, y}, codes{kc, vc}, scales{ks, vs}, row(first + static_cast<int>(threadIdx.x >> 2)), end(rows) {}
+  template <int I>
+  __device__ __forceinline__ void piece() {
+    const int64_t r = min(row, end - 1), part = threadIdx.x & 3;
+    if (end <= 0) return;  // no such tile
+    const uint8_t* from = codes[I] + r * (DT / 2) + part * (DT / 8);
+    if constexpr (N == 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(from);
+      c[I][0] = x.x, c[I][1] = x.y, c[I][2] = x.z, c[I][3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) c[I][e] = reinterpret_cast<const uint32_t*>(from)[e];
+    }
+    const uint8_t* b = scales[I] + r * N;
+    s[I][0] = b[part * (DT / 4) / 32];
+    if constexpr (DT == 96) s[I][1] = b[(24 * part + 16) / 32];  // 24 channels, of one block or two
+  }
+  __device__ __forceinline__ void all() {
+    piece<0>();
+    piece<1>();
+  }
+  __device__ __forceinline__ void finish() const {
+    if (end <= 0) return;
+    const int r = static_cast<int>(threadIdx.x >> 2), part = static_cast<int>(threadIdx.x & 3);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        uint32_t scale = s[i][0];
+        if constexpr (DT == 96) scale = e == 0 || (e == 1 && part != 1) ? s[i][0] : s[i][1];
+        const bool bad = scale == kC4Bad, none = row >= end;
+        uint4 y[2];
+        if constexpr (sizeof(T) == 2) {
+          y[0] = __builtin_bit_cast(uint4, c4_bf16(c[i][e], c4_scale(scale)));
+        } else {
+          float v[8];
+          c4_f32(c[i][e], c4_scale(scale), v);
+          y[0] = uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+          y[1] = uint4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        }
+        constexpr int pieces = sizeof(T) == 2 ? 1 : 2;
+#pragma unroll
+        for (int j = 0; j < pieces; ++j) {
+          if (bad) y[j] = uint4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN of either type
+          if (none) y[j] = uint4{0u, 0u, 0u, 0u};
+          *reinterpret_cast<uint4*>(to[i] + r * Tile::ROW + (((pieces * (part * N + e) + j) ^ Tile::swizzle(r)) << 4)) = y[j];
+        }
+      }
+  }
 };
 
 // A causal chunk that not every row of the workgroup sees whole: the weights of its unseen pairs are zeros, and
@@ -792,7 +864,8 @@ __device__ __forceinline__ void pk_mask(at_f16& s, int k0, int lo, int span, int
 // Forward. A workgroup takes 128 rows and walks over the keys that they see, 64 at a time, with a running
 // reference score m and sum l. m starts at the first chunk's maximum (whose weight, the largest of a short
 // row, is then 1 and rounds to itself) and moves when a chunk's exceeds it by 2^8.
-template <typename T, int DT, int MOD>
+// CACHE4: over a cache in 4 bits.
+template <typename T, int DT, int MOD, bool CACHE4 = false>
 __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 : DT <= 64 ? 3 : 2) : 1) pk_fwd_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
@@ -833,20 +906,24 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, min(ri, w.rows - 1), grp);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
-  const T* kp = static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
-  const T* vp = static_cast<const T*>(p.v) + w.k_first * p.st[kPkV][0] + w.kv_head * p.st[kPkV][1];
+  const int64_t head_rows = static_cast<int64_t>(w.kv_head) * p.k_rows + w.k_first;  // of a cache in 4 bits
+  const T* kp = CACHE4 ? nullptr : static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
+  const T* vp = CACHE4 ? nullptr : static_cast<const T*>(p.v) + w.k_first * p.st[kPkV][0] + w.kv_head * p.st[kPkV][1];
   float m = 0.0f, l = 0.0f;  // l: of the lane's half of the keys
   bool fresh = true;         // no key seen yet
   at_f16 o[DT / 32];
 #pragma unroll
   for (int nd = 0; nd < DT / 32; ++nd) o[nd] = at_zero16();
 
-  using Pair = typename Stream::Pair;
   auto tile = [&](unsigned char* K, unsigned char* V, int c) {  // behind the last: zeros, which nothing reads
-    return Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < c1 ? w.m : 0, p.dim);
+    if constexpr (CACHE4)
+      return PkCachePair<T, DT>(K, V, static_cast<const uint8_t*>(p.k) + head_rows * (DT / 2), p.k_scales + head_rows * (DT / 32),
+                                static_cast<const uint8_t*>(p.v) + head_rows * (DT / 2), p.v_scales + head_rows * (DT / 32), c * kPkChunk, c < c1 ? w.m : 0);
+    else
+      return typename Stream::Pair(K, kp, p.st[kPkK][0], V, vp, p.st[kPkV][0], c * kPkChunk, c < c1 ? w.m : 0, p.dim);
   };
   bool sick = false;  // pk_settle found some
-  auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, const Pair& next) {
+  auto chunk = [&](unsigned char* Kb, unsigned char* Vb, int turn, int c, auto&& next) {
     PkLds K = (PkLds)(Kb), V = (PkLds)(Vb);
     const int k0 = c * kPkChunk;
     if (MOD != 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;  // settled chunks at both ends of the range, others between them
@@ -857,6 +934,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     }
     if (k0 >= wend || (MOD != 0 && k0 + kPkChunk <= wbegin)) {
       next.all();
+      next.finish();
       return;
     }
     at_f16 s0 = at_zero16(), s1 = at_zero16();
@@ -948,7 +1026,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           },
           [&](auto i) {
             constexpr int b = i / KS, t = i % KS;
-            if constexpr (i < 2 * Stream::NV) next.template piece<i>();
+            if constexpr (i < std::decay_t<decltype(next)>::kPieces) next.template piece<i>();
             if constexpr (b == 1) soft(s0, k0, PkInt<t>{});
             if constexpr (b == 2) soft(s1, k0 + 32, PkInt<t>{});
             if constexpr ((b == 1 || b == 2) && t == KS - 1) {
@@ -1011,8 +1089,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       }
       pk_accumulate2<T, DT, PF>(o, V, s0, o, V + 32 * Tile::ROW, s1, at);
     }
+    next.finish();
   };
-  if (c0 < c1) tile(X0, Y0, c0).all();
+  if (c0 < c1) {
+    auto head = tile(X0, Y0, c0);
+    head.all();
+    head.finish();
+  }
   for (int c = c0; c < c1; c += 2) {
     pk_barrier();  // tile c is there, and every wave is done with tile c - 1
     chunk(X0, Y0, 0, c, tile(X1, Y1, c + 1));
@@ -1044,7 +1127,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           const int ch = 32 * nd + 8 * (i >> 2) + 4 * grp + (i & 3);
           float x = 0.0f;
           if (ch < p.dim) {
-            if constexpr (sizeof(T) == 2) x = bf16_to_f32(vp[j * p.st[kPkV][0] + ch]);
+            if constexpr (CACHE4) x = p.v_scales[(head_rows + j) * (DT / 32) + nd] == kC4Bad ? NAN : 0.0f;
+            else if constexpr (sizeof(T) == 2) x = bf16_to_f32(vp[j * p.st[kPkV][0] + ch]);
             else x = vp[j * p.st[kPkV][0] + ch];
           }
           if (x - x != 0.0f) y[nd][i] += x;

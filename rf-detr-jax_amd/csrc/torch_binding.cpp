@@ -55,6 +55,10 @@ struct Library {
   decltype(&msda_packed_attention_shaped_bwd) packed_bwd;
   decltype(&msda_packed_attention_shaped_fwd_workspace_size) packed_fwd_workspace_size;
   decltype(&msda_packed_attention_shaped_bwd_workspace_size) packed_bwd_workspace_size;
+  decltype(&msda_cache4_write) cache4_write;
+  decltype(&msda_cache4_read) cache4_read;
+  decltype(&msda_cache4_attention) cache4_attention;
+  decltype(&msda_cache4_attention_workspace_size) cache4_attention_workspace_size;
   decltype(&msda_rotary) rotary;
   decltype(&msda_norm_rotary_fwd) norm_rotary_fwd;
   decltype(&msda_norm_rotary_bwd) norm_rotary_bwd;
@@ -86,6 +90,10 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_packed_attention_shaped_bwd", lib.packed_bwd);
   get("msda_packed_attention_shaped_fwd_workspace_size", lib.packed_fwd_workspace_size);
   get("msda_packed_attention_shaped_bwd_workspace_size", lib.packed_bwd_workspace_size);
+  get("msda_cache4_write", lib.cache4_write);
+  get("msda_cache4_read", lib.cache4_read);
+  get("msda_cache4_attention", lib.cache4_attention);
+  get("msda_cache4_attention_workspace_size", lib.cache4_attention_workspace_size);
   get("msda_rotary", lib.rotary);
   get("msda_norm_rotary_fwd", lib.norm_rotary_fwd);
   get("msda_norm_rotary_bwd", lib.norm_rotary_bwd);
@@ -672,7 +680,40 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
 };
 
-// q [T, H, D], k and v [S, Hk, D]; scale, cap: a Python float, or None; window: a Python int, or None
+// Offsets and lengths of an ordinary call.
+bool places(const Tensor& like, const Tensor* o, const Tensor* ko, const Tensor* kl) {
+  for (const Tensor* t : {o, ko, kl})
+    if (t != nullptr && (t->dim() != 1 || t->scalar_type() != at::kInt || t->device() != like.device() || !t->is_contiguous())) return false;
+  return ko->numel() == o->numel() && (kl == nullptr || kl->numel() == o->numel() - 1);
+}
+
+// What an ordinary call says of its scores; scale, cap: a Python float, or None; window: a Python int, or None
+struct Scores {
+  double scale, cap;
+  int64_t window;
+};
+std::optional<Scores> scores_of(const Tensor& q, const Tensor& offsets, bool causal, const py::handle& scale, const py::handle& cap, const Tensor* slopes,
+                                const py::handle& window, const Tensor* prefix) {
+  if (slopes != nullptr && (slopes->dim() != 1 || slopes->size(0) != q.size(1) || !f32(*slopes) || slopes->device() != q.device() ||
+                            !slopes->is_contiguous() || slopes->requires_grad()))
+    return std::nullopt;
+  if (prefix != nullptr && (!causal || prefix->dim() != 1 || prefix->numel() != offsets.numel() - 1 || prefix->scalar_type() != at::kInt ||
+                            prefix->device() != q.device() || !prefix->is_contiguous()))
+    return std::nullopt;
+  if ((!scale.is_none() && !PyFloat_CheckExact(scale.ptr())) || (!cap.is_none() && !PyFloat_CheckExact(cap.ptr())) ||
+      (!window.is_none() && !PyLong_CheckExact(window.ptr())))
+    return std::nullopt;
+  Scores s{scale.is_none() ? 1.0 / std::sqrt(static_cast<double>(q.size(2))) : PyFloat_AS_DOUBLE(scale.ptr()),
+           cap.is_none() ? 0.0 : PyFloat_AS_DOUBLE(cap.ptr()), window.is_none() ? 0 : PyLong_AsLongLong(window.ptr())};
+  if (!window.is_none() && (s.window < 1 || s.window >= (int64_t{1} << 31))) {
+    PyErr_Clear();
+    return std::nullopt;
+  }
+  if (!(s.scale >= 0x1p-64 && s.scale <= 0x1p64) || (!cap.is_none() && !(s.cap >= 0x1p-32 && s.cap <= 0x1p32))) return std::nullopt;
+  return s;
+}
+
+// q [T, H, D], k and v [S, Hk, D]
 py::object packed_attention(const py::handle& q, const py::handle& k, const py::handle& v, const py::handle& offsets, const py::handle& key_offsets,
                             const py::handle& key_lengths, bool causal, const py::handle& scale, const py::handle& cap, const py::handle& slopes,
                             const py::handle& window, const py::handle& prefix_lengths) {
@@ -690,26 +731,102 @@ py::object packed_attention(const py::handle& q, const py::handle& k, const py::
   if (b->sizes() != c->sizes() || b->size(2) != a->size(2) || a->size(1) == 0 || b->size(1) == 0 || a->size(1) % b->size(1) != 0 || a->size(1) > 64 * b->size(1) ||
       a->size(2) == 0 || a->size(2) % 8 != 0 || a->size(2) > 128)
     return py::none();
-  if (sl != nullptr && (sl->dim() != 1 || sl->size(0) != a->size(1) || !f32(*sl) || sl->device() != a->device() || !sl->is_contiguous() || sl->requires_grad()))
-    return py::none();
-  if (pl != nullptr && (!causal || pl->numel() != o->numel() - 1)) return py::none();
-  for (const Tensor* t : {o, ko, kl, pl})
-    if (t != nullptr && (t->dim() != 1 || t->scalar_type() != at::kInt || t->device() != a->device() || !t->is_contiguous())) return py::none();
-  if (ko->numel() != o->numel() || (kl != nullptr && kl->numel() != o->numel() - 1)) return py::none();
-  if (!scale.is_none() && !PyFloat_CheckExact(scale.ptr())) return py::none();
-  const double s = scale.is_none() ? 1.0 / std::sqrt(static_cast<double>(a->size(2))) : PyFloat_AS_DOUBLE(scale.ptr());
-  if (!(s >= 0x1p-64 && s <= 0x1p64)) return py::none();
-  if ((!cap.is_none() && !PyFloat_CheckExact(cap.ptr())) || (!window.is_none() && !PyLong_CheckExact(window.ptr()))) return py::none();
-  const double top = cap.is_none() ? 0.0 : PyFloat_AS_DOUBLE(cap.ptr());
-  if (!cap.is_none() && !(top >= 0x1p-32 && top <= 0x1p32)) return py::none();
-  const int64_t reach = window.is_none() ? 0 : PyLong_AsLongLong(window.ptr());
-  if (!window.is_none() && (reach < 1 || reach >= (int64_t{1} << 31))) {
-    PyErr_Clear();
-    return py::none();
-  }
-  const Packed p(*a, *b, *o, causal, s, top, reach, sl != nullptr ? *sl : Tensor(), pl != nullptr ? *pl : Tensor());
+  if (!places(*a, o, ko, kl)) return py::none();
+  const auto scores = scores_of(*a, *o, causal, scale, cap, sl, window, pl);
+  if (!scores) return py::none();
+  const Packed p(*a, *b, *o, causal, scores->scale, scores->cap, scores->window, sl != nullptr ? *sl : Tensor(), pl != nullptr ? *pl : Tensor());
   if (!wants_grad({a, b, c})) return py::cast(packed_forward(*a, *b, *c, *o, *ko, kl != nullptr ? *kl : Tensor(), p, false)[0]);
   return py::cast(PackedAttention::apply(*a, *b, *c, *o, *ko, kl != nullptr ? std::optional<Tensor>(*kl) : std::nullopt, p));
+}
+
+// ---- a cache in 4 bits ------------------------------------------------------------------------
+
+// The cache of an ordinary call: its four tensors, and the head dim.
+struct Cache {
+  const Tensor *keys, *key_scales, *values, *value_scales;
+  int64_t dim;
+  bool get(const py::handle& k, const py::handle& ks, const py::handle& v, const py::handle& vs, const py::handle& head_dim) {
+    if ((keys = plain(k)) == nullptr || (key_scales = plain(ks)) == nullptr || (values = plain(v)) == nullptr || (value_scales = plain(vs)) == nullptr ||
+        !PyLong_CheckExact(head_dim.ptr()))
+      return false;
+    dim = PyLong_AsLongLong(head_dim.ptr());
+    if (dim < 8 || dim > 128 || dim % 8 != 0) {
+      PyErr_Clear();
+      return false;
+    }
+    const int64_t blocks = (dim + 31) / 32;
+    for (const Tensor* t : {keys, key_scales, values, value_scales}) {
+      const bool codes = t == keys || t == values;
+      if (t->dim() != 3 || t->scalar_type() != at::kByte || t->size(0) != keys->size(0) || t->size(1) != keys->size(1) || t->size(1) >= (int64_t{1} << 31) ||
+          t->size(2) != (codes ? 16 * blocks : blocks) || !t->is_contiguous() || t->device() != keys->device() ||
+          (codes && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0))
+        return false;
+    }
+    return true;
+  }
+  static uint8_t* at(const Tensor* t) { return static_cast<uint8_t*>(t->data_ptr()); }
+};
+
+// k, v [T, Hk, D], written into the cache or read from it; True, or None for a call that is not an ordinary one
+py::object cache4_rows(const py::handle& keys, const py::handle& key_scales, const py::handle& values, const py::handle& value_scales,
+                       const py::handle& head_dim, const py::handle& k, const py::handle& v, const py::handle& offsets, const py::handle& key_offsets,
+                       const py::handle& key_lengths, bool write) {
+  Cache c;
+  const Tensor *a, *b, *o, *ko, *kl = nullptr;
+  if (!ordinary_state() || !c.get(keys, key_scales, values, value_scales, head_dim) || (a = plain(k)) == nullptr || (b = plain(v)) == nullptr ||
+      (o = plain(offsets)) == nullptr || (ko = key_offsets.is_none() ? o : plain(key_offsets)) == nullptr ||
+      (!key_lengths.is_none() && (kl = plain(key_lengths)) == nullptr))
+    return py::none();
+  for (const Tensor* t : {a, b})
+    if (!value_type(*t) || t->scalar_type() != a->scalar_type() || !packed_rows(*t) || t->sizes() != a->sizes() || t->size(1) != c.keys->size(0) ||
+        t->size(2) != c.dim || t->size(0) >= (int64_t{1} << 31) || t->device() != c.keys->device() || wants_grad({t}))
+      return py::none();
+  if (!places(*a, o, ko, kl)) return py::none();
+  const int64_t st[4] = {a->stride(0), a->stride(1), b->stride(0), b->stride(1)};
+  const int n = static_cast<int>(o->numel() - 1), tokens = static_cast<int>(a->size(0)), rows = static_cast<int>(c.keys->size(1));
+  const int heads = static_cast<int>(c.keys->size(0)), dim = static_cast<int>(c.dim);
+  launch(*a, [&](void* stream) {
+    if (write)
+      return lib.cache4_write(ptr(*a), ptr(*b), code(*a), Cache::at(c.keys), Cache::at(c.key_scales), Cache::at(c.values), Cache::at(c.value_scales), iptr(*o),
+                              iptr(*ko), kl != nullptr ? iptr(*kl) : nullptr, n, tokens, rows, heads, dim, st, stream);
+    return lib.cache4_read(Cache::at(c.keys), Cache::at(c.key_scales), Cache::at(c.values), Cache::at(c.value_scales), ptr(*a), ptr(*b), code(*a), iptr(*o),
+                           iptr(*ko), kl != nullptr ? iptr(*kl) : nullptr, n, tokens, rows, heads, dim, st, stream);
+  });
+  return py::bool_(true);
+}
+
+py::object cache4_attention(const py::handle& q, const py::handle& keys, const py::handle& key_scales, const py::handle& values,
+                            const py::handle& value_scales, const py::handle& head_dim, const py::handle& offsets, const py::handle& key_offsets,
+                            const py::handle& key_lengths, bool causal, const py::handle& scale, const py::handle& cap, const py::handle& slopes,
+                            const py::handle& window, const py::handle& prefix_lengths) {
+  Cache c;
+  const Tensor *a, *o, *ko, *kl = nullptr, *sl = nullptr, *pl = nullptr;
+  if (!ordinary_state() || !c.get(keys, key_scales, values, value_scales, head_dim) || (a = plain(q)) == nullptr || (o = plain(offsets)) == nullptr ||
+      (ko = key_offsets.is_none() ? o : plain(key_offsets)) == nullptr || (!key_lengths.is_none() && (kl = plain(key_lengths)) == nullptr) ||
+      (!slopes.is_none() && (sl = plain(slopes)) == nullptr) || (!prefix_lengths.is_none() && (pl = plain(prefix_lengths)) == nullptr))
+    return py::none();
+  const int64_t hk = c.keys->size(0);
+  if (!value_type(*a) || !packed_rows(*a, 64) || a->size(2) != c.dim || a->size(0) >= (int64_t{1} << 31) || a->size(1) >= (int64_t{1} << 31) ||
+      a->size(1) % hk != 0 || a->size(1) > 64 * hk || a->device() != c.keys->device() || wants_grad({a}) || !places(*a, o, ko, kl))
+    return py::none();
+  const auto s = scores_of(*a, *o, causal, scale, cap, sl, window, pl);
+  if (!s) return py::none();
+  const int n = static_cast<int>(o->numel() - 1), tokens = static_cast<int>(a->size(0)), rows = static_cast<int>(c.keys->size(1));
+  const int heads = static_cast<int>(a->size(1)), kv_heads = static_cast<int>(hk), dim = static_cast<int>(c.dim);
+  const msda_score_shape shape{static_cast<float>(s->cap), static_cast<int>(s->window), sl != nullptr ? static_cast<const float*>(ptr(*sl)) : nullptr,
+                               pl != nullptr ? iptr(*pl) : nullptr};
+  const Tensor out = at::empty(a->sizes(), a->options());
+  Tensor ws;
+  const int64_t bytes = lib.cache4_attention_workspace_size(code(*a), n, tokens, rows, heads, kv_heads, dim, shape.window);
+  check(bytes);
+  if (bytes != 0) ws = workspace(bytes, *a);
+  const int64_t st[4] = {a->stride(0), a->stride(1), out.stride(0), out.stride(1)};
+  launch(*a, [&](void* stream) {
+    return lib.cache4_attention(ptr(*a), code(*a), ptr(out), Cache::at(c.keys), Cache::at(c.key_scales), Cache::at(c.values), Cache::at(c.value_scales),
+                                iptr(*o), iptr(*ko), kl != nullptr ? iptr(*kl) : nullptr, n, tokens, rows, heads, kv_heads, dim, st, causal,
+                                static_cast<float>(s->scale), &shape, ptr(ws), bytes, stream);
+  });
+  return py::cast(out);
 }
 
 struct RotaryPlan {
@@ -986,6 +1103,8 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("grid_sample", &grid_sample);
   m.def("attention", &attention);
   m.def("packed_attention", &packed_attention);
+  m.def("cache4_rows", &cache4_rows);
+  m.def("cache4_attention", &cache4_attention);
   m.def("rotary", &rotary);
   m.def("norm_rotary", &norm_rotary);
 }

@@ -8,7 +8,8 @@ kernels, the segmentation head's point sampling (``bilinear_grid_sample``, ``poi
 decoder's grouped self-attention (``MultiheadAttention``, ``scaled_dot_product_attention``,
 layers.py:54-99, :491-548). Beside it, without a counterpart in the reference, attention over packed
 sequences of different lengths with grouped heads (``packed_attention``), rotary positions on several axes
-(``rotary_embed``), and these with a norm of every head in the same pass (``norm_rotary_embed``).
+(``rotary_embed``), these with a norm of every head in the same pass (``norm_rotary_embed``), and attention over a cache of
+keys and values in 4 bits (``cache4_attention`` and what writes the cache).
 """
 
 from .attention import (
@@ -18,6 +19,7 @@ from .attention import (
     grouped_attention,
     scaled_dot_product_attention,
 )
+from .cache4 import Cache4, cache4_attention, cache4_read, cache4_write, new_cache4
 from .grid_sample import bilinear_grid_sample, point_sample
 from .norm_rotary import norm_rotary_embed
 from .ops import (
@@ -36,10 +38,14 @@ from .rotary import rotary_embed
 from .value_proj import MSDeformAttn, value_proj_rows
 
 __all__ = [
+    "Cache4",
     "MSDeformAttn",
     "MultiheadAttention",
     "SAMPLERS",
     "bilinear_grid_sample",
+    "cache4_attention",
+    "cache4_read",
+    "cache4_write",
     "decoder_self_attention",
     "dropout_keep_mask",
     "grouped_attention",
@@ -51,6 +57,7 @@ __all__ = [
     "ms_deform_attn_fused",
     "ms_deform_attn_fused_backward",
     "ms_deform_attn_fused_forward",
+    "new_cache4",
     "norm_rotary_embed",
     "packed_attention",
     "packed_attention_backward",

@@ -71,6 +71,10 @@ SIGNATURES = {
     "msda_packed_attention_shaped_bwd_workspace_size": ([_I] * 8, _I64),
     "msda_packed_attention_shaped_fwd": ([_P, _P, _P, _I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _P, _I64, _P], _I),
     "msda_packed_attention_shaped_bwd": ([_P] * 8 + [_I] + [_P] * 6 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _P, _I64, _P], _I),
+    "msda_cache4_write": ([_P, _P, _I] + [_P] * 7 + [_I] * 5 + [_P, _P], _I),
+    "msda_cache4_read": ([_P] * 6 + [_I] + [_P] * 3 + [_I] * 5 + [_P, _P], _I),
+    "msda_cache4_attention_workspace_size": ([_I] * 8, _I64),
+    "msda_cache4_attention": ([_P, _I] + [_P] * 8 + [_I] * 6 + [_P, _I, ctypes.c_float, _P, _P, _I64, _P], _I),
     "msda_rotary": ([_P] * 4 + [_I, _P] + [_I] * 5 + [_P] * 3 + [_I, ctypes.c_double] + [_I] * 3 + [_P], _I),
     "msda_norm_rotary_fwd": ([_P] * 4 + [_I, _P, _P, _I, _P] + [_I] * 5 + [_P] * 3 + [_I, ctypes.c_double, _I, _I, ctypes.c_double, _P], _I),
     "msda_norm_rotary_bwd_workspace_size": ([_I, _I], _I64),
@@ -137,7 +141,7 @@ def lib(path: str | None = None) -> ctypes.CDLL:
 class _NoBinding:
     """Leaves every call to the Python autograd functions."""
 
-    core = fused = value_proj = grid_sample = attention = packed_attention = rotary = norm_rotary = staticmethod(lambda *args: None)
+    core = fused = value_proj = grid_sample = attention = packed_attention = rotary = norm_rotary = cache4_rows = cache4_attention = staticmethod(lambda *args: None)
 
 
 def binding():

@@ -29,10 +29,12 @@ SOURCES = [os.path.join(CSRC, f) for f in ("msda_abi.hip", "msda_fwd_f32.hip", "
                                            "packed_attention_fwd_bf16.hip", "packed_attention_bwd_f32.hip",
                                            "packed_attention_bwd_bf16.hip",
                                            *(f"packed_attention_shaped_{d}{c}_{t}.hip" for d in ("bwd", "fwd") for c in ("_cap", "") for t in ("bf16", "f32")),
+                                           "cache4_abi.hip", *(f"cache4_attention_{c}_{t}.hip" for c in ("cap", "shaped", "plain") for t in ("bf16", "f32")),
                                            "rotary_abi.hip", "norm_rotary_abi.hip", "probe_abi.hip")]
 HEADERS = [os.path.join(CSRC, f) for f in ("msda_kernels.h", "msda_band_kernels.h", "msda_gather_kernels.h", "msda_fused_bwd_kernels.h", "msda_launch.h", "grid_sample_kernels.h",
                                            "value_proj_kernels.h", "value_proj_mfma_kernels.h", "attention_common.h", "attention_kernels.h",
-                                           "attention_split_kernels.h", "packed_attention_kernels.h", "packed_attention_launch.h", "packed_attention_parts.h",
+                                           "attention_split_kernels.h", "packed_attention_kernels.h", "packed_attention_launch.h", "packed_attention_parts.h", "packed_attention_host.h",
+                                           "cache4_common.h", "cache4_kernels.h", "cache4_launch.h",
                                            "rotary_kernels.h", "norm_rotary_kernels.h")] + [
     os.path.join(INCLUDE, "msda.h"), os.path.join(INCLUDE, "msda_probe.h")]
 BUILD_DIR = os.path.join(ROOT, "_build")
