@@ -82,6 +82,7 @@ struct PackParams {
 // whose ranges begin at 0.
 enum PackShaped { kPkRanges = 4, kPkCap = 1, kPkSlope = 2 };
 
+constexpr float kPkShare = 0.5f;
 constexpr int kPkPart = 32;  // chunks of a workgroup on the key side, unless that makes more parts than the host gave room for
 constexpr int kPkJoin = 32;   // workgroups that join a key tile's parts
 
@@ -984,7 +985,9 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
         }
         if constexpr (t == HA) {
           bm = at_max_halves(bm);
-          const bool move = bm > kAtLazy || (fresh && bm != -INFINITY);
+          bool move = bm > kAtLazy || (fresh && bm != -INFINITY);
+          // a weight that is much of its row's sum becomes 1, which is rounded to itself
+          if constexpr (MOD != 0) move = move || (bm > 0.0f && at_exp2(bm) > kPkShare * at_sum_halves(l));
           if (__any(move)) {
             const float d = move ? bm : 0.0f, a = fresh ? 0.0f : at_exp2(-d);
             alpha *= a;
