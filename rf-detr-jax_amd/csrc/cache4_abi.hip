@@ -16,8 +16,8 @@ using msda_host::aligned_to;
 using msda_host::fail;
 
 // Few rows to a sequence on average: the kernel that takes 16 rows at a time and gives every wave keys of its own. More:
-// tiles of 128 rows. A sequence of more rows than 16 reads its keys once for each 16 there. One sequence of 16,000 keys,
-// 4 key heads of 128 channels, us a call, rows of 16 and tiles: @@FEW@@
+// tiles of 128 rows. A sequence of more rows than 16 reads its keys once for each 16 there.
+//
 bool c4_few(const PackShape& s) { return static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads) <= static_cast<int64_t>(16) * s.sequences; }
 
 // The parts of a sequence's keys in the kernel of few rows: chunks of one, and how many at most.

@@ -48,6 +48,9 @@ int pk_parts(const PackShape& s, int window) {
   constexpr int64_t kWant = 2048, kMost = 8;
   if (s.sequences == 0 || s.k_rows == 0) return 1;
   const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
+  // Inside a window all tiles have about the same work: parts only where the tiles do not fill the CUs' two places
+  // (12,093 tokens, 16 heads to 8 of 128 channels, a window of 1,024, 756 tiles: the join of two parts alone took 44 us).
+  if (window < s.k_rows / s.sequences && tiles >= 512) return 1;
   // The rows of one sequence, if it is 4 times the average: a longer one takes longer parts, and batches of short
   // sequences start no second kernel (4 us).
   // No more than a window's see a tile.

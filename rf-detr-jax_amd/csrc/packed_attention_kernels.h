@@ -253,6 +253,18 @@ __device__ __forceinline__ bool pk_far(const PackParams& p, const at_f16& s) {
   return __any(most * p.inner >= kPkNear<T>);
 }
 
+// A block of scores through the tanh, in place: the near side of it where all lie there.
+template <typename T>
+__device__ __forceinline__ void pk_bend(const PackParams& p, at_f16& s) {
+  if (pk_far<T>(p, s)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = pk_bent<T>(p, s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = pk_near<T>(s[i] * p.inner);
+  }
+}
+
 // One row's bias: of the key that lies `ahead` of the lane's first key of a block.
 struct PkBias {
   float slope;  // -slope log2(e)
@@ -390,11 +402,11 @@ __device__ __forceinline__ void pk_pipe(Read&& read, Use&& use, Beside&& beside)
 }
 
 // Vector work beside the KS products of a phase: a product's result is there one product later, so step t
-// takes part t - 1 of KS - 1 of the 16 registers.
-template <int KS, int T, typename F>
+// takes part t - 1 of KS - 1 of the 16 registers (or of N things).
+template <int KS, int T, int N = 16, typename F>
 __device__ __forceinline__ void pk_beside(F&& f) {
   if constexpr (T >= 1) {
-    constexpr int lo = 16 * (T - 1) / (KS - 1), hi = 16 * T / (KS - 1);
+    constexpr int lo = N * (T - 1) / (KS - 1), hi = N * T / (KS - 1);
     pk_for<hi - lo>([&](auto i) { f(lo + i); });
   }
 }
@@ -512,6 +524,8 @@ __device__ __forceinline__ void pk_accumulate2(at_f16 (&ax)[DT / 32], PkLds X, c
 
 typedef __bf16 pk_bf16 __attribute__((ext_vector_type(16)));
 typedef __bf16 pk_bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pk_bf2 __attribute__((ext_vector_type(2)));
+typedef float pk_f2 __attribute__((ext_vector_type(2)));
 
 // What the rounding to bf16 leaves.
 __device__ __forceinline__ at_f16 pk_rest(const at_f16& x) { return x - __builtin_convertvector(__builtin_convertvector(x, pk_bf16), at_f16); }
@@ -1230,14 +1244,14 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
 
 // dq, and the rows' numbers for the key side (alone when gq is null).
 template <typename T, int DT, int MOD>
-__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_q_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && MOD == 0 ? 3 : 2) : 1) pk_bwd_q_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
   __shared__ __align__(16) unsigned char X0[Tile::BYTES], Y0[Tile::BYTES], X1[Tile::BYTES], Y1[Tile::BYTES];
   __shared__ uint32_t bad[2][2];  // pk_settle's rows of a chunk, by turns
   if (threadIdx.x < 4) bad[threadIdx.x >> 1][threadIdx.x & 1] = 0;
-  constexpr int PF = sizeof(T) == 2 ? 3 : 2;
+  constexpr int PF = sizeof(T) == 2 && !(MOD != 0 && DT == 128) ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
   const PkQueries<MOD> w(p, lane, std::false_type());
@@ -1290,6 +1304,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   if (gq == nullptr) return;
   constexpr bool bf = sizeof(T) == 2;
   if (bf) m += ll;  // rounded at its own size, 2^-24 of it
+  // With ranges 14 registers were spilled at 128 channels, pieces of the cotangent among them, whose reloads waited for the
+  // tile in flight: the last KEEP pieces wait in LDS (as on the key side).
+  constexpr int KEEP = bf && DT == 128 && MOD != 0 ? 3 : 0;
+  __shared__ __align__(16) unsigned char kept_rows[KEEP > 0 ? KEEP * kPkWaves * 1024 : 16];
+  if constexpr (KEEP > 0)  // of this lane, so no barrier
+    for (int j = 0; j < KEEP; ++j) *reinterpret_cast<at_bf8*>(kept_rows + threadIdx.x * 16 + j * kPkWaves * 1024) = go.x[DT / 16 - KEEP + j];
   const T* kp = static_cast<const T*>(p.k) + w.k_first * p.st[kPkK][0] + w.kv_head * p.st[kPkK][1];
   const T* vp = static_cast<const T*>(p.v) + w.k_first * p.st[kPkV][0] + w.kv_head * p.st[kPkV][1];
   at_f16 dq[DT / 32];
@@ -1325,6 +1345,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       typename P::Weights wa, wb;
       PkLane<T, DT> now = at;  // as in pk_bwd_kv_kernel
       asm volatile("" : "+v"(now.row), "+v"(now.tr));
+      uint32_t kept = 0;
+      if constexpr (KEEP > 0) {
+        kept = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((MSDA_LDS unsigned char*)(kept_rows))) + threadIdx.x * 16;
+        asm volatile("" : "+v"(kept));
+      }
+      at_bf8 last[KEEP > 0 ? KEEP : 1];
       bool far = false;
       // MOD: weights, times the slope of the cap
       auto weigh = [&](at_f16& s, int k, auto t) {
@@ -1368,9 +1394,11 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
           [&](auto i, const auto& a) {
             constexpr int b = i / KS, t = i % KS;
             if constexpr (b == 0) P::score(sa, a, q, t);
-            if constexpr (b == 1) P::score(da, a, go, t);
+            if constexpr (b == 1 && t < KS - KEEP) P::score(da, a, go, t);
+            if constexpr (b == 1 && t >= KS - KEEP) P::score(da, a, last[t - (KS - KEEP)]);
             if constexpr (b == 2) P::score(sb, a, q, t);
-            if constexpr (b == 3) P::score(db, a, go, t);
+            if constexpr (b == 3 && t < KS - KEEP) P::score(db, a, go, t);
+            if constexpr (b == 3 && t >= KS - KEEP) P::score(db, a, last[t - (KS - KEEP)]);
             if constexpr (b == 4) P::sum(dq, a, wa, t);
             if constexpr (b == 5) P::sum(dq, a, wb, t);
           },
@@ -1378,6 +1406,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
             constexpr int b = i / KS;
             constexpr PkInt<i % KS> t{};
             if constexpr (i < 2 * Stream::NV) next.template piece<i>();
+            if constexpr (KEEP > 0 && (b == 1 || b == 3) && t + 2 >= KS - KEEP && t + 2 < KS)
+              last[t + 2 - (KS - KEEP)] = *reinterpret_cast<const MSDA_LDS at_bf8*>(reinterpret_cast<PkLds>(static_cast<uintptr_t>(kept)) + (t + 2 - (KS - KEEP)) * kPkWaves * 1024);
             if constexpr (b == 1) weigh(sa, k0, t);
             if constexpr (b == 2) slope(sa, da, wa, k0, t);
             if constexpr (b == 3) weigh(sb, k0 + 32, t);
@@ -1434,6 +1464,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
 
 // ---- keys on their own side: dk and dv ---------------------------------------------------------
 
+// The keys of a tile that a row sees, [lo, hi) of 0 .. kPkTile, in one number.
+struct PkSeen {
+  static __device__ __forceinline__ int pack(int lo, int hi) {
+    lo = min(max(lo, 0), kPkTile);
+    return lo | max(min(hi, kPkTile) - lo, 0) << 16;
+  }
+  static __device__ __forceinline__ bool key(int seen, int k) { return static_cast<uint32_t>(k - (seen & 0xffff)) < static_cast<uint32_t>(seen) >> 16; }
+};
+
 template <bool RANGES>
 struct PkKeys {
   PkPlace w;
@@ -1488,7 +1527,7 @@ struct PkKeys {
 // head's group) that see them, 64 at a time. A tile that many rows see is shared by several workgroups,
 // whose sums pk_join_kv_kernel adds in their order.
 template <typename T, int DT, int MOD>
-__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 : 2) : 1) pk_bwd_kv_kernel(const PackParams p) {
+__global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && MOD == 0 ? 3 : 2) : 1) pk_bwd_kv_kernel(const PackParams p) {
   using Tile = PkTile<T, DT>;
   using Stream = PkStream<T, DT>;
   // arrays of their own, so that the compiler knows that the transfers under way do not write what it reads
@@ -1498,9 +1537,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
   // of the tile's rows: the numbers that its scores and dP start from (bf16), or m, log2 l and delta (f32);
   // the keys that the row sees
   __shared__ __align__(16) float row_s[2][kPkChunk], row_d[2][kPkChunk], row_l[2][sizeof(T) == 2 ? 4 : kPkChunk];
-  __shared__ __align__(16) int row_lim[2][kPkChunk];
-  // MOD: the first of these keys, the row's place less the tile's first key, and its slope, which the head gives
-  __shared__ __align__(16) int row_lo[2][MOD != 0 ? kPkChunk : 4];
+  __shared__ __align__(16) int row_lim[2][kPkChunk];  // MOD: those of the tile, from the first of them: (PkSeen)
+  // MOD: the row's place less the tile's first key, and its slope, which the head gives
   __shared__ __align__(16) float row_place[2][(MOD & kPkSlope) != 0 ? kPkChunk : 4], row_slope[(MOD & kPkSlope) != 0 ? kPkChunk : 4];
   constexpr bool bf = sizeof(T) == 2;
   constexpr int PF = bf && DT != 64 && DT != 128 ? 3 : 2;
@@ -1569,13 +1607,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     if constexpr (MOD == 0) {
       if (wave == 3) row_lim[buf][x] = x >= count ? 0 : p.causal ? min(max(t0 + t + shift + 1, 0), m) : m;
     } else if (wave == 3) {
-      row_lim[buf][x] = x >= count ? 0 : w.hi(p, t0 + t);
-      row_lo[buf][x] = w.lo(p, t0 + t);
+      row_lim[buf][x] = x >= count ? 0 : PkSeen::pack(w.lo(p, t0 + t) - wb, w.hi(p, t0 + t) - wb);
       if constexpr ((MOD & kPkSlope) != 0) row_place[buf][x] = static_cast<float>(t0 + t + shift - w.b0);
     }
   };
   // One 32-row block; `all`: every row sees every key of the wave.
-  auto block = [&](bool all, PkLds Q, PkLds G, int h, const float* rs, const float* rd, const float* rl, const int* lims, const int* los, const float* places,
+  auto block = [&](bool all, PkLds Q, PkLds G, int h, const float* rs, const float* rd, const float* rl, const int* lims, const float* places,
                    const float* slopes) {
     // All that a lane's place gives is formed anew in each block, the operands' offsets in each phase: kept, they spill
     // at 128 channels.
@@ -1607,11 +1644,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
       if constexpr (MOD != 0) {
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
-          const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp), lf = *reinterpret_cast<const int4*>(los + 8 * c4 + 4 * grp);
-          x[4 * c4] = kj < lm.x && kj >= lf.x ? x[4 * c4] : 0.0f;
-          x[4 * c4 + 1] = kj < lm.y && kj >= lf.y ? x[4 * c4 + 1] : 0.0f;
-          x[4 * c4 + 2] = kj < lm.z && kj >= lf.z ? x[4 * c4 + 2] : 0.0f;
-          x[4 * c4 + 3] = kj < lm.w && kj >= lf.w ? x[4 * c4 + 3] : 0.0f;
+          const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
+          x[4 * c4] = PkSeen::key(lm.x, kj - wb) ? x[4 * c4] : 0.0f;
+          x[4 * c4 + 1] = PkSeen::key(lm.y, kj - wb) ? x[4 * c4 + 1] : 0.0f;
+          x[4 * c4 + 2] = PkSeen::key(lm.z, kj - wb) ? x[4 * c4 + 2] : 0.0f;
+          x[4 * c4 + 3] = PkSeen::key(lm.w, kj - wb) ? x[4 * c4 + 3] : 0.0f;
+          __builtin_amdgcn_sched_barrier(0);  // one read at a time: registers
         }
         return;
       }
@@ -1624,12 +1662,71 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
         x[4 * c4 + 3] = kj < lm.w ? x[4 * c4 + 3] : 0.0f;
       }
     };
-    if constexpr (bf) {
+    if constexpr (bf && (MOD & kPkCap) != 0 && DT == 128) {
+      // The weights and their slopes take as long as the products. Beside these they need 20 registers more than there are,
+      // and what is spilled comes back through the counter of the tile in flight; so the phases follow one another here,
+      // the scores first in place through the tanh, then two of them and two dP at a time into a pair of weights and a pair
+      // of ds, and a CU's other workgroup has the matrix units meanwhile.
+      constexpr int KS = P::kScores;
+      typename P::Weights w, ds;
+      at_bf8 last[KEEP];
+      pk_pipe<2 * KS, PF>(
+          [&](auto i) { return P::row_operand(i < KS ? Q : G, now, i % KS); },
+          [&](auto i, const auto& a) {
+            constexpr int t = i % KS;
+            if constexpr (i < KS) P::score(s, a, k, t);
+            else if constexpr (t < KS - KEEP) P::score(dp, a, v, t);
+            else P::score(dp, a, last[t - (KS - KEEP)]);
+          },
+          [&](auto i) {
+            constexpr int t = i % KS;
+            if constexpr (i == KS - 1) start(dp, rd, false);
+            if constexpr (i >= KS && t + 2 >= KS - KEEP && t + 2 < KS)
+              last[t + 2 - (KS - KEEP)] = *reinterpret_cast<const MSDA_LDS at_bf8*>(reinterpret_cast<PkLds>(static_cast<uintptr_t>(kept)) + (t + 2 - (KS - KEEP)) * kPkWaves * 1024);
+          });
+      pk_bend<T>(p, s);
+      uint32_t wp[8], dsp[8];
+      pk_for<8>([&](auto pair) {
+        const int a = 8 * (pair >> 1) + 4 * grp + 2 * (pair & 1);
+        const pk_f2 number = *reinterpret_cast<const pk_f2*>(rs + a);
+        float ws[2], es[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float bent = s[2 * pair + j];
+          float x = fmaf(bent, p.cap2, number[j]);
+          if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[a + j], fabsf(places[a + j] - static_cast<float>(kj - wb)), x);
+          ws[j] = at_exp2(x);
+          es[j] = ws[j] * fmaf(-bent, bent, 1.0f) * dp[2 * pair + j];
+        }
+        if (!all) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const bool sees = PkSeen::key(lims[a + j], kj - wb);
+            ws[j] = sees ? ws[j] : 0.0f;
+            es[j] = sees ? es[j] : 0.0f;
+          }
+        }
+        wp[pair] = __builtin_bit_cast(uint32_t, __builtin_convertvector((pk_f2{ws[0], ws[1]}), pk_bf2));
+        dsp[pair] = __builtin_bit_cast(uint32_t, __builtin_convertvector((pk_f2{es[0], es[1]}), pk_bf2));
+        if constexpr (pair % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+      });
+      w.b[0] = __builtin_bit_cast(at_bf8, uint4{wp[0], wp[1], wp[2], wp[3]});
+      w.b[1] = __builtin_bit_cast(at_bf8, uint4{wp[4], wp[5], wp[6], wp[7]});
+      ds.b[0] = __builtin_bit_cast(at_bf8, uint4{dsp[0], dsp[1], dsp[2], dsp[3]});
+      ds.b[1] = __builtin_bit_cast(at_bf8, uint4{dsp[4], dsp[5], dsp[6], dsp[7]});
+      asm volatile("" : "+v"(now.row), "+v"(now.tr));
+      pk_pipe<2 * KS, PF>([&](auto i) { return P::sum_operand(i < KS ? G : Q, now, i % KS); },
+                          [&](auto i, const auto& a) {
+                            if constexpr (i < KS) P::sum(dv, a, w, i % KS);
+                            else P::sum(dk, a, ds, i % KS);
+                          },
+                          [](auto) {});
+    } else if constexpr (bf) {
       // Phases of KS products: S, dP beside the weights, dv beside ds, dk.
       constexpr int KS = P::kScores;
       typename P::Weights w, ds;
       bool far = false;
-      at_f16 bend;  // the slopes of the cap
+      uint32_t wp[8];  // with the cap: the weights as the products take them; s has them times the slopes of the cap
       at_bf8 last[KEEP > 0 ? KEEP : 1];
       pk_pipe<4 * KS, PF>(
           [&](auto i) {
@@ -1655,21 +1752,39 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
             if constexpr (b == 1 && MOD == 0) pk_beside<KS, t>([&](int j) { s[j] = at_exp2(s[j] * p.scale2); });
             if constexpr (b == 1 && MOD != 0) {
               if constexpr ((MOD & kPkCap) != 0 && t == 1) far = pk_far<T>(p, s);
-              // register j, its row's number (with the cap; else the products started from it) and bias
-              auto shape = [&](int j, float bent) {
+              // registers j and j + 1; a row's number (with the cap; else the products started from it) and bias
+              auto score = [&](int j, float bent) {
                 const int row = 8 * (j >> 2) + 4 * grp + (j & 3);
                 float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, rs[row]) : s[j] * p.scale2;
-                if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[row], fabsf(places[row] - static_cast<float>(kj - static_cast<int>(wb))), x);
-                s[j] = at_exp2(x);
-                if constexpr ((MOD & kPkCap) != 0) bend[j] = fmaf(-bent, bent, 1.0f);
+                if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[row], fabsf(places[row] - static_cast<float>(kj - wb)), x);
+                return at_exp2(x);
               };
-              if ((MOD & kPkCap) != 0 && far) pk_beside<KS, t>([&](int j) { shape(j, pk_bent<T>(p, s[j])); });
-              else pk_beside<KS, t>([&](int j) { shape(j, pk_near<T>(s[j] * p.inner)); });
+              auto capped = [&](int j, float b0, float b1) {
+                const float w0 = score(j, b0), w1 = score(j + 1, b1);
+                wp[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((pk_f2{w0, w1}), pk_bf2));
+                s[j] = w0 * fmaf(-b0, b0, 1.0f);
+                s[j + 1] = w1 * fmaf(-b1, b1, 1.0f);
+              };
+              if constexpr ((MOD & kPkCap) == 0) pk_beside<KS, t>([&](int j) { s[j] = score(j, 0.0f); });
+              else if (far) pk_beside<KS, t, 8>([&](int i) { capped(2 * i, pk_bent<T>(p, s[2 * i]), pk_bent<T>(p, s[2 * i + 1])); });
+              else pk_beside<KS, t, 8>([&](int i) { capped(2 * i, pk_near<T>(s[2 * i] * p.inner), pk_near<T>(s[2 * i + 1] * p.inner)); });
             }
             if constexpr (b == 1 && t == KS - 1) {
               unseen(s);
-              w.set(s);
-              if constexpr ((MOD & kPkCap) != 0) s *= bend;
+              if constexpr ((MOD & kPkCap) == 0) {
+                w.set(s);
+              } else {
+                if (!all) {
+#pragma unroll
+                  for (int c4 = 0; c4 < 4; ++c4) {
+                    const int4 lm = *reinterpret_cast<const int4*>(lims + 8 * c4 + 4 * grp);
+                    wp[2 * c4] &= (PkSeen::key(lm.x, kj - wb) ? 0xffffu : 0u) | (PkSeen::key(lm.y, kj - wb) ? 0xffff0000u : 0u);
+                    wp[2 * c4 + 1] &= (PkSeen::key(lm.z, kj - wb) ? 0xffffu : 0u) | (PkSeen::key(lm.w, kj - wb) ? 0xffff0000u : 0u);
+                  }
+                }
+                w.b[0] = __builtin_bit_cast(at_bf8, uint4{wp[0], wp[1], wp[2], wp[3]});
+                w.b[1] = __builtin_bit_cast(at_bf8, uint4{wp[4], wp[5], wp[6], wp[7]});
+              }
             }
             if constexpr (b == 2) pk_beside<KS, t>([&](int j) { dp[j] *= s[j]; });
             if constexpr (b == 2 && t == KS - 1) {
@@ -1721,7 +1836,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     if constexpr (MOD != 0) {
       for (uint64_t left = sick; left != 0; left &= left - 1) {
         const int x = static_cast<int>(__builtin_ctzll(left));
-        spoilt = spoilt || (wb0 + col < row_lim[buf][x] && wb0 + col >= row_lo[buf][x]);
+        spoilt = spoilt || PkSeen::key(row_lim[buf][x], wb0 + col - wb);
       }
       return;
     }
@@ -1742,7 +1857,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 ? 3 
     const bool full = __builtin_amdgcn_readfirstlane(seen) != 0;
 #pragma unroll 1
     for (int h = 0; h < count; h += 32)
-      block(full, Q, G, h, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h, row_lo[buf] + (MOD != 0 ? h : 0),
+      block(full, Q, G, h, row_s[buf] + h, row_d[buf] + h, row_l[buf] + (bf ? 0 : h), row_lim[buf] + h,
             row_place[buf] + ((MOD & kPkSlope) != 0 ? h : 0), row_slope + ((MOD & kPkSlope) != 0 ? h : 0));
   };
   if (c0 < c1) stage(X0, Y0, 0, c0);
