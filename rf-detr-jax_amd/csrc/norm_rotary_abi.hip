@@ -15,13 +15,17 @@ using msda::NormRotaryParams;
 using msda_host::aligned_to;
 using msda_host::fail;
 
-// Workgroups of the backward, each with one row of partial sums: enough for 8 to a CU.
-constexpr int64_t kMostGroups = 2048;
+// Workgroups of the backward, each with one row of partial sums: four to a CU, as many as fit, where there are the tokens.
+constexpr int64_t kMostGroups = 1024;
 
-int tokens_of(int64_t tokens) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, tokens / 1024))); }
+// Tokens of a step of a workgroup: few enough for four workgroups a CU; at most 8 (the angles of 8 tokens keep 256 threads
+// busy for one or two steps), in the backward 16, so that 16,000 tokens are one step.
+int tokens_of(int64_t tokens, bool backward) {
+  return static_cast<int>(std::max<int64_t>(1, backward ? std::min<int64_t>(16, (tokens + kMostGroups - 1) / kMostGroups) : std::min<int64_t>(8, tokens / 1024)));
+}
 
 int64_t groups_of(int64_t tokens, bool backward) {
-  const int64_t n = (tokens + tokens_of(tokens) - 1) / tokens_of(tokens);
+  const int64_t per = tokens_of(tokens, backward), n = (tokens + per - 1) / per;
   return backward ? std::min(n, kMostGroups) : n;
 }
 
@@ -64,7 +68,7 @@ int run(const NormRotaryParams& p, bool backward, bool neighbours, hipStream_t s
 // The checks and parameters that both directions share; p.tokens 0: nothing to do.
 int plan(NormRotaryParams& p, int dtype, const void* positions, int position_type, int weight_type, int tokens, int heads, int kv_heads, int head_dim,
          const int64_t* strides, int nstrides, const int64_t* position_strides, const int32_t* sections, int axes, double base, int shared_frequencies,
-         double eps) {
+         double eps, bool backward) {
   if (dtype != MSDA_DTYPE_F32 && dtype != MSDA_DTYPE_BF16) return fail(MSDA_ERR_UNSUPPORTED, "norm rotary: unsupported dtype code %d", dtype);
   if (weight_type != MSDA_DTYPE_F32 && weight_type != MSDA_DTYPE_BF16) return fail(MSDA_ERR_UNSUPPORTED, "norm rotary: unsupported weight type code %d", weight_type);
   if (position_type < MSDA_POSITION_I32 || position_type > MSDA_POSITION_F32)
@@ -97,7 +101,7 @@ int plan(NormRotaryParams& p, int dtype, const void* positions, int position_typ
   p.heads[1] = kv_heads;
   p.dim = head_dim;
   p.pairs = static_cast<int>(pairs);
-  p.per = tokens_of(tokens);
+  p.per = tokens_of(tokens, backward);
   p.eps = static_cast<float>(eps);
   p.inverse_dim = 1.0f / static_cast<float>(head_dim);
   const double log_base = std::log(base);
@@ -128,7 +132,7 @@ int msda_norm_rotary_fwd(const void* q, void* q_out, const void* k, void* k_out,
   msda_host::clear_error();
   NormRotaryParams p{};
   int rc = plan(p, dtype, positions, position_type, weight_type, tokens, heads, kv_heads, head_dim, strides, 8, position_strides, sections, axes, base,
-                shared_frequencies, eps);
+                shared_frequencies, eps, false);
   if (rc != MSDA_OK || p.tokens == 0) return rc;
   const size_t e = dtype == MSDA_DTYPE_BF16 ? 2 : 4, pe = position_type == MSDA_POSITION_I64 ? 8 : 4, we = weight_type == MSDA_DTYPE_BF16 ? 2 : 4;
   if (positions == nullptr || (heads != 0 && (q == nullptr || q_out == nullptr)) || (kv_heads != 0 && (k == nullptr || k_out == nullptr)))
@@ -162,7 +166,7 @@ int msda_norm_rotary_bwd(const void* q, const void* grad_q_out, void* grad_q, co
   msda_host::clear_error();
   NormRotaryParams p{};
   int rc = plan(p, dtype, positions, position_type, weight_type, tokens, heads, kv_heads, head_dim, strides, 12, position_strides, sections, axes, base,
-                shared_frequencies, eps);
+                shared_frequencies, eps, true);
   if (rc != MSDA_OK) return rc;
   const bool sums = grad_q_weight != nullptr || grad_k_weight != nullptr;
   const size_t e = dtype == MSDA_DTYPE_BF16 ? 2 : 4, pe = position_type == MSDA_POSITION_I64 ? 8 : 4, we = weight_type == MSDA_DTYPE_BF16 ? 2 : 4;

@@ -160,28 +160,36 @@ __global__ void __launch_bounds__(256) norm_rotary_kernel(const NormRotaryParams
   }
 }
 
+// Queries, then keys: with the sums of both at a time 161 registers left 3 waves a SIMD (16,000 tokens of 40 heads, 128
+// channels, bf16: 151 us, now 121 us).
 template <typename T, int LPR, bool NEIGHBOURS>
-__global__ void __launch_bounds__(256) norm_rotary_bwd_kernel(const NormRotaryParams p) {
+__global__ void __launch_bounds__(256, 4) norm_rotary_bwd_kernel(const NormRotaryParams p) {
   extern __shared__ __align__(16) float2 nr_cs[];
   constexpr int E = 16 / static_cast<int>(sizeof(T)), SLOTS = 256 / LPR;
   __shared__ float sums[4][LPR][2 * E + 1];
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6, u = lane % LPR;
   const NrUnit<T, NEIGHBOURS> unit(p, u);
-  float dw[2][2 * E] = {};
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per; t0 < p.tokens; t0 += static_cast<int64_t>(gridDim.x) * p.per) {
-    const int nt = static_cast<int>(min(static_cast<int64_t>(p.per), p.tokens - t0));
-    __syncthreads();  // the last step's angles are read
-    nr_angles<-1>(p, nr_cs, t0, nt);
-    __syncthreads();
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int heads = p.heads[which];
-      float w[2 * E], x[2 * E], g[2 * E];
-      unit.weights(p, which, w);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * p.per;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int heads = p.heads[which];
+    float w[2 * E], dw[2 * E] = {};
+    unit.weights(p, which, w);
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.per; t0 < p.tokens; t0 += stride) {
+      const int nt = static_cast<int>(min(static_cast<int64_t>(p.per), p.tokens - t0));
+      if (which == 0 || stride < p.tokens) {  // (one step: they are there)
+        __syncthreads();                       // the last step's angles are read
+        nr_angles<-1>(p, nr_cs, t0, nt);
+        __syncthreads();
+      }
+      const T* px = static_cast<const T*>(p.x[which]) + t0 * p.xs[which][0];
+      const T* pg = static_cast<const T*>(p.dy[which]) + t0 * p.gs[which][0];
+      T* py = static_cast<T*>(p.y[which]);
       for (int row = static_cast<int>(threadIdx.x) / LPR; row < nt * heads; row += SLOTS) {
         const int t = row / heads, h = row - t * heads;
-        unit.load(static_cast<const T*>(p.x[which]) + (t0 + t) * p.xs[which][0] + h * p.xs[which][1], x);
-        unit.load(static_cast<const T*>(p.dy[which]) + (t0 + t) * p.gs[which][0] + h * p.gs[which][1], g);
+        float x[2 * E], g[2 * E];
+        unit.load(px + t * p.xs[which][0] + h * p.xs[which][1], x);
+        unit.load(pg + t * p.gs[which][0] + h * p.gs[which][1], g);
         unit.turn(g, nr_cs + t * p.pairs, p.pairs);
         float xx = 0.0f, ux = 0.0f;
 #pragma unroll
@@ -194,20 +202,17 @@ __global__ void __launch_bounds__(256) norm_rotary_bwd_kernel(const NormRotaryPa
         const float r = rsqrtf(fmaf(xx, p.inverse_dim, p.eps)), back = r * r * (ux * p.inverse_dim);
 #pragma unroll
         for (int j = 0; j < 2 * E; ++j) {
-          dw[which][j] = fmaf(g[j], x[j] * r, dw[which][j]);
+          dw[j] = fmaf(g[j], x[j] * r, dw[j]);
           x[j] = r * fmaf(-x[j], back, g[j] * w[j]);
         }
-        if (p.y[which] != nullptr) unit.store(static_cast<T*>(p.y[which]) + (t0 + t) * p.ys[which][0] + h * p.ys[which][1], x);
+        if (py != nullptr) unit.store(py + (t0 + t) * p.ys[which][0] + h * p.ys[which][1], x);
       }
     }
-  }
-  if (p.part == nullptr) return;
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
+    if (p.part == nullptr) continue;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2 * E; ++j) {
-      float s = dw[which][j];
+      float s = dw[j];
 #pragma unroll
       for (int m = LPR; m < 64; m *= 2) s += __shfl_xor(s, m);
       if (lane < LPR) sums[wave][u][j] = s;
@@ -302,25 +307,33 @@ __global__ void __launch_bounds__(256) norm_rotary_any_kernel(const NormRotaryPa
   }
 }
 
-// The workgroups' sums of the weights' gradients, in their order: 16 columns of [2][dim] to a workgroup, 64 threads a
-// column.
+// The workgroups' sums of the weights' gradients, in their order: 16 columns of [2][dim] to a workgroup, 4 to a thread.
 __global__ void __launch_bounds__(1024) norm_rotary_join_kernel(const float* part, int rows, int dim, void* q, void* k, int weight_type) {
-  __shared__ float sums[64][17];
-  const int col = static_cast<int>(threadIdx.x) & 15, at = static_cast<int>(threadIdx.x) >> 4, c = static_cast<int>(blockIdx.x) * 16 + col;
-  float s = 0.0f;
-  if (c < 2 * dim) {
-#pragma unroll 8
-    for (int r = at; r < rows; r += 64) s += part[static_cast<int64_t>(r) * 2 * dim + c];
+  __shared__ float sums[256][17];
+  const int quad = static_cast<int>(threadIdx.x) & 3, at = static_cast<int>(threadIdx.x) >> 2, c = static_cast<int>(blockIdx.x) * 16 + 4 * quad;
+  float4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < 2 * dim) {  // (2 dim is a multiple of 4)
+#pragma unroll 4
+    for (int r = at; r < rows; r += 256) {
+      const float4 x = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(r) * 2 * dim + c);
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
   }
-  sums[at][col] = s;
+  sums[at][4 * quad] = s.x, sums[at][4 * quad + 1] = s.y, sums[at][4 * quad + 2] = s.z, sums[at][4 * quad + 3] = s.w;
+  __syncthreads();
+  // 16 columns of 64 threads each
+  const int col = static_cast<int>(threadIdx.x) & 15, row = static_cast<int>(threadIdx.x) >> 4, to_col = static_cast<int>(blockIdx.x) * 16 + col;
+  float t = (sums[row][col] + sums[row + 64][col]) + (sums[row + 128][col] + sums[row + 192][col]);
+  __syncthreads();
+  sums[row][col] = t;
   __syncthreads();
   for (int n = 32; n > 0; n /= 2) {
-    if (at < n) sums[at][col] += sums[at + n][col];
+    if (row < n) sums[row][col] += sums[row + n][col];
     __syncthreads();
   }
-  if (at != 0 || c >= 2 * dim) return;
-  void* to = c < dim ? q : k;
-  const int ch = c < dim ? c : c - dim;
+  if (row != 0 || to_col >= 2 * dim) return;
+  void* to = to_col < dim ? q : k;
+  const int ch = to_col < dim ? to_col : to_col - dim;
   if (to == nullptr) return;
   if (weight_type == 0) static_cast<float*>(to)[ch] = sums[0][col];
   else rot_put(static_cast<bf16_t*>(to)[ch], sums[0][col]);

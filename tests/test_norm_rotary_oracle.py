@@ -118,7 +118,7 @@ def test_refusals(direction, change, code, text):
 def test_workspace():
     lib = _native.lib()
     assert lib.msda_norm_rotary_bwd_workspace_size(4, 32) == 4 * 2 * 32 * 4
-    assert lib.msda_norm_rotary_bwd_workspace_size(10 ** 8, 256) == 2048 * 2 * 256 * 4
+    assert lib.msda_norm_rotary_bwd_workspace_size(10 ** 8, 256) == 1024 * 2 * 256 * 4
     assert lib.msda_norm_rotary_bwd_workspace_size(-1, 32) == INVALID and lib.msda_norm_rotary_bwd_workspace_size(4, 7) == UNSUPPORTED
     for change in ({"ws": None}, {"ws_bytes": 100}, {"ws": ODD}):
         rc, msg = _call("bwd", **change)
