@@ -165,31 +165,37 @@ __device__ __forceinline__ float c4_sum_groups(float x) {
   return at_sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+typedef uint32_t c4_u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t c4_u3 __attribute__((ext_vector_type(3)));
+typedef uint32_t c4_u4 __attribute__((ext_vector_type(4)));
+
 // A lane's share of 16 rows of the cache: a quarter of one row's channels.
 template <int DT>
 struct C4Rows {
   static constexpr int N = DT / 32, B = DT / 32;  // dwords of a share, blocks of a row
   uint32_t codes[N];
   uint32_t scale[DT == 96 ? 2 : 1];
-  // row `r` of the head's
-  __device__ __forceinline__ void load(const uint8_t* c, const uint8_t* s, int64_t r, int grp) {
-    const uint8_t* at = c + r * (DT / 2) + grp * (DT / 8);
+  // Row 16 j + col of a chunk, whose codes and scales the two buffers hold: zeros behind its last row.
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t c, __amdgpu_buffer_rsrc_t s, int j, int col, int grp) {
+    const int at = col * (DT / 2) + grp * (DT / 8), first = 16 * j * (DT / 2);
     if constexpr (N == 4) {
-      const uint4 x = *reinterpret_cast<const uint4*>(at);
-      codes[0] = x.x, codes[1] = x.y, codes[2] = x.z, codes[3] = x.w;
+      const c4_u4 x = __builtin_amdgcn_raw_buffer_load_b128(c, at + first, 0, 0);
+      codes[0] = x[0], codes[1] = x[1], codes[2] = x[2], codes[3] = x[3];
+    } else if constexpr (N == 3) {
+      const c4_u3 x = __builtin_amdgcn_raw_buffer_load_b96(c, at + first, 0, 0);
+      codes[0] = x[0], codes[1] = x[1], codes[2] = x[2];
     } else if constexpr (N == 2) {
-      const uint2 x = *reinterpret_cast<const uint2*>(at);
-      codes[0] = x.x, codes[1] = x.y;
+      const c4_u2 x = __builtin_amdgcn_raw_buffer_load_b64(c, at + first, 0, 0);
+      codes[0] = x[0], codes[1] = x[1];
     } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) codes[e] = reinterpret_cast<const uint32_t*>(at)[e];
+      codes[0] = __builtin_amdgcn_raw_buffer_load_b32(c, at + first, 0, 0);
     }
-    const uint8_t* b = s + r * B;
+    const int row = col * B + 16 * j * B;
     if constexpr (DT == 96) {  // 24 channels, of one block or two
-      scale[0] = b[24 * grp / 32];
-      scale[1] = b[(24 * grp + 16) / 32];
+      scale[0] = __builtin_amdgcn_raw_buffer_load_b8(s, row + 24 * grp / 32, 0, 0);
+      scale[1] = __builtin_amdgcn_raw_buffer_load_b8(s, row + (24 * grp + 16) / 32, 0, 0);
     } else {
-      scale[0] = b[grp * (DT / 4) / 32];
+      scale[0] = __builtin_amdgcn_raw_buffer_load_b8(s, row + grp * (DT / 4) / 32, 0, 0);
     }
   }
   __device__ __forceinline__ uint32_t scale_of(int e, int grp) const {  // of dword e, channels grp DT / 4 + 8 e ..
@@ -205,7 +211,7 @@ struct C4Rows {
 };
 
 template <typename T, int DT, bool SHAPED>
-__global__ void __launch_bounds__(256, 2) cache4_attention_kernel(const PackParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_kernel(const PackParams p) {
   constexpr int DP = DT == 96 ? 128 : DT, CPR = DP / 8;  // channels and 16-byte pieces of a row in LDS
   constexpr int N = DT / 32, MT = DT / 16, QT = kC4QTerms<T>, PT = kC4PTerms<T>;
   __shared__ __align__(16) unsigned char area[4][64 * DP];  // a wave's 32 rows of values, later its sums
@@ -247,7 +253,12 @@ __global__ void __launch_bounds__(256, 2) cache4_attention_kernel(const PackPara
   const uint8_t* ks = p.k_scales + head_rows * (DT / 32);
   const uint8_t* vs = p.v_scales + head_rows * (DT / 32);
   unsigned char* const mine = area[wave];
-  auto swizzle = [](int r) { return CPR == 16 ? r & 15 : CPR == 8 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  // Piece c of row r lies at c ^ swizzle(r): 16 rows of one piece (the writes), and 8 rows of two neighbouring ones (half
+  // a wave's transposing read), fall on 256 bytes of banks. Rows 16 apart have the same.
+  auto swizzle = [](int r) { return (r / (16 / CPR) % (CPR / 2)) * 2 | (r >> 3 & 1); };
+  // lane 4 j + a of a group reads key 4 grp + j, channels 4 a .. of 16
+  const int key = 4 * grp + (col >> 2), quad = col & 3;
+  const uint32_t read_at = key * (2 * DP) + (((quad >> 1) ^ swizzle(key)) << 4) + 8 * (quad & 1), write_at = col * (2 * DP);
 
   for (int r0 = 0; r0 < n * p.group; r0 += kC4Rows) {
     const int r = r0 + col, rc = min(r, n * p.group - 1), tok = rc / p.group, g = rc - tok * p.group, head = kv_head * p.group + g;
@@ -278,14 +289,17 @@ __global__ void __launch_bounds__(256, 2) cache4_attention_kernel(const PackPara
     for (int i = 0; i < MT; ++i) o[i] = at_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
     C4Rows<DT> kr[4], vr[4];
-    auto load_keys = [&](int c) {
+    // A chunk is two buffers, whose addresses are the wave's: a lane adds a constant, and rows behind the last key need no
+    // test of their own.
+    auto load = [&](C4Rows<DT>(&x)[4], const uint8_t* codes, const uint8_t* scales, int c) {
+      const int rows = __builtin_amdgcn_readfirstlane(min(m - c * kPkChunk, kPkChunk));
+      const __amdgpu_buffer_rsrc_t cb = pk_buffer(codes + static_cast<int64_t>(c) * (kPkChunk * (DT / 2)), rows * (DT / 2));
+      const __amdgpu_buffer_rsrc_t sb = pk_buffer(scales + static_cast<int64_t>(c) * (kPkChunk * (DT / 32)), rows * (DT / 32));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kr[j].load(kc, ks, min(c * kPkChunk + 16 * j + col, m - 1), grp);
+      for (int j = 0; j < 4; ++j) x[j].load(cb, sb, j, col, grp);
     };
-    auto load_values = [&](int c) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vr[j].load(vc, vs, min(c * kPkChunk + 16 * j + col, m - 1), grp);
-    };
+    auto load_keys = [&](int c) { load(kr, kc, ks, c); };
+    auto load_values = [&](int c) { load(vr, vc, vs, c); };
     // chunks that the tile's rows see
     const int ca = max(c0, tile_first / kPkChunk), cz = min(c1, (tile_end + kPkChunk - 1) / kPkChunk);
     int c = ca + wave;
@@ -307,6 +321,7 @@ __global__ void __launch_bounds__(256, 2) cache4_attention_kernel(const PackPara
 #pragma unroll
           for (int t = QT - 1; t >= 0; --t) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[e][t], s[j], 0, 0, 0);
         }
+        if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // left to itself the compiler converts everything first: 230 registers
       }
       if (c + 4 < cz) load_keys(c + 4);
       if (SHAPED && p.cap2 != 0.0f) {
@@ -363,26 +378,25 @@ __global__ void __launch_bounds__(256, 2) cache4_attention_kernel(const PackPara
           const C4Rows<DT>& x = vr[2 * h + j];
           const bool spoilt = __any(x.bad());
           sick = sick || spoilt;
-          const int row = 16 * j + col;
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             uint4 y = __builtin_bit_cast(uint4, x.bf16(e, grp));
             if (spoilt && x.scale_of(e, grp) == kC4Bad) y = uint4{0u, 0u, 0u, 0u};  // its rows get it in the end
-            *reinterpret_cast<uint4*>(mine + row * (2 * DP) + (((grp * N + e) ^ swizzle(row)) << 4)) = y;
+            *reinterpret_cast<uint4*>(mine + (write_at + (((grp * N + e) ^ swizzle(col)) << 4)) + 16 * j * (2 * DP)) = y;
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
         if (h == 1 && c + 4 < cz) load_values(c + 4);
         at_bf8 w[PT];
         c4_terms(at_f8{s[2 * h][0], s[2 * h][1], s[2 * h][2], s[2 * h][3], s[2 * h + 1][0], s[2 * h + 1][1], s[2 * h + 1][2], s[2 * h + 1][3]}, w);
         pk_wave_sync();
-        // lane 4 j + a of a group addresses key 4 grp + j, channels 4 a ..
-        const int key = 4 * grp + (col >> 2), quad = col & 3;
-        auto piece = [&](int row, int i) { return (PkLds)(mine) + row * (2 * DP) + (((2 * i + (quad >> 1)) ^ swizzle(row)) << 4) + 8 * (quad & 1); };
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const at_bf8 a = at_bf8_of(pk_read_tr(piece(key, i)), pk_read_tr(piece(16 + key, i)));
+          const PkLds at = (PkLds)(mine) + (read_at ^ (i << 5));
+          const at_bf8 a = at_bf8_of(pk_read_tr(at), pk_read_tr(at + 16 * (2 * DP)));
 #pragma unroll
           for (int t = PT - 1; t >= 0; --t) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[t], o[i], 0, 0, 0);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
         pk_wave_sync();
       }

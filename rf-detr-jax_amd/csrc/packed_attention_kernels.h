@@ -648,7 +648,8 @@ struct PkStream {
 
 // The same of a cache in 4 bits: a thread takes a quarter of one row of keys and of values, DT / 4 channels, loads its codes
 // and scales before the products of a chunk and writes them behind these, as T, where the transfers of Pair would have
-// put them. A row is DT / 2 bytes of codes and DT / 32 of scales.
+// put them. A row is DT / 2 bytes of codes and DT / 32 of scales. 16 lanes take one quarter of 16 rows, whose pieces the
+// swizzle spreads over all banks (four quarters of 4 rows met on 4 of 16 places), a wave whole rows.
 template <typename T, int DT>
 struct PkCachePair {
   using Tile = PkTile<T, DT>;
@@ -661,10 +662,12 @@ struct PkCachePair {
   uint32_t c[2][N], s[2][DT == 96 ? 2 : 1];
   __device__ __forceinline__ PkCachePair(unsigned char* x, unsigned char* y, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
                                          int first, int rows)
-      : to{x, y}, codes{kc, vc}, scales{ks, vs}, row(first + static_cast<int>(threadIdx.x >> 2)), end(rows) {}
+      : to{x, y}, codes{kc, vc}, scales{ks, vs}, row(first + own()), end(rows) {}
+  static __device__ __forceinline__ int own() { return static_cast<int>(threadIdx.x >> 6) * 16 + static_cast<int>(threadIdx.x & 15); }
+  static __device__ __forceinline__ int quarter() { return static_cast<int>(threadIdx.x >> 4 & 3); }
   template <int I>
   __device__ __forceinline__ void piece() {
-    const int64_t r = min(row, end - 1), part = threadIdx.x & 3;
+    const int64_t r = min(row, end - 1), part = quarter();
     if (end <= 0) return;  // no such tile
     const uint8_t* from = codes[I] + r * (DT / 2) + part * (DT / 8);
     if constexpr (N == 4) {
@@ -684,7 +687,7 @@ struct PkCachePair {
   }
   __device__ __forceinline__ void finish() const {
     if (end <= 0) return;
-    const int r = static_cast<int>(threadIdx.x >> 2), part = static_cast<int>(threadIdx.x & 3);
+    const int r = own(), part = quarter();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
