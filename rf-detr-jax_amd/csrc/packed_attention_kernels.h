@@ -962,7 +962,6 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
       // products of one wave; a CU's other workgroup fills the rest.
       using P = PkProducts<T, DT>;
       constexpr int KS = P::kScores, HA = KS >= 4 ? KS / 2 - 1 : 1, HB = KS - 1 - HA;  // steps up to the maximum, behind it
-      bool far = false;
       float bm, alpha = 1.0f, late = 1.0f;  // late: what scales the first half's weights after their rounding
       // step t of the softmax of block x, whose keys start at k: x = scale2 s - m and its maximum, m moved if it
       // has to, weights and their sum (a lane sums its half of the keys until the end)
@@ -972,7 +971,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           if constexpr (MOD == 0) {
             if (k + 32 > wfull) pk_mask(x, k, lim, grp);
           }
-          if constexpr ((MOD & kPkCap) != 0) far = pk_far<T>(p, x);
+          if constexpr ((MOD & kPkCap) != 0) pk_bend<T>(p, x);
           bm = -INFINITY;
         }
         if constexpr (t >= 1 && t <= HA) {
@@ -986,12 +985,11 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
             float to = -m;
             PkBias b = bias;
             if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
-            auto shape = [&](int i, float bent) {
-              x[i] = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, to) : fmaf(x[i], p.scale2, to);
+            pk_for<i1 - i0>([&](auto j) {
+              constexpr int i = i0 + j;
+              x[i] = fmaf(x[i], (MOD & kPkCap) != 0 ? p.cap2 : p.scale2, to);
               if constexpr ((MOD & kPkSlope) != 0) x[i] = b.add(x[i], 8 * (i >> 2) + (i & 3));
-            };
-            if ((MOD & kPkCap) != 0 && far) pk_for<i1 - i0>([&](auto i) { shape(i0 + i, pk_bent<T>(p, x[i0 + i])); });
-            else pk_for<i1 - i0>([&](auto i) { shape(i0 + i, pk_near<T>(x[i0 + i] * p.inner)); });
+            });
             if (k + 32 > wfull || k < wlo)
               pk_for<i1 - i0>([&](auto j) {
                 constexpr int i = i0 + j;
@@ -1354,23 +1352,21 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
         asm volatile("" : "+v"(kept));
       }
       at_bf8 last[KEEP > 0 ? KEEP : 1];
-      bool far = false;
       // MOD: weights, times the slope of the cap
       auto weigh = [&](at_f16& s, int k, auto t) {
         if constexpr (MOD == 0) {
           pk_beside<KS, t>([&](int i) { s[i] = at_exp2(fmaf(s[i], p.scale2, -m)); });
         } else {
-          if constexpr ((MOD & kPkCap) != 0 && t == 1) far = pk_far<T>(p, s);
+          if constexpr ((MOD & kPkCap) != 0 && t == 1) pk_bend<T>(p, s);
           PkBias b = bias;
           if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
-          auto shape = [&](int i, float bent) {
-            float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, -m) : fmaf(s[i], p.scale2, -m);
+          pk_beside<KS, t>([&](int i) {
+            const float bent = s[i];
+            float x = fmaf(bent, (MOD & kPkCap) != 0 ? p.cap2 : p.scale2, -m);
             if constexpr ((MOD & kPkSlope) != 0) x = b.add(x, 8 * (i >> 2) + (i & 3));
             s[i] = at_exp2(x);
             if constexpr ((MOD & kPkCap) != 0) s[i] *= fmaf(-bent, bent, 1.0f);
-          };
-          if ((MOD & kPkCap) != 0 && far) pk_beside<KS, t>([&](int i) { shape(i, pk_bent<T>(p, s[i])); });
-          else pk_beside<KS, t>([&](int i) { shape(i, pk_near<T>(s[i] * p.inner)); });
+          });
         }
       };
       auto slope = [&](at_f16& s, const at_f16& d, typename P::Weights& w, int k, auto t) {
@@ -1727,6 +1723,14 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
     } else if constexpr (bf) {
       // Phases of KS products: S, dP beside the weights, dv beside ds, dk.
       constexpr int KS = P::kScores;
+      // What a row adds to its scores, four rows to a read; at more channels there are no registers to hold it.
+      constexpr bool HELD = MOD != 0 && DT <= 64;
+      at_f16 number, place, slope;
+      if constexpr (HELD && (MOD & kPkCap) != 0) start(number, rs, false);
+      if constexpr (HELD && (MOD & kPkSlope) != 0) {
+        start(place, places, false);
+        start(slope, slopes, false);
+      }
       typename P::Weights w, ds;
       bool far = false;
       uint32_t wp[8];  // with the cap: the weights as the products take them; s has them times the slopes of the cap
@@ -1758,8 +1762,9 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
               // registers j and j + 1; a row's number (with the cap; else the products started from it) and bias
               auto score = [&](int j, float bent) {
                 const int row = 8 * (j >> 2) + 4 * grp + (j & 3);
-                float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, rs[row]) : s[j] * p.scale2;
-                if constexpr ((MOD & kPkSlope) != 0) x = fmaf(slopes[row], fabsf(places[row] - static_cast<float>(kj - wb)), x);
+                float x = (MOD & kPkCap) != 0 ? fmaf(bent, p.cap2, HELD ? number[j] : rs[row]) : s[j] * p.scale2;
+                if constexpr ((MOD & kPkSlope) != 0)
+                  x = fmaf(HELD ? slope[j] : slopes[row], fabsf((HELD ? place[j] : places[row]) - static_cast<float>(kj - wb)), x);
                 return at_exp2(x);
               };
               auto capped = [&](int j, float b0, float b1) {

@@ -318,3 +318,62 @@ def test_image_and_text_with_rotary_positions(dtype):
     cache = [torch.cat([x, torch.full_like(x, float("nan"))]) for x in (k, v)]
     last = packed_attention(q[-1:], *cache, _int([0, 1]), _int([0, 2 * n]), _int([n]), **kw)
     _within(last, want[-1:], bound[0][-1:], "token")
+
+
+#      lengths, keys, heads, key heads, head dim
+WIDE = {
+    "thousands": ([int(i * 7919 % 4) for i in range(3000)], None, 2, 1, 8),  # searched, not counted
+    "sixty_four_to_a_head": ([40, 3], [150, 3], 64, 1, 64),
+    "thirty_three_to_a_head": ([30, 66], None, 66, 2, 32),
+    "one_token_in_many": ([0] * 100 + [1] + [0] * 100, [0] * 100 + [333] + [0] * 100, 64, 2, 128),
+    "long_keys": ([130, 2], [4000, 3000], 2, 1, 128),
+    "long_rows": ([3100, 2], None, 2, 1, 32),
+}
+
+
+@TYPES
+@pytest.mark.parametrize("name", sorted(WIDE))
+def test_many_sequences_wide_groups_and_long_keys(name, dtype):
+    lengths, keys, h, hk, d = WIDE[name]
+    keys = lengths if keys is None else keys
+    sys.stderr.write(f"[gpu] shaped attention {name} {dtype}\n")
+    off, koff = np.cumsum([0, *lengths]), np.cumsum([0, *keys])
+    q, k, v, g = _normal(26, dtype, (off[-1], h, d), (koff[-1], hk, d), (koff[-1], hk, d), (off[-1], h, d))
+    for options in (dict(cap=3.0, slopes=_slopes(h), prefixes=_prefixes(keys)), dict(window=100, slopes=_slopes(h))):
+        kw, shape = _options(**options)
+        got = _run(q, k, v, g, _int(off), _int(koff), **kw)
+        _compare(q, k, v, g, got, PA.sequences(off, koff), shape)
+
+
+@TYPES
+def test_caps_of_every_size(dtype):
+    """From one that flattens everything to one that changes nothing, beside scales of other sizes: far, near and both in
+    a block."""
+    off = [0, 100, 171]
+    q, k, v, g = _normal(27, dtype, (171, 2, 64), (171, 1, 64), (171, 1, 64), (171, 2, 64))
+    for cap, scale in ((2.0 ** -32, None), (0.01, None), (1.0, 3.0), (4.0, 1.0), (1000.0, 2.0), (2.0 ** 20, None), (2.0 ** 32, 0.5), (30.0, 2.0 ** -40)):
+        kw, shape = _options(cap=cap)
+        shape.scale = scale
+        got = _run(q, k, v, g, _int(off), scale=scale, **kw)
+        _compare(q, k, v, g, got, PA.sequences(off), shape)
+
+
+@TYPES
+def test_layouts_and_one_gradient_at_a_time(dtype):
+    """Slices of a projection, head-major tensors, a cotangent by stride 0; gradients wanted one by one: the same bits."""
+    off, h, hk, d = [0, 50, 131], 4, 2, 64
+    (qkv,) = _normal(28, dtype, (131, h + 2 * hk, d))
+    parts = [qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]]
+    (g,) = _normal(29, dtype, (131, h, d))
+    kw, shape = _options(cap=2.0, slopes=_slopes(h), window=60, prefixes=[20, 131])
+    want = _run(*(x.contiguous() for x in parts), g, _int(off), **kw)
+    _compare(*parts, g, want, PA.sequences(off), shape)
+    for other in (parts, [x.transpose(0, 1).contiguous().transpose(0, 1) for x in parts], [x.transpose(1, 2).contiguous().transpose(1, 2) for x in parts]):
+        assert all(torch.equal(a, b) for a, b in zip(_run(*other, g, _int(off), **kw), want))
+    out, saved = packed_attention_forward(*parts, _int(off), **kw)
+    for i in range(3):
+        needs = [j == i for j in range(3)]
+        got = packed_attention_backward(*parts, out, saved, g, _int(off), needs=needs, **kw)
+        assert [x is not None for x in got] == needs and torch.equal(got[i], want[i + 1])
+    ones = torch.ones((), dtype=dtype, device=_dev()).expand(131, h, d)
+    _compare(*parts, ones, _run(*parts, ones, _int(off), **kw), PA.sequences(off), shape)
