@@ -220,6 +220,9 @@ struct PkRange {
 //   x = cap tanh(y) - slope |place - j|,  and d x / d (scale q.k) = 1 - tanh(y)^2,
 // over the keys with |place - j| < window and (not causal, or j <= place, or j < prefix): one range [lo, hi), whose
 // ends rise with the query, so that tiles, waves and rows skip and mask keys as the causal kernels do.
+// What bounds them is the vector units: with a cap a score takes 15 instructions beside its products for 8 (prompts of
+// 15,902 tokens, 32 heads to 8 of 128 channels: vector units 75 % and matrix units 32 % busy, 787 us, where the products
+// alone would take 497). The template's flags (PackShaped) keep what a call does not ask for out of the loops.
 
 __device__ __forceinline__ int pk_lo(const PackParams& p, int place) { return place < p.window ? 0 : place - p.window + 1; }
 __device__ __forceinline__ int pk_hi(const PackParams& p, int place, int prefix, int m) {
