@@ -519,7 +519,8 @@ int msda_packed_attention_bwd_const(const void* q, const void* k, const void* v,
  * all its queries see: a prompt or an image before a text; 0 and less: none).
  * shape NULL: the calls above. A window makes keys, tiles and the work that lie outside it go away.
  * Backward: msda_packed_attention_bwd_const's arguments. slopes have no gradient.
- * Workspaces: as above, with the window (0: none).
+ * Workspaces: as above, with the window (0: none); the backward's holds partial sums of grad_q, too, where the tiles of
+ * queries are fewer than the CUs.
  */
 typedef struct msda_score_shape {
   float cap;

@@ -41,10 +41,12 @@ int64_t pk_fwd_workspace(const PackShape& s, int window) {
   return parts == 1 ? 0 : (parts * (s.head_dim + 2) + 1) * rows * 4;
 }
 
+int pk_part(const PackShape& s, bool shaped) { return shaped && s.dtype == MSDA_DTYPE_F32 ? msda::kPkPartF32 : msda::kPkPart; }
+
 // The number of workgroups that may share a tile of keys in the backward: a causal sequence's first keys are
 // seen by all its rows, so with few tiles the longest one sets the time. A part is kPkPart chunks (more where
 // that makes more than kMost parts, or the tiles alone are several rounds of workgroups).
-int pk_parts(const PackShape& s, int window) {
+int pk_parts(const PackShape& s, int window, bool shaped) {
   constexpr int64_t kWant = 2048, kMost = 8;
   if (s.sequences == 0 || s.k_rows == 0) return 1;
   const int64_t tiles = std::min<int64_t>(s.k_rows, s.k_rows / msda::kPkTile + s.sequences) * s.kv_heads;
@@ -55,14 +57,29 @@ int pk_parts(const PackShape& s, int window) {
   // sequences start no second kernel (4 us).
   // No more than a window's see a tile.
   const int64_t rows = std::min<int64_t>({s.q_rows, 4 * (static_cast<int64_t>(s.q_rows) / s.sequences + 1), msda::pk_in_window(window)});
-  const int64_t chunks = rows * (s.heads / s.kv_heads) / msda::kPkChunk;
-  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, (chunks + msda::kPkPart - 1) / msda::kPkPart, kMost})));
+  const int64_t chunks = rows * (s.heads / s.kv_heads) / msda::kPkChunk, part = pk_part(s, shaped);
+  return static_cast<int>(std::max<int64_t>(1, std::min({kWant / tiles, (chunks + part - 1) / part, kMost})));
+}
+
+// Workgroups that share a tile of queries in the backward of shaped scores: two to a CU where the tiles are fewer than
+// the CUs, with 4 chunks of keys each at least (3,260 tokens of 8 heads, 32 channels, f32, 208 tiles: 86 us, in three parts 49 and 5 for their join).
+int pk_q_parts(const PackShape& s, int window) {
+  if (s.sequences == 0 || s.q_rows == 0) return 1;
+  const int64_t rows = static_cast<int64_t>(s.q_rows) * (s.heads / s.kv_heads), tiles = std::min<int64_t>(rows, rows / msda::kPkTile + s.sequences) * s.kv_heads;
+  const int64_t chunks = std::min(s.k_rows / s.sequences, msda::pk_in_window(window)) / msda::kPkChunk;
+  return tiles >= 256 ? 1 : static_cast<int>(std::clamp<int64_t>(std::min((512 + tiles - 1) / tiles, chunks / 4), 1, 8));
 }
 
 // Bytes of the parts' f32 sums of dk and dv.
-int64_t pk_bwd_workspace(const PackShape& s, int window) {
-  const int parts = pk_parts(s, window);
+int64_t pk_kv_workspace(const PackShape& s, int window, bool shaped) {
+  const int parts = pk_parts(s, window, shaped);
   return parts == 1 ? 0 : static_cast<int64_t>(parts) * 2 * s.k_rows * s.kv_heads * s.head_dim * 4;
+}
+
+// Those of dq, and the rows' numbers of parts.
+int64_t pk_q_workspace(const PackShape& s, int window) {
+  const int64_t parts = pk_q_parts(s, window);
+  return parts == 1 ? 0 : (parts * s.head_dim + 1) * static_cast<int64_t>(s.q_rows) * s.heads * 4;
 }
 
 template <typename T>
@@ -102,7 +119,7 @@ int64_t msda_packed_attention_bwd_workspace_size(int dtype, int sequences, int q
   msda_host::clear_error();
   const PackShape s{dtype, sequences, q_rows, k_rows, heads, kv_heads, head_dim};
   const int rc = pk_bwd_shape(s);
-  return rc != MSDA_OK ? rc : pk_bwd_workspace(s, 0x7fffffff);
+  return rc != MSDA_OK ? rc : pk_kv_workspace(s, 0x7fffffff, false);
 }
 
 int64_t msda_packed_attention_shaped_fwd_workspace_size(int dtype, int sequences, int q_rows, int k_rows, int heads, int kv_heads, int head_dim, int window) {
@@ -120,7 +137,8 @@ int64_t msda_packed_attention_shaped_bwd_workspace_size(int dtype, int sequences
   const msda_score_shape shape{0.0f, window, nullptr, nullptr};
   int rc;
   if ((rc = pk_bwd_shape(s)) != MSDA_OK || (rc = pk_check_shape(&shape, 1)) != MSDA_OK) return rc;
-  return pk_bwd_workspace(s, pk_window(&shape));
+  // (of a call without a shape, too)
+  return std::max(pk_kv_workspace(s, pk_window(&shape), true) + pk_q_workspace(s, pk_window(&shape)), pk_kv_workspace(s, pk_window(&shape), false));
 }
 
 int msda_packed_attention_shaped_fwd(const void* q, const void* k, const void* v, int dtype, void* out, void* out_rest, float* stats,
@@ -205,12 +223,17 @@ int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v
   p.stats = const_cast<float*>(stats);  // (the backward reads it)
   p.numbers = grad_k != nullptr || grad_v != nullptr ? row_numbers : nullptr;
   const int mod = pk_set_shape(p, shape);
-  if (grad_k != nullptr || grad_v != nullptr) p.splits = pk_parts(s, p.window);
-  if (p.splits > 1) {
-    const int64_t need = pk_bwd_workspace(s, p.window);
+  const bool keys = grad_k != nullptr || grad_v != nullptr;
+  if (keys) p.splits = pk_parts(s, p.window, mod != 0);
+  p.part = pk_part(s, mod != 0);
+  p.q_parts = mod != 0 && grad_q != nullptr ? pk_q_parts(s, p.window) : 1;
+  const int64_t kv_bytes = p.splits > 1 ? pk_kv_workspace(s, p.window, mod != 0) : 0, need = kv_bytes + (p.q_parts > 1 ? pk_q_workspace(s, p.window) : 0);
+  if (need != 0) {
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_packed_attention_bwd: the workspace must hold %lld bytes, aligned to 16", static_cast<long long>(need));
     p.part_kv = static_cast<float*>(workspace);
+    p.part_q = p.part_kv + kv_bytes / 4;
+    p.part_q_n = reinterpret_cast<int32_t*>(p.part_q + static_cast<int64_t>(p.q_parts) * q_rows * heads * head_dim);
   }
   const int q_slots = q_rows == 0 ? 0 : static_cast<int>(pk_slots(static_cast<int64_t>(q_rows) * p.group, sequences));
   const int k_slots = k_rows == 0 ? 0 : static_cast<int>(pk_slots(k_rows, sequences));

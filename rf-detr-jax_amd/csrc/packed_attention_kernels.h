@@ -61,11 +61,14 @@ struct PackParams {
   float* part_ml;            // [splits][q_rows * heads][2]: m, l
   int32_t* part_n;           // [q_rows * heads]: the row's parts
   float* part_kv;            // key side: [splits][dk, dv][k_rows * kv_heads][dim]
+  float* part_q;             // shaped scores, queries' side of the backward: [q_parts][q_rows * heads][dim]
+  int32_t* part_q_n;         // [q_rows * heads]: q_parts, or 1 where the row is outside every sequence
   int64_t st[kPkTensors][2];  // element strides (row, head) of each tensor
   int sequences, q_rows, k_rows, heads, kv_heads, group, dim, causal;
   int splits;    // at most so many workgroups share a tile's streamed rows
-  int part;      // forward: chunks of one of them, unless that makes more
+  int part;      // chunks of one of them, unless that makes more (forward; key side of shaped scores)
   int slots;     // tiles of the kernel's own side
+  int q_parts;   // shaped scores, backward: workgroups that share a tile of queries
   float scale;   // of the scores
   float scale2;  // scale log2(e)
   // shaped scores (PackShaped)
@@ -84,6 +87,7 @@ enum PackShaped { kPkRanges = 4, kPkCap = 1, kPkSlope = 2 };
 
 constexpr float kPkShare = 0.5f;
 constexpr int kPkPart = 32;  // chunks of a workgroup on the key side, unless that makes more parts than the host gave room for
+constexpr int kPkPartF32 = 8;  // shaped scores in f32, whose products take 16 times as long
 constexpr int kPkJoin = 32;   // workgroups that join a key tile's parts
 
 __device__ __align__(16) const uint32_t pk_zeros[4] = {0u, 0u, 0u, 0u};
@@ -785,10 +789,10 @@ struct PkQueries {
   int m, shift;     // keys; a row of token t stands at place t + shift, and sees the keys up to there
   int prefix;
   template <bool SPLIT>
-  __device__ PkQueries(const PackParams& p, int lane, std::bool_constant<SPLIT>) {
+  __device__ PkQueries(const PackParams& p, int lane, int block, std::bool_constant<SPLIT>) {
     // key heads fastest: with 8 of them each stays on one XCD, whose L2 then holds its keys; the last
     // tiles, which see the most keys of a causal sequence, first
-    const int b = static_cast<int>(blockIdx.x), rest = b / p.kv_heads;
+    const int b = block, rest = b / p.kv_heads;
     kv_head = b - rest * p.kv_heads;
     parts = 1;
     split = 0;
@@ -897,7 +901,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   constexpr int PF = sizeof(T) == 2 ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries<MOD> w(p, lane, std::true_type());
+  const PkQueries<MOD> w(p, lane, static_cast<int>(blockIdx.x), std::true_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* out = static_cast<T*>(p.out);
@@ -1258,11 +1262,17 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   constexpr int PF = sizeof(T) == 2 && !(MOD != 0 && DT == 128) ? 3 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;
   const PkLane<T, DT> at(lane);
-  const PkQueries<MOD> w(p, lane, std::false_type());
+  // with shaped scores several workgroups may share a tile's keys (the grid of tiles, one part behind the other)
+  const int tiles = MOD != 0 ? static_cast<int>(gridDim.x) / p.q_parts : 0, qpart = MOD != 0 ? static_cast<int>(blockIdx.x) / tiles : 0;
+  const int place = static_cast<int>(blockIdx.x) - qpart * tiles;  // every second part backwards: the longest tiles beside the shortest
+  const PkQueries<MOD> w(p, lane, (qpart & 1) != 0 ? tiles - 1 - place : place, std::false_type());
   if (w.r0 >= w.rows) return;
   const int r1 = min(w.r0 + kPkTile, w.rows);
   T* gq = static_cast<T*>(p.gq);
+  if (MOD != 0 && p.q_parts > 1 && qpart == 0)
+    for (int r = w.r0 + static_cast<int>(threadIdx.x); r < r1; r += 64 * kPkWaves) p.part_q_n[w.stat(p, r)] = w.w.seq < 0 ? 1 : p.q_parts;
   if (w.w.seq < 0) {
+    if (MOD != 0 && qpart != 0) return;
     if (gq != nullptr) pk_zero_rows<T>(w.r0, r1, p.dim, [&](int r) { return w.row(p, gq, kPkGQ, r); });
     return;
   }
@@ -1277,7 +1287,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   const int wbegin = MOD != 0 && wr0 < w.rows ? w.from(p, wr0) : 0;
   const int wlo = MOD != 0 && wr0 < w.rows ? w.from(p, min(wr0 + 31, w.rows - 1)) : 0, alo = MOD != 0 ? w.from(p, r1 - 1) : 0;
   const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = MOD != 0 && p.window < kPkChunk;
-  const int cb = w.from(p, w.r0) / kPkChunk, chunks = (end + kPkChunk - 1) / kPkChunk;
+  int cb = w.from(p, w.r0) / kPkChunk, chunks = (end + kPkChunk - 1) / kPkChunk;
+  if constexpr (MOD != 0) {
+    const int per = (max(chunks - cb, 0) + p.q_parts - 1) / p.q_parts;
+    cb += qpart * per;
+    chunks = min(chunks, cb + per);
+  }
   PkBias bias{0.0f, 0.0f};
   if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, rc, grp);
   PkRow<T, DT> q, go;
@@ -1302,7 +1317,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
     ll = p.stats[row + 1];
     // for the key side: delta; bf16: -delta and -(m + log2 l) / scale2, which its sums start from (the weight is
     // 2^(scale2 s) then; the number is rounded at its own size, 2^-24 of it)
-    if (p.numbers != nullptr && valid && grp == 0)
+    if (p.numbers != nullptr && valid && grp == 0 && qpart == 0)
       *reinterpret_cast<at_f4*>(p.numbers + row) = sizeof(T) == 2 ? at_f4{m, ll, -delta, (MOD & kPkCap) != 0 ? -(m + ll) : -(m + ll) / p.scale2} : at_f4{m, ll, delta, 0.0f};
   }
   if (gq == nullptr) return;
@@ -1460,8 +1475,33 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   }
   pk_barrier();
   unsigned char* const scratch = (wave / 2 % 4 == 0 ? X0 : wave / 2 % 4 == 1 ? Y0 : wave / 2 % 4 == 2 ? X1 : Y1) + wave % 2 * (Tile::BYTES / 2);
+  if (MOD != 0 && p.q_parts > 1) {
+    if (!valid) return;
+    float* to = p.part_q + (static_cast<int64_t>(qpart) * p.q_rows * p.heads + w.stat(p, ri)) * p.dim;
+#pragma unroll
+    for (int nd = 0; nd < DT / 32; ++nd)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int ch = 32 * nd + 8 * c + 4 * grp;
+        if (ch < p.dim) *reinterpret_cast<at_f4*>(to + ch) = at_f4{dq[nd][4 * c], dq[nd][4 * c + 1], dq[nd][4 * c + 2], dq[nd][4 * c + 3]} * factor;
+      }
+    return;
+  }
   pk_store<T, DT>(dq, factor, scratch, p.dim, lane,
                   [&](int r) { return wr0 + r < w.rows ? w.row(p, gq, kPkGQ, wr0 + r) : static_cast<T*>(nullptr); });
+}
+
+// The parts of dq of every row, in their order, four channels to a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) pk_join_q_kernel(const PackParams p) {
+  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.heads, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / (p.dim / 4);
+  if (row >= rows || p.part_q_n[row] != p.q_parts) return;  // (written already)
+  const int ch = 4 * static_cast<int>(i - row * (p.dim / 4));
+  at_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < p.q_parts; ++s) a += *reinterpret_cast<const at_f4*>(p.part_q + (s * rows + row) * p.dim + ch);
+  const int64_t tok = row / p.heads;
+  pk_put4(static_cast<T*>(p.gq) + tok * p.st[kPkGQ][0] + (row - tok * p.heads) * p.st[kPkGQ][1] + ch, a);
 }
 
 // ---- keys on their own side: dk and dv ---------------------------------------------------------
@@ -1511,7 +1551,8 @@ struct PkKeys {
       end = static_cast<int>(min(max(static_cast<int64_t>(min(b1, m)) - 1 + p.window - shift, static_cast<int64_t>(first)), static_cast<int64_t>(n)));
     }
     chunks = b0 < m ? (end - first + walk.tokens - 1) / walk.tokens : 0;
-    parts = min(max((chunks + kPkPart - 1) / kPkPart, 1), p.splits);
+    const int part = RANGES ? p.part : kPkPart;
+    parts = min(max((chunks + part - 1) / part, 1), p.splits);
   }
   template <typename T>
   __device__ T* row(const PackParams& p, T* base, int t, int j) const {
@@ -1554,7 +1595,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   // the parts of a tile are a grid of tiles apart, the last of all tiles first: of shared tiles all parts are full,
   // those of one part, down to a few rows, come last and even out
   const int tiles = static_cast<int>(gridDim.x) / p.splits, turn = static_cast<int>(blockIdx.x) / tiles;
-  const PkKeys<MOD != 0> w(p, walk, lane, static_cast<int>(blockIdx.x) - turn * tiles, p.splits - 1 - turn);
+  const int place = static_cast<int>(blockIdx.x) - turn * tiles, part = p.splits - 1 - turn;
+  const PkKeys<MOD != 0> w(p, walk, lane, MOD != 0 && (part & 1) != 0 ? tiles - 1 - place : place, part);
   if (w.b0 >= w.w.own || w.part >= w.parts) return;
   T* gk = static_cast<T*>(p.gk);
   T* gv = static_cast<T*>(p.gv);

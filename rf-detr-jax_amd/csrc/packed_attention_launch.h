@@ -29,7 +29,10 @@ int pk_fwd(const msda::PackParams& p, hipStream_t st) {
 template <typename T, int DT, int MOD>
 int pk_bwd(msda::PackParams p, int q_slots, int k_slots, hipStream_t st) {
   p.slots = q_slots;
-  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT, MOD>, static_cast<int64_t>(q_slots) * p.kv_heads, p, st, "packed attention backward (queries)");
+  const int q_parts = MOD != 0 ? p.q_parts : 1;
+  int rc = pk_launch(msda::pk_bwd_q_kernel<T, DT, MOD>, static_cast<int64_t>(q_slots) * p.kv_heads * q_parts, p, st, "packed attention backward (queries)");
+  if (rc == MSDA_OK && q_parts > 1 && p.gq != nullptr)
+    rc = pk_launch(msda::pk_join_q_kernel<T>, (static_cast<int64_t>(p.q_rows) * p.heads * (p.dim / 4) + 255) / 256, p, st, "packed attention backward (queries, join)");
   if (rc != MSDA_OK || (p.gk == nullptr && p.gv == nullptr)) return rc;
   p.slots = k_slots;
   rc = pk_launch(msda::pk_bwd_kv_kernel<T, DT, MOD>, static_cast<int64_t>(k_slots) * p.splits * p.kv_heads, p, st,

@@ -54,7 +54,8 @@ struct Library {
   decltype(&msda_packed_attention_shaped_fwd) packed_fwd;
   decltype(&msda_packed_attention_shaped_bwd) packed_bwd;
   decltype(&msda_packed_attention_shaped_fwd_workspace_size) packed_fwd_workspace_size;
-  decltype(&msda_packed_attention_shaped_bwd_workspace_size) packed_bwd_workspace_size;
+  decltype(&msda_packed_attention_bwd_workspace_size) packed_bwd_workspace_size;
+  decltype(&msda_packed_attention_shaped_bwd_workspace_size) packed_shaped_bwd_workspace_size;
   decltype(&msda_cache4_write) cache4_write;
   decltype(&msda_cache4_read) cache4_read;
   decltype(&msda_cache4_attention) cache4_attention;
@@ -89,7 +90,8 @@ void bind(const py::dict& address, const py::object& check, const py::object& pa
   get("msda_packed_attention_shaped_fwd", lib.packed_fwd);
   get("msda_packed_attention_shaped_bwd", lib.packed_bwd);
   get("msda_packed_attention_shaped_fwd_workspace_size", lib.packed_fwd_workspace_size);
-  get("msda_packed_attention_shaped_bwd_workspace_size", lib.packed_bwd_workspace_size);
+  get("msda_packed_attention_bwd_workspace_size", lib.packed_bwd_workspace_size);
+  get("msda_packed_attention_shaped_bwd_workspace_size", lib.packed_shaped_bwd_workspace_size);
   get("msda_cache4_write", lib.cache4_write);
   get("msda_cache4_read", lib.cache4_read);
   get("msda_cache4_attention", lib.cache4_attention);
@@ -592,6 +594,7 @@ struct Packed {  // one call's sizes
       : sequences(static_cast<int>(offsets.numel() - 1)), q_rows(static_cast<int>(q.size(0))), k_rows(static_cast<int>(k.size(0))),
         heads(static_cast<int>(q.size(1))), kv_heads(static_cast<int>(k.size(1))), dim(static_cast<int>(q.size(2))), causal(c),
         scale(static_cast<float>(s)), cap(static_cast<float>(cap_)), window(static_cast<int>(window_)), slopes(slopes_), prefix(prefix_) {}
+  bool shaped() const { return cap != 0.0f || window != 0 || slopes.defined() || prefix.defined(); }
   msda_score_shape shape() const;
 };
 
@@ -656,9 +659,9 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     Tensor gq = like(ctx->needs_input_grad(0), q), gk = like(ctx->needs_input_grad(1), k), gv = like(ctx->needs_input_grad(2), v), ws;
     // what the kernels hand on: other calls may read the statistics
     const Tensor numbers = like(gk.defined() || gv.defined(), stats);
-    const int64_t bytes = gk.defined() || gv.defined()
-                              ? lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, p.window)
-                              : 0;
+    int64_t bytes = 0;
+    if (p.shaped()) bytes = lib.packed_shaped_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim, p.window);
+    else if (gk.defined() || gv.defined()) bytes = lib.packed_bwd_workspace_size(code(q), p.sequences, p.q_rows, p.k_rows, p.heads, p.kv_heads, p.dim);
     check(bytes);
     if (bytes != 0) ws = workspace(bytes, q);
     int64_t st[16] = {};

@@ -125,6 +125,7 @@ class _Shape:
                 raise ValueError("prefix_lengths belong to causal attention: without causal every query sees every key")
             prefix_lengths = _int32(prefix_lengths, (sequences,), "prefix_lengths", device)
         self.prefix = prefix_lengths
+        self.any = self.cap != 0.0 or self.window != 0 or slopes is not None or prefix_lengths is not None
 
     def pointer(self):
         return ctypes.byref(_native.ScoreShape(self.cap, self.window, _ptr(self.slopes), _ptr(self.prefix)))
@@ -160,7 +161,11 @@ def _backward(q, k, v, out, rest, stats, grad_out, seq, causal, scale, shape, ne
     lib, code = _native.lib(), _DTYPES[q.dtype]
     dims = (seq.count, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
     with torch.cuda.device(q.device):
-        nbytes = lib.msda_packed_attention_shaped_bwd_workspace_size(code, *dims, shape.window) if needs[1] or needs[2] else 0
+        nbytes = 0
+        if shape.any:
+            nbytes = lib.msda_packed_attention_shaped_bwd_workspace_size(code, *dims, shape.window)
+        elif needs[1] or needs[2]:
+            nbytes = lib.msda_packed_attention_bwd_workspace_size(code, *dims)
         _native.check(min(nbytes, 0))
         ws = _native.workspace(nbytes, q.device) if nbytes else None
         numbers = torch.empty_like(stats) if needs[1] or needs[2] else None  # what the kernels hand on: other calls may read stats
