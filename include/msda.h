@@ -556,7 +556,7 @@ int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v
  * 32 channels of a row are a block with one power of two 2^e, held as e + 127; a channel is 4 bits, the first of two in
  * the lower half of their byte: a sign (8) and the code of {0, 1/2, 1, 3/2, 2, 3, 4, 6} times 2^e. Writing takes the least
  * e with every magnitude within 7 2^e, from -120 to 125, and the nearest value for each channel, the even code between
- * two. A block that holds an infinity or NaN reads as NaN (scale 255). Channels behind head_dim are zeros.
+ * two. A block that holds an infinity or NaN reads as NaN (scale 255; 253 and 254, which no block gets, too). Channels behind head_dim are zeros.
  *
  * Sequences as above: sequence i's keys are the rows from k_offsets[i] on, as many as k_lengths[i] says (NULL: all before
  * k_offsets[i + 1]), and its tokens q_offsets[i] .. q_offsets[i + 1] - 1 are the newest of them: its last token is its

@@ -53,5 +53,5 @@ def encode(x):
 def decode(codes, scales, d):
     codes = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], -1)
     value = np.array(MAGNITUDES)[codes & 7] * np.where(codes & 8, -1.0, 1.0)
-    scale = np.where(scales == BAD, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
+    scale = np.where(scales > HIGH + 127, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
     return (value.reshape(*value.shape[:-1], -1, 32) * scale[..., None]).reshape(value.shape)[..., :d]

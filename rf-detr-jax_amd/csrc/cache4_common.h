@@ -3,7 +3,7 @@
 // The numbers. 32 channels of a row share a power of two 2^e, one byte e + 127; a channel is a sign and 3 bits for
 // {0, 1/2, 1, 3/2, 2, 3, 4, 6} of it. e is the least with every magnitude within 7 2^e (6 and what rounds to it), from
 // -120 to 125; a channel goes to the nearest, to the even code between two. A block that holds an infinity or NaN reads
-// as NaN (byte 255). Every value is a bf16 number exactly, so that products on bf16 matrix instructions lose nothing.
+// as NaN (byte 255; 253 and 254, which no block gets, do too). Every value is a bf16 number exactly, so that products on bf16 matrix instructions lose nothing.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -17,7 +17,9 @@ namespace msda {
 typedef __bf16 c4_bf2 __attribute__((ext_vector_type(2)));
 typedef float c4_f2 __attribute__((ext_vector_type(2)));
 
-constexpr uint32_t kC4Bad = 255;  // the scale of a block that is not finite
+// The scale of a block that is not finite as it is written, and the largest of one that is: what lies between (in memory that
+// nothing wrote) would be values past bf16's largest, infinities, and counts as not finite.
+constexpr uint32_t kC4Bad = 255, kC4Most = 252;
 
 __device__ __forceinline__ float c4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4Params p) 
     const int64_t block = (at.head * static_cast<int64_t>(p.rows) + row) * p.blocks + at.block;
     const uint32_t scale = p.scales[at.which][block];
     c4_f32(*reinterpret_cast<const uint32_t*>(p.codes[at.which] + block * 16 + 4 * at.quarter), c4_scale(scale), v);
-    if (scale == kC4Bad) {
+    if (scale > kC4Most) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = NAN;
     }
@@ -205,8 +205,8 @@ struct C4Rows {
   }
   __device__ __forceinline__ at_bf8 bf16(int e, int grp) const { return c4_bf16(codes[e], c4_scale(scale_of(e, grp))); }
   __device__ __forceinline__ bool bad() const {
-    bool b = scale[0] == kC4Bad;
-    if constexpr (DT == 96) b = b || scale[1] == kC4Bad;
+    bool b = scale[0] > kC4Most;
+    if constexpr (DT == 96) b = b || scale[1] > kC4Most;
     return b;
   }
 };
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           at_bf8 a = kr[j].bf16(e, grp);
-          if (spoilt && kr[j].scale_of(e, grp) == kC4Bad) a[0] = static_cast<__bf16>(NAN);
+          if (spoilt && kr[j].scale_of(e, grp) > kC4Most) a[0] = static_cast<__bf16>(NAN);
 #pragma unroll
           for (int t = QT - 1; t >= 0; --t) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[e][t], s[j], 0, 0, 0);
         }
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             uint4 y = __builtin_bit_cast(uint4, x.bf16(e, grp));
-            if (spoilt && x.scale_of(e, grp) == kC4Bad) y = uint4{0u, 0u, 0u, 0u};  // its rows get it in the end
+            if (spoilt && x.scale_of(e, grp) > kC4Most) y = uint4{0u, 0u, 0u, 0u};  // its rows get it in the end
             *reinterpret_cast<uint4*>(mine + (write_at + (((grp * N + e) ^ swizzle(col)) << 4)) + 16 * j * (2 * DP)) = y;
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_
         for (int j = c * kPkChunk; j < min((c + 1) * kPkChunk, m); ++j)
 #pragma unroll
           for (int i = 0; i < MT; ++i)
-            if (vs[static_cast<int64_t>(j) * (DT / 32) + i / 2] == kC4Bad && j >= lo && j < lim) o[i] += at_f4{NAN, NAN, NAN, NAN};
+            if (vs[static_cast<int64_t>(j) * (DT / 32) + i / 2] > kC4Most && j >= lo && j < lim) o[i] += at_f4{NAN, NAN, NAN, NAN};
     }
     l = c4_sum_groups(l);
     if (grp == 0) ml[wave][col] = float2{top, l};

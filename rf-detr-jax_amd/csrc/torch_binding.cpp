@@ -760,7 +760,7 @@ struct Cache {
     const int64_t blocks = (dim + 31) / 32;
     for (const Tensor* t : {keys, key_scales, values, value_scales}) {
       const bool codes = t == keys || t == values;
-      if (t->dim() != 3 || t->scalar_type() != at::kByte || t->size(0) != keys->size(0) || t->size(1) != keys->size(1) || t->size(1) >= (int64_t{1} << 31) ||
+      if (t->dim() != 3 || t->size(0) == 0 || t->scalar_type() != at::kByte || t->size(0) != keys->size(0) || t->size(1) != keys->size(1) || t->size(1) >= (int64_t{1} << 31) ||
           t->size(2) != (codes ? 16 * blocks : blocks) || !t->is_contiguous() || t->device() != keys->device() ||
           (codes && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0))
         return false;

@@ -29,7 +29,7 @@ from .packed_attention import _DTYPES, _Shape, _int32, _ptr, _rows16, _scale, _s
 class Cache4(NamedTuple):
     """Keys and values in 4 bits. With ``B = ceil(head_dim / 32)`` blocks of a row: ``keys`` and ``values`` uint8
     ``[Hk, rows, 16 B]``, two channels to a byte, the first in its lower half (sign 8, code 0 to 7); ``key_scales`` and
-    ``value_scales`` uint8 ``[Hk, rows, B]``, the block's exponent + 127. All contiguous, on one GPU."""
+    ``value_scales`` uint8 ``[Hk, rows, B]``, the block's exponent + 127 (more than 252: not finite). All contiguous, on one GPU."""
 
     keys: torch.Tensor
     key_scales: torch.Tensor
@@ -61,6 +61,8 @@ def _check_cache(cache):
     d = cache.head_dim
     if d % 8 or not 8 <= d <= 128:
         raise ValueError(f"head_dim must be a multiple of 8 up to 128, got {d}")
+    if cache.keys.dim() != 3 or cache.kv_heads < 1:
+        raise ValueError(f"the cache's keys must be [Hk, rows, bytes] with at least one head, got {tuple(cache.keys.shape)}")
     blocks = (d + 31) // 32
     for name, width in (("keys", 16 * blocks), ("key_scales", blocks), ("values", 16 * blocks), ("value_scales", blocks)):
         t = getattr(cache, name)

@@ -128,3 +128,13 @@ def test_front_end_refusals():
         cache4_read(cache, 4, off, dtype=torch.float16)
     with pytest.raises(ValueError, match="tokens"):
         cache4_read(cache, -1, off)
+    for empty in (Cache4(*(torch.empty(0, 8, n, dtype=torch.uint8) for n in (32, 2) * 2), 40), cache._replace(keys=cache.keys[0])):
+        for call in (lambda: cache4_write(empty, x, x, off), lambda: cache4_attention(x, empty, off)):
+            with pytest.raises(ValueError, match="at least one head"):
+                call()
+
+
+def test_scales_that_no_block_gets_are_not_finite():
+    codes, scales = np.full((3, 16), 0x22, np.uint8), np.array([[252], [253], [255]], np.uint8)
+    got = C4.decode(codes, scales, 32)
+    assert (got[0] == 2.0 ** 125).all() and np.isnan(got[1:]).all()

@@ -303,6 +303,29 @@ def test_rows_before_and_behind_and_blocks_that_are_not_finite(name, dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("name", ["tokens", "chunks", "chunks96", "mixed"])
+def test_memory_that_nothing_wrote(name, dtype):
+    """Any bytes where no key is seen, scales of no finite block (253 and more) among them."""
+    lengths, fill, room, h, hk, d = SHAPES[name]
+    off, koff = np.cumsum([0, *lengths]), np.arange(len(fill) + 1) * room
+    cache = _random_cache(22, koff[-1], hk, d)
+    (q,) = _normal(23, dtype, (off[-1], h, d))
+    g = torch.Generator().manual_seed(24)
+    kw, _ = _options(window=100)
+    args = (_int(off), _int(koff), _int(fill))
+    want = cache4_attention(q, cache, *args, **kw)
+    for scale in (0, 253, 254, None):
+        other = Cache4(*(t.clone() for t in cache[:4]), d)
+        for (q0, n, k0, m) in PA.sequences(off, koff, fill):
+            for rows in (slice(k0 + m, k0 + room), slice(k0, k0 + max(m - max(n, 1) - 99, 0))):
+                for t in other[:4]:
+                    t[:, rows] = torch.randint(0, 256, t[:, rows].shape, generator=g, dtype=torch.uint8).to(_dev())
+                if scale is not None:
+                    other.key_scales[:, rows] = other.value_scales[:, rows] = scale
+        assert torch.equal(cache4_attention(q, other, *args, **kw), want), scale
+
+
+@TYPES
 def test_large_scores(dtype):
     """Scores that rise and fall by hundreds along the keys, in both kernels."""
     d, m = 64, 900
