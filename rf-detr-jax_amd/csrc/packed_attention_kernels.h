@@ -701,7 +701,7 @@ struct PkCachePair {
       for (int e = 0; e < N; ++e) {
         uint32_t scale = s[i][0];
         if constexpr (DT == 96) scale = e == 0 || (e == 1 && part != 1) ? s[i][0] : s[i][1];
-        const bool bad = scale == kC4Bad, none = row >= end;
+        const bool bad = scale > kC4Most, none = row >= end;
         uint4 y[2];
         if constexpr (sizeof(T) == 2) {
           y[0] = __builtin_bit_cast(uint4, c4_bf16(c[i][e], c4_scale(scale)));
@@ -1152,7 +1152,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           const int ch = 32 * nd + 8 * (i >> 2) + 4 * grp + (i & 3);
           float x = 0.0f;
           if (ch < p.dim) {
-            if constexpr (CACHE4) x = p.v_scales[(head_rows + j) * (DT / 32) + nd] == kC4Bad ? NAN : 0.0f;
+            if constexpr (CACHE4) x = p.v_scales[(head_rows + j) * (DT / 32) + nd] > kC4Most ? NAN : 0.0f;
             else if constexpr (sizeof(T) == 2) x = bf16_to_f32(vp[j * p.st[kPkV][0] + ch]);
             else x = vp[j * p.st[kPkV][0] + ch];
           }
@@ -1286,7 +1286,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   const int lo = MOD != 0 && valid ? w.from(p, ri) : 0, span = max(lim - lo, 0);  // as in the forward
   const int wbegin = MOD != 0 && wr0 < w.rows ? w.from(p, wr0) : 0;
   const int wlo = MOD != 0 && wr0 < w.rows ? w.from(p, min(wr0 + 31, w.rows - 1)) : 0, alo = MOD != 0 ? w.from(p, r1 - 1) : 0;
-  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = MOD != 0 && p.window < kPkChunk;
+  const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk;
+  // Few channels: the keys that a sharp row weighs most share a large part along q, which cancels in the sum of ds k, as
+  // ds adds up to 0, while the roundings of ds do not. One rounding of ds left grad_q 1.86, 1.64, 1.54, 1.51, 1.49 and 1.49 times as
+  // far off as the exact one rounded at 8, 16, 32, 40, 64 and 80 channels (1.47 at 96 and 128), with scores of four standard
+  // deviations. So ds keeps its rest there, as in narrow windows: 1.02 to 1.14, for 5 % of a training step. Scores without a
+  // cap are smaller, or would have one (one standard deviation, 64 channels: 1.34).
+  const bool narrow = MOD != 0 && (p.window < kPkChunk || p.dim <= ((MOD & kPkCap) != 0 ? 80 : 48));
   int cb = w.from(p, w.r0) / kPkChunk, chunks = (end + kPkChunk - 1) / kPkChunk;
   if constexpr (MOD != 0) {
     const int per = (max(chunks - cb, 0) + p.q_parts - 1) / p.q_parts;

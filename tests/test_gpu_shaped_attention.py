@@ -377,3 +377,22 @@ def test_layouts_and_one_gradient_at_a_time(dtype):
         assert [x is not None for x in got] == needs and torch.equal(got[i], want[i + 1])
     ones = torch.ones((), dtype=dtype, device=_dev()).expand(131, h, d)
     _compare(*parts, ones, _run(*parts, ones, _int(off), **kw), PA.sequences(off), shape)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [8, 16, 32, 40, 64, 80])
+def test_gradients_of_few_channels(dim, causal):
+    """bf16, scores of four standard deviations: the keys that a row weighs most lie along its query, and what they share
+    cancels in the sum of ds k. One rounding of each ds would not cancel: it alone is the result's own rounding again (their
+    sum the square root of two of it), times the root of (a^2 + D) / D, a the shared part in standard deviations. So grad_q
+    has to be nearer than the square root of two: its own rounding, and delta's error, smaller than that."""
+    n, h, hk = 900, 4, 2
+    q, k, v, g = _normal(31 + dim, torch.float32, (n, h, dim), (n, hk, dim), (n, hk, dim), (n, h, dim))
+    q, k, v, g = (x.bfloat16() for x in (4.0 * q, k, v, g))
+    kw, shape = _options(causal=causal, cap=50.0)
+    off = np.array([0, n])
+    got = _run(q, k, v, g, _int(off), causal=causal, **kw)
+    arrays = [_np(x) for x in (q, k, v, g)]
+    want = SA.attention_vjp(*arrays, PA.sequences(off, off, None), shape)[0]
+    rounded = np.linalg.norm(_np(torch.from_numpy(want).bfloat16()) - want)
+    assert np.linalg.norm(_np(got[1]) - want) < 2 ** 0.5 * rounded
