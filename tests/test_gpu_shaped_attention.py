@@ -396,3 +396,24 @@ def test_gradients_of_few_channels(dim, causal):
     want = SA.attention_vjp(*arrays, PA.sequences(off, off, None), shape)[0]
     rounded = np.linalg.norm(_np(torch.from_numpy(want).bfloat16()) - want)
     assert np.linalg.norm(_np(got[1]) - want) < 2 ** 0.5 * rounded
+
+
+@TYPES
+@pytest.mark.parametrize("kind", ["all", "cap", "open", "prefix"])
+def test_tiles_that_workgroups_share(kind, dtype):
+    """Few tiles of queries over many keys, rows in front of the first sequence and behind the last, a sequence without keys
+    and one that sees its first keys alone; twice, with the same bits."""
+    lengths, keys, h, hk, d = [300, 0, 45, 131], [1900, 7, 0, 1400], 4, 2, 64
+    off, koff = np.cumsum([0, *lengths]) + 3, np.cumsum([0, *keys]) + 2
+    q, k, v, g = _normal(41, dtype, (off[-1] + 5, h, d), (koff[-1] + 4, hk, d), (koff[-1] + 4, hk, d), (off[-1] + 5, h, d))
+    for x, ends in ((q, off), (g, off), (k, koff), (v, koff)):
+        x[:ends[0]] = x[ends[-1]:] = float("nan")
+    kw, shape = _options(**KINDS[kind](h, keys))
+    causal = kind != "open"
+    got = _run(q, k, v, g, _int(off), _int(koff), causal=causal, **kw)
+    for x, ends in zip(got, (off, off, koff, koff)):
+        assert not x[:ends[0]].any() and not x[ends[-1]:].any()
+    for a, b in zip(got, _run(q, k, v, g, _int(off), _int(koff), causal=causal, **kw)):
+        assert torch.equal(a, b)
+    inner, outer = slice(off[0], off[-1]), slice(koff[0], koff[-1])
+    _compare(q[inner], k[outer], v[outer], g[inner], [x[s] for x, s in zip(got, (inner, inner, outer, outer))], PA.sequences(off - 3, koff - 2), shape)

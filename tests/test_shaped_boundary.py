@@ -62,6 +62,11 @@ def test_workspaces():
     assert lib.msda_packed_attention_shaped_bwd_workspace_size(*train, 128) == 0
     for name in ("fwd", "bwd"):
         assert getattr(lib, f"msda_packed_attention_shaped_{name}_workspace_size")(*train, -1) == INVALID
+    # few tiles of queries: parts of dq, of 4 chunks of keys each at least, and each row's number of them
+    few = (1, 1, 256, 256 * 16, 2, 1, 64)
+    parts = lib.msda_packed_attention_shaped_bwd_workspace_size(*few, 0) - lib.msda_packed_attention_bwd_workspace_size(*few)
+    assert parts == (8 * 64 + 1) * 256 * 2 * 4
+    assert lib.msda_packed_attention_shaped_bwd_workspace_size(1, 1, 256, 448, 2, 1, 64, 0) == lib.msda_packed_attention_bwd_workspace_size(1, 1, 256, 448, 2, 1, 64)
 
 
 CPU = torch.device("cpu")
