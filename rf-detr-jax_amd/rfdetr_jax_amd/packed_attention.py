@@ -92,6 +92,11 @@ class _Sequences:
         self.lengths = None if key_lengths is None else _int32(key_lengths, (self.count,), "key_lengths", q.device)
 
 
+def _no_gradient(slopes):
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes get no gradient: pass them detached")
+
+
 def _scale(scale, head_dim):
     scale = head_dim ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -64 <= scale <= 2.0 ** 64:
@@ -116,8 +121,7 @@ class _Shape:
                 raise ValueError(f"slopes must be [{heads}], got {tuple(slopes.shape)}")
             if slopes.device != device:
                 raise ValueError(f"slopes are on {slopes.device}, the queries on {device}")
-            if slopes.requires_grad and torch.is_grad_enabled():
-                raise ValueError("slopes get no gradient: pass them detached")
+            _no_gradient(slopes)
             slopes = slopes.detach().contiguous()
         self.slopes = slopes
         if prefix_lengths is not None:
@@ -253,7 +257,7 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
         scale: of the scores, from ``2 ** -64`` to ``2 ** 64``; ``D ** -0.5`` when None.
         cap: a score ``s = scale q.k`` becomes ``cap tanh(s / cap)``; from ``2 ** -32`` to ``2 ** 32``.
         slopes: float32 ``[H]`` on the same GPU: behind the cap, head ``h``'s scores fall by ``slopes[h]`` for each place
-            between query and key, ``|t + m - n - j|``. Finite; they get no gradient.
+            between query and key, ``|t + m - n - j|``. Finite; they get no gradient, and ones that need one are refused.
         window: keys at this distance and farther are not seen, on either side (1: a query's own place alone). What lies
             outside costs nothing.
         prefix_lengths: int32 ``[N]``, with ``causal``: the first so many keys of a sequence are seen by all its queries,
@@ -281,4 +285,5 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
     out = _native.binding().packed_attention(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale, cap, slopes, window, prefix_lengths)
     if out is not None:
         return out
+    _no_gradient(slopes)  # here: inside an autograd function's forward no gradients are recorded
     return _PackedAttention.apply(q, k, v, offsets, key_offsets, key_lengths, bool(causal), scale, cap, slopes, window, prefix_lengths)
