@@ -272,11 +272,15 @@ __device__ __forceinline__ void pk_bend(const PackParams& p, at_f16& s) {
   }
 }
 
-// One row's bias: of the key that lies `ahead` of the lane's first key of a block.
+// One row's bias.
 struct PkBias {
   float slope;  // -slope log2(e)
-  float first;  // the first key's number less the row's place
-  __device__ __forceinline__ float add(float x, int ahead) const { return fmaf(slope, fabsf(first + static_cast<float>(ahead)), x); }
+  int first;    // the lane's first key of a chunk less the row's place
+  // How far the lane's first key of the block at key k lies ahead of the row: subtracted as integers, because from 2^24 on
+  // a float does not hold every place.
+  __device__ __forceinline__ float from(int k) const { return static_cast<float>(first + k); }
+  // of the key that lies `ahead` of that one
+  __device__ __forceinline__ float add(float x, float at, int ahead) const { return fmaf(slope, fabsf(at + static_cast<float>(ahead)), x); }
 };
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -850,7 +854,7 @@ struct PkQueries {
   __device__ int from(const PackParams& p, int r) const { return MOD != 0 ? pk_lo(p, r / p.group + shift) : 0; }
   __device__ PkBias bias(const PackParams& p, int r, int grp) const {
     const int tok = r / p.group;
-    return PkBias{p.slopes[kv_head * p.group + r - tok * p.group] * -1.44269504f, static_cast<float>(4 * grp - (tok + shift))};
+    return PkBias{p.slopes[kv_head * p.group + r - tok * p.group] * -1.44269504f, 4 * grp - (tok + shift)};
   }
   template <typename T>
   __device__ T* row(const PackParams& p, T* base, int t, int r) const {
@@ -927,7 +931,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
   const int wlo = MOD != 0 && wr0 < w.rows ? w.from(p, min(wr0 + 31, w.rows - 1)) : 0, alo = MOD != 0 ? w.from(p, r1 - 1) : 0;
   const bool few = wr0 < w.rows && w.seen(p, wr0) < kPkChunk, narrow = w.rows <= 32 || (MOD != 0 && p.window < kPkChunk);
   const int per = (chunks + parts - 1) / parts, c0 = cb + w.split * per, c1 = min(cb + chunks, c0 + per);
-  PkBias bias{0.0f, 0.0f};
+  PkBias bias{0.0f, 0};
   if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, min(ri, w.rows - 1), grp);
   PkRow<T, DT> q;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, min(ri, w.rows - 1)), valid, p.dim, grp);
@@ -989,13 +993,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
               bm = fmaxf(bm, x[i0 + i]);
             });
           } else {
-            float to = -m;
-            PkBias b = bias;
-            if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
+            float to = -m, away = 0.0f;
+            if constexpr ((MOD & kPkSlope) != 0) away = bias.from(k);
             pk_for<i1 - i0>([&](auto j) {
               constexpr int i = i0 + j;
               x[i] = fmaf(x[i], (MOD & kPkCap) != 0 ? p.cap2 : p.scale2, to);
-              if constexpr ((MOD & kPkSlope) != 0) x[i] = b.add(x[i], 8 * (i >> 2) + (i & 3));
+              if constexpr ((MOD & kPkSlope) != 0) x[i] = bias.add(x[i], away, 8 * (i >> 2) + (i & 3));
             });
             if (k + 32 > wfull || k < wlo)
               pk_for<i1 - i0>([&](auto j) {
@@ -1077,15 +1080,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           pk_mask(s1, k0 + 32, lim, grp);
         }
       } else {
-        PkBias b = bias;
-        if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k0);
+        float away = 0.0f;
+        if constexpr ((MOD & kPkSlope) != 0) away = bias.from(k0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s0[i] = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s0[i]) * p.cap2 : s0[i] * p.scale2;
           s1[i] = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s1[i]) * p.cap2 : s1[i] * p.scale2;
           if constexpr ((MOD & kPkSlope) != 0) {
-            s0[i] = b.add(s0[i], 8 * (i >> 2) + (i & 3));
-            s1[i] = b.add(s1[i], 32 + 8 * (i >> 2) + (i & 3));
+            s0[i] = bias.add(s0[i], away, 8 * (i >> 2) + (i & 3));
+            s1[i] = bias.add(s1[i], away, 32 + 8 * (i >> 2) + (i & 3));
           }
         }
         if (k0 + kPkChunk > wfull || k0 < wlo) {
@@ -1299,7 +1302,7 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
     cb += qpart * per;
     chunks = min(chunks, cb + per);
   }
-  PkBias bias{0.0f, 0.0f};
+  PkBias bias{0.0f, 0};
   if constexpr ((MOD & kPkSlope) != 0) bias = w.bias(p, rc, grp);
   PkRow<T, DT> q, go;
   q.load(w.row(p, static_cast<const T*>(p.q), kPkQ, rc), valid, p.dim, grp);
@@ -1382,12 +1385,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
           pk_beside<KS, t>([&](int i) { s[i] = at_exp2(fmaf(s[i], p.scale2, -m)); });
         } else {
           if constexpr ((MOD & kPkCap) != 0 && t == 1) pk_bend<T>(p, s);
-          PkBias b = bias;
-          if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k);
+          float away = 0.0f;
+          if constexpr ((MOD & kPkSlope) != 0) away = bias.from(k);
           pk_beside<KS, t>([&](int i) {
             const float bent = s[i];
             float x = fmaf(bent, (MOD & kPkCap) != 0 ? p.cap2 : p.scale2, -m);
-            if constexpr ((MOD & kPkSlope) != 0) x = b.add(x, 8 * (i >> 2) + (i & 3));
+            if constexpr ((MOD & kPkSlope) != 0) x = bias.add(x, away, 8 * (i >> 2) + (i & 3));
             s[i] = at_exp2(x);
             if constexpr ((MOD & kPkCap) != 0) s[i] *= fmaf(-bent, bent, 1.0f);
           });
@@ -1452,13 +1455,13 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
             for (int i = 0; i < 16; ++i) s[i] = k0 + h + 8 * (i >> 2) + 4 * grp + (i & 3) < lim ? s[i] : 0.0f;
           }
         } else {
-          PkBias b = bias;
-          if constexpr ((MOD & kPkSlope) != 0) b.first += static_cast<float>(k0 + h);
+          float away = 0.0f;
+          if constexpr ((MOD & kPkSlope) != 0) away = bias.from(k0 + h);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float bent = (MOD & kPkCap) != 0 ? pk_bent<T>(p, s[i]) : 0.0f;
             float x = (MOD & kPkCap) != 0 ? bent * p.cap2 : s[i] * p.scale2;
-            if constexpr ((MOD & kPkSlope) != 0) x = b.add(x, 8 * (i >> 2) + (i & 3));
+            if constexpr ((MOD & kPkSlope) != 0) x = bias.add(x, away, 8 * (i >> 2) + (i & 3));
             s[i] = at_exp2((x - m) - ll) * (dp[i] - delta);
             if constexpr ((MOD & kPkCap) != 0) s[i] *= fmaf(-bent, bent, 1.0f);
           }

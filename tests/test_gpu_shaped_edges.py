@@ -1,0 +1,81 @@
+"""Packed attention with shaped scores on an MI355X: learned slopes, places past 2^24, parts of a call that another part
+outweighs. Tolerances are the oracle's ``bounds``."""
+
+from __future__ import annotations
+
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import packed_attention_ref as PA
+from oracle import shaped_attention_ref as SA
+from rfdetr_jax_amd import _native, packed_attention
+
+pytestmark = pytest.mark.gpu
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    return torch.device("cuda:0")
+
+
+def _int(x):
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device=_dev())
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _normal(seed, dtype, *shapes):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(dtype).to(_dev()) for s in shapes]
+
+
+def _within(got, want, bound, what):
+    got = _np(got)
+    assert got.shape == want.shape and np.isfinite(got).all(), f"{what}: not finite"
+    over = np.abs(got - want) - bound
+    at = np.unravel_index(np.argmax(over), over.shape)
+    assert over[at] <= 0, f"{what}: off by {abs(got[at] - want[at]):.3e} at {at}, {bound[at]:.3e} allowed"
+
+
+@pytest.mark.parametrize("path", ["binding", "python"])
+def test_learned_slopes_are_refused(path, monkeypatch):
+    q, k, v = _normal(1, torch.bfloat16, (9, 4, 64), (9, 2, 64), (9, 2, 64))
+    slopes = torch.nn.Parameter(torch.full((4,), 0.5, device=_dev()))
+    if path == "python":
+        monkeypatch.setattr(_native, "binding", lambda: _native._NoBinding)
+    want = packed_attention(q, k, v, _int([0, 9]), slopes=slopes.detach())
+    for x in (q, q.detach().requires_grad_(True)):
+        with pytest.raises(ValueError, match="slopes get no gradient"):
+            packed_attention(x, k, v, _int([0, 9]), slopes=slopes)
+        with torch.no_grad():
+            assert torch.equal(packed_attention(x, k, v, _int([0, 9]), slopes=slopes), want)
+
+
+@TYPES
+@pytest.mark.parametrize("dim", [8, 40])
+def test_distances_past_2_to_the_24(dim, dtype):
+    """The newest queries of a sequence of more than 2^24 keys, inside a window: their distances are small whole numbers,
+    and their place is one that a float does not hold. What lies before the window holds NaN and is not seen."""
+    m, n, h, window, tail = (1 << 24) + 301, 5, 2, 70, 200
+    sys.stderr.write(f"[gpu] distances past 2^24, {dim} channels {dtype}\n")
+    q, kt, vt, g = _normal(2, dtype, (n, h, dim), (tail, 1, dim), (tail, 1, dim), (n, h, dim))
+    k, v = (torch.cat([torch.full((m - tail, 1, dim), float("nan"), dtype=dtype, device=_dev()), x]).requires_grad_(True) for x in (kt, vt))
+    slopes = torch.tensor([1.0, 0.37], device=_dev())
+    q.requires_grad_(True)
+    for kw in (dict(), dict(cap=3.0), dict(cap=3.0, causal=False), dict(causal=False)):
+        out = packed_attention(q, k, v, _int([0, n]), _int([0, m]), slopes=slopes, window=window, **kw)
+        grads = torch.autograd.grad(out, (q, k, v), g)
+        shape = SA.Shape(kw.get("causal", True), None, kw.get("cap"), _np(slopes), window)
+        arrays, seqs = [_np(x) for x in (q, kt, vt, g)], PA.sequences([0, n], [0, tail])
+        want = [SA.attention(*arrays[:3], seqs, shape), *SA.attention_vjp(*arrays, seqs, shape)]
+        got = [out, grads[0], grads[1][-tail:], grads[2][-tail:]]
+        for name, x, w, b in zip(("out", "grad_q", "grad_k", "grad_v"), got, want, SA.bounds(*arrays, seqs, HALF_STEP[dtype], shape)):
+            _within(x, w, b, f"{name} {kw}")
+        assert not grads[1][:-tail].any() and not grads[2][:-tail].any()
