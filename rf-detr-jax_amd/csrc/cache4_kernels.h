@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_
     }
     float slope = 0.0f;
     if (SHAPED && p.slopes != nullptr) slope = p.slopes[head] * -1.44269504f;
-    const float place = static_cast<float>(tok + shift);
+    const int place = tok + shift;
     float top = 0.0f, l = 0.0f;  // the running reference score; the sum over the lane's keys
     bool fresh = true, sick = false;
     at_f4 o[MT];  // channels 16 i + 4 grp .. of the lane's row
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) cache4_attention_
           for (int i = 0; i < 4; ++i) s[j][i] = fmaf(s[j][i], p.scale2, -top);
       }
       if (SHAPED && p.slopes != nullptr) {
-        const float ahead = static_cast<float>(k0 + 4 * grp) - place;
+        const float ahead = static_cast<float>(k0 + 4 * grp - place);  // (as integers: places from 2^24 on are not all floats)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll

@@ -1,0 +1,78 @@
+"""Attention over a cache in 4 bits on an MI355X: places past 2^24, blocks that are not finite wherever the parts of a
+call fall. Tolerances are those of shaped_attention_ref's ``bounds``."""
+
+from __future__ import annotations
+
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache4_ref as C4
+from oracle import shaped_attention_ref as SA
+from rfdetr_jax_amd import Cache4, cache4_attention
+
+pytestmark = pytest.mark.gpu
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a visible MI355X"
+    return torch.device("cuda:0")
+
+
+def _int(x):
+    return torch.tensor([int(i) for i in x], dtype=torch.int32, device=_dev())
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _normal(seed, dtype, *shapes):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(dtype).to(_dev()) for s in shapes]
+
+
+def _random_cache(seed, rows, hk, d):
+    r = np.random.default_rng(seed)
+    blocks = (d + 31) // 32
+    out = []
+    for _ in range(2):
+        codes = r.integers(0, 16, (hk, rows, 32 * blocks)).astype(np.uint8)
+        codes[..., d:] = 0
+        out += [codes[..., 0::2] | codes[..., 1::2] << 4, (126 + r.integers(-2, 2, (hk, rows, blocks))).astype(np.uint8)]
+    return Cache4(*(torch.from_numpy(x).to(_dev()) for x in out), d)
+
+
+def _held(cache):
+    b = [t.cpu().numpy() for t in cache[:4]]
+    return [C4.decode(b[i], b[i + 1], cache.head_dim).transpose(1, 0, 2) for i in (0, 2)]
+
+
+def _check(out, q, cache, seqs, shape):
+    arrays, u = [_np(q), *_held(cache)], HALF_STEP[q.dtype]
+    want = SA.attention(*arrays, seqs, shape)
+    bound = SA.bounds(*arrays, np.zeros(arrays[0].shape), seqs, u, shape)[0]
+    got = _np(out)
+    assert np.isfinite(got).all()
+    over = np.abs(got - want) - bound
+    at = np.unravel_index(np.argmax(over), over.shape)
+    assert over[at] <= 0, f"off by {abs(got[at] - want[at]):.3e} at {at}, {bound[at]:.3e} allowed"
+
+
+@TYPES
+@pytest.mark.parametrize("n", [1, 3, 50], ids=["token", "tokens", "chunk"])  # 50: rows in tiles
+def test_distances_past_2_to_the_24(n, dtype):
+    """The newest queries of a sequence of more than 2^24 keys, inside a window; unseen blocks are not finite."""
+    m, h, d, window, tail = (1 << 24) + 301, 2, 40, 70, 256
+    sys.stderr.write(f"[gpu] cache in 4 bits, distances past 2^24, {n} tokens {dtype}\n")
+    small = _random_cache(1, tail, 1, d)
+    cache = Cache4(*(torch.cat([torch.full((1, m - tail, t.shape[2]), 255, dtype=torch.uint8, device=_dev()), t], 1) for t in small[:4]), d)
+    (q,) = _normal(2, dtype, (n, h, d))
+    slopes = torch.tensor([1.0, 0.37], device=_dev())
+    for kw in (dict(), dict(cap=3.0), dict(causal=False)):
+        out = cache4_attention(q, cache, _int([0, n]), _int([0, m]), slopes=slopes, window=window, **kw)
+        _check(out, q, small, [(0, n, 0, tail)], SA.Shape(kw.get("causal", True), None, kw.get("cap"), _np(slopes), window))
