@@ -1223,7 +1223,8 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
   for (int x = LPR / 2; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x, LPR));
 #pragma unroll
   for (int i = 0; i < kPkMostParts / LPR; ++i) {
-    ml[i].x = ml[i].y != 0.0f ? at_exp2(ml[i].x - m) : 0.0f;  // the part's weight
+    // the part's weight; -1: it saw no key
+    ml[i].x = ml[i].y != 0.0f ? at_exp2(ml[i].x - m) : -1.0f;
     l += ml[i].y * ml[i].x;
   }
 #pragma unroll
@@ -1240,7 +1241,12 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
 #pragma unroll 4
       for (int s = LPR * i; s < min(parts, LPR * (i + 1)); ++s) {
         const float w = __shfl(ml[i].x, s - LPR * i, LPR);
-        if (mine && w != 0.0f) a += *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch) * w;
+        if (!mine || w < 0.0f) continue;
+        const at_f4 x = *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch);
+        if (w != 0.0f) a += x * w;
+        else  // outweighed by 2^126 or more: what is no finite number stays one, however a call is split
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[j] += x[j] - x[j] != 0.0f ? x[j] : 0.0f;
       }
     if (!mine) continue;
     a *= inv;

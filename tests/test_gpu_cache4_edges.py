@@ -76,3 +76,23 @@ def test_distances_past_2_to_the_24(n, dtype):
     for kw in (dict(), dict(cap=3.0), dict(causal=False)):
         out = cache4_attention(q, cache, _int([0, n]), _int([0, m]), slopes=slopes, window=window, **kw)
         _check(out, q, small, [(0, n, 0, tail)], SA.Shape(kw.get("causal", True), None, kw.get("cap"), _np(slopes), window))
+
+
+@TYPES
+@pytest.mark.parametrize("n", [1, 3, 50], ids=["token", "tokens", "chunk"])
+def test_a_bad_value_of_a_part_that_weighs_nothing(n, dtype):
+    """Slopes so steep that the first part of the keys weighs 0 beside the last: a block of its values that is not finite
+    makes the rows that see it NaN all the same, in its channels alone."""
+    m, h, hk, d = 5000, 4, 2, 64
+    cache = _random_cache(3, m, hk, d)
+    (q,) = _normal(4, dtype, (n, h, d))
+    args = (_int([0, n]), _int([0, m]))
+    slopes = torch.full((h,), 0.5, device=_dev())
+    want = cache4_attention(q, cache, *args, slopes=slopes)
+    _check(want, q, cache, [(0, n, 0, m)], SA.Shape(slopes=_np(slopes)))
+    for key in (10, 2600):
+        bad = Cache4(*(t.clone() for t in cache[:4]), d)
+        bad.value_scales[1, key, 1] = 255
+        got = cache4_attention(q, bad, *args, slopes=slopes)
+        assert torch.isnan(got[:, 2:, 32:]).all()
+        assert torch.equal(got[:, 2:, :32], want[:, 2:, :32]) and torch.equal(got[:, :2], want[:, :2])

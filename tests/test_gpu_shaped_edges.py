@@ -79,3 +79,22 @@ def test_distances_past_2_to_the_24(dim, dtype):
         for name, x, w, b in zip(("out", "grad_q", "grad_k", "grad_v"), got, want, SA.bounds(*arrays, seqs, HALF_STEP[dtype], shape)):
             _within(x, w, b, f"{name} {kw}")
         assert not grads[1][:-tail].any() and not grads[2][:-tail].any()
+
+
+@TYPES
+@pytest.mark.parametrize("n", [1, 20], ids=["token", "chunk"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_value_that_is_not_finite_in_a_part_that_weighs_nothing(value, n, dtype):
+    """Slopes so steep that the first keys weigh 0 beside the last: a value of theirs that is not finite shows in the rows
+    that see it, whichever workgroup took it, and in its channel alone."""
+    m, h, hk, d = 5000, 4, 2, 64
+    q, k, v = _normal(3, dtype, (n, h, d), (m, hk, d), (m, hk, d))
+    slopes = torch.full((h,), 0.5, device=_dev())
+    want = packed_attention(q, k, v, _int([0, n]), _int([0, m]), slopes=slopes)
+    for key in (10, 2600):
+        odd = v.clone()
+        odd[key, 1, 33] = value
+        got = packed_attention(q, k, odd, _int([0, n]), _int([0, m]), slopes=slopes)
+        assert not torch.isfinite(got[:, 2:, 33]).any()
+        rest = [c for c in range(d) if c != 33]
+        assert torch.equal(got[:, 2:, rest], want[:, 2:, rest]) and torch.equal(got[:, :2], want[:, :2])
