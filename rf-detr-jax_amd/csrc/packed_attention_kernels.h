@@ -1119,6 +1119,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     }
     next.finish();
   };
+  if constexpr (CACHE4 && Tile::DP != DT) {
+    // Channels past DT, which no row of the cache has and pk_settle searches: zeros once. (Left as they were, a NaN there from
+    // an earlier kernel sent every row through its keys again at the end: 200 tokens, 96 channels, a window of 4,000, 31 us or 1,350.)
+    constexpr int C = DT / Tile::E, none = Tile::CPR - C;
+    for (int i = threadIdx.x; i < kPkChunk * none; i += 64 * kPkWaves) {
+      const int r = i / none, at = r * Tile::ROW + (((C + i - r * none) ^ Tile::swizzle(r)) << 4);
+      *reinterpret_cast<uint4*>(Y0 + at) = *reinterpret_cast<uint4*>(Y1 + at) = uint4{0u, 0u, 0u, 0u};
+    }
+  }
   if (c0 < c1) {
     auto head = tile(X0, Y0, c0);
     head.all();
