@@ -18,10 +18,15 @@ using msda_host::fail;
 // Workgroups of the backward, each with one row of partial sums: four to a CU, as many as fit, where there are the tokens.
 constexpr int64_t kMostGroups = 1024;
 
-// Tokens of a step of a workgroup: few enough for four workgroups a CU; at most 8 (the angles of 8 tokens keep 256 threads
-// busy for one or two steps), in the backward 16, so that 16,000 tokens are one step.
+// Tokens of a step of a workgroup, which forms their angles together: few enough for four workgroups a CU and at most 8 in the
+// forward (the angles of 8 tokens keep 256 threads busy for one or two steps), at most 16 in the backward, whose workgroups
+// take several steps where that leaves tokens over: then smaller ones, so that all workgroups have about as many tokens (40
+// heads of 128 channels, bf16, the weights' sums included: 16,384 tokens 123 us, 16,400 139 and 33,000 241; in steps of 16,
+// a few workgroups with one more than the others, 171 and 274).
 int tokens_of(int64_t tokens, bool backward) {
-  return static_cast<int>(std::max<int64_t>(1, backward ? std::min<int64_t>(16, (tokens + kMostGroups - 1) / kMostGroups) : std::min<int64_t>(8, tokens / 1024)));
+  if (!backward) return static_cast<int>(std::clamp<int64_t>(tokens / 1024, 1, 8));
+  const int64_t steps = std::max<int64_t>(1, (tokens + 16 * kMostGroups - 1) / (16 * kMostGroups)), all = steps * kMostGroups;
+  return static_cast<int>(std::max<int64_t>(1, (tokens + all - 1) / all));
 }
 
 int64_t groups_of(int64_t tokens, bool backward) {
