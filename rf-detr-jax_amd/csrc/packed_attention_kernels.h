@@ -1308,8 +1308,9 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   // Few channels: the keys that a sharp row weighs most share a large part along q, which cancels in the sum of ds k, as
   // ds adds up to 0, while the roundings of ds do not. One rounding of ds left grad_q 1.86, 1.64, 1.54, 1.51, 1.49 and 1.49 times as
   // far off as the exact one rounded at 8, 16, 32, 40, 64 and 80 channels (1.47 at 96 and 128), with scores of four standard
-  // deviations. So ds keeps its rest there, as in narrow windows: 1.02 to 1.14, for 5 % of a training step. Scores without a
-  // cap are smaller, or would have one (one standard deviation, 64 channels: 1.34).
+  // deviations. So ds keeps its rest there, as in narrow windows: 1.02 to 1.14, for 5 % of a training step. Of scores
+  // without a cap, which are smaller or would have one, from 56 channels on it does not (64 channels: one standard deviation
+  // 1.34, four 1.49). What is left is the root of 1 + (a^2 + D) / D at most, a = 4 deviations of the keys along q.
   const bool narrow = MOD != 0 && (p.window < kPkChunk || p.dim <= ((MOD & kPkCap) != 0 ? 80 : 48));
   int cb = w.from(p, w.r0) / kPkChunk, chunks = (end + kPkChunk - 1) / kPkChunk;
   if constexpr (MOD != 0) {

@@ -266,10 +266,12 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
     Documents that must not see each other are sequences of their own.
 
     Sums, softmax and statistics are float32. Of bfloat16 inputs the softmax weights and their gradients are rounded to
-    bfloat16 for the matrix products: results lie 1.2 to 1.5 times as far from the exact ones as these rounded;
-    new tokens (a sequence's tokens times ``H / Hk`` up to 32) keep their weights in two bfloat16 numbers. Float32
-    inputs are float32 throughout. Calls whose work does not fill the GPU evenly take a workspace of partial sums, in
-    float32 prompts up to some hundred MB (``msda_packed_attention_fwd_workspace_size``).
+    bfloat16 for the matrix products: results lie 1.2 to 1.5 times as far from the exact ones as these rounded. Farther:
+    gradients of k where a few tokens see a key, whose errors do not average out (4 to 31 tokens up to 1.8 times, two tokens
+    2.4), and, without the options behind ``scale``, gradients of q and k of scores of several standard deviations (four: up
+    to 1.9 times, of 8 channels 2.5). New tokens (a sequence's tokens times ``H / Hk`` up to 32) keep their weights in two
+    bfloat16 numbers. Float32 inputs are float32 throughout. Calls whose work does not fill the GPU evenly take a workspace
+    of partial sums, in float32 prompts up to some hundred MB (``msda_packed_attention_fwd_workspace_size``).
 
     A query that sees no key gives zeros. Rows of the result, and of the gradients, outside every sequence are
     zeros. Pairs that are not seen take no part, whatever their rows hold (infinities and NaN too; a key that is not
