@@ -564,7 +564,7 @@ int msda_packed_attention_shaped_bwd(const void* q, const void* k, const void* v
  * msda_cache4_read gives the values that the rows there stand for, in dtype (exact in both). Tokens of no sequence, and
  * those older than its keys, are not written, and read as zeros; other rows of the cache stay as they are. Sequences whose
  * rows overlap write over each other in no order. k, v: [tokens, kv_heads, head_dim], strides [2][2] in elements (token,
- * head), channels contiguous, rows on 16-byte boundaries.
+ * head), channels contiguous, rows on 16-byte boundaries; tokens ceil(kv_heads B / 8) < 2^26.
  *
  * msda_cache4_attention: msda_packed_attention_shaped_fwd over the cache (shape NULL: plain scores), without statistics;
  * strides of q and out [2][2]. Every value of the cache is a bf16 number exactly; with bf16 queries weights and out are
@@ -619,7 +619,7 @@ int msda_rotary(const void* q, void* q_out, const void* k, void* k_out, int dtyp
  *   weight_type: enum msda_dtype of the weights and of their gradients, f32 or bf16.
  *   strides: element strides (token, head), forward of q, q_out, k, k_out [4][2]; backward of q, grad_q_out, grad_q, k,
  *   grad_k_out, grad_k [6][2]. An output may be its input.
- * eps: 2^-126 to 2^126. Sums are f32, results rounded once.
+ * eps: 2^-126 to 2^126. Sums are f32, results rounded once. The forward takes fewer than 2^27 tokens.
  * Backward, for the cotangents of q_out and k_out: grad_q, grad_k and the weights' gradients (each may be NULL), the last
  * as sums over all tokens and heads in a fixed order, which take the workspace (NULL without them).
  */

@@ -92,7 +92,7 @@ int c4_rows(msda::Cache4Params& p, const void* const (&tensors)[2], int dtype, c
 template <typename K>
 int c4_launch(K kernel, const msda::Cache4Params& p, hipStream_t st, const char* what) {
   const int64_t waves = (2 * static_cast<int64_t>(p.kv_heads) * p.blocks * 4 + 63) / 64, grid = (waves * p.tokens + 3) / 4;
-  if (grid >= int64_t{1} << 31) return fail(MSDA_ERR_UNSUPPORTED, "cache in 4 bits: too many workgroups");
+  if (grid >= int64_t{1} << 24) return fail(MSDA_ERR_UNSUPPORTED, "cache in 4 bits: too many workgroups");  // a launch's threads are counted in 32 bits
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, st, p);
   return msda_host::check_launch(what);
 }

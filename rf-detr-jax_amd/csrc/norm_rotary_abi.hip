@@ -50,11 +50,11 @@ int run(const NormRotaryParams& p, bool backward, hipStream_t st) {
     for (int j = 0; j < 2; ++j) whole = whole && p.xs[i][j] % E == 0 && p.ys[i][j] % E == 0 && p.gs[i][j] % E == 0;
   }
   const int64_t grid = groups_of(p.tokens, backward);
+  if (grid >= int64_t{1} << 24) return fail(MSDA_ERR_UNSUPPORTED, "norm rotary: too many tokens");  // a launch's threads are counted in 32 bits
   const int lds = p.per * p.pairs * static_cast<int>(sizeof(float2));
   if (!whole) {
-    const int64_t any = grid;
-    if (backward) hipLaunchKernelGGL((msda::norm_rotary_any_kernel<T, NEIGHBOURS, true>), dim3(static_cast<unsigned>(any)), dim3(256), lds, st, p);
-    else hipLaunchKernelGGL((msda::norm_rotary_any_kernel<T, NEIGHBOURS, false>), dim3(static_cast<unsigned>(any)), dim3(256), lds, st, p);
+    if (backward) hipLaunchKernelGGL((msda::norm_rotary_any_kernel<T, NEIGHBOURS, true>), dim3(static_cast<unsigned>(grid)), dim3(256), lds, st, p);
+    else hipLaunchKernelGGL((msda::norm_rotary_any_kernel<T, NEIGHBOURS, false>), dim3(static_cast<unsigned>(grid)), dim3(256), lds, st, p);
   } else {
     const int turned = NEIGHBOURS ? 0 : p.pairs / E, units = turned + (p.dim - (NEIGHBOURS ? 0 : 2 * p.pairs) + 2 * E - 1) / (2 * E);
     if (units <= 4) launch_pieces<T, 4, NEIGHBOURS>(p, backward, grid, lds, st);
