@@ -1611,8 +1611,9 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 64 && M
   constexpr bool bf = sizeof(T) == 2;
   constexpr int PF = bf && DT != 64 && DT != 128 ? 3 : 2;
   // At 128 channels k, v, dk and dv take 192 of a wave's 256 registers. The last KEEP pieces of v wait in LDS: in
-  // registers the compiler spilled them, and each reload from scratch memory waited for the tile in flight. Three
-  // registers of other values are spilled still, two of them read back in the loop, behind a chunk's products.
+  // registers the compiler spilled them, and each reload from scratch memory waited for the tile in flight. Some are
+  // spilled still: three, two of them read back behind a chunk's products; with ranges alone one piece, read back in each
+  // block; with a cap four pieces, read back once a chunk behind its blocks; with slopes and no cap none in the loop.
   constexpr int KEEP = bf && DT == 128 ? 3 : 0;
   __shared__ __align__(16) unsigned char kept_rows[KEEP > 0 ? KEEP * kPkWaves * 1024 : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)), grp = lane >> 5, col = lane & 31;

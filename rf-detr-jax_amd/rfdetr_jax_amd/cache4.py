@@ -170,6 +170,11 @@ def cache4_attention(q, cache, offsets, key_offsets=None, key_lengths=None, caus
     ``q`` is float32 or bfloat16 ``[T, H, D]``, ``H`` a multiple of the cache's heads. The cache's values are bfloat16 numbers
     exactly and lose nothing more: results lie as far from the exact ones for these values as there.
 
+    A batch whose sequences have up to 16 rows (tokens times ``H / Hk``) on average takes one kernel, others another. The first
+    reads a sequence's keys once for each 16 of its rows, so a chunk among many single tokens is best called by itself: 63
+    tokens and a chunk of 190 over 8,000 keys in bfloat16, 32 heads to 8, 639 us in one call, and with a chunk of 194, which
+    the other kernel takes, 141.
+
     A query that sees no key, and rows outside every sequence, give zeros. Keys that are not seen take no part, whatever
     their rows hold; a block that is not finite makes the results of the queries that see it NaN (a key: all channels; a
     value: the block's). Not differentiable.

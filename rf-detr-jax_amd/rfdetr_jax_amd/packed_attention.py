@@ -269,7 +269,8 @@ def packed_attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causa
     bfloat16 for the matrix products: results lie 1.2 to 1.5 times as far from the exact ones as these rounded. Farther:
     gradients of k where a few tokens see a key, whose errors do not average out (4 to 31 tokens up to 1.8 times, two tokens
     2.4), and, without the options behind ``scale``, gradients of q and k of scores of several standard deviations (four: up
-    to 1.9 times, of 8 channels 2.5). New tokens (a sequence's tokens times ``H / Hk`` up to 32) keep their weights in two
+    to 1.9 times, of 8 channels 2.5). Where a row's gradients all but cancel (one weight near 1), what is left of them is good
+    to 2^-16 of its terms. New tokens (a sequence's tokens times ``H / Hk`` up to 32) keep their weights in two
     bfloat16 numbers. Float32 inputs are float32 throughout. Calls whose work does not fill the GPU evenly take a workspace
     of partial sums, in float32 prompts up to some hundred MB (``msda_packed_attention_fwd_workspace_size``).
 
