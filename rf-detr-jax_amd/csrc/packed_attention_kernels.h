@@ -1222,7 +1222,6 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
   const int parts = row < rows ? min(p.part_n[row], p.splits) : 0;
   float2 ml[kPkMostParts / LPR];  // of parts lane, lane + LPR, ..
   float m = -INFINITY, l = 0.0f;
-  bool lost = false;
 #pragma unroll
   for (int i = 0; i < kPkMostParts / LPR; ++i) {
     const int s = lane + LPR * i;
@@ -1233,13 +1232,11 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
   for (int x = LPR / 2; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x, LPR));
 #pragma unroll
   for (int i = 0; i < kPkMostParts / LPR; ++i) {
-    // the part's weight; -1: it saw keys, and is outweighed by 2^126 or more
-    const float w = ml[i].y != 0.0f ? at_exp2(ml[i].x - m) : 0.0f;
-    l += ml[i].y * w;
-    ml[i].x = ml[i].y != 0.0f && w == 0.0f ? -1.0f : w;
-    lost = lost || ml[i].x < 0.0f;
+    // The part's weight: never 0 where it saw keys, so that what is no finite number in it stays one, however a call is split.
+    const float w = at_exp2(ml[i].x - m);
+    ml[i].x = ml[i].y == 0.0f ? 0.0f : w < 0x1p-126f ? 0x1p-126f : w;
+    l += ml[i].y * ml[i].x;
   }
-  lost = __any(lost);
 #pragma unroll
   for (int x = LPR / 2; x > 0; x /= 2) l += __shfl_xor(l, x, LPR);
   if (parts <= 1) return;  // written already
@@ -1249,24 +1246,13 @@ __global__ void __launch_bounds__(256) pk_join_kernel(const PackParams p) {
   for (int ch = 4 * lane; ch < p.dim + 4 * (LPR - 1); ch += 4 * LPR) {  // every lane takes part in the shuffles
     const bool mine = ch < p.dim;
     at_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto add = [&](auto&& plus) {
 #pragma unroll
-      for (int i = 0; i < kPkMostParts / LPR; ++i)
+    for (int i = 0; i < kPkMostParts / LPR; ++i)
 #pragma unroll 4
-        for (int s = LPR * i; s < min(parts, LPR * (i + 1)); ++s) {
-          const float w = __shfl(ml[i].x, s - LPR * i, LPR);
-          if (mine && w != 0.0f) a = plus(a, *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch), w);
-        }
-    };
-    if (!lost) {
-      add([](const at_f4& a, const at_f4& x, float w) { return a + x * w; });
-    } else {  // what is no finite number in such a part stays one, however a call is split
-      add([](at_f4 a, const at_f4& x, float w) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = !(w < 0.0f) ? fmaf(x[j], w, a[j]) : x[j] - x[j] != 0.0f ? a[j] + x[j] : a[j];
-        return a;
-      });
-    }
+      for (int s = LPR * i; s < min(parts, LPR * (i + 1)); ++s) {
+        const float w = __shfl(ml[i].x, s - LPR * i, LPR);
+        if (mine && w != 0.0f) a += *reinterpret_cast<const at_f4*>(p.part_o + (s * rows + row) * p.dim + ch) * w;
+      }
     if (!mine) continue;
     a *= inv;
     pk_put4(out + ch, a);
