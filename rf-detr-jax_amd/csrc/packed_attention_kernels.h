@@ -1174,7 +1174,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[nd][i] = y[nd][i] != 0.0f ? y[nd][i] : o[nd][i];
+      for (int i = 0; i < 16; ++i)  // (the plain kernels' o has those of the chunks in front of the diagonal)
+        if (y[nd][i] != 0.0f) o[nd][i] = MOD == 0 && !odd && o[nd][i] - o[nd][i] != 0.0f ? o[nd][i] + y[nd][i] : y[nd][i];
   }
   l = at_sum_halves(l);
   pk_barrier();  // the tiles hold the waves' scratch from here

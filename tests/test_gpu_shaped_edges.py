@@ -98,3 +98,32 @@ def test_a_value_that_is_not_finite_in_a_part_that_weighs_nothing(value, n, dtyp
         assert not torch.isfinite(got[:, 2:, 33]).any()
         rest = [c for c in range(d) if c != 33]
         assert torch.equal(got[:, 2:, rest], want[:, 2:, rest]) and torch.equal(got[:, :2], want[:, :2])
+
+
+@TYPES
+@pytest.mark.parametrize("kw", [{}, dict(cap=4.0), dict(window=250), dict(window=100)], ids=["plain", "cap", "window", "narrow"])
+def test_values_that_are_not_finite_at_both_ends_of_what_a_row_sees(kw, dtype):
+    """Two values of one channel that are not finite, one in a chunk that every row of the workgroup sees and one on the
+    diagonal or at the window's end: the rows that see both get their sum, those that see one get it."""
+    n, h, hk, d = 400, 4, 2, 64
+    q, k, v = _normal(4, dtype, (n, h, d), (n, hk, d), (n, hk, d))
+    q = 0.1 * q  # every weight is well above 0
+    clean = packed_attention(q, k, v, _int([0, n]), **kw)
+    inf, nan = float("inf"), float("nan")
+    places = torch.arange(n, device=_dev())
+
+    def sees(key):
+        return (places >= key) & (places - key < kw.get("window", n))
+
+    for first, last, a, b in ((20, 300, inf, -inf), (20, 300, nan, inf), (140, 390, -inf, inf), (200, 270, inf, -inf), (20, 300, inf, inf)):
+        odd = v.clone()
+        odd[first, :, 5], odd[last, :, 5] = a, b
+        got = packed_attention(q, k, odd, _int([0, n]), **kw)
+        both, one, other = sees(first) & sees(last), sees(first) & ~sees(last), sees(last) & ~sees(first)
+        for rows, value in ((both, a + b), (one, a), (other, b)):
+            x = got[rows][..., 5].float()
+            assert torch.isnan(x).all() if value != value else (x == value).all(), (first, last, a, b, value)
+        none = ~(sees(first) | sees(last))
+        assert torch.equal(got[none], clean[none])
+        rest = [c for c in range(d) if c != 5]
+        assert torch.equal(got[..., rest], clean[..., rest])
