@@ -960,7 +960,8 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     if (min(k0 + kPkChunk, w.m) > all || (MOD != 0 && k0 < alo)) {
       if (MOD == 0 && threadIdx.x < 2) bad[turn ^ 1][threadIdx.x] = 0;
       pk_settle<T, DT>(Vb, bad[turn]);
-      sick = sick || pk_settled(bad[turn]) != 0;
+      const bool found = pk_settled(bad[turn]) != 0;  // (its barrier in front of every such chunk's products)
+      sick = sick || found;
     }
     if (k0 >= wend || (MOD != 0 && k0 + kPkChunk <= wbegin)) {
       next.all();

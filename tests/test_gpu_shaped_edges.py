@@ -127,3 +127,30 @@ def test_values_that_are_not_finite_at_both_ends_of_what_a_row_sees(kw, dtype):
         assert torch.equal(got[none], clean[none])
         rest = [c for c in range(d) if c != 5]
         assert torch.equal(got[..., rest], clean[..., rest])
+
+
+@TYPES
+@pytest.mark.parametrize("kw", [{}, dict(cap=4.0), dict(window=100), dict(window=30, cap=4.0), dict(window=90, causal=False)],
+                         ids=["plain", "cap", "window", "narrow", "open"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunk_after_chunk_of_values_that_are_not_finite(dim, kw, dtype):
+    """Values that are not finite in every chunk on a tile's diagonal and at its window's ends, one chunk behind the other:
+    each is searched and settled before any wave multiplies with it. Rows that see none of them keep their bits, in call
+    after call, and those that see one have NaN in its channel alone."""
+    n, h, hk = 700, 2, 2
+    q, k, v = _normal(5, dtype, (n, h, dim), (n, hk, dim), (n, hk, dim))
+    off, window, causal = _int([0, n]), kw.get("window", n), kw.get("causal", True)
+    clean = packed_attention(q, k, v, off, **kw)
+    keys = list(range(40, n, 61))
+    odd = v.clone()
+    odd[keys, :, 7] = float("nan")
+    odd[keys, :, dim - 3] = float("nan")
+    place, key = torch.arange(n, device=_dev())[:, None], torch.tensor(keys, device=_dev())[None]
+    sees = ((place - key).abs() < window) & ((key <= place) if causal else torch.ones_like(key <= place))
+    sees = sees.any(1)
+    rest = [c for c in range(dim) if c not in (7, dim - 3)]
+    for _ in range(10):
+        got = packed_attention(q, k, odd, off, **kw)
+        assert torch.equal(got[~sees], clean[~sees])
+        assert torch.isnan(got[sees][..., [7, dim - 3]]).all()
+        assert torch.equal(got[sees][..., rest], clean[sees][..., rest])
