@@ -1157,8 +1157,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
     at_f16 y[DT / 32];
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd) y[nd] = at_zero16();
+    // Where only pk_settle found some: the chunks that it searched, which begin in front of `alo` or end behind `all`.
+    const int near = (alo + kPkChunk - 1) / kPkChunk * kPkChunk, far = odd ? near : max(all / kPkChunk * kPkChunk, near);
 #pragma unroll 1
-    for (int j = MOD != 0 ? max(c0 * kPkChunk, lo) : (odd ? c0 : max(all / kPkChunk, c0)) * kPkChunk; j < min(c1 * kPkChunk, lim); ++j)
+    for (int j = max(c0 * kPkChunk, lo); j < min(c1 * kPkChunk, lim); ++j) {
+      if (j >= near && j < far) j = far;
+      if (j >= min(c1 * kPkChunk, lim)) break;
 #pragma unroll
       for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
@@ -1172,11 +1176,12 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
           }
           if (x - x != 0.0f) y[nd][i] += x;
         }
+    }
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)  // (the plain kernels' o has those of the chunks in front of the diagonal)
-        if (y[nd][i] != 0.0f) o[nd][i] = MOD == 0 && !odd && o[nd][i] - o[nd][i] != 0.0f ? o[nd][i] + y[nd][i] : y[nd][i];
+      for (int i = 0; i < 16; ++i)  // (o has those of the chunks between)
+        if (y[nd][i] != 0.0f) o[nd][i] = !odd && o[nd][i] - o[nd][i] != 0.0f ? o[nd][i] + y[nd][i] : y[nd][i];
   }
   l = at_sum_halves(l);
   pk_barrier();  // the tiles hold the waves' scratch from here
