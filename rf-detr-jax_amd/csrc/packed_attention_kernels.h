@@ -61,11 +61,14 @@ struct PackParams {
   float* part_ml;            // [splits][q_rows * heads][2]: m, l
   int32_t* part_n;           // [q_rows * heads]: the row's parts
   float* part_kv;            // key side: [splits][dk, dv][k_rows * kv_heads][dim]
+  float* part_q;             // shaped scores, queries' side of the backward: [q_parts][q_rows * heads][dim]
+  int32_t* part_q_n;         // [q_rows * heads]: q_parts, or 1 where the row is outside every sequence
   int64_t st[kPkTensors][2];  // element strides (row, head) of each tensor
   int sequences, q_rows, k_rows, heads, kv_heads, group, dim, causal;
   int splits;    // at most so many workgroups share a tile's streamed rows
   int part;      // chunks of one of them, unless that makes more (forward; key side of shaped scores)
   int slots;     // tiles of the kernel's own side
+  int q_parts;   // shaped scores, backward: workgroups that share a tile of queries
   float scale;   // of the scores
   float scale2;  // scale log2(e)
   // shaped scores (PackShaped)
@@ -76,10 +79,6 @@ struct PackParams {
   // a cache in 4 bits (cache4_kernels.h): k and v are its codes
   const uint8_t* k_scales;
   const uint8_t* v_scales;
-  // the backward of shaped scores, queries' side
-  float* part_q;      // [q_parts][q_rows * heads][dim]
-  int32_t* part_q_n;  // [q_rows * heads]: q_parts, or 1 where the row is outside every sequence
-  int q_parts;        // workgroups that share a tile of queries
 };
 
 // What a kernel of shaped scores does besides the ranges [lo, hi) of keys that a query sees; 0: the plain kernels,
