@@ -1152,16 +1152,15 @@ __global__ void __launch_bounds__(64 * kPkWaves, sizeof(T) == 2 ? (DT <= 32 ? 4 
         for (int i = 0; i < 16; ++i) odd = odd || o[nd][i] != o[nd][i];
       odd = __any(odd);
     }
-  if (sick || odd) {
+  if (__builtin_expect(sick || odd, 0)) {
     at_f16 y[DT / 32];
 #pragma unroll
     for (int nd = 0; nd < DT / 32; ++nd) y[nd] = at_zero16();
     // Where only pk_settle found some: the chunks that it searched, which begin in front of `alo` or end behind `all`.
     const int near = (alo + kPkChunk - 1) / kPkChunk * kPkChunk, far = odd ? near : max(all / kPkChunk * kPkChunk, near);
+    const int stop = min(c1 * kPkChunk, lim);
 #pragma unroll 1
-    for (int j = max(c0 * kPkChunk, lo); j < min(c1 * kPkChunk, lim); ++j) {
-      if (j >= near && j < far) j = far;
-      if (j >= min(c1 * kPkChunk, lim)) break;
+    for (int j = max(c0 * kPkChunk, lo); j < stop; j = j + 1 >= near && j + 1 < far ? far : j + 1) {
 #pragma unroll
       for (int nd = 0; nd < DT / 32; ++nd)
 #pragma unroll
